@@ -17,6 +17,7 @@
 #include <string>
 
 #include "hkx.h"
+#include "hkx_api.hpp"
 #include "hkx_launch.hpp"
 
 namespace {
@@ -506,6 +507,23 @@ int scratch_for_current_device(void** out) {
 }
 
 }  // namespace
+
+namespace hkx {
+
+int api_fail(int code, const char* fmt, ...) {
+  char buf[512];
+  va_list ap;
+  va_start(ap, fmt);
+  vsnprintf(buf, sizeof buf, fmt, ap);
+  va_end(ap);
+  return fail(code, "%s", buf);
+}
+
+void api_clear() { g_err.clear(); }
+int api_launched(hipError_t e, const char* what) { return launched(e, what); }
+int api_cus() { return cu_count(); }
+
+}  // namespace hkx
 
 extern "C" {
 

@@ -25,6 +25,7 @@ OK, ERR_SHAPE, ERR_DTYPE, ERR_WORKSPACE, ERR_LAUNCH, ERR_ARG = range(6)
 BF16, FP16, FP32, FP8E4M3, INT8 = range(5)
 #: ab_dtype codes of fp8 operand pairs with e5m2: both, A e4m3 x B e5m2, A e5m2 x B e4m3
 FP8E5M2, FP8_E4M3_E5M2, FP8_E5M2_E4M3 = 5, 6, 7
+FP4E2M1 = 8  #: packed e2m1, two a byte (the MXFP4 calls)
 ROW, COL, TILE = 1, 2, 3
 EP_NONE, EP_FUSED, EP_PROGRAM, EP_SILU_MUL = range(4)
 ACT_NONE, ACT_GELU_TANH, ACT_SILU, ACT_RELU = range(4)
@@ -74,11 +75,41 @@ class HkxGemmArgs(Structure):
                 ("counters", c_void_p), ("counters_len", c_int64)]
 
 
+class HkxMx4GemmArgs(Structure):
+    _fields_ = [("size", c_int32), ("a_dtype", c_int32), ("a", c_void_p), ("b", c_void_p),
+                ("sa", c_void_p), ("sb", c_void_p), ("bias", c_void_p), ("c", c_void_p),
+                ("lda", c_int64), ("ldb", c_int64), ("sa_ld", c_int64), ("sb_ld", c_int64),
+                ("ldc", c_int64), ("m", c_int32), ("n", c_int32), ("k", c_int32),
+                ("bias_dtype", c_int32), ("silu_mul", c_int32), ("reserved", c_int32),
+                ("ws", c_void_p), ("ws_bytes", c_size_t)]
+
+
+class HkxBlockNormArgs(Structure):
+    _fields_ = [("size", c_int32), ("x_dtype", c_int32), ("r_dtype", c_int32),
+                ("w_dtype", c_int32), ("gate_dtype", c_int32), ("rows", c_int32), ("d", c_int32),
+                ("gate_rows", c_int32), ("gate_col", c_int32), ("quant", c_int32),
+                ("branch_scale", c_float), ("residual_scale", c_float), ("eps", c_float),
+                ("reserved", c_int32), ("x", c_void_p), ("residual", c_void_p),
+                ("post", c_void_p), ("pre", c_void_p), ("gate", c_void_p), ("h", c_void_p),
+                ("y", c_void_p), ("y_scales", c_void_p), ("rstd", c_void_p), ("ldx", c_int64),
+                ("ldr", c_int64), ("ldh", c_int64), ("ldy", c_int64), ("ldys", c_int64)]
+
+
+class HkxBlockNormGradArgs(Structure):
+    _fields_ = [("size", c_int32), ("reserved", c_int32), ("f", HkxBlockNormArgs),
+                ("dh", c_void_p), ("dy", c_void_p), ("dx", c_void_p), ("dresidual", c_void_p),
+                ("dpost", c_void_p), ("dpre", c_void_p), ("dgate", c_void_p), ("lddh", c_int64),
+                ("lddy", c_int64), ("lddx", c_int64), ("lddr", c_int64), ("ws", c_void_p),
+                ("ws_bytes", c_size_t)]
+
+
 #: Every function include/hkx.h declares.
 SYMBOLS = ("hkx_abi_version", "hkx_abi_sizes", "hkx_last_error", "hkx_gemm_workspace",
            "hkx_gemm_counters",
            "hkx_gemm_check", "hkx_gemm", "hkx_scaled_mm", "hkx_mx_gemm", "hkx_mx_gemm_workspace",
-           "hkx_mx_quant", "hkx_gemm_noalloc")
+           "hkx_mx_quant", "hkx_gemm_noalloc", "hkx_mx4_quant", "hkx_mx_dequant", "hkx_mx4_gemm",
+           "hkx_mx4_gemm_workspace", "hkx_block_norm", "hkx_block_norm_backward",
+           "hkx_block_norm_backward_workspace")
 
 _LIB = None
 _LOCK = threading.Lock()
@@ -130,6 +161,17 @@ def lib() -> ctypes.CDLL:
         L.hkx_scaled_mm.argtypes = [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64,
                                     c_void_p, c_int32, c_void_p, c_void_p, c_int64, c_int32,
                                     c_int32, c_int32, c_void_p, c_size_t, c_void_p]
+        L.hkx_mx4_quant.argtypes = [c_void_p, c_int64, c_int32, c_void_p, c_int64, c_void_p,
+                                    c_int64, c_int32, c_int32, c_void_p]
+        L.hkx_mx_dequant.argtypes = [c_void_p, c_int64, c_int32, c_void_p, c_int64, c_void_p,
+                                     c_int64, c_int32, c_int32, c_int32, c_void_p]
+        L.hkx_mx4_gemm.argtypes = [POINTER(HkxMx4GemmArgs), c_void_p]
+        L.hkx_mx4_gemm_workspace.argtypes = [POINTER(HkxMx4GemmArgs)]
+        L.hkx_mx4_gemm_workspace.restype = c_size_t
+        L.hkx_block_norm.argtypes = [POINTER(HkxBlockNormArgs), c_void_p]
+        L.hkx_block_norm_backward.argtypes = [POINTER(HkxBlockNormGradArgs), c_void_p]
+        L.hkx_block_norm_backward_workspace.argtypes = [POINTER(HkxBlockNormGradArgs)]
+        L.hkx_block_norm_backward_workspace.restype = c_size_t
         sizes = (c_size_t * 4)()
         L.hkx_abi_sizes(sizes)
         want = [ctypes.sizeof(t) for t in (HkxOperand, HkxInstr, HkxEpilogue, HkxGemmArgs)]

@@ -125,6 +125,44 @@ def quant(x, out=None):
     return q, s
 
 
+def dequant(q, s, dtype=None):
+    """The numbers that (q, s) stand for: q float8_e4m3fn [M, K] with E8M0 scales s [M, K/32], as
+    bf16 or `dtype` (fp16, fp32), rounded once. A block of scale 255 is NaN."""
+    import torch  # noqa: PLC0415
+
+    if q.dtype != torch.float8_e4m3fn or q.dim() != 2:
+        raise TypeError(f"mxfp8.dequant: q is float8_e4m3fn (M, K), got {q.dtype} {tuple(q.shape)}")
+    return _dequant("mxfp8.dequant", q, s, dtype, nat.FP8E4M3, q.shape[1])
+
+
+def _dequant(call, q, s, dtype, code, k):
+    import torch  # noqa: PLC0415
+
+    dtype = torch.bfloat16 if dtype is None else dtype
+    if dtype not in (torch.bfloat16, torch.float16, torch.float32):
+        raise TypeError(f"{call}: numbers as bf16, fp16 or fp32, got {dtype}")
+    m = q.shape[0]
+    if k % 32:
+        raise ValueError(f"{call}: K={k}, a multiple of 32")
+    if s.dtype != torch.uint8 or tuple(s.shape) != (m, k // 32):
+        raise ValueError(f"{call}: s is uint8 ({m}, {k // 32}), got {s.dtype} {tuple(s.shape)}")
+    if not q.is_cuda:
+        raise ValueError(f"{call}: q is on a GPU, got {q.device}")
+    _on(q.device, call, s=s)
+    if q.stride(1) != 1 or q.stride(0) % 8 or q.data_ptr() % 8:
+        q = q.contiguous()
+    if s.stride(1) != 1:
+        s = s.contiguous()
+    y = nat.empty(q, (m, k), dtype)
+    if m == 0 or k == 0:
+        return y
+    nat.check(nat.lib().hkx_mx_dequant(
+        q.data_ptr(), max(q.stride(0), q.shape[1]), code, s.data_ptr(),
+        max(s.stride(0), k // 32), y.data_ptr(), k, nat.dtype_code(dtype), m, k,
+        nat.stream_of(q.device)))
+    return y
+
+
 def linear(x, w, ws):
     """bf16 x [M, K] @ (ws . w)^T, w fp8 [N, K] with E8M0 row scales ws [N, K/32]: the
     activation quantized (`quant`), then `gemm`."""
@@ -132,4 +170,4 @@ def linear(x, w, ws):
     return gemm(xq, w, xs, ws)
 
 
-__all__ = ["gemm", "quant", "linear", "expand_block_scales"]
+__all__ = ["gemm", "quant", "dequant", "linear", "expand_block_scales"]

@@ -74,6 +74,7 @@ extern "C" {
 #define HKX_FP8E5M2 5        /* A and B e5m2 */
 #define HKX_FP8_E4M3_E5M2 6  /* A e4m3, B e5m2 (e.g. activations against a gradient) */
 #define HKX_FP8_E5M2_E4M3 7  /* A e5m2, B e4m3 */
+#define HKX_FP4E2M1 8 /* OCP e2m1, two a byte, the even column in the low bits: the MXFP4 calls only */
 
 /* Epilogue operand kinds: what an operand is against C (M, N) -- templates/gemm.py:116-135. */
 #define HKX_ROW 1  /* (N,) or (1, N): one value per column of C (a bias, a per-channel scale) */
@@ -314,6 +315,98 @@ size_t hkx_mx_gemm_workspace(int32_t m, int32_t n, int32_t k);
  * q and s). */
 int hkx_mx_quant(const void* x, int64_t ldx, void* q, int64_t ldq, uint8_t* s, int64_t lds,
                  int32_t m, int32_t k, void* stream);
+
+/* ---------------------------------------------------------------- MXFP4, and the block norm */
+
+/* x (M, K) of x_dtype (bf16, fp16, fp32) -> q (M, K/2 bytes) packed e2m1 and s (M, K/32) E8M0
+ * bytes: per 32-column block e = ceil(log2(amax / 6)) at least -127, q = x / 2^e rounded to the
+ * nearest, ties to the even code, s = e + 127; a block with an infinity or a NaN has s = 255
+ * (E8M0's NaN) and codes 0. K a multiple of 32; x's rows 16-byte aligned, q's 4-byte; strides in
+ * elements of x and bytes of q and s. */
+int hkx_mx4_quant(const void* x, int64_t ldx, int32_t x_dtype, void* q, int64_t ldq, uint8_t* s,
+                  int64_t lds, int32_t m, int32_t k, void* stream);
+
+/* The numbers MX values stand for: q (M, K) packed e2m1 (HKX_FP4E2M1) or e4m3 (HKX_FP8E4M3) with s
+ * (M, K/32) E8M0 bytes -> y (M, K) of y_dtype, rounded once; a block of scale 255 is NaN. y's rows
+ * 16-byte aligned, q's 4-byte (8-byte for e4m3). */
+int hkx_mx_dequant(const void* q, int64_t ldq, int32_t q_dtype, const uint8_t* s, int64_t lds,
+                   void* y, int64_t ldy, int32_t y_dtype, int32_t m, int32_t k, void* stream);
+
+/* bf16 C (M, N) = (sa . A)(sb . B)^T (+ bias): A (M, K) packed e2m1 or e4m3, B (N, K) packed e2m1,
+ * sa (M, K/32) and sb (N, K/32) E8M0 bytes. silu_mul: B has 2N rows, Z = (sa . A)(sb . B)^T (+ bias
+ * of 2N) and C = silu(Z[:, :N]) * Z[:, N:]. Sums in fp32, one rounding. Any M and N, K a multiple of
+ * 32. Row strides lda, ldb, sa_ld, sb_ld in bytes, ldc in elements; A's and B's rows 16-byte, the
+ * scales' 4-byte aligned (up to 3 bytes past a scale row's K/32, within its last dword, are read). */
+typedef struct {
+  int32_t size; /* sizeof(HkxMx4GemmArgs): the library refuses another layout */
+  int32_t a_dtype;
+  const void* a;
+  const void* b;
+  const uint8_t* sa;
+  const uint8_t* sb;
+  const void* bias; /* NULL: none */
+  void* c;
+  int64_t lda, ldb, sa_ld, sb_ld, ldc;
+  int32_t m, n, k;
+  int32_t bias_dtype; /* HKX_BF16 / HKX_FP16 / HKX_FP32 */
+  int32_t silu_mul;
+  int32_t reserved;
+  void* ws; /* hkx_mx4_gemm_workspace() bytes, 16-byte aligned; NULL where that is 0 */
+  size_t ws_bytes;
+} HkxMx4GemmArgs;
+int hkx_mx4_gemm(const HkxMx4GemmArgs* args, void* stream);
+size_t hkx_mx4_gemm_workspace(const HkxMx4GemmArgs* args);
+
+/* Between two blocks, a row at a time: u = x rsqrt(mean x^2 + eps) post (u = x without post), h =
+ * residual_scale residual + branch_scale gate u, y = h rsqrt(mean h^2 + eps) pre (no y without pre).
+ * x and y of x_dtype (bf16, fp16, fp32), residual and h of r_dtype (the same or fp32), post and pre
+ * (d,) of w_dtype and gate of gate_dtype (x's or fp32). The gate's rows, d long (gate_col 1) or one
+ * value (0), stand one after another, each for gate_rows rows of x. quant 1: y as MXFP8 (e4m3, ldy
+ * bytes a row) with y_scales, 2: as MXFP4; d then a multiple of 32 and every row 16-byte aligned.
+ * rstd (rows, 2) fp32 keeps the two norms' factors for the backward pass (NULL: not kept). d at most
+ * 16384, in the backward pass 8192. Strides in elements. */
+typedef struct {
+  int32_t size; /* sizeof(HkxBlockNormArgs) */
+  int32_t x_dtype, r_dtype, w_dtype, gate_dtype;
+  int32_t rows, d;
+  int32_t gate_rows, gate_col;
+  int32_t quant;
+  float branch_scale, residual_scale, eps;
+  int32_t reserved;
+  const void* x;
+  const void* residual;
+  const void* post;
+  const void* pre;
+  const void* gate;
+  void* h;
+  void* y;
+  uint8_t* y_scales;
+  float* rstd;
+  int64_t ldx, ldr, ldh, ldy, ldys;
+} HkxBlockNormArgs;
+int hkx_block_norm(const HkxBlockNormArgs* args, void* stream);
+
+/* Its gradients from dh and dy (NULL: zero): dx (x's type), dresidual (its type), dpost and dpre
+ * (w_dtype), dgate (the gate's shape and type, summed over the rows and columns it is broadcast
+ * over); dpost, dpre and dgate may be NULL. f as in the forward call, with its rstd; f's h, y and
+ * y_scales are not used. Sums in fp32 in a fixed order: the same bits every call. */
+typedef struct {
+  int32_t size; /* sizeof(HkxBlockNormGradArgs) */
+  int32_t reserved;
+  HkxBlockNormArgs f;
+  const void* dh;
+  const void* dy;
+  void* dx;
+  void* dresidual;
+  void* dpost;
+  void* dpre;
+  void* dgate;
+  int64_t lddh, lddy, lddx, lddr;
+  void* ws; /* hkx_block_norm_backward_workspace() bytes, 16-byte aligned */
+  size_t ws_bytes;
+} HkxBlockNormGradArgs;
+int hkx_block_norm_backward(const HkxBlockNormGradArgs* args, void* stream);
+size_t hkx_block_norm_backward_workspace(const HkxBlockNormGradArgs* args);
 
 #ifdef __cplusplus
 }
