@@ -91,7 +91,8 @@ int forward_args(const HkxBlockNormArgs& g, const char* what, NormArgs& a) {
   return HKX_OK;
 }
 
-// A backward call's workers: two waves a SIMD of the GPU, at least 2 rows each.
+// A backward call's workers: two waves a SIMD of the GPU, at least 2 rows each. (Their number, and so
+// the workspace, goes by the shape alone, not by how a call's rows are aligned.)
 struct Grad {
   int workers, parts, groups, group_rows;
   NormShape shape;

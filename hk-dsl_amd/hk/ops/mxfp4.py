@@ -9,6 +9,9 @@ The OCP MX layout: two e2m1 codes a byte, the even column in the low bits (uint8
 float4_e2m1fn_x2), and one E8M0 byte (2^(s - 127); 255 is NaN) a row and 32 columns. Scales whose rows
 start at multiples of 4 bytes are read in place (`quant` makes such rows at any K); others are copied
 every call, so a weight's scales are best laid out once by `scale_rows`.
+
+A call's checks and layout are kept by the shapes, strides and types they depend on, as a template of
+the library's arguments; a call of known layout fills in its addresses.
 """
 
 from __future__ import annotations
@@ -31,41 +34,47 @@ def _packed(t, call, name):
     raise TypeError(f"{call}: {name} holds packed 4-bit codes (uint8 or float4_e2m1fn_x2), got {t.dtype}")
 
 
+def _e8m0(s, shape, name):
+    import torch  # noqa: PLC0415
+
+    if s.dtype == torch.float8_e8m0fnu:
+        s = s.view(torch.uint8)
+    if s.dtype != torch.uint8:
+        raise TypeError(f"mxfp4.gemm: {name} holds E8M0 bytes (uint8), got {s.dtype}")
+    if tuple(s.shape) != shape:
+        raise ValueError(f"mxfp4.gemm: {name} is {tuple(s.shape)}, expected {shape}")
+    return s
+
+
 def scale_rows(s):
     """E8M0 scales (rows, K/32) with rows that start at multiples of 4 bytes: `s` itself where it has
     them, else a copy."""
-    if s.stride(1) == 1 and s.stride(0) % 4 == 0 and s.data_ptr() % 4 == 0:
-        return s
     rows, k32 = s.shape
+    st = s.stride()
+    if s.data_ptr() % 4 == 0 and st[1] == 1 and (rows < 2 or (st[0] % 4 == 0 and st[0] >= k32)):
+        return s
     out = s.new_empty((rows, (k32 + 3) // 4 * 4))[:, :k32]
     out.copy_(s)
     return out
 
 
-def _scales(s, rows, k, name):
-    import torch  # noqa: PLC0415
-
-    if s.dtype != torch.uint8 and s.dtype != torch.float8_e8m0fnu:
-        raise TypeError(f"mxfp4.gemm: {name} holds E8M0 bytes (uint8), got {s.dtype}")
-    if s.shape != (rows, k // 32):
-        raise ValueError(f"mxfp4.gemm: {name} is {tuple(s.shape)}, expected ({rows}, {k // 32})")
-    if s.dtype != torch.uint8:
-        s = s.view(torch.uint8)
-    return scale_rows(s)
-
-
 def _rows16(t):
     """`t` with rows the kernels read in place: unit stride along K, 16-byte aligned."""
-    st = t.stride()
-    if st[1] == 1 and st[0] % 16 == 0 and t.data_ptr() % 16 == 0 and (st[0] >= t.shape[1]):
+    rows, st = t.shape[0], t.stride()
+    if t.data_ptr() % 16 == 0 and st[1] == 1 and (rows < 2 or (st[0] % 16 == 0 and st[0] >= t.shape[1])):
         return t
-    return t.clone(memory_format=_contiguous())
+    out = t.new_empty(t.shape)
+    out.copy_(t)
+    return out
 
 
-def _contiguous():
-    import torch  # noqa: PLC0415
+def _ld(t, least):
+    """A matrix's row stride (a single row's is anything)."""
+    return t.stride(0) if t.shape[0] > 1 else least
 
-    return torch.contiguous_format
+
+#: What quant knows of a layout of x: (M, K, x's type code, x's row stride, the scales' row stride).
+_QUANT: dict = {}
 
 
 def quant(x, out=None):
@@ -73,6 +82,25 @@ def quant(x, out=None):
     uint8 (M, K/32). A block's scale is 2^ceil(log2(amax / 6)) (nothing is clamped), its codes x over
     that rounded to the nearest, ties to even; a block with an infinity or a NaN is NaN (scale 255).
     `out`: (q, s) to write into."""
+    key = (x.shape, x.stride(), x.dtype)
+    plan = _QUANT.get(key)
+    if plan is None or out is not None or x.data_ptr() & 15 or x.get_device() < 0:
+        return _quant(x, out, key)
+    import torch  # noqa: PLC0415
+
+    m, k, code, ldx, lds = plan
+    if type(x) is torch.Tensor:
+        q = x.new_empty((m, k >> 1), dtype=torch.uint8)
+        s = x.new_empty_strided((m, k >> 5), (lds, 1), dtype=torch.uint8)
+    else:
+        q = nat.empty(x, (m, k >> 1), torch.uint8)
+        s = torch.empty_strided((m, k >> 5), (lds, 1), dtype=torch.uint8, device=x.device)
+    nat.check(nat.lib().hkx_mx4_quant(x.data_ptr(), ldx, code, q.data_ptr(), k >> 1, s.data_ptr(), lds,
+                                      m, k, nat.stream_of(x.device)))
+    return q, s
+
+
+def _quant(x, out, key):
     import torch  # noqa: PLC0415
 
     if x.dtype not in (torch.bfloat16, torch.float16, torch.float32) or x.dim() != 2:
@@ -82,98 +110,140 @@ def quant(x, out=None):
         raise ValueError(f"mxfp4.quant: K={k}, a multiple of 32")
     if not x.is_cuda:
         raise ValueError(f"mxfp4.quant: x is on a GPU, got {x.device}")
-    per = 16 // x.element_size()
-    if x.stride(1) != 1 or x.stride(0) % per or x.stride(0) < k or x.data_ptr() % 16:
-        x = x.clone(memory_format=torch.contiguous_format)
+    per, ldx = 16 // x.element_size(), _ld(x, k)
+    if x.stride(1) != 1 or ldx % per or ldx < k or x.data_ptr() % 16:
+        x, ldx = x.clone(memory_format=torch.contiguous_format), k
+    elif m:
+        nat.remember(_QUANT, key, (m, k, nat.dtype_code(x.dtype), ldx, (k // 32 + 3) // 4 * 4), 4096)
     if out is not None:
         q, s = out
         q = _packed(q, "mxfp4.quant", "out")
+        ldq, lds = _ld(q, k // 2), _ld(s, k // 32)
         if (tuple(q.shape) != (m, k // 2) or tuple(s.shape) != (m, k // 32) or s.dtype != torch.uint8
-                or q.stride(1) != 1 or s.stride(1) != 1 or q.stride(0) % 4 or q.data_ptr() % 4
-                or q.stride(0) < k // 2 or s.stride(0) < k // 32):
+                or q.stride(1) != 1 or s.stride(1) != 1 or ldq % 4 or q.data_ptr() % 4
+                or ldq < k // 2 or lds < k // 32):
             raise ValueError(f"mxfp4.quant: out is uint8 ({m}, {k // 2}) with 4-byte aligned rows and "
                              f"uint8 ({m}, {k // 32})")
         _on(x.device, "mxfp4.quant", q=q, s=s)
     else:
+        ldq, lds = k // 2, (k // 32 + 3) // 4 * 4
         q = nat.empty(x, (m, k // 2), torch.uint8)
-        s = nat.empty(x, (m, (k // 32 + 3) // 4 * 4), torch.uint8)
-        if k % 128:
-            s = s[:, :k // 32]
-    if m == 0:
-        return q, s
-    nat.check(nat.lib().hkx_mx4_quant(x.data_ptr(), x.stride(0), nat.dtype_code(x.dtype),
-                                      q.data_ptr(), q.stride(0), s.data_ptr(), s.stride(0), m, k,
-                                      nat.stream_of(x.device)))
+        s = torch.empty_strided((m, k // 32), (lds, 1), dtype=torch.uint8, device=x.device)
+    if m:
+        nat.check(nat.lib().hkx_mx4_quant(x.data_ptr(), ldx, nat.dtype_code(x.dtype), q.data_ptr(), ldq,
+                                          s.data_ptr(), lds, m, k, nat.stream_of(x.device)))
     return q, s
 
 
 def dequant(q, s, dtype=None):
-    """The numbers that (q, s) stand for, (M, K) bf16 or `dtype` (fp16, fp32), rounded once."""
-    if q.dim() != 2:
-        raise ValueError(f"mxfp4.dequant: q is (M, K/2), got {tuple(q.shape)}")
-    q = _packed(q, "mxfp4.dequant", "q")
-    return _dequant("mxfp4.dequant", q, s, dtype, nat.FP4E2M1, 2 * q.shape[1])
+    """The numbers that (q, s) stand for, (..., K) bf16 or `dtype` (fp16, fp32), rounded once: q (...,
+    K/2) packed codes with E8M0 scales s (..., K/32). A block of scale 255 is NaN."""
+    return _dequant("mxfp4.dequant", _packed(q, "mxfp4.dequant", "q"), s, dtype, nat.FP4E2M1, 2)
+
+
+#: Layouts of gemm's operands: (arguments filled in but for their addresses, workspace bytes, C's shape).
+_GEMM: dict = {}
 
 
 def gemm(a, b, sa, sb, *, bias=None, silu_mul=False, out=None):
-    """bf16 (M, N) = (sa . a)(sb . b)^T (+ bias): a (M, K/2) packed codes or (M, K) float8_e4m3fn, b
-    (N, K/2) packed codes, sa and sb their E8M0 scales (rows, K/32), bias (N,) bf16, fp16 or fp32. With
-    silu_mul, b (2N, K/2) holds gate rows, then up rows: silu(z[:, :N]) * z[:, N:] of z (M, 2N) with its
-    bias. Any M and N, K a multiple of 32; sums in fp32, rounded once."""
+    """bf16 (..., N) = (sa . a)(sb . b)^T (+ bias): a (..., K/2) packed codes or (..., K)
+    float8_e4m3fn, b (N, K/2) packed codes, sa and sb their E8M0 scales (..., K/32), bias (N,) bf16, fp16
+    or fp32. With silu_mul, b (2N, K/2) holds gate rows, then up rows: silu(z[..., :N]) * z[..., N:] of z
+    (..., 2N) with its bias. Any sizes, K a multiple of 32; sums in fp32, rounded once."""
+    key = (a.shape, a.stride(), a.dtype, b.shape, b.stride(), b.dtype, sa.shape, sa.stride(), sa.dtype,
+           sb.shape, sb.stride(), sb.dtype, bias is None or (bias.shape, bias.stride(), bias.dtype), silu_mul)
+    plan = _GEMM.get(key)
+    if plan is None or out is not None:
+        return _gemm(a, b, sa, sb, bias, silu_mul, out, key)
+    pa, pb, ps, pt = a.data_ptr(), b.data_ptr(), sa.data_ptr(), sb.data_ptr()
+    d = a.get_device()
+    if ((pa | pb) & 15 or (ps | pt) & 3 or d < 0 or b.get_device() != d or sa.get_device() != d
+            or sb.get_device() != d or (bias is not None and bias.get_device() != d)):
+        return _gemm(a, b, sa, sb, bias, silu_mul, out, None)
+    args, need, shape = plan
+    g = nat.HkxMx4GemmArgs.from_buffer_copy(args)
+    return _launch(g, need, a, pa, pb, ps, pt, bias, nat.empty(a, shape, _bf16()))
+
+
+_BF16: list = []
+
+
+def _bf16():
+    if not _BF16:
+        import torch  # noqa: PLC0415
+
+        _BF16.append(torch.bfloat16)
+    return _BF16[0]
+
+
+def _launch(g, need, a, pa, pb, ps, pt, bias, out):
+    g.a, g.b, g.sa, g.sb, g.c = pa, pb, ps, pt, out.data_ptr()
+    if bias is not None:
+        g.bias = bias.data_ptr()
+    if need:
+        ws = nat.workspace(a.device, need)
+        g.ws, g.ws_bytes = ws.data_ptr(), need
+    nat.check(nat.lib().hkx_mx4_gemm(ctypes.byref(g), nat.stream_of(a.device)))
+    return out
+
+
+def _gemm(a, b, sa, sb, bias, silu_mul, out, key):
     import torch  # noqa: PLC0415
 
-    if a.dim() != 2 or b.dim() != 2:
-        raise ValueError(f"mxfp4.gemm: a and b are matrices, got {tuple(a.shape)} and {tuple(b.shape)}")
+    if a.dim() < 1 or b.dim() != 2:
+        raise ValueError(f"mxfp4.gemm: a (..., K) and b a matrix, got {tuple(a.shape)} and {tuple(b.shape)}")
+    given = (a, b, sa, sb, bias)
     b = _packed(b, "mxfp4.gemm", "b")
     wide = a.dtype == torch.float8_e4m3fn
     if not wide:
         a = _packed(a, "mxfp4.gemm", "a")
-    m, k = a.shape
-    rows, kb = b.shape
-    if not wide:
-        k *= 2
-    if k != 2 * kb or k % 32 or k == 0:
-        raise ValueError(f"mxfp4.gemm: K is {k} in a and {2 * kb} in b, the same multiple of 32")
+    lead, rows = tuple(a.shape[:-1]), b.shape[0]
+    k = a.shape[-1] if wide else 2 * a.shape[-1]
+    if k != 2 * b.shape[1] or k % 32 or k == 0:
+        raise ValueError(f"mxfp4.gemm: K is {k} in a and {2 * b.shape[1]} in b, the same multiple of 32")
     n = rows
     if silu_mul:
         if rows % 2:
             raise ValueError(f"mxfp4.gemm: silu_mul takes gate rows, then as many up rows: b has {rows}")
         n = rows // 2
-    d = a.get_device()
-    if d < 0 or b.get_device() != d:
+    if not a.is_cuda or b.device != a.device:
         raise ValueError("mxfp4.gemm: a and b are on one GPU")
-    if sa.get_device() != d or sb.get_device() != d:
-        _on(a.device, "mxfp4.gemm", sa=sa, sb=sb)
-    sa, sb = _scales(sa, m, k, "sa"), _scales(sb, rows, k, "sb")
-    if bias is not None:
-        if bias.dtype not in (torch.bfloat16, torch.float16, torch.float32) or bias.shape != (rows,):
-            raise ValueError(f"mxfp4.gemm: bias is bf16, fp16 or fp32 ({rows},), got {bias.dtype} "
-                             f"{tuple(bias.shape)}")
-        _on(a.device, "mxfp4.gemm", bias=bias)
-        bias = bias.contiguous()
+    _on(a.device, "mxfp4.gemm", sa=sa, sb=sb, bias=bias, out=out)
+    sa = _e8m0(sa, (*lead, k // 32), "sa")
+    sb = _e8m0(sb, (rows, k // 32), "sb")
+    if bias is not None and (bias.dtype not in (torch.bfloat16, torch.float16, torch.float32)
+                             or bias.shape != (rows,)):
+        raise ValueError(f"mxfp4.gemm: bias is bf16, fp16 or fp32 ({rows},), got {bias.dtype} "
+                         f"{tuple(bias.shape)}")
     if out is None:
-        out = nat.empty(a, (m, n), torch.bfloat16)
-    else:
-        if out.dtype != torch.bfloat16 or tuple(out.shape) != (m, n) or out.stride(1) != 1 or out.stride(0) < n:
-            raise ValueError(f"mxfp4.gemm: out is bf16 ({m}, {n}) with unit column stride")
-        _on(a.device, "mxfp4.gemm", out=out)
+        out = nat.empty(a, (*lead, n), torch.bfloat16)
+    elif out.dtype != torch.bfloat16 or tuple(out.shape) != (*lead, n):
+        raise ValueError(f"mxfp4.gemm: out is bf16 {(*lead, n)}, got {out.dtype} {tuple(out.shape)}")
+    m = a.numel() // a.shape[-1]
     if m == 0 or n == 0:
         return out
-    a, b = _rows16(a), _rows16(b)
+    a, sa = a.reshape(m, a.shape[-1]), sa.reshape(m, k // 32)
+    c = out if out.dim() == 2 else out.view(m, n)
+    if c.stride(1) != 1 or (m > 1 and c.stride(0) < n):
+        raise ValueError("mxfp4.gemm: out has unit column stride and rows that do not overlap")
+    a, b, sa, sb = _rows16(a), _rows16(b), scale_rows(sa), scale_rows(sb)
+    if bias is not None:
+        bias = bias.contiguous()
     g = nat.HkxMx4GemmArgs()
     g.size = ctypes.sizeof(g)
     g.a_dtype = nat.FP8E4M3 if wide else nat.FP4E2M1
-    g.a, g.b, g.sa, g.sb, g.c = a.data_ptr(), b.data_ptr(), sa.data_ptr(), sb.data_ptr(), out.data_ptr()
-    g.lda, g.ldb, g.sa_ld, g.sb_ld, g.ldc = a.stride(0), b.stride(0), sa.stride(0), sb.stride(0), out.stride(0)
+    g.lda, g.ldb = _ld(a, a.shape[1]), _ld(b, k // 2)
+    up4 = (k // 32 + 3) // 4 * 4
+    g.sa_ld, g.sb_ld, g.ldc = _ld(sa, up4), _ld(sb, up4), _ld(c, n)
     g.m, g.n, g.k, g.silu_mul = m, n, k, 1 if silu_mul else 0
     if bias is not None:
-        g.bias, g.bias_dtype = bias.data_ptr(), nat.dtype_code(bias.dtype)
-    L = nat.lib()
-    need = L.hkx_mx4_gemm_workspace(ctypes.byref(g))
-    if need:
-        ws = nat.workspace(a.device, need)
-        g.ws, g.ws_bytes = ws.data_ptr(), need
-    nat.check(L.hkx_mx4_gemm(ctypes.byref(g), nat.stream_of(a.device)))
+        g.bias_dtype = nat.dtype_code(bias.dtype)
+    need = nat.lib().hkx_mx4_gemm_workspace(ctypes.byref(g))
+    # (a template only where every operand was read where it is, and C is a plain new tensor)
+    if key is not None and g.ldc == n and all(
+            x is None or x.data_ptr() == y.data_ptr() for x, y in zip((a, b, sa, sb, bias), given)):
+        nat.remember(_GEMM, key, (bytes(g), need, (*lead, n)), 4096)
+    _launch(g, need, a, a.data_ptr(), b.data_ptr(), sa.data_ptr(), sb.data_ptr(), bias, c)
     return out
 
 

@@ -126,40 +126,48 @@ def quant(x, out=None):
 
 
 def dequant(q, s, dtype=None):
-    """The numbers that (q, s) stand for: q float8_e4m3fn [M, K] with E8M0 scales s [M, K/32], as
+    """The numbers that (q, s) stand for: q float8_e4m3fn (..., K) with E8M0 scales s (..., K/32), as
     bf16 or `dtype` (fp16, fp32), rounded once. A block of scale 255 is NaN."""
     import torch  # noqa: PLC0415
 
-    if q.dtype != torch.float8_e4m3fn or q.dim() != 2:
-        raise TypeError(f"mxfp8.dequant: q is float8_e4m3fn (M, K), got {q.dtype} {tuple(q.shape)}")
-    return _dequant("mxfp8.dequant", q, s, dtype, nat.FP8E4M3, q.shape[1])
+    if q.dtype != torch.float8_e4m3fn:
+        raise TypeError(f"mxfp8.dequant: q is float8_e4m3fn, got {q.dtype}")
+    return _dequant("mxfp8.dequant", q, s, dtype, nat.FP8E4M3, 1)
 
 
-def _dequant(call, q, s, dtype, code, k):
+def _dequant(call, q, s, dtype, code, per):
+    """`per` values a byte of q."""
     import torch  # noqa: PLC0415
 
     dtype = torch.bfloat16 if dtype is None else dtype
     if dtype not in (torch.bfloat16, torch.float16, torch.float32):
         raise TypeError(f"{call}: numbers as bf16, fp16 or fp32, got {dtype}")
-    m = q.shape[0]
-    if k % 32:
+    if q.dim() < 1:
+        raise ValueError(f"{call}: q is (..., K), got {tuple(q.shape)}")
+    lead, kb = q.shape[:-1], q.shape[-1]
+    k = per * kb
+    if k % 32 or k == 0:
         raise ValueError(f"{call}: K={k}, a multiple of 32")
-    if s.dtype != torch.uint8 or tuple(s.shape) != (m, k // 32):
-        raise ValueError(f"{call}: s is uint8 ({m}, {k // 32}), got {s.dtype} {tuple(s.shape)}")
-    if not q.is_cuda:
+    if s.dtype != torch.uint8 or s.shape[:-1] != lead or s.dim() < 1 or s.shape[-1] != k // 32:
+        raise ValueError(f"{call}: s is uint8 {(*lead, k // 32)}, got {s.dtype} {tuple(s.shape)}")
+    d = q.get_device()
+    if d < 0:
         raise ValueError(f"{call}: q is on a GPU, got {q.device}")
-    _on(q.device, call, s=s)
-    if q.stride(1) != 1 or q.stride(0) % 8 or q.data_ptr() % 8:
-        q = q.contiguous()
-    if s.stride(1) != 1:
-        s = s.contiguous()
-    y = nat.empty(q, (m, k), dtype)
-    if m == 0 or k == 0:
+    if s.get_device() != d:
+        _on(q.device, call, s=s)
+    y = nat.empty(q, (*lead, k), dtype)
+    m = q.numel() // kb
+    if m == 0:
         return y
-    nat.check(nat.lib().hkx_mx_dequant(
-        q.data_ptr(), max(q.stride(0), q.shape[1]), code, s.data_ptr(),
-        max(s.stride(0), k // 32), y.data_ptr(), k, nat.dtype_code(dtype), m, k,
-        nat.stream_of(q.device)))
+    if q.dim() != 2:
+        q, s = q.reshape(m, kb), s.reshape(m, k // 32)
+    ldq, lds = (q.stride(0), s.stride(0)) if m > 1 else (kb, k // 32)
+    if q.stride(1) != 1 or ldq % 8 or ldq < kb or q.data_ptr() % 8:
+        q, ldq = q.clone(memory_format=torch.contiguous_format), kb
+    if s.stride(1) != 1 or lds < k // 32:
+        s, lds = s.contiguous(), k // 32
+    nat.check(nat.lib().hkx_mx_dequant(q.data_ptr(), ldq, code, s.data_ptr(), lds, y.data_ptr(), k,
+                                       nat.dtype_code(dtype), m, k, nat.stream_of(q.device)))
     return y
 
 

@@ -13,12 +13,14 @@ or are fp32. The gate is broadcast over x: (D,), (B, 1, D), (B, S, 1), (B, S, D)
 leading sizes are x's, then ones. Sums and both norms are fp32; h is rounded only as it is stored.
 D up to 16384 (8192 where gradients are taken).
 
-quant="mxfp8" or "mxfp4" gives y as (q, s), an MX product's operand (hk.ops.mxfp8.gemm, hk.ops.mxfp4.gemm)
-without another pass: x is then 2-dimensional or y's rows are x's leading dimensions flattened, and D a
-multiple of 32.
+quant="mxfp8" or "mxfp4" gives y as (q, s), the operand of an MX product (hk.ops.mxfp4.gemm), without
+another pass: q (..., D) float8_e4m3fn, or (..., D/2) packed codes, and s (..., D/32); D a multiple of 32.
 
 Differentiable in x, residual, post, pre and gate (not through a quantized y): one backward pass over the
 same bytes, with the gradients of post, pre and a broadcast gate summed in fp32 in a fixed order.
+
+A call's checks and layout are kept by the shapes, strides and types they depend on, as a template of
+the library's arguments; a call of known layout fills in its addresses.
 """
 
 from __future__ import annotations
@@ -91,34 +93,59 @@ def _args(x, residual, post, pre, gate, branch_scale, residual_scale, eps):
     return g, keep
 
 
-def _forward(x, residual, post, pre, gate, branch_scale, residual_scale, eps, quant, keep_rstd):
+#: Layouts of a call: (arguments filled in but for their addresses, the shapes of the outputs).
+_PLANS: dict = {}
+
+
+def _forward(x, residual, post, pre, gate, scales, quant, keep_rstd):
+    """(h, y, the norms' factors): a checked call."""
     import torch  # noqa: PLC0415
 
     d = x.shape[-1]
-    g, keep = _args(x, residual, post, pre, gate, branch_scale, residual_scale, eps)
-    h = nat.empty(residual, residual.shape, residual.dtype)
-    rows = g.rows
-    y = scales = rstd = None
-    g.h, g.ldh = h.data_ptr(), d
+    g, keep = _args(x, residual, post, pre, gate, *scales)
+    g.ldh = d
+    y_shape = y_type = s_shape = s_stride = None
     if pre is not None:
         g.quant = QUANT[quant]
-        if quant is None:
-            y = nat.empty(x, x.shape, x.dtype)
-            g.ldy = d
-        else:
-            y = (nat.empty(x, (rows, d), torch.float8_e4m3fn) if quant == "mxfp8"
-                 else nat.empty(x, (rows, d // 2), torch.uint8))
-            scales = nat.empty(x, (rows, (d // 32 + 3) // 4 * 4), torch.uint8)
-            g.y_scales, g.ldys, g.ldy = scales.data_ptr(), scales.stride(0), y.stride(0)
-            if d % 128:
-                scales = scales[:, :d // 32]
+        y_shape, y_type = tuple(x.shape), x.dtype
+        if quant is not None:
+            y_type = torch.float8_e4m3fn if quant == "mxfp8" else torch.uint8
+            y_shape = (*x.shape[:-1], d if quant == "mxfp8" else d // 2)
+            s_shape = (*x.shape[:-1], d // 32)
+            s_stride, step = [1], (d // 32 + 3) // 4 * 4
+            for n in reversed(s_shape[:-1]):
+                s_stride.insert(0, step)
+                step *= n
+            g.ldys = (d // 32 + 3) // 4 * 4
+        g.ldy = y_shape[-1]
+    plan = (g.rows, y_shape, y_type, s_shape, s_stride)
+    out = _run(g, plan, x, residual, keep_rstd)
+    return out, bytes(g), plan, keep
+
+
+def _run(g, plan, x, residual, keep_rstd):
+    """Outputs for arguments whose inputs are in place, and the launch."""
+    rows, y_shape, y_type, s_shape, s_stride = plan
+    h = nat.empty(residual, residual.shape, residual.dtype)
+    g.h = h.data_ptr()
+    y = rstd = None
+    if y_shape is not None:
+        y = nat.empty(x, y_shape, y_type)
         g.y = y.data_ptr()
+        if s_shape is not None:
+            import torch  # noqa: PLC0415
+
+            s = torch.empty_strided(s_shape, s_stride, dtype=torch.uint8, device=x.device)
+            g.y_scales = s.data_ptr()
+            y = (y, s)
     if keep_rstd:
+        import torch  # noqa: PLC0415
+
         rstd = nat.empty(x, (rows, 2), torch.float32)
         g.rstd = rstd.data_ptr()
     if rows:
         nat.check(nat.lib().hkx_block_norm(ctypes.byref(g), nat.stream_of(x.device)))
-    return h, (y if quant is None else (y, scales)), rstd
+    return h, y, rstd
 
 
 _FUNCTION: list = []
@@ -133,7 +160,7 @@ def _function():
     class BlockNorm(torch.autograd.Function):
         @staticmethod
         def forward(ctx, x, residual, post, pre, gate, scales):
-            h, y, rstd = _forward(x, residual, post, pre, gate, *scales, None, True)
+            h, y, rstd = _call(x, residual, post, pre, gate, scales, None, True)
             ctx.save_for_backward(x, residual, post, pre, gate, rstd)
             ctx.scales = scales
             ctx.set_materialize_grads(False)
@@ -150,55 +177,129 @@ def _function():
     return BlockNorm
 
 
+#: Layouts of a backward call: (arguments filled in but for their addresses, workspace bytes, the
+#: types of dpost and dpre as the kernels write them).
+_GRAD_PLANS: dict = {}
+
+
 def _backward(x, residual, post, pre, gate, rstd, dh, dy, scales, need):
+    """The gradients of (x, residual, post, pre, gate); post, pre and gate's None where not needed."""
+    if dh is None and dy is None:
+        return (None,) * 5
+    key = (_layout(x), _layout(residual), _layout(post), _layout(pre), _layout(gate), _layout(dh),
+           _layout(dy), scales, need)
+    plan, keep = _GRAD_PLANS.get(key), None
+    if plan is None:
+        plan, keep = _grad_plan(x, residual, post, pre, gate, dh, dy, scales, need)
+        if keep is None:
+            nat.remember(_GRAD_PLANS, key, plan, 4096)
+    args, nws, tpost, tpre = plan
+    q = nat.HkxBlockNormGradArgs.from_buffer_copy(args)
+    f = q.f
+    f.x, f.residual, f.post, f.pre, f.gate, q.dh, q.dy = keep[0] if keep is not None else [
+        None if t is None else t.data_ptr() for t in (x, residual, post, pre, gate, dh, dy)]
+    f.rstd = rstd.data_ptr()
+    dx, dr = nat.empty(x, x.shape, x.dtype), nat.empty(residual, residual.shape, residual.dtype)
+    q.dx, q.dresidual = dx.data_ptr(), dr.data_ptr()
+    dpost = dpre = dgate = None
+    if post is not None and need[2]:
+        dpost = nat.empty(x, post.shape, tpost)
+        q.dpost = dpost.data_ptr()
+    if pre is not None and need[3]:
+        dpre = nat.empty(x, pre.shape, tpre)
+        q.dpre = dpre.data_ptr()
+    if gate is not None and need[4]:
+        dgate = nat.empty(x, gate.shape, gate.dtype)
+        q.dgate = dgate.data_ptr()
+    if f.rows == 0:
+        for t in (dpost, dpre, dgate):
+            if t is not None:
+                t.zero_()
+    else:
+        if nws:
+            ws = nat.workspace(x.device, nws)
+            q.ws, q.ws_bytes = ws.data_ptr(), nws
+        nat.check(nat.lib().hkx_block_norm_backward(ctypes.byref(q), nat.stream_of(x.device)))
+    if dpost is not None and tpost != post.dtype:
+        dpost = dpost.to(post.dtype)
+    if dpre is not None and tpre != pre.dtype:
+        dpre = dpre.to(pre.dtype)
+    return dx, dr, dpost, dpre, dgate
+
+
+def _grad_plan(x, residual, post, pre, gate, dh, dy, scales, need):
+    """(the plan, None), or with (the operands' addresses, what holds them) where one had to be copied."""
     import torch  # noqa: PLC0415
 
     d = x.shape[-1]
-    if dh is None and dy is None:
-        return (None,) * 5
     q = nat.HkxBlockNormGradArgs()
     q.size = ctypes.sizeof(q)
     q.f, keep = _args(x, residual, post, pre, gate, *scales)
-    q.f.rstd = rstd.data_ptr()
+    ptr = [q.f.x, q.f.residual, q.f.post, q.f.pre, q.f.gate]
     for name, t in (("dh", dh), ("dy", dy)):
         if t is not None:
             t = _rows(t, d)
             keep.append(t)
             setattr(q, name, t.data_ptr())
             setattr(q, "ld" + name, _ld(t, d))
-    dx, dr = nat.empty(x, x.shape, x.dtype), nat.empty(residual, residual.shape, residual.dtype)
-    q.dx, q.dresidual, q.lddx, q.lddr = dx.data_ptr(), dr.data_ptr(), d, d
-    wt = None if post is None else post.dtype
-    if post is not None and pre is not None and pre.dtype != wt:
-        wt = torch.float32  # mixed types go to the kernels as fp32
-    wt = pre.dtype if wt is None and pre is not None else wt
-    dpost = nat.empty(x, (d,), wt) if post is not None and need[2] else None
-    dpre = nat.empty(x, (d,), wt) if pre is not None and need[3] else None
-    dgate = nat.empty(x, gate.shape, gate.dtype) if gate is not None and need[4] else None
-    for name, t in (("dpost", dpost), ("dpre", dpre), ("dgate", dgate)):
-        if t is not None:
-            setattr(q, name, t.data_ptr())
-    if q.f.rows == 0:
-        for t in (dpost, dpre, dgate):
-            if t is not None:
-                t.zero_()
-    else:
-        L = nat.lib()
-        nws = L.hkx_block_norm_backward_workspace(ctypes.byref(q))
-        if nws:
-            ws = nat.workspace(x.device, nws)
-            q.ws, q.ws_bytes = ws.data_ptr(), nws
-        nat.check(L.hkx_block_norm_backward(ctypes.byref(q), nat.stream_of(x.device)))
-    if dpost is not None and dpost.dtype != post.dtype:
-        dpost = dpost.to(post.dtype)
-    if dpre is not None and dpre.dtype != pre.dtype:
-        dpre = dpre.to(pre.dtype)
-    return dx, dr, dpost, dpre, dgate
+        ptr.append(None if t is None else t.data_ptr())
+    q.lddx = q.lddr = d
+    tpost, tpre = (None if w is None else w.dtype for w in (post, pre))
+    if tpost != tpre and tpost is not None and tpre is not None:
+        tpost = tpre = torch.float32  # (weights of two types go to the kernels as fp32)
+    # which sums are wanted, for the workspace's size: any address that is not null
+    q.dpost = 16 if post is not None and need[2] else None
+    q.dpre = 16 if pre is not None and need[3] else None
+    q.dgate = 16 if gate is not None and need[4] else None
+    q.dx = q.dresidual = 16
+    nws = nat.lib().hkx_block_norm_backward_workspace(ctypes.byref(q))
+    q.dpost = q.dpre = q.dgate = q.dx = q.dresidual = None
+    plan = (bytes(q), nws, tpost, tpre)
+    mine = [None if t is None else t.data_ptr() for t in (x, residual, post, pre, gate, dh, dy)]
+    return plan, None if [p or None for p in ptr] == [p or None for p in mine] else (ptr, keep)
+
+
+def _layout(t):
+    return None if t is None else (t.shape, t.stride(), t.dtype)
+
+
+def _call(x, residual, post, pre, gate, scales, quant, grad):
+    key = (_layout(x), _layout(residual), _layout(post), _layout(pre), _layout(gate), scales, quant, grad)
+    plan = _PLANS.get(key)
+    d = x.get_device()
+    ptr = [None if t is None else t.data_ptr() for t in (x, residual, post, pre, gate)]
+    if plan is None or d < 0 or any(t is not None and t.get_device() != d for t in (residual, post, pre, gate)) or (
+            quant is not None and any(p and p & 15 for p in ptr)):
+        x, residual, post, pre, gate = _checked(x, residual, post, pre, gate, quant, grad)
+        out, args, plan, keep = _forward(x, residual, post, pre, gate, scales, quant, grad)
+        # (a template only where every operand was read where it is)
+        if all(a is None or a == b.data_ptr() for a, b in zip(ptr, (x, residual, post, pre, gate))) and all(
+                t is None or t.data_ptr() in ptr for t in keep):
+            nat.remember(_PLANS, key, (args, plan), 4096)
+        return out
+    args, plan = plan
+    g = nat.HkxBlockNormArgs.from_buffer_copy(args)
+    g.x, g.residual, g.post, g.pre, g.gate = ptr
+    return _run(g, plan, x, residual, grad)
 
 
 def block_norm(x, residual, *, post=None, pre=None, gate=None, branch_scale=1.0, residual_scale=1.0,
                eps=1e-6, quant=None):
     """(h, y): see the module's docstring."""
+    import torch  # noqa: PLC0415
+
+    scales = (float(branch_scale), float(residual_scale), float(eps))
+    if torch.is_grad_enabled() and (x.requires_grad or residual.requires_grad or any(
+            t is not None and t.requires_grad for t in (post, pre, gate))):
+        if quant is not None:
+            raise ValueError("block_norm: no gradient through a quantized y")
+        return _function().apply(x, residual, post, pre, gate, scales)
+    return _call(x, residual, post, pre, gate, scales, quant, False)[:2]
+
+
+def _checked(x, residual, post, pre, gate, quant, grad):
+    """The operands, refused where the kernels do not take them (copied where a quantized y needs
+    them aligned)."""
     import torch  # noqa: PLC0415
 
     floats = (torch.bfloat16, torch.float16, torch.float32)
@@ -228,24 +329,13 @@ def block_norm(x, residual, *, post=None, pre=None, gate=None, branch_scale=1.0,
         raise ValueError(f"block_norm: quant is None, 'mxfp8' or 'mxfp4', got {quant!r}")
     if quant is not None and (pre is None or d % 32):
         raise ValueError(f"block_norm: a quantized y needs pre and D={d} a multiple of 32")
-    limit = 16384
-    grad = torch.is_grad_enabled() and any(
-        t is not None and t.requires_grad for t in (x, residual, post, pre, gate))
-    if grad:
-        if quant is not None:
-            raise ValueError("block_norm: no gradient through a quantized y")
-        limit = 8192
+    limit = 8192 if grad else 16384
     if d > limit:
         raise ValueError(f"block_norm: D={d}, at most {limit}{' where gradients are taken' if grad else ''}")
-    scales = (float(branch_scale), float(residual_scale), float(eps))
-    if quant is not None:  # (rows of 16-byte pieces)
-        x, residual, post, pre, gate = (
-            t if t is None or (t.data_ptr() % 16 == 0 and t.is_contiguous()) else t.clone(
-                memory_format=torch.contiguous_format) for t in (x, residual, post, pre, gate))
-    if grad:
-        return _function().apply(x, residual, post, pre, gate, scales)
-    h, y, _ = _forward(x, residual, post, pre, gate, *scales, quant, False)
-    return h, y
+    if quant is None:
+        return x, residual, post, pre, gate
+    return tuple(t if t is None or (t.data_ptr() % 16 == 0 and t.is_contiguous())
+                 else t.clone(memory_format=torch.contiguous_format) for t in (x, residual, post, pre, gate))
 
 
 __all__ = ["block_norm"]

@@ -161,6 +161,8 @@ def test_quantized(shape, types, quant):
     rh, ry = O.block_norm(**a, **SCALES)
     d = shape[-1]
     ry = ry.reshape(-1, d)
+    assert q.shape[:-1] == s.shape[:-1] == shape[:-1]
+    q, s = q.flatten(0, -2), s.flatten(0, -2)
     v = O.values(q.cpu(), s.cpu())
     _near(h, rh, TYPES[types][1], a["residual"].double().abs() + _rowmax(rh))
     assert s.shape == (ry.shape[0], d // 32)

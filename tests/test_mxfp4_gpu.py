@@ -281,6 +281,20 @@ def test_linear_quantizes_the_activation():
         assert ((y.cpu().double() - ref).abs() <= err).all()
 
 
+def test_leading_dimensions():
+    g = _gen(11)
+    a, sa = _operand(30, 416, True, g)
+    b, sb = _operand(24, 416, False, g)
+    c = mxfp4.gemm(a.to(DEV), b.to(DEV), sa.to(DEV), sb.to(DEV))
+    for lead in ((2, 3, 5), (30,), (1, 30)):
+        a3, s3 = a.to(DEV).view(*lead, 416), sa.to(DEV).view(*lead, 13)
+        for _ in range(2):  # the first call of a layout, and one that knows it
+            assert torch.equal(mxfp4.gemm(a3, b.to(DEV), s3, sb.to(DEV)), c.view(*lead, 24))
+        assert torch.equal(mxfp8.dequant(a3, s3).view(30, 416), mxfp8.dequant(a.to(DEV), sa.to(DEV)))
+    one = mxfp4.gemm(a.to(DEV)[3], b.to(DEV), sa.to(DEV)[3], sb.to(DEV))
+    assert torch.equal(one, mxfp4.gemm(a.to(DEV)[3:4], b.to(DEV), sa.to(DEV)[3:4], sb.to(DEV))[0])
+
+
 def test_gemm_of_nothing():
     b, sb = torch.zeros(8, 32, dtype=torch.uint8, device=DEV), torch.zeros(8, 2, dtype=torch.uint8, device=DEV)
     c = mxfp4.gemm(b[:0], b, sb[:0], sb)
