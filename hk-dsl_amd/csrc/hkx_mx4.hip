@@ -2,7 +2,7 @@
 #include <algorithm>
 
 #include "hkx_api.hpp"
-#include "hkx_mx4.hpp"
+#include "hkx_mx4_quad.hpp"
 
 namespace hkx {
 
@@ -49,17 +49,41 @@ hipError_t launch_mx4_reduce(const Mx4ReduceArgs& r, hipStream_t s) {
 namespace {
 
 struct Plan {
-  int bm, splits;
+  int kernel, splits;
 };
 
-Plan plan(int m, int n, int k, bool pair, int cus) {
-  const int outw = pair ? 64 : 128;
-  const int bm = m <= 64 ? 64 : 128;
-  const int tiles = ((m + bm - 1) / bm) * ((n + outw - 1) / outw);
-  const int units = (k + 255) / 256;
-  int s = std::max(1, std::min({cus / tiles, units / 2, 8}));
+int rows_of(int kernel) { return kernel == HKX_MX4_QUAD ? 256 : kernel == HKX_MX4_TILE128 ? 128 : 64; }
+int cols_of(int kernel, bool pair) { return (kernel == HKX_MX4_QUAD ? 256 : 128) / (pair ? 2 : 1); }
+
+// 256-K units a split of s: the quadrant kernel's start at whole chunks of its packed scales.
+int split_units(int kernel, int units, int s) {
   const int per = (units + s - 1) / s;
-  return {bm, (units + per - 1) / per};
+  return kernel == HKX_MX4_QUAD && s > 1 ? (per + 1) / 2 * 2 : per;
+}
+
+// At most s splits, none empty.
+int whole_splits(int kernel, int units, int s) {
+  const int per = split_units(kernel, units, s);
+  return (units + per - 1) / per;
+}
+
+// The quadrant kernel's epilogue: 32-bit offsets into C, and a paired bias whose up half starts at a
+// multiple of 4 bytes.
+bool quad_ok(const HkxMx4GemmArgs& g) {
+  const int64_t rows = ((int64_t)g.m + 255) / 256 * 256;
+  return rows * std::max(g.ldc * 2, ((int64_t)g.n + 3) / 4 * 4 * (g.silu_mul ? 8 : 4)) < ((int64_t)1 << 32) - 65536 &&
+         (!g.bias || !g.silu_mul || g.bias_dtype == HKX_FP32 || g.n % 2 == 0);
+}
+
+Plan plan(const HkxMx4GemmArgs& g) {
+  const bool pair = g.silu_mul != 0;
+  const int units = (g.k + 255) / 256, cus = api_cus();
+  if (g.kernel != HKX_MX4_AUTO) return {g.kernel, whole_splits(g.kernel, units, std::max(1, std::min(g.splits, units)))};
+  const int64_t big = ((int64_t)g.m + 255) / 256 * ((g.n + cols_of(HKX_MX4_QUAD, pair) - 1) / cols_of(HKX_MX4_QUAD, pair));
+  const int kernel = g.m > 128 && 4 * big >= 3 * cus && quad_ok(g) ? HKX_MX4_QUAD : g.m <= 64 ? HKX_MX4_TILE64 : HKX_MX4_TILE128;
+  const int bm = rows_of(kernel), bn = cols_of(kernel, pair);
+  const int tiles = ((g.m + bm - 1) / bm) * ((g.n + bn - 1) / bn);
+  return {kernel, whole_splits(kernel, units, std::max(1, std::min({cus / tiles, units / 2, 8})))};
 }
 
 int64_t share_ld(const HkxMx4GemmArgs& g, int& up) {
@@ -67,11 +91,22 @@ int64_t share_ld(const HkxMx4GemmArgs& g, int& up) {
   return g.silu_mul ? 2 * (int64_t)up : up;
 }
 
-size_t ws_bytes(const HkxMx4GemmArgs& g) {
-  if (g.m < 1 || g.n < 1 || g.k < 32) return 0;
-  const Plan q = plan(g.m, g.n, g.k, g.silu_mul != 0, api_cus());
+// The workspace: a split's shares, then the quadrant kernel's packed scales of A and of B.
+struct Room {
+  size_t shares, sa, sb;
+  size_t all() const { return shares + sa + sb; }
+};
+
+Room room(const HkxMx4GemmArgs& g, const Plan& q) {
+  Room r{};
   int up;
-  return q.splits > 1 ? (size_t)q.splits * g.m * share_ld(g, up) * 4 : 0;
+  if (q.splits > 1) r.shares = ((size_t)q.splits * g.m * share_ld(g, up) * 4 + 15) / 16 * 16;
+  if (q.kernel == HKX_MX4_QUAD) {
+    const size_t chunks = (size_t)(g.k + 511) / 512;
+    r.sa = (size_t)((g.m + 255) / 256) * chunks * 4096;
+    r.sb = (size_t)((g.n + cols_of(q.kernel, g.silu_mul) - 1) / cols_of(q.kernel, g.silu_mul)) * chunks * 4096;
+  }
+  return r;
 }
 
 }  // namespace
@@ -80,8 +115,8 @@ size_t ws_bytes(const HkxMx4GemmArgs& g) {
 extern "C" {
 
 size_t hkx_mx4_gemm_workspace(const HkxMx4GemmArgs* args) {
-  if (!args || args->size != sizeof *args) return 0;
-  return hkx::ws_bytes(*args);
+  if (!args || args->size != sizeof *args || args->m < 1 || args->n < 1 || args->k < 32) return 0;
+  return hkx::room(*args, hkx::plan(*args)).all();
 }
 
 int hkx_mx4_gemm(const HkxMx4GemmArgs* args, void* stream) {
@@ -112,8 +147,13 @@ int hkx_mx4_gemm(const HkxMx4GemmArgs* args, void* stream) {
   constexpr int64_t kMost = ((int64_t)1 << 32) - 65536;
   if (mr * g.lda >= kMost || nr * g.ldb >= kMost || mr * g.sa_ld >= kMost || nr * g.sb_ld >= kMost)
     return api_fail(HKX_ERR_SHAPE, "mx4_gemm: A, B or their scales span 4 GiB or more; split the call");
-  const Plan q = plan(g.m, g.n, g.k, pair, api_cus());
-  const size_t need = ws_bytes(g);
+  if (g.kernel < HKX_MX4_AUTO || g.kernel > HKX_MX4_QUAD || g.splits < 0)
+    return api_fail(HKX_ERR_ARG, "mx4_gemm: kernel %d, splits %d", g.kernel, g.splits);
+  if (g.bias && !api_aligned(g.bias, 16)) return api_fail(HKX_ERR_SHAPE, "mx4_gemm: the bias needs 16-byte alignment");
+  if (g.kernel == HKX_MX4_QUAD && !quad_ok(g)) return api_fail(HKX_ERR_SHAPE, "mx4_gemm: the quadrant kernel does not take this call");
+  const Plan q = plan(g);
+  const Room rm = room(g, q);
+  const size_t need = rm.all();
   if (need && (!g.ws || g.ws_bytes < need || !api_aligned(g.ws, 16)))
     return api_fail(HKX_ERR_WORKSPACE, "mx4_gemm: needs %zu bytes of 16-byte aligned workspace, got %zu", need,
                     g.ws ? g.ws_bytes : (size_t)0);
@@ -141,12 +181,39 @@ int hkx_mx4_gemm(const HkxMx4GemmArgs* args, void* stream) {
   t.units = t.units_split = (g.k + 255) / 256;
   t.wgm = 8;
   t.c_vec = api_aligned(g.c, 16) && g.ldc % 8 == 0 && g.n % 8 == 0;
-  const int outw = pair ? 64 : 128;
-  t.tiles_m = (g.m + q.bm - 1) / q.bm;
-  t.tiles_n = (g.n + outw - 1) / outw;
+  const int bm = rows_of(q.kernel), bn = cols_of(q.kernel, pair);
+  t.tiles_m = (g.m + bm - 1) / bm;
+  t.tiles_n = (g.n + bn - 1) / bn;
   const hipStream_t s = (hipStream_t)stream;
-  const dim3 grid((unsigned)(t.tiles_m * t.tiles_n), (unsigned)q.splits);
-  if (q.splits == 1) return api_launched(launch_mx4_tile(t, a8, pair, false, q.bm, grid, s), "mx4 GEMM");
+  if (q.kernel == HKX_MX4_QUAD) {
+    Mx4PackArgs pa{}, pb{};
+    pa.s = g.sa;
+    pa.out = (uint8_t*)g.ws + rm.shares;
+    pa.ld = t.sa_ld;
+    pa.rows = (uint32_t)g.m;
+    pa.k32 = pb.k32 = g.k / 32;
+    pa.chunks = pb.chunks = (t.units + 1) / 2;
+    pa.tiles = t.tiles_m;
+    pb.s = g.sb;
+    pb.out = pa.out + rm.sa;
+    pb.ld = t.sb_ld;
+    pb.rows = (uint32_t)g.n;
+    pb.tiles = t.tiles_n;
+    pb.is_b = 1;
+    pb.pair = pair;
+    if (int rc = api_launched(launch_mx4_pack(pa, pb, s), "mx4 GEMM (scales)")) return rc;
+    t.sa = pa.out;
+    t.sb = pb.out;
+    t.sa_bytes = (uint32_t)rm.sa;
+    t.sb_bytes = (uint32_t)rm.sb;
+  }
+  auto launch = [&](bool share) {
+    const int tiles = t.tiles_m * t.tiles_n;
+    if (q.kernel == HKX_MX4_QUAD)
+      return launch_mx4_quad(t, a8, pair, share, dim3((unsigned)std::min(tiles, std::max(1, api_cus() / q.splits)), (unsigned)q.splits), s);
+    return launch_mx4_tile(t, a8, pair, share, bm, dim3((unsigned)tiles, (unsigned)q.splits), s);
+  };
+  if (q.splits == 1) return api_launched(launch(false), "mx4 GEMM");
   Mx4ReduceArgs r{};
   r.ws = (const float*)g.ws;
   r.ws_ld = share_ld(g, r.share_up);
@@ -164,8 +231,8 @@ int hkx_mx4_gemm(const HkxMx4GemmArgs* args, void* stream) {
   t.ldc = r.ws_ld;
   t.split_stride = r.split_stride;
   t.share_up = r.share_up;
-  t.units_split = (t.units + q.splits - 1) / q.splits;
-  int rc = api_launched(launch_mx4_tile(t, a8, pair, true, q.bm, grid, s), "mx4 GEMM (split over K)");
+  t.units_split = split_units(q.kernel, t.units, q.splits);
+  int rc = api_launched(launch(true), "mx4 GEMM (split over K)");
   return rc ? rc : api_launched(launch_mx4_reduce(r, s), "mx4 GEMM (sum of the splits)");
 }
 

@@ -158,7 +158,8 @@ def gemm(a, b, sa, sb, *, bias=None, silu_mul=False, out=None):
     pa, pb, ps, pt = a.data_ptr(), b.data_ptr(), sa.data_ptr(), sb.data_ptr()
     d = a.get_device()
     if ((pa | pb) & 15 or (ps | pt) & 3 or d < 0 or b.get_device() != d or sa.get_device() != d
-            or sb.get_device() != d or (bias is not None and bias.get_device() != d)):
+            or sb.get_device() != d
+            or (bias is not None and (bias.get_device() != d or bias.data_ptr() & 15))):
         return _gemm(a, b, sa, sb, bias, silu_mul, out, None)
     args, need, shape = plan
     g = nat.HkxMx4GemmArgs.from_buffer_copy(args)
@@ -229,6 +230,8 @@ def _gemm(a, b, sa, sb, bias, silu_mul, out, key):
     a, b, sa, sb = _rows16(a), _rows16(b), scale_rows(sa), scale_rows(sb)
     if bias is not None:
         bias = bias.contiguous()
+        if bias.data_ptr() % 16:
+            bias = bias.clone()
     g = nat.HkxMx4GemmArgs()
     g.size = ctypes.sizeof(g)
     g.a_dtype = nat.FP8E4M3 if wide else nat.FP4E2M1

@@ -337,6 +337,10 @@ int hkx_mx_dequant(const void* q, int64_t ldq, int32_t q_dtype, const uint8_t* s
  * of 2N) and C = silu(Z[:, :N]) * Z[:, N:]. Sums in fp32, one rounding. Any M and N, K a multiple of
  * 32. Row strides lda, ldb, sa_ld, sb_ld in bytes, ldc in elements; A's and B's rows 16-byte, the
  * scales' 4-byte aligned (up to 3 bytes past a scale row's K/32, within its last dword, are read). */
+#define HKX_MX4_AUTO 0
+#define HKX_MX4_TILE64 1  /* 64 x 128 tiles, 4 waves */
+#define HKX_MX4_TILE128 2 /* 128 x 128 tiles, 4 waves */
+#define HKX_MX4_QUAD 3    /* 256 x 256 tiles, 8 waves, persistent; C under 4 GiB */
 typedef struct {
   int32_t size; /* sizeof(HkxMx4GemmArgs): the library refuses another layout */
   int32_t a_dtype;
@@ -350,6 +354,8 @@ typedef struct {
   int32_t m, n, k;
   int32_t bias_dtype; /* HKX_BF16 / HKX_FP16 / HKX_FP32 */
   int32_t silu_mul;
+  int32_t kernel; /* HKX_MX4_AUTO, or the kernel to run (tuning, tests) */
+  int32_t splits; /* of K, where kernel is given (0: 1); no split is empty */
   int32_t reserved;
   void* ws; /* hkx_mx4_gemm_workspace() bytes, 16-byte aligned; NULL where that is 0 */
   size_t ws_bytes;

@@ -343,3 +343,49 @@ def test_refusals():
     with pytest.raises(nat.HkxError):
         nat.check(nat.lib().hkx_mx4_gemm(g, None))
     assert hk.ops.mxfp4 is mxfp4
+
+
+def _forced(kernel, splits, a, b, sa, sb, bias=None, silu_mul=False):
+    """A product on a kernel and split given (hk.ops.mxfp4.gemm picks them)."""
+    import ctypes
+
+    m, n = a.shape[0], b.shape[0] // (2 if silu_mul else 1)
+    g = nat.HkxMx4GemmArgs()
+    g.size = ctypes.sizeof(g)
+    g.a_dtype = nat.FP8E4M3 if a.dtype == torch.float8_e4m3fn else nat.FP4E2M1
+    out = torch.empty(m, n, dtype=BF16, device=DEV)
+    sa, sb = mxfp4.scale_rows(sa), mxfp4.scale_rows(sb)
+    g.a, g.b, g.sa, g.sb, g.c = (t.data_ptr() for t in (a, b, sa, sb, out))
+    g.lda, g.ldb, g.ldc = a.stride(0), b.stride(0), n
+    g.sa_ld, g.sb_ld = (t.stride(0) if t.shape[0] > 1 else (t.shape[1] + 3) // 4 * 4 for t in (sa, sb))
+    g.m, g.n, g.k, g.silu_mul, g.kernel, g.splits = m, n, 2 * b.shape[1], int(silu_mul), kernel, splits
+    if bias is not None:
+        g.bias, g.bias_dtype = bias.data_ptr(), nat.dtype_code(bias.dtype)
+    need = nat.lib().hkx_mx4_gemm_workspace(g)
+    ws = torch.full((need // 4 + 4,), float("nan"), device=DEV)
+    g.ws, g.ws_bytes = ws.data_ptr(), need
+    nat.check(nat.lib().hkx_mx4_gemm(g, nat.stream_of(a.device)))
+    return out
+
+
+@pytest.mark.parametrize("kernel", [nat.MX4_TILE64, nat.MX4_TILE128, nat.MX4_QUAD])
+@pytest.mark.parametrize("wide", [False, True], ids=["a4", "a8"])
+@pytest.mark.parametrize("m,n,k,splits,pair", [
+    (1, 8, 32, 1, False), (5, 40, 256, 1, True), (300, 300, 288, 1, False), (260, 513, 1120, 3, False),
+    (129, 130, 2048, 4, True), (520, 1000, 768, 1, True), (513, 264, 4096, 8, False), (700, 1032, 544, 2, False),
+    (2304, 2560, 96, 1, False), (2100, 4352, 512, 1, False), (1500, 2400, 1312, 1, True)])
+def test_every_kernel_takes_every_shape(m, n, k, splits, pair, wide, kernel):
+    """Also several tiles a workgroup of the persistent kernel (2304 x 2560 and more), each K unit
+    count from one, and both forms of its stores (N a multiple of 8 or not)."""
+    print(f"case forced {kernel} {m}x{n}x{k}/{splits} pair={pair} wide={wide}", flush=True)
+    g = _gen(m, n, k, 3)
+    a, sa = _operand(m, k, wide, g, 2)
+    b, sb = _operand(2 * n if pair else n, k, False, g, 2)
+    if pair:
+        sb -= 6
+    bias = torch.randn(b.shape[0], generator=g).to([BF16, F16, F32][m % 3]) if n % 2 == 0 else None
+    dev = [t.to(DEV) if t is not None else None for t in (a, b, sa, sb, bias)]
+    c = _forced(kernel, splits, *dev, pair)
+    ref, err = O.gemm(a, b, sa, sb, bias, pair)
+    bad = ~((c.cpu().double() - ref).abs() <= err)
+    assert not bad.any(), f"{int(bad.sum())} of {bad.numel()} off, first at {bad.nonzero()[0].tolist()}"
