@@ -25,7 +25,7 @@ OK, ERR_SHAPE, ERR_DTYPE, ERR_WORKSPACE, ERR_LAUNCH, ERR_ARG = range(6)
 BF16, FP16, FP32, FP8E4M3, INT8 = range(5)
 #: ab_dtype codes of fp8 operand pairs with e5m2: both, A e4m3 x B e5m2, A e5m2 x B e4m3
 FP8E5M2, FP8_E4M3_E5M2, FP8_E5M2_E4M3 = 5, 6, 7
-MX4_AUTO, MX4_TILE64, MX4_TILE128, MX4_QUAD = range(4)
+MX4_AUTO, MX4_TILE64, MX4_TILE128, MX4_QUAD, MX4_SKINNY = range(5)
 FP4E2M1 = 8  #: packed e2m1, two a byte (the MXFP4 calls)
 ROW, COL, TILE = 1, 2, 3
 EP_NONE, EP_FUSED, EP_PROGRAM, EP_SILU_MUL = range(4)

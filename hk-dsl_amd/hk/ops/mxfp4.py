@@ -6,9 +6,7 @@
     y = hk.ops.mxfp4.gemm(a, q, sa, s, silu_mul=True)  # q: gate rows, then up rows
 
 The OCP MX layout: two e2m1 codes a byte, the even column in the low bits (uint8, or torch's
-float4_e2m1fn_x2), and one E8M0 byte (2^(s - 127); 255 is NaN) a row and 32 columns. Scales whose rows
-start at multiples of 4 bytes are read in place (`quant` makes such rows at any K); others are copied
-every call, so a weight's scales are best laid out once by `scale_rows`.
+float4_e2m1fn_x2), and one E8M0 byte (2^(s - 127); 255 is NaN) a row and 32 columns.
 
 A call's checks and layout are kept by the shapes, strides and types they depend on, as a template of
 the library's arguments; a call of known layout fills in its addresses.
@@ -46,16 +44,9 @@ def _e8m0(s, shape, name):
     return s
 
 
-def scale_rows(s):
-    """E8M0 scales (rows, K/32) with rows that start at multiples of 4 bytes: `s` itself where it has
-    them, else a copy."""
-    rows, k32 = s.shape
-    st = s.stride()
-    if s.data_ptr() % 4 == 0 and st[1] == 1 and (rows < 2 or (st[0] % 4 == 0 and st[0] >= k32)):
-        return s
-    out = s.new_empty((rows, (k32 + 3) // 4 * 4))[:, :k32]
-    out.copy_(s)
-    return out
+def _scale_rows(s):
+    """`s` with unit stride along K (the kernels read rows at any alignment)."""
+    return s if s.stride(1) == 1 and (s.shape[0] < 2 or s.stride(0) >= s.shape[1]) else s.contiguous()
 
 
 def _rows16(t):
@@ -141,7 +132,8 @@ def dequant(q, s, dtype=None):
     return _dequant("mxfp4.dequant", _packed(q, "mxfp4.dequant", "q"), s, dtype, nat.FP4E2M1, 2)
 
 
-#: Layouts of gemm's operands: (arguments filled in but for their addresses, workspace bytes, C's shape).
+#: Layouts of gemm's operands: (arguments filled in but for their addresses, workspace bytes, C's shape,
+#: the scales' alignment that the workspace is for).
 _GEMM: dict = {}
 
 
@@ -155,13 +147,13 @@ def gemm(a, b, sa, sb, *, bias=None, silu_mul=False, out=None):
     plan = _GEMM.get(key)
     if plan is None or out is not None:
         return _gemm(a, b, sa, sb, bias, silu_mul, out, key)
+    args, need, shape, align = plan
     pa, pb, ps, pt = a.data_ptr(), b.data_ptr(), sa.data_ptr(), sb.data_ptr()
     d = a.get_device()
-    if ((pa | pb) & 15 or (ps | pt) & 3 or d < 0 or b.get_device() != d or sa.get_device() != d
+    if ((pa | pb) & 15 or (ps | pt) & 3 != align or d < 0 or b.get_device() != d or sa.get_device() != d
             or sb.get_device() != d
             or (bias is not None and (bias.get_device() != d or bias.data_ptr() & 15))):
         return _gemm(a, b, sa, sb, bias, silu_mul, out, None)
-    args, need, shape = plan
     g = nat.HkxMx4GemmArgs.from_buffer_copy(args)
     return _launch(g, need, a, pa, pb, ps, pt, bias, nat.empty(a, shape, _bf16()))
 
@@ -227,7 +219,7 @@ def _gemm(a, b, sa, sb, bias, silu_mul, out, key):
     c = out if out.dim() == 2 else out.view(m, n)
     if c.stride(1) != 1 or (m > 1 and c.stride(0) < n):
         raise ValueError("mxfp4.gemm: out has unit column stride and rows that do not overlap")
-    a, b, sa, sb = _rows16(a), _rows16(b), scale_rows(sa), scale_rows(sb)
+    a, b, sa, sb = _rows16(a), _rows16(b), _scale_rows(sa), _scale_rows(sb)
     if bias is not None:
         bias = bias.contiguous()
         if bias.data_ptr() % 16:
@@ -238,6 +230,7 @@ def _gemm(a, b, sa, sb, bias, silu_mul, out, key):
     g.lda, g.ldb = _ld(a, a.shape[1]), _ld(b, k // 2)
     up4 = (k // 32 + 3) // 4 * 4
     g.sa_ld, g.sb_ld, g.ldc = _ld(sa, up4), _ld(sb, up4), _ld(c, n)
+    g.sa, g.sb = sa.data_ptr(), sb.data_ptr()  # (the workspace goes by their alignment)
     g.m, g.n, g.k, g.silu_mul = m, n, k, 1 if silu_mul else 0
     if bias is not None:
         g.bias_dtype = nat.dtype_code(bias.dtype)
@@ -245,7 +238,7 @@ def _gemm(a, b, sa, sb, bias, silu_mul, out, key):
     # (a template only where every operand was read where it is, and C is a plain new tensor)
     if key is not None and g.ldc == n and all(
             x is None or x.data_ptr() == y.data_ptr() for x, y in zip((a, b, sa, sb, bias), given)):
-        nat.remember(_GEMM, key, (bytes(g), need, (*lead, n)), 4096)
+        nat.remember(_GEMM, key, (bytes(g), need, (*lead, n), (g.sa | g.sb) & 3), 4096)
     _launch(g, need, a, a.data_ptr(), b.data_ptr(), sa.data_ptr(), sb.data_ptr(), bias, c)
     return out
 
@@ -259,4 +252,4 @@ def linear(x, w, ws, *, bias=None, silu_mul=False, act="mxfp8"):
     return gemm(xq, w, xs, ws, bias=bias, silu_mul=silu_mul)
 
 
-__all__ = ["quant", "dequant", "gemm", "linear", "scale_rows"]
+__all__ = ["quant", "dequant", "gemm", "linear"]

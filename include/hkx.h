@@ -336,10 +336,12 @@ int hkx_mx_dequant(const void* q, int64_t ldq, int32_t q_dtype, const uint8_t* s
  * sa (M, K/32) and sb (N, K/32) E8M0 bytes. silu_mul: B has 2N rows, Z = (sa . A)(sb . B)^T (+ bias
  * of 2N) and C = silu(Z[:, :N]) * Z[:, N:]. Sums in fp32, one rounding. Any M and N, K a multiple of
  * 32. Row strides lda, ldb, sa_ld, sb_ld in bytes, ldc in elements; A's and B's rows 16-byte, the
- * scales' 4-byte aligned (up to 3 bytes past a scale row's K/32, within its last dword, are read). */
+ * scales' anywhere (whole aligned dwords of them are read: up to 3 bytes before the first and past the
+ * last). */
 #define HKX_MX4_AUTO 0
 #define HKX_MX4_TILE64 1  /* 64 x 128 tiles, 4 waves */
 #define HKX_MX4_TILE128 2 /* 128 x 128 tiles, 4 waves */
+#define HKX_MX4_SKINNY 4  /* the decode kernel: M up to 16, or 32 at K up to 4096; no splits */
 #define HKX_MX4_QUAD 3    /* 256 x 256 tiles, 8 waves, persistent; C under 4 GiB */
 typedef struct {
   int32_t size; /* sizeof(HkxMx4GemmArgs): the library refuses another layout */
