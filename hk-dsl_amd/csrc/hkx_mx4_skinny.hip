@@ -5,18 +5,15 @@ namespace hkx {
 
 template <int MF, bool A8, bool PAIR>
 static hipError_t launch(const Mx4SkinnyArgs& a, dim3 grid, hipStream_t s) {
-  constexpr int per = A8 ? 8 : 16;  // units a round
-  if (a.units <= per) {
+  if (a.units <= 8) {
     hipLaunchKernelGGL((mx4_skinny_kernel<MF, A8, PAIR, 1>), grid, dim3(512), 0, s, a);
     return hipGetLastError();
   }
-  if constexpr (MF == 1 || A8) {
-    if (a.units <= 2 * per) {
-      hipLaunchKernelGGL((mx4_skinny_kernel<MF, A8, PAIR, 2>), grid, dim3(512), 0, s, a);
-      return hipGetLastError();
-    }
+  if (a.units <= 16) {
+    hipLaunchKernelGGL((mx4_skinny_kernel<MF, A8, PAIR, 2>), grid, dim3(512), 0, s, a);
+    return hipGetLastError();
   }
-  if constexpr (MF == 1) {
+  if constexpr (MF == 1 || !A8) {
     hipLaunchKernelGGL((mx4_skinny_kernel<MF, A8, PAIR, 0>), grid, dim3(512), 0, s, a);
     return hipGetLastError();
   }
@@ -30,13 +27,15 @@ static hipError_t launch_form(const Mx4SkinnyArgs& a, bool a8, bool pair, dim3 g
 }
 
 hipError_t launch_mx4_skinny(Mx4SkinnyArgs a, bool a8, bool pair, int cus, hipStream_t s) {
-  // the most blocks a workgroup, up to 4, that leave two workgroups a CU and the blocks as even over
-  // the CUs as one each
+  // the most blocks a workgroup, up to 4, that leave the CUs full and the blocks as even over them as
+  // one each
+  const int nq = a.units <= 8 ? 1 : a.units <= 16 ? 2 : 0;
+  const int resident = mx4_skinny_resident(a.M <= 16 ? 1 : 2, a8, pair, nq);
   const int blocks = (a.N + (pair ? 7 : 15)) / (pair ? 8 : 16), least = (blocks + cus - 1) / cus;
   a.nb = 1;
   for (int nb = 2; nb <= 4; ++nb) {
     const int wgs = (blocks + nb - 1) / nb;
-    if (wgs >= 2 * cus && nb * ((wgs + cus - 1) / cus) <= least) a.nb = nb;
+    if (wgs >= resident * cus && nb * ((wgs + cus - 1) / cus) <= least) a.nb = nb;
   }
   const dim3 grid((unsigned)((blocks + a.nb - 1) / a.nb));
   return a.M <= 16 ? launch_form<1>(a, a8, pair, grid, s) : launch_form<2>(a, a8, pair, grid, s);

@@ -4,11 +4,13 @@
 //
 // * A block is 16 rows of W (a 16 x 16 x 128 MFMA fragment): 16 columns of C, or in the paired form 8
 //   gate rows and the 8 up rows of the same columns, whose sums meet by a shuffle. A workgroup owns nb
-//   (1-4) blocks and 8 waves cut K: in round q of a block wave w takes RK K units (256 K, a line of
-//   W's row) from (8 q + w) RK on: two with 4-bit X, one with 8-bit X, 256 bytes of each row of X.
-// * Two rounds are in flight, and two workgroups fit a CU. Up to NQ = 2 rounds a block X stays in
-//   registers for all the workgroup's blocks; past that it is streamed with the rounds.
-// * X is read in whole lines and turned into the MFMA's layout through the slot.
+//   (1-4) blocks and 8 waves cut K: in round q of a block wave w takes K unit 8 q + w, 256 K: a line of
+//   each row of W and one (4-bit) or two (8-bit) of each row of X.
+// * Two rounds are in flight. One fragment of tokens (M <= 16) fits three workgroups a CU, 96 KB of W in
+//   flight (two rounds of two units, two workgroups a CU and one unit each with 8-bit X before: 12288 x
+//   4096 at M = 1 took 10.9 us). Up to NQ = 2 rounds a block (K = 4096) X stays in registers for all the
+//   workgroup's blocks; past that it is streamed with the rounds.
+// * X is read in whole lines and turned into the MFMA's layout through the slot, a line at a time.
 // * Scales: lane r < 16 (of X: r < 16 MF) reads row r's bytes of the round as dwords, at any
 //   alignment (one dword more, joined by the byte offset), masks those past K, and hands them to the
 //   lanes by ds_bpermute.
@@ -36,16 +38,19 @@ struct Mx4SkinnyArgs {
   int32_t c_vec;  // C's rows 8-byte aligned and N a multiple of 4: 8-byte stores
 };
 
-// M up to 32; past 16 K up to 4096, whose X stays in registers (streamed, two 16-row fragments spilled).
-inline bool mx4_skinny_takes(int m, int k) { return m <= 16 || (m <= 32 && k <= 4096); }
+// M up to 32; past 16 with 8-bit X only K up to 4096, whose X stays in registers (streamed, it spilled).
+inline bool mx4_skinny_takes(int m, int k, bool a8) { return m <= 16 || (m <= 32 && (!a8 || k <= 4096)); }
+
+// Workgroups a CU: three where the registers allow it.
+constexpr int mx4_skinny_resident(int mf, bool a8, bool pair, int nq) {
+  return mf == 1 && (!a8 || nq == 1 || (nq == 2 && !pair)) ? 3 : 2;
+}
 
 template <int MF, bool A8, bool PAIR, int NQ>
-__global__ void __launch_bounds__(512, 4) mx4_skinny_kernel(const Mx4SkinnyArgs p) {
+__global__ void __launch_bounds__(512, 2 * mx4_skinny_resident(MF, A8, PAIR, NQ)) mx4_skinny_kernel(const Mx4SkinnyArgs p) {
   constexpr int NW = 8;
-  static_assert(MF == 1 || NQ == (A8 ? 2 : 1) || (A8 && NQ == 1), "two fragments: X in registers");
-  constexpr int RK = A8 ? 1 : 2;          // units of a wave a round
-  constexpr int ND = 2 * RK;              // scale dwords of a row a round
-  constexpr int SLOT = 16 * 256;          // W's 16 rows x RK lines; X turned: 16 rows x 256 bytes
+  constexpr int NL = A8 ? 2 : 1;          // lines of a row of X a unit
+  constexpr int SLOT = 16 * 128;          // 16 rows of W, or of X as a line is turned
   constexpr int RED = NW * 2 * SLOT;      // then the waves' sums of a block: [wave][fragment][lane]
   constexpr int BC = PAIR ? 8 : 16;       // columns a block
   __shared__ __attribute__((aligned(16))) uint8_t lds[RED + NW * MF * 1024];
@@ -55,7 +60,7 @@ __global__ void __launch_bounds__(512, 4) mx4_skinny_kernel(const Mx4SkinnyArgs 
   const int rf = lane & 15, g = lane >> 4;
   const int n0 = blockIdx.x * BC * p.nb;
   const int nb = min(p.nb, (p.N - n0 + BC - 1) / BC);
-  const int nq = NQ ? NQ : (p.units + NW * RK - 1) / (NW * RK);
+  const int nq = NQ ? NQ : (p.units + NW - 1) / NW;
   const int nu = nb * nq;  // steps: (block, round)
   uint8_t* own = lds + wave * 2 * SLOT;
 
@@ -94,123 +99,102 @@ __global__ void __launch_bounds__(512, 4) mx4_skinny_kernel(const Mx4SkinnyArgs 
     asm volatile("" : "+v"(v));
     return v;
   };
-  struct Scales {
-    i32x4 d;       // the row's dwords of a round from the aligned one on
-    uint32_t e;    // 4-bit X: the fifth
-  };
-  constexpr int SLOADS = A8 ? 1 : 2;
-  constexpr int WDMA = A8 ? 2 : 4;
-  constexpr int WLOADS = WDMA + SLOADS;
-  constexpr int XLOADS = 4 * MF + SLOADS;
+  using Scales = i32x4;  // the row's dwords of a unit from the aligned one on: two, and the next one's part
+  constexpr int WLOADS = 3;
+  constexpr int XLOADS = 2 * NL * MF + 1;
   struct XRegs {
-    i32x4 x[MF][4];
+    i32x4 x[MF][NL][2];
     Scales s;
   };
-  auto load_scales = [&](__amdgpu_buffer_rsrc_t r, uint32_t at, bool ok) {
-    Scales s;
-    s.d = buf_load16(r, ok ? at & ~3u : kMx4Out, 0);
-    s.e = A8 ? 0u : __builtin_amdgcn_raw_buffer_load_b32(r, ok ? (at & ~3u) + 16u : kMx4Out, 0, 0);
-    return s;
-  };
-  // dword d of a round's row, in place: bytes 4 d .. of it, those past K 0
+  // dword d of a unit's row, in place: bytes 4 d .. of it, those past K 0
   auto scale_dword = [&](const Scales& s, uint32_t at, int d, int left) -> uint32_t {
-    const uint32_t hi = d == 3 ? s.e : (uint32_t)s.d[(d + 1) & 3];
-    return __builtin_amdgcn_alignbyte(hi, (uint32_t)s.d[d], at & 3) & mx4_mask(left - 4 * d);
+    return __builtin_amdgcn_alignbyte((uint32_t)s[d + 1], (uint32_t)s[d], at & 3) & mx4_mask(left - 4 * d);
   };
-  // step u's fills into slot u & 1, and W's scales
+  // step u's fills into slot u & 1 (8 rows x 128 bytes each), and W's scales
   auto issue_w = [&](int u, Scales& sw) {
     const int j = NQ == 1 ? u : u / nq;
-    const int k = ((u - j * nq) * NW + wave) * RK;  // its first unit
-    const bool in = u < nu;
+    const int k = (u - j * nq) * NW + wave;  // its unit
+    const bool in = u < nu && k < p.units;
     uint8_t* slot = own + (u & 1) * SLOT;
     __builtin_amdgcn_sched_barrier(0);
-    const int ln = fresh(lane), g = ln >> 4, rf = ln & 15;
-    sw = load_scales(rsw, sw0 + wrow(j, rf) * p.sb_ld + (uint32_t)k * 8u, in && lane < 16 && wok(j, rf) && k < p.units);
-    if constexpr (A8) {
+    const int ln = fresh(lane), r = ln & 15;
+    sw = buf_load16(rsw, in && ln < 16 && wok(j, r) ? (sw0 + wrow(j, r) * p.sb_ld + (uint32_t)k * 8u) & ~3u : kMx4Out, 0);
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {  // 8 rows x 128 bytes
-        const int row = 8 * i + (ln >> 3), piece = (ln & 7) ^ ((row >> 1) & 7);
-        buf_load16_lds<kNonTemporal>(rw, slot + i * 1024,
-                                     in && k < p.units && wok(j, row)
-                                         ? wrow(j, row) * p.ldb + (uint32_t)k * 128u + (uint32_t)piece * 16u
-                                         : kMx4Out, 0);
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {  // 4 rows x 256 bytes
-        const int row = 4 * i + g, piece = rf ^ row;
-        buf_load16_lds<kNonTemporal>(rw, slot + i * 1024,
-                                     in && k + (piece >> 3) < p.units && wok(j, row)
-                                         ? wrow(j, row) * p.ldb + (uint32_t)k * 128u + (uint32_t)piece * 16u
-                                         : kMx4Out, 0);
-      }
+    for (int i = 0; i < 2; ++i) {
+      const int row = 8 * i + (ln >> 3), piece = (ln & 7) ^ ((row >> 1) & 7);
+      buf_load16_lds<kNonTemporal>(
+          rw, slot + i * 1024,
+          in && wok(j, row) ? wrow(j, row) * p.ldb + (uint32_t)k * 128u + (uint32_t)piece * 16u : kMx4Out, 0);
     }
     __builtin_amdgcn_sched_barrier(0);
   };
   // round q of X in line order, and its scales
   auto issue_x = [&](int q, XRegs& r) {
-    const int k = (q * NW + wave) * RK;
-    const int ln = fresh(lane), g = ln >> 4, rf = ln & 15;
-    const uint32_t at = (uint32_t)k * (A8 ? 256u : 128u) + (uint32_t)rf * 16u;
-    const bool in = at < (uint32_t)(A8 ? p.K : p.units * 128);
-    r.s = load_scales(rsx, sx0 + (uint32_t)ln * p.sa_ld + (uint32_t)k * 8u, ln < p.M && k < p.units);
+    const int k = q * NW + wave;
+    const int ln = fresh(lane);
+    const bool in = k < p.units;
+    r.s = buf_load16(rsx, in && ln < p.M ? (sx0 + (uint32_t)ln * p.sa_ld + (uint32_t)k * 8u) & ~3u : kMx4Out, 0);
 #pragma unroll
     for (int f = 0; f < MF; ++f)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int row = 16 * f + 4 * i + g;
-        r.x[f][i] = buf_load16(rx, in && row < p.M ? (uint32_t)row * p.lda + at : kMx4Out, 0);
-      }
+      for (int l = 0; l < NL; ++l)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int row = 16 * f + 8 * i + (ln >> 3);
+          const uint32_t at = (uint32_t)(k * NL + l) * 128u + (uint32_t)(ln & 7) * 16u;
+          r.x[f][l][i] = buf_load16(
+              rx, in && row < p.M && (!A8 || at < (uint32_t)p.K) ? (uint32_t)row * p.lda + at : kMx4Out, 0);
+        }
     __builtin_amdgcn_sched_barrier(0);
   };
-  // into the MFMA's layout: x[f][i] the 16-byte piece 4 i + g of row rf
+  // into the MFMA's layout: x[f][l][i] the 16-byte piece 4 i + g of row rf's line l
+  const uint32_t wr = (uint32_t)((lane >> 3) * 128 + (((lane & 7) ^ ((lane >> 4) & 7)) << 4));
+  const uint32_t rd0 = (uint32_t)(rf * 128 + ((g ^ ((rf >> 1) & 7)) << 4)), rd1 = (uint32_t)(rf * 128 + (((4 + g) ^ ((rf >> 1) & 7)) << 4));
   auto turn_x = [&](int u, XRegs& r) {
     uint8_t* slot = own + (u & 1) * SLOT;
 #pragma unroll
-    for (int f = 0; f < MF; ++f) {
+    for (int f = 0; f < MF; ++f)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) *(i32x4*)(slot + (4 * i + g) * 256 + ((rf ^ (4 * i + g)) << 4)) = r.x[f][i];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) r.x[f][i] = *(const i32x4*)(slot + rf * 256 + (((4 * i + g) ^ rf) << 4));
-    }
+      for (int l = 0; l < NL; ++l) {
+        *(i32x4*)(slot + wr) = r.x[f][l][0];  // rows 0-7, and 8-15 with the piece's other half
+        *(i32x4*)(slot + 1024 + (wr ^ 64)) = r.x[f][l][1];
+        r.x[f][l][0] = *(const i32x4*)(slot + rd0);
+        r.x[f][l][1] = *(const i32x4*)(slot + rd1);
+      }
   };
 
   f32x4 acc[MF];
 #pragma unroll
   for (int f = 0; f < MF; ++f) acc[f] = f32x4{0.f, 0.f, 0.f, 0.f};
-  i32x4 w[ND];  // [unit][K-half]
+  i32x4 w[2];  // [K-half]
   auto read_w = [&](int u) {
     const uint8_t* slot = own + (u & 1) * SLOT;
-#pragma unroll
-    for (int i = 0; i < ND; ++i) {
-      if constexpr (A8) w[i] = *(const i32x4*)(slot + rf * 128 + (((4 * i + g) ^ ((rf >> 1) & 7)) << 4));
-      else w[i] = *(const i32x4*)(slot + rf * 256 + (((4 * i + g) ^ rf) << 4));
-    }
+    w[0] = *(const i32x4*)(slot + rd0);
+    w[1] = *(const i32x4*)(slot + rd1);
   };
   auto wide = [](i32x4 v) { return i32x8{v.x, v.y, v.z, v.w, 0, 0, 0, 0}; };
   // W's registers of a step (round q) against X's
   auto mma = [&](int q, const XRegs& r, const Scales& sw) {
-    const int k = (q * NW + wave) * RK;
-    const int left = (int)k32 - 8 * k;
-    // (only their last two bits count, which a block's first row and a round's first byte leave alone)
+    const int left = (int)k32 - 8 * (q * NW + wave);
+    // (only their last two bits count, which a block's first row and a unit's first byte leave alone)
     const int ln = fresh(lane);
     const uint32_t atw = sw0 + (uint32_t)(PAIR ? (ln & 7) + (ln & 8 ? p.N : 0) : ln & 15) * p.sb_ld;
     const uint32_t atx = sx0 + (uint32_t)ln * p.sa_ld;
 #pragma unroll
-    for (int i = 0; i < ND; ++i) {
-      const int wsc = (int)((uint32_t)__builtin_amdgcn_ds_bpermute(4 * rf, (int)scale_dword(sw, atw, i, left)) >> (8 * g));
-      const uint32_t xd = scale_dword(r.s, atx, i, left);
+    for (int h = 0; h < 2; ++h) {
+      const int wsc = (int)((uint32_t)__builtin_amdgcn_ds_bpermute(4 * rf, (int)scale_dword(sw, atw, h, left)) >> (8 * g));
+      const uint32_t xd = scale_dword(r.s, atx, h, left);
 #pragma unroll
       for (int f = 0; f < MF; ++f) {
         const int xsc = (int)((uint32_t)__builtin_amdgcn_ds_bpermute(4 * (16 * f + rf), (int)xd) >> (8 * g));
         i32x8 x;
         if constexpr (A8) {
-          const i32x4 lo = r.x[f][2 * i], hi = r.x[f][2 * i + 1];
+          const i32x4 lo = r.x[f][NL - 1 ? h : 0][0], hi = r.x[f][NL - 1 ? h : 0][1];
           x = i32x8{lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
         } else {
-          x = wide(r.x[f][i]);
+          x = wide(r.x[f][0][h]);
         }
-        acc[f] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wide(w[i]), x, acc[f], 4, A8 ? 0 : 4, 0, wsc, 0, xsc);
+        acc[f] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wide(w[h]), x, acc[f], 4, A8 ? 0 : 4, 0, wsc, 0, xsc);
       }
     }
   };
