@@ -103,7 +103,7 @@ Plan plan(const HkxMx4GemmArgs& g) {
   const int units = (g.k + 255) / 256, cus = api_cus();
   if (g.kernel == HKX_MX4_SKINNY) return {g.kernel, 1};
   if (g.kernel != HKX_MX4_AUTO) return {g.kernel, whole_splits(g.kernel, units, std::max(1, std::min(g.splits, units)))};
-  if (mx4_skinny_takes(g.m, g.k, g.a_dtype == HKX_FP8E4M3)) return {HKX_MX4_SKINNY, 1};
+  if (g.m <= kMx4SkinnyM) return {HKX_MX4_SKINNY, 1};
   const int64_t big = ((int64_t)g.m + 255) / 256 * ((g.n + cols_of(HKX_MX4_QUAD, pair) - 1) / cols_of(HKX_MX4_QUAD, pair));
   const int kernel = g.m > 128 && 4 * big >= 3 * cus && quad_ok(g) ? HKX_MX4_QUAD : g.m <= 64 ? HKX_MX4_TILE64 : HKX_MX4_TILE128;
   const int bm = rows_of(kernel), bn = cols_of(kernel, pair);
@@ -187,8 +187,8 @@ int hkx_mx4_gemm(const HkxMx4GemmArgs* args, void* stream) {
     return api_fail(HKX_ERR_ARG, "mx4_gemm: kernel %d, splits %d", g.kernel, g.splits);
   if (g.bias && !api_aligned(g.bias, 16)) return api_fail(HKX_ERR_SHAPE, "mx4_gemm: the bias needs 16-byte alignment");
   if (g.kernel == HKX_MX4_QUAD && !quad_ok(g)) return api_fail(HKX_ERR_SHAPE, "mx4_gemm: the quadrant kernel does not take this call");
-  if (g.kernel == HKX_MX4_SKINNY && !mx4_skinny_takes(g.m, g.k, g.a_dtype == HKX_FP8E4M3))
-    return api_fail(HKX_ERR_SHAPE, "mx4_gemm: the decode kernel does not take M=%d K=%d", g.m, g.k);
+  if (g.kernel == HKX_MX4_SKINNY && g.m > kMx4SkinnyM)
+    return api_fail(HKX_ERR_SHAPE, "mx4_gemm: the decode kernel takes M <= %d, got %d", kMx4SkinnyM, g.m);
   const Plan q = plan(g);
   const Room rm = room(g, q);
   const size_t need = rm.all();

@@ -13,11 +13,8 @@ static hipError_t launch(const Mx4SkinnyArgs& a, dim3 grid, hipStream_t s) {
     hipLaunchKernelGGL((mx4_skinny_kernel<MF, A8, PAIR, 2>), grid, dim3(512), 0, s, a);
     return hipGetLastError();
   }
-  if constexpr (MF == 1 || !A8) {
-    hipLaunchKernelGGL((mx4_skinny_kernel<MF, A8, PAIR, 0>), grid, dim3(512), 0, s, a);
-    return hipGetLastError();
-  }
-  return hipErrorInvalidValue;
+  hipLaunchKernelGGL((mx4_skinny_kernel<MF, A8, PAIR, 0>), grid, dim3(512), 0, s, a);
+  return hipGetLastError();
 }
 
 template <int MF>

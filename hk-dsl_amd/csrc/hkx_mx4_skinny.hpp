@@ -6,7 +6,8 @@
 //   gate rows and the 8 up rows of the same columns, whose sums meet by a shuffle. A workgroup owns nb
 //   (1-4) blocks and 8 waves cut K: in round q of a block wave w takes K unit 8 q + w, 256 K: a line of
 //   each row of W and one (4-bit) or two (8-bit) of each row of X.
-// * Two rounds are in flight. One fragment of tokens (M <= 16) fits three workgroups a CU, 96 KB of W in
+// * Two rounds are in flight, four of a long K (a workgroup a CU at 4096 columns: two took 4096 x 12288
+//   at M = 16 from 9 to 14 us). One fragment of tokens (M <= 16) fits three workgroups a CU, 96 KB of W in
 //   flight (two rounds of two units, two workgroups a CU and one unit each with 8-bit X before: 12288 x
 //   4096 at M = 1 took 10.9 us). Up to NQ = 2 rounds a block (K = 4096) X stays in registers for all the
 //   workgroup's blocks; past that it is streamed with the rounds.
@@ -38,12 +39,12 @@ struct Mx4SkinnyArgs {
   int32_t c_vec;  // C's rows 8-byte aligned and N a multiple of 4: 8-byte stores
 };
 
-// M up to 32; past 16 with 8-bit X only K up to 4096, whose X stays in registers (streamed, it spilled).
-inline bool mx4_skinny_takes(int m, int k, bool a8) { return m <= 16 || (m <= 32 && (!a8 || k <= 4096)); }
+constexpr int kMx4SkinnyM = 32;
 
-// Workgroups a CU: three where the registers allow it.
+// Workgroups a CU, as the registers allow: three where a round's X is few, one where four are in flight
+// and many.
 constexpr int mx4_skinny_resident(int mf, bool a8, bool pair, int nq) {
-  return mf == 1 && (!a8 || nq == 1 || (nq == 2 && !pair)) ? 3 : 2;
+  return mf == 1 && nq > 0 && (!a8 || nq == 1 || !pair) ? 3 : (a8 || mf == 2) && nq == 0 ? 1 : 2;
 }
 
 template <int MF, bool A8, bool PAIR, int NQ>
@@ -51,7 +52,8 @@ __global__ void __launch_bounds__(512, 2 * mx4_skinny_resident(MF, A8, PAIR, NQ)
   constexpr int NW = 8;
   constexpr int NL = A8 ? 2 : 1;          // lines of a row of X a unit
   constexpr int SLOT = 16 * 128;          // 16 rows of W, or of X as a line is turned
-  constexpr int RED = NW * 2 * SLOT;      // then the waves' sums of a block: [wave][fragment][lane]
+  constexpr int NS = NQ ? 2 : 4;          // rounds in flight, a slot each
+  constexpr int RED = NW * NS * SLOT;     // then the waves' sums of a block: [wave][fragment][lane]
   constexpr int BC = PAIR ? 8 : 16;       // columns a block
   __shared__ __attribute__((aligned(16))) uint8_t lds[RED + NW * MF * 1024];
 
@@ -62,7 +64,7 @@ __global__ void __launch_bounds__(512, 2 * mx4_skinny_resident(MF, A8, PAIR, NQ)
   const int nb = min(p.nb, (p.N - n0 + BC - 1) / BC);
   const int nq = NQ ? NQ : (p.units + NW - 1) / NW;
   const int nu = nb * nq;  // steps: (block, round)
-  uint8_t* own = lds + wave * 2 * SLOT;
+  uint8_t* own = lds + wave * NS * SLOT;
 
   const __amdgpu_buffer_rsrc_t rw = make_rsrc(p.b, p.b_bytes), rx = make_rsrc(p.a, p.a_bytes);
   // the scales' buffers begin at an aligned dword and end with the one that holds the last byte
@@ -78,28 +80,31 @@ __global__ void __launch_bounds__(512, 2 * mx4_skinny_resident(MF, A8, PAIR, NQ)
     if constexpr (PAIR) return (uint32_t)(n0 + 8 * j + (r & 7) + (r & 8 ? p.N : 0));
     else return (uint32_t)(n0 + 16 * j + r);
   };
-  auto wok = [&](int j, int r) { return PAIR ? n0 + 8 * j + (r & 7) < p.N : n0 + 16 * j + r < p.N; };
 
   // the bias of the workgroup's columns, one a lane (paired: gates, then ups from lane 32 on), as
   // 32 and as 16 bits, without a branch
   const int bc = PAIR ? n0 + (lane & 31) + (lane & 32 ? p.N : 0) : n0 + lane;
-  const bool bok = p.bias && (PAIR ? n0 + (lane & 31) < p.N : bc < p.N) && wave < MF;
   const __amdgpu_buffer_rsrc_t rbias = make_rsrc(p.bias, p.bias ? (uint32_t)((PAIR ? 2 : 1) * p.N) * (p.bias_dt == HKX_FP32 ? 4u : 2u) : 0u);
   float bias32 = 0.0f;
   uint16_t bias16 = 0;
   auto load_bias = [&]() {
-    bias32 = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(
-        rbias, bok && p.bias_dt == HKX_FP32 ? (uint32_t)bc * 4u : kMx4Out, 0, 0));
-    bias16 = __builtin_amdgcn_raw_buffer_load_b16(rbias, bok && p.bias_dt != HKX_FP32 ? (uint32_t)bc * 2u : kMx4Out, 0, 0);
+    const uint32_t o32 = p.bias_dt == HKX_FP32 ? 0u : kMx4Out, o16 = p.bias_dt == HKX_FP32 ? kMx4Out : 0u;
+    bias32 = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(rbias, ((uint32_t)bc * 4u) | o32, 0, 0));
+    bias16 = __builtin_amdgcn_raw_buffer_load_b16(rbias, ((uint32_t)bc * 2u) | o16, 0, 0);
   };
-  if constexpr (NQ > 0) load_bias();  // (a long K reads it at a block's end: no registers are left)
+  load_bias();
   __builtin_amdgcn_sched_barrier(0);
 
   auto fresh = [](int v) {  // (as in the 8-bit kernel: offsets made again a round, not held)
     asm volatile("" : "+v"(v));
     return v;
   };
-  using Scales = i32x4;  // the row's dwords of a unit from the aligned one on: two, and the next one's part
+  // The row's dwords of a unit from the aligned one on: two, and the next one's part. (Three: of a load of
+  // four the compiler used the fourth's register at once, and so waited for the load there.)
+  typedef int Scales __attribute__((ext_vector_type(3)));
+  auto load_scales = [](__amdgpu_buffer_rsrc_t r, uint32_t off) {
+    return __builtin_bit_cast(Scales, __builtin_amdgcn_raw_buffer_load_b96(r, off, 0, 0));
+  };
   constexpr int WLOADS = 3;
   constexpr int XLOADS = 2 * NL * MF + 1;
   struct XRegs {
@@ -110,21 +115,22 @@ __global__ void __launch_bounds__(512, 2 * mx4_skinny_resident(MF, A8, PAIR, NQ)
   auto scale_dword = [&](const Scales& s, uint32_t at, int d, int left) -> uint32_t {
     return __builtin_amdgcn_alignbyte((uint32_t)s[d + 1], (uint32_t)s[d], at & 3) & mx4_mask(left - 4 * d);
   };
-  // step u's fills into slot u & 1 (8 rows x 128 bytes each), and W's scales
+  // (Out of range by or-ed bits, not branches. Rows past M and past B's last are out of range by
+  // themselves; the paired form's gate rows past N are up rows, whose columns are never stored.)
+  // step u's fills into its slot (8 rows x 128 bytes each), and W's scales
   auto issue_w = [&](int u, Scales& sw) {
     const int j = NQ == 1 ? u : u / nq;
     const int k = (u - j * nq) * NW + wave;  // its unit
-    const bool in = u < nu && k < p.units;
-    uint8_t* slot = own + (u & 1) * SLOT;
+    const uint32_t out = u < nu && k < p.units ? 0u : kMx4Out;
+    uint8_t* slot = own + (u & (NS - 1)) * SLOT;
     __builtin_amdgcn_sched_barrier(0);
-    const int ln = fresh(lane), r = ln & 15;
-    sw = buf_load16(rsw, in && ln < 16 && wok(j, r) ? (sw0 + wrow(j, r) * p.sb_ld + (uint32_t)k * 8u) & ~3u : kMx4Out, 0);
+    const int ln = fresh(lane);
+    sw = load_scales(rsw, ((sw0 + wrow(j, ln & 15) * p.sb_ld + (uint32_t)k * 8u) & ~3u) | out | (ln < 16 ? 0u : kMx4Out));
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       const int row = 8 * i + (ln >> 3), piece = (ln & 7) ^ ((row >> 1) & 7);
-      buf_load16_lds<kNonTemporal>(
-          rw, slot + i * 1024,
-          in && wok(j, row) ? wrow(j, row) * p.ldb + (uint32_t)k * 128u + (uint32_t)piece * 16u : kMx4Out, 0);
+      buf_load16_lds<kNonTemporal>(rw, slot + i * 1024,
+                                   (wrow(j, row) * p.ldb + (uint32_t)k * 128u + (uint32_t)piece * 16u) | out, 0);
     }
     __builtin_amdgcn_sched_barrier(0);
   };
@@ -132,8 +138,8 @@ __global__ void __launch_bounds__(512, 2 * mx4_skinny_resident(MF, A8, PAIR, NQ)
   auto issue_x = [&](int q, XRegs& r) {
     const int k = q * NW + wave;
     const int ln = fresh(lane);
-    const bool in = k < p.units;
-    r.s = buf_load16(rsx, in && ln < p.M ? (sx0 + (uint32_t)ln * p.sa_ld + (uint32_t)k * 8u) & ~3u : kMx4Out, 0);
+    const uint32_t out = k < p.units ? 0u : kMx4Out;
+    r.s = load_scales(rsx, ((sx0 + (uint32_t)ln * p.sa_ld + (uint32_t)k * 8u) & ~3u) | out);
 #pragma unroll
     for (int f = 0; f < MF; ++f)
 #pragma unroll
@@ -142,8 +148,7 @@ __global__ void __launch_bounds__(512, 2 * mx4_skinny_resident(MF, A8, PAIR, NQ)
         for (int i = 0; i < 2; ++i) {
           const int row = 16 * f + 8 * i + (ln >> 3);
           const uint32_t at = (uint32_t)(k * NL + l) * 128u + (uint32_t)(ln & 7) * 16u;
-          r.x[f][l][i] = buf_load16(
-              rx, in && row < p.M && (!A8 || at < (uint32_t)p.K) ? (uint32_t)row * p.lda + at : kMx4Out, 0);
+          r.x[f][l][i] = buf_load16(rx, ((uint32_t)row * p.lda + at) | out | (!A8 || at < (uint32_t)p.K ? 0u : kMx4Out), 0);
         }
     __builtin_amdgcn_sched_barrier(0);
   };
@@ -151,7 +156,7 @@ __global__ void __launch_bounds__(512, 2 * mx4_skinny_resident(MF, A8, PAIR, NQ)
   const uint32_t wr = (uint32_t)((lane >> 3) * 128 + (((lane & 7) ^ ((lane >> 4) & 7)) << 4));
   const uint32_t rd0 = (uint32_t)(rf * 128 + ((g ^ ((rf >> 1) & 7)) << 4)), rd1 = (uint32_t)(rf * 128 + (((4 + g) ^ ((rf >> 1) & 7)) << 4));
   auto turn_x = [&](int u, XRegs& r) {
-    uint8_t* slot = own + (u & 1) * SLOT;
+    uint8_t* slot = own + (u & (NS - 1)) * SLOT;
 #pragma unroll
     for (int f = 0; f < MF; ++f)
 #pragma unroll
@@ -168,7 +173,7 @@ __global__ void __launch_bounds__(512, 2 * mx4_skinny_resident(MF, A8, PAIR, NQ)
   for (int f = 0; f < MF; ++f) acc[f] = f32x4{0.f, 0.f, 0.f, 0.f};
   i32x4 w[2];  // [K-half]
   auto read_w = [&](int u) {
-    const uint8_t* slot = own + (u & 1) * SLOT;
+    const uint8_t* slot = own + (u & (NS - 1)) * SLOT;
     w[0] = *(const i32x4*)(slot + rd0);
     w[1] = *(const i32x4*)(slot + rd1);
   };
@@ -211,9 +216,6 @@ __global__ void __launch_bounds__(512, 2 * mx4_skinny_resident(MF, A8, PAIR, NQ)
     __builtin_amdgcn_s_waitcnt(0xc07f);
     __builtin_amdgcn_s_barrier();
     if (wave >= MF) return;
-    if constexpr (NQ == 0) {
-      if (p.bias) load_bias();
-    }
     f32x4 v = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll 1
     for (int h = 0; h < NW; h += 4) {
@@ -260,7 +262,7 @@ __global__ void __launch_bounds__(512, 2 * mx4_skinny_resident(MF, A8, PAIR, NQ)
   } while (0)
 
   Scales s0{}, s1{};
-  XRegs x0, x1;  // NQ = 1: x0 alone; 2: round 0's and 1's; 0: alternating with the steps
+  XRegs x0, x1;  // NQ = 1: x0 alone; 2: round 0's and 1's; 0: turning with the steps, as x2 and x3
   // a step: its fills landed (the newest are the next one's), W read, X turned in its first block
   if constexpr (NQ > 0) {
     auto odd = [&]() -> XRegs& {
@@ -300,37 +302,52 @@ __global__ void __launch_bounds__(512, 2 * mx4_skinny_resident(MF, A8, PAIR, NQ)
         issue_w(u + 2, sw);
         if (NQ == 1 || (u & 1)) finish(NQ == 1 ? u : u >> 1);
       };
-      for (int u = 2; u < nu; u += 2) {
+      for (int u = 2;; u += 2) {
         step(u, x0, s0);
-        if (u + 1 < nu) step(u + 1, odd(), s1);
+        if (u + 1 >= nu) break;
+        step(u + 1, odd(), s1);
+        if (u + 2 >= nu) break;
       }
     } else {
       finish(NQ == 1 ? 1 : 0);
     }
   } else {
+    Scales s2{}, s3{};
+    XRegs x2, x3;
+    auto round_of = [&](int u) { return u < nq ? u : u % nq; };
     issue_x(0, x0);
     issue_w(0, s0);
-    issue_x(1, x1);
+    issue_x(round_of(1), x1);
     issue_w(1, s1);
-    int j = 0, q = 0;         // step u's block and round
-    int qx = nq > 2 ? 2 : 0;  // round of step u + 2
+    issue_x(round_of(2), x2);
+    issue_w(2, s2);
+    issue_x(round_of(3), x3);
+    issue_w(3, s3);
+    int j = 0, q = 0;      // step u's block and round
+    int qx = round_of(4);  // round of step u + 4
     auto step = [&](int u, XRegs& x, Scales& sw) {
-      HKX_SKINNY_WAIT(WLOADS + XLOADS);
+      HKX_SKINNY_WAIT(3 * (WLOADS + XLOADS));
       read_w(u);
       turn_x(u, x);
       mma(q, x, sw);
       __builtin_amdgcn_s_waitcnt(0xc07f);
       issue_x(qx, x);
-      issue_w(u + 2, sw);
+      issue_w(u + 4, sw);
       if (++qx == nq) qx = 0;
       if (++q == nq) {
         finish(j++);
         q = 0;
       }
     };
-    for (int u = 0; u < nu; u += 2) {
+    for (int u = 0;; u += 4) {  // (each exit leaves the loop: a step the compiler sees skipped costs waits)
       step(u, x0, s0);
-      if (u + 1 < nu) step(u + 1, x1, s1);
+      if (u + 1 >= nu) break;
+      step(u + 1, x1, s1);
+      if (u + 2 >= nu) break;
+      step(u + 2, x2, s2);
+      if (u + 3 >= nu) break;
+      step(u + 3, x3, s3);
+      if (u + 4 >= nu) break;
     }
   }
 #undef HKX_SKINNY_WAIT
