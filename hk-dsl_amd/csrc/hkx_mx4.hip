@@ -71,45 +71,30 @@ hipError_t launch_mx4_reduce(const Mx4ReduceArgs& r, hipStream_t s) {
 
 namespace {
 
-struct Plan {
-  int kernel, splits;
-};
+static_assert(kMx4Tile64 == HKX_MX4_TILE64 && kMx4Tile128 == HKX_MX4_TILE128 && kMx4Quad == HKX_MX4_QUAD &&
+                  kMx4Skinny == HKX_MX4_SKINNY, "kernels");
 
-int rows_of(int kernel) { return kernel == HKX_MX4_QUAD ? 256 : kernel == HKX_MX4_TILE128 ? 128 : 64; }
-int cols_of(int kernel, bool pair) { return (kernel == HKX_MX4_QUAD ? 256 : 128) / (pair ? 2 : 1); }
-
-// 256-K units a split of s: the quadrant kernel's start at whole chunks of its packed scales.
-int split_units(int kernel, int units, int s) {
-  const int per = (units + s - 1) / s;
-  return kernel == HKX_MX4_QUAD && s > 1 ? (per + 1) / 2 * 2 : per;
-}
-
-// At most s splits, none empty.
-int whole_splits(int kernel, int units, int s) {
-  const int per = split_units(kernel, units, s);
-  return (units + per - 1) / per;
-}
-
-// The quadrant kernel's epilogue: 32-bit offsets into C, and a paired bias whose up half starts at a
-// multiple of 4 bytes.
+// The quadrant kernel's epilogue: 32-bit offsets into C or the shares, and a paired bias whose up half
+// starts at a multiple of 4 bytes.
 bool quad_ok(const HkxMx4GemmArgs& g) {
   const int64_t rows = ((int64_t)g.m + 255) / 256 * 256;
   return rows * std::max(g.ldc * 2, ((int64_t)g.n + 3) / 4 * 4 * (g.silu_mul ? 8 : 4)) < ((int64_t)1 << 32) - 65536 &&
          (!g.bias || !g.silu_mul || g.bias_dtype == HKX_FP32 || g.n % 2 == 0);
 }
 
-Plan plan(const HkxMx4GemmArgs& g) {
-  const bool pair = g.silu_mul != 0;
-  const int units = (g.k + 255) / 256, cus = api_cus();
-  if (g.kernel == HKX_MX4_SKINNY) return {g.kernel, 1};
-  if (g.kernel != HKX_MX4_AUTO) return {g.kernel, whole_splits(g.kernel, units, std::max(1, std::min(g.splits, units)))};
-  if (g.m <= kMx4SkinnyM) return {HKX_MX4_SKINNY, 1};
-  const int64_t big = ((int64_t)g.m + 255) / 256 * ((g.n + cols_of(HKX_MX4_QUAD, pair) - 1) / cols_of(HKX_MX4_QUAD, pair));
-  const int kernel = g.m > 128 && 4 * big >= 3 * cus && quad_ok(g) ? HKX_MX4_QUAD : g.m <= 64 ? HKX_MX4_TILE64 : HKX_MX4_TILE128;
-  const int bm = rows_of(kernel), bn = cols_of(kernel, pair);
-  const int tiles = ((g.m + bm - 1) / bm) * ((g.n + bn - 1) / bn);
-  return {kernel, whole_splits(kernel, units, std::max(1, std::min({cus / tiles, units / 2, 8})))};
+// C's rows are 16-byte aligned and N a multiple of 8. (By the row stride where C is not there yet: the
+// workspace's size is asked before.)
+bool c_vec(const HkxMx4GemmArgs& g) { return api_aligned(g.c, 16) && g.ldc % 8 == 0 && g.n % 8 == 0; }
+
+Mx4Plan plan(const HkxMx4GemmArgs& g) {
+  if (g.kernel == HKX_MX4_AUTO)
+    return mx4_plan(g.m, g.n, g.k, g.a_dtype == HKX_FP8E4M3, g.silu_mul != 0, quad_ok(g), c_vec(g), api_cus());
+  const int units = (g.k + 255) / 256;
+  return {g.kernel, g.kernel == HKX_MX4_SKINNY ? 1 : mx4_splits(g.kernel, units, std::max(1, std::min(g.splits, units)))};
 }
+
+// Whether the sums leave through fp32 shares and a second pass.
+bool shared(const HkxMx4GemmArgs& g, const Mx4Plan& q) { return q.splits > 1 || (q.kernel == HKX_MX4_QUAD && !c_vec(g)); }
 
 int64_t share_ld(const HkxMx4GemmArgs& g, int& up) {
   up = (g.n + 3) / 4 * 4;
@@ -129,14 +114,14 @@ struct Room {
   size_t all() const { return shares + sa + sb; }
 };
 
-Room room(const HkxMx4GemmArgs& g, const Plan& q) {
+Room room(const HkxMx4GemmArgs& g, const Mx4Plan& q) {
   Room r{};
   int up;
-  if (q.splits > 1) r.shares = ((size_t)q.splits * g.m * share_ld(g, up) * 4 + 15) / 16 * 16;
+  if (shared(g, q)) r.shares = ((size_t)q.splits * g.m * share_ld(g, up) * 4 + 15) / 16 * 16;
   if (q.kernel == HKX_MX4_QUAD) {
     const size_t chunks = (size_t)(g.k + 511) / 512;
     r.sa = (size_t)((g.m + 255) / 256) * chunks * 4096;
-    r.sb = (size_t)((g.n + cols_of(q.kernel, g.silu_mul) - 1) / cols_of(q.kernel, g.silu_mul)) * chunks * 4096;
+    r.sb = (size_t)((g.n + mx4_cols(q.kernel, g.silu_mul) - 1) / mx4_cols(q.kernel, g.silu_mul)) * chunks * 4096;
   }
   if (q.kernel == HKX_MX4_TILE64 || q.kernel == HKX_MX4_TILE128) {
     const size_t row = (size_t)(g.k / 32 + 3) / 4 * 4;
@@ -189,7 +174,7 @@ int hkx_mx4_gemm(const HkxMx4GemmArgs* args, void* stream) {
   if (g.kernel == HKX_MX4_QUAD && !quad_ok(g)) return api_fail(HKX_ERR_SHAPE, "mx4_gemm: the quadrant kernel does not take this call");
   if (g.kernel == HKX_MX4_SKINNY && g.m > kMx4SkinnyM)
     return api_fail(HKX_ERR_SHAPE, "mx4_gemm: the decode kernel takes M <= %d, got %d", kMx4SkinnyM, g.m);
-  const Plan q = plan(g);
+  const Mx4Plan q = plan(g);
   const Room rm = room(g, q);
   const size_t need = rm.all();
   if (need && (!g.ws || g.ws_bytes < need || !api_aligned(g.ws, 16)))
@@ -218,7 +203,7 @@ int hkx_mx4_gemm(const HkxMx4GemmArgs* args, void* stream) {
   t.K = g.k;
   t.units = t.units_split = (g.k + 255) / 256;
   t.wgm = 8;
-  t.c_vec = api_aligned(g.c, 16) && g.ldc % 8 == 0 && g.n % 8 == 0;
+  t.c_vec = c_vec(g);
   const hipStream_t s = (hipStream_t)stream;
   if (q.kernel == HKX_MX4_SKINNY) {
     Mx4SkinnyArgs d{};
@@ -243,7 +228,7 @@ int hkx_mx4_gemm(const HkxMx4GemmArgs* args, void* stream) {
     d.c_vec = api_aligned(g.c, 8) && g.ldc % 4 == 0 && g.n % 4 == 0;
     return api_launched(launch_mx4_skinny(d, a8, pair, api_cus(), s), "mx4 decode GEMM");
   }
-  const int bm = rows_of(q.kernel), bn = cols_of(q.kernel, pair);
+  const int bm = mx4_rows(q.kernel), bn = mx4_cols(q.kernel, pair);
   t.tiles_m = (g.m + bm - 1) / bm;
   t.tiles_n = (g.n + bn - 1) / bn;
   if (q.kernel != HKX_MX4_QUAD && !scales_ok(g)) {
@@ -296,9 +281,10 @@ int hkx_mx4_gemm(const HkxMx4GemmArgs* args, void* stream) {
     const int tiles = t.tiles_m * t.tiles_n;
     if (q.kernel == HKX_MX4_QUAD)
       return launch_mx4_quad(t, a8, pair, share, dim3((unsigned)std::min(tiles, std::max(1, api_cus() / q.splits)), (unsigned)q.splits), s);
-    return launch_mx4_tile(t, a8, pair, share, bm, dim3((unsigned)tiles, (unsigned)q.splits), s);
+    // (two workgroups a CU past one a CU)
+    return launch_mx4_tile(t, a8, pair, share, bm, tiles * q.splits > api_cus(), dim3((unsigned)tiles, (unsigned)q.splits), s);
   };
-  if (q.splits == 1) return api_launched(launch(false), "mx4 GEMM");
+  if (!shared(g, q)) return api_launched(launch(false), "mx4 GEMM");
   Mx4ReduceArgs r{};
   r.ws = (const float*)g.ws;
   r.ws_ld = share_ld(g, r.share_up);
@@ -316,7 +302,7 @@ int hkx_mx4_gemm(const HkxMx4GemmArgs* args, void* stream) {
   t.ldc = r.ws_ld;
   t.split_stride = r.split_stride;
   t.share_up = r.share_up;
-  t.units_split = split_units(q.kernel, t.units, q.splits);
+  t.units_split = mx4_split_units(q.kernel, t.units, q.splits);
   int rc = api_launched(launch(true), "mx4 GEMM (split over K)");
   return rc ? rc : api_launched(launch_mx4_reduce(r, s), "mx4 GEMM (sum of the splits)");
 }

@@ -52,8 +52,11 @@ HKX_DEV uint32_t mx4_mask(int left) { return left >= 4 ? 0xffffffffu : left <= 0
 //   fragment reads of 16 rows hit distinct banks; filled by 16-byte DMA of whole lines, the swizzle
 //   applied on the global side.
 // * A unit's scales: the 16 bytes of two units of every row by DMA, into one of two buffers.
-// * The fills of unit t + NST - 1 go into the stage unit t - 1 left, right after the one barrier of a
-//   unit; a wave waits for its own fills of the next unit only (buffer loads land in order).
+// * Fragment reads run a k-step of 64 K ahead of their MFMAs, the next unit's first ones under the last
+//   k-step, after the unit's one barrier (read just before them, 4096 x 4096 of 4-bit K = 12288 at M =
+//   777 took 39.6 us). After that barrier the unit's stage takes the fills of unit t + NST; a wave
+//   waits for its own fills of the next unit only (buffer loads land in order).
+// * RES = 2: two workgroups a CU, for grids of more than one a CU, in half the LDS.
 template <int BM, int BN, bool A8, bool PAIR, bool SHARE, int RES>
 __global__ void __launch_bounds__(256, RES) mx4_tile_kernel(const Mx4Args p) {
   constexpr int TM = BM / 2, TN = BN / 2;
@@ -160,8 +163,9 @@ __global__ void __launch_bounds__(256, RES) mx4_tile_kernel(const Mx4Args p) {
       }
     }
   };
-  uint32_t sca[FM][2], scb[FN][2];
-  auto read_scales = [&](int kt) {
+  using ScaleA = uint32_t[FM][2];
+  using ScaleB = uint32_t[FN][2];
+  auto read_scales = [&](int kt, ScaleA& sca, ScaleB& scb) {
     const uint8_t* sc = smem + SCO + ((kt >> 1) & 1) * ROWS * 16 + (kt & 1) * 8 + rf * 16;
     const int left = p.K / 32 - 8 * (kt0 + kt);
     const uint32_t k0 = mx4_mask(left), k1 = mx4_mask(left - 4);
@@ -183,6 +187,8 @@ __global__ void __launch_bounds__(256, RES) mx4_tile_kernel(const Mx4Args p) {
   for (int i = 0; i < FM; ++i)
 #pragma unroll
     for (int j = 0; j < FN; ++j) acc[i][j] = f32x16{};
+  ScaleA sca, nsca;
+  ScaleB scb, nscb;
   auto mma = [&](const AFrag (&af)[FM], const i32x4 (&bf)[FN], int ks) {
 #pragma unroll
     for (int i = 0; i < FM; ++i)
@@ -215,29 +221,53 @@ __global__ void __launch_bounds__(256, RES) mx4_tile_kernel(const Mx4Args p) {
     __builtin_amdgcn_s_barrier();
     __builtin_amdgcn_sched_barrier(0);
   };
-  // stages 0 .. NST - 2; unit 0 landed. (A fill past the last unit fetches that unit again.)
-  scale_fill(0);
+  // one LDS read or two after each MFMA of a k-step, then what is left of either
+  auto interleave = [&]() {
+    constexpr int reads = FN + FM * AL, mfmas = FM * FN, each = (reads + mfmas - 1) / mfmas;
 #pragma unroll
-  for (int s = 0; s < NST - 1; ++s) fill(min(s, nkt - 1), s);
-  sync();
+    for (int q = 0; q < mfmas; ++q) {
+      __builtin_amdgcn_sched_group_barrier(0x100, each, 0);
+      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+    }
+  };
+  // all stages; unit 0 landed. (A fill past the last unit fetches that unit again.)
+  scale_fill(0);
+  scale_fill(1);
+#pragma unroll
+  for (int s = 0; s < NST; ++s) fill(min(s, nkt - 1), s);
+  __builtin_amdgcn_s_waitcnt((((NST - 1) * NCH) & 15) | ((((NST - 1) * NCH) >> 4) << 14) | (7 << 4));
+  __builtin_amdgcn_s_barrier();
+  __builtin_amdgcn_sched_barrier(0);
   AFrag a0[FM], a1[FM];
   i32x4 b0[FN], b1[FN];
+  read(0, 0, a0, b0);
+  read_scales(0, sca, scb);
   for (int kt = 0; kt < nkt; ++kt) {
     const int s = kt % NST;
-    // (two units ahead, before the fills: the waits that leave up to two units' fills in flight
-    // cover it, and its buffer's last reads were two units ago)
-    if (!(kt & 1) && kt + 2 < nkt) scale_fill((kt >> 1) + 1);
-    fill(min(kt + NST - 1, nkt - 1), (kt + NST - 1) % NST);
-    read_scales(kt);
-    read(s, 0, a0, b0);
     read(s, 1, a1, b1);
     mma(a0, b0, 0);
+    interleave();
+    __builtin_amdgcn_sched_barrier(0);
     read(s, 2, a0, b0);
     mma(a1, b1, 1);
+    interleave();
+    __builtin_amdgcn_sched_barrier(0);
     read(s, 3, a1, b1);
     mma(a0, b0, 2);
+    interleave();
+    sync();  // every wave is past stage s, and unit kt + 1 landed
+    // (a buffer of scales: its last reads were a barrier ago, its next are two units on)
+    if ((kt & 1) && kt + 3 < nkt) scale_fill((kt + 3) >> 1);
+    fill(min(kt + NST, nkt - 1), s);
+    read((kt + 1) % NST, 0, a0, b0);  // (past the last unit: never used)
+    read_scales(kt + 1, nsca, nscb);
     mma(a1, b1, 3);
-    sync();
+    interleave();
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int i = 0; i < FM; ++i) sca[i][0] = nsca[i][0], sca[i][1] = nsca[i][1];
+#pragma unroll
+    for (int j = 0; j < FN; ++j) scb[j][0] = nscb[j][0], scb[j][1] = nscb[j][1];
   }
   __builtin_amdgcn_s_waitcnt(0x3f70);  // the last fills land before LDS is reused
   __syncthreads();
@@ -307,7 +337,8 @@ struct Mx4ReduceArgs {
   int32_t bias_dt, splits, M, N, share_up, pair, c_vec;
 };
 
-hipError_t launch_mx4_tile(const Mx4Args& a, bool a8, bool pair, bool share, int bm, dim3 grid, hipStream_t s);
+// two: two workgroups a CU.
+hipError_t launch_mx4_tile(const Mx4Args& a, bool a8, bool pair, bool share, int bm, bool two, dim3 grid, hipStream_t s);
 hipError_t launch_mx4_reduce(const Mx4ReduceArgs& r, hipStream_t s);
 
 }  // namespace hkx

@@ -243,7 +243,8 @@ __global__ void __launch_bounds__(512, 1) mx4_quad_kernel(const Mx4Args p) {
   constexpr std::integral_constant<int, 1> I1{};
 
   // ---- the epilogue of local tile lt: lane (rf, q) holds row rf, columns 4 q + [0, 4) of each 16 x 16
-  // fragment; two fragments trade quarters (v_permlane16_swap) so that a lane stores 16 bytes
+  // fragment; two fragments trade quarters (v_permlane16_swap) so that a lane stores 16 bytes (C's rows
+  // are whole 16-byte pieces; others leave as shares)
   auto bias4 = [&](int lt, int half, int col) -> f32x4 {
     const uint8_t* s = smem + EPV + (lt % 3) * 2048 + half * 1024;
     if (p.bias_dt == HKX_FP32) return *(const f32x4*)(s + 4 * col);
@@ -260,13 +261,6 @@ __global__ void __launch_bounds__(512, 1) mx4_quad_kernel(const Mx4Args p) {
     const uint32_t row_b = (uint32_t)p.ldc * (SHARE ? 4u : 2u);
     const __amdgpu_buffer_rsrc_t rc = make_rsrc(
         SHARE ? (const void*)((const float*)p.c + (int64_t)blockIdx.y * p.split_stride) : p.c, (uint32_t)rows * row_b);
-    auto store_odd = [&](u32x2 w, int m, int n) {  // four columns one by one
-      const uint32_t h[4] = {w.x, w.x >> 16, w.y, w.y >> 16};
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (n + i < p.N)
-          __builtin_amdgcn_raw_buffer_store_b16((uint16_t)h[i], rc, (uint32_t)m * row_b + (uint32_t)(n + i) * 2u, 0, 0);
-    };
     int m0, n0;
     tile_at(lt, m0, n0);
     m0 += 64 * grp;
@@ -298,19 +292,14 @@ __global__ void __launch_bounds__(512, 1) mx4_quad_kernel(const Mx4Args p) {
 #pragma unroll
             for (int f = 0; f < 2; ++f)
               w[f] = pack4<2>(HKX_BF16, silu_mul4(acc[i][j][2 * a + f][0] + bg, acc[i][j][2 * a + f][1] + bu));
-            if (p.c_vec) {
-              uint32_t ax = w[0].x, ay = w[0].y, bx = w[1].x, by = w[1].y;
-              swap16(ax, bx);
-              swap16(ay, by);
-              const int n = n0 + col + 8 * (ln >> 5);
-              if (n < p.N)
-                __builtin_amdgcn_raw_buffer_store_b128(
-                    i32x4{(int)ax, (int)ay, (int)bx, (int)by}, rc,
-                    (uint32_t)(m0 + 128 * i + 32 * a + 16 * (q & 1) + rf) * row_b + (uint32_t)n * 2u, 0, 0);
-            } else {
-#pragma unroll
-              for (int f = 0; f < 2; ++f) store_odd(w[f], m0 + 128 * i + 32 * a + 16 * f + rf, n0 + col + 4 * q);
-            }
+            uint32_t ax = w[0].x, ay = w[0].y, bx = w[1].x, by = w[1].y;
+            swap16(ax, bx);
+            swap16(ay, by);
+            const int n = n0 + col + 8 * (ln >> 5);
+            if (n < p.N)
+              __builtin_amdgcn_raw_buffer_store_b128(
+                  i32x4{(int)ax, (int)ay, (int)bx, (int)by}, rc,
+                  (uint32_t)(m0 + 128 * i + 32 * a + 16 * (q & 1) + rf) * row_b + (uint32_t)n * 2u, 0, 0);
           }
         } else {
           const int col = 128 * j + 32 * wc;
@@ -321,18 +310,13 @@ __global__ void __launch_bounds__(512, 1) mx4_quad_kernel(const Mx4Args p) {
             __builtin_amdgcn_sched_barrier(0);
             const u32x2 wa = pack4<2>(HKX_BF16, acc[i][j][f][0] + b0), wb = pack4<2>(HKX_BF16, acc[i][j][f][1] + b1);
             const int m = m0 + 128 * i + 16 * f + rf;
-            if (p.c_vec) {
-              uint32_t x0 = wa.x, x1 = wb.x, y0 = wa.y, y1 = wb.y;
-              swap16(x0, x1);
-              swap16(y0, y1);
-              const int n = n0 + col + 16 * (q & 1) + 8 * (q >> 1);
-              if (n < p.N)
-                __builtin_amdgcn_raw_buffer_store_b128(i32x4{(int)x0, (int)y0, (int)x1, (int)y1}, rc,
-                                                       (uint32_t)m * row_b + (uint32_t)n * 2u, 0, 0);
-            } else {
-              store_odd(wa, m, n0 + col + 4 * q);
-              store_odd(wb, m, n0 + col + 16 + 4 * q);
-            }
+            uint32_t x0 = wa.x, x1 = wb.x, y0 = wa.y, y1 = wb.y;
+            swap16(x0, x1);
+            swap16(y0, y1);
+            const int n = n0 + col + 16 * (q & 1) + 8 * (q >> 1);
+            if (n < p.N)
+              __builtin_amdgcn_raw_buffer_store_b128(i32x4{(int)x0, (int)y0, (int)x1, (int)y1}, rc,
+                                                     (uint32_t)m * row_b + (uint32_t)n * 2u, 0, 0);
           }
         }
       }

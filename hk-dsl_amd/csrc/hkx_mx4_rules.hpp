@@ -1,0 +1,89 @@
+// The MXFP4 product's choice between its kernels, by shape and CUs alone: plain C++, no HIP, so that a
+// host program can ask it.
+#pragma once
+
+#include <algorithm>
+#include <cstdint>
+
+namespace hkx {
+
+constexpr int kMx4SkinnyM = 32;  // the decode kernel's rows
+
+// The kernels (HKX_MX4_* of hkx.h).
+constexpr int kMx4Tile64 = 1, kMx4Tile128 = 2, kMx4Quad = 3, kMx4Skinny = 4;
+
+struct Mx4Plan {
+  int kernel, splits;
+};
+
+inline int mx4_rows(int kernel) { return kernel == kMx4Quad ? 256 : kernel == kMx4Tile128 ? 128 : 64; }
+inline int mx4_cols(int kernel, bool pair) { return (kernel == kMx4Quad ? 256 : 128) / (pair ? 2 : 1); }
+
+// 256-K units a split of at most s: the quadrant kernel's start at whole chunks of two units.
+inline int mx4_split_units(int kernel, int units, int s) {
+  const int per = (units + s - 1) / s;
+  return kernel == kMx4Quad && s > 1 ? (per + 1) / 2 * 2 : per;
+}
+// The splits that leaves, none empty.
+inline int mx4_splits(int kernel, int units, int s) {
+  const int per = mx4_split_units(kernel, units, s);
+  return (units + per - 1) / per;
+}
+
+// Whether up to 32 rows run on the decode kernel; its rate over the 64 x 128 tiles' of the best split,
+// cold weights (rows of B: twice the columns in the paired form), M = 1-8, 16, 24, 32:
+// * K to 4096: any up to M = 16; past it 1.13-1.8 to 16384 rows, 0.58-0.83 at 28672;
+// * past it X is streamed with every 16 rows of B: 4-bit X 1.36-1.63, 1.24-1.45, 1.01-1.33, 0.92-1.28 to
+//   4096 rows, 1.06-1.10, 0.93-1.03, 0.87-1.01, 0.8-0.96 at 8192, 0.98-1.08, 0.86-0.93, .. at 16384;
+//   8-bit X 1.26-1.52, 1.11-1.41, 0.86-1.15, 0.8-1.09 to 4096, 1.04-1.14, 0.89-1.05, 0.72-0.81, .. at 8192,
+//   0.92-1.02, 0.78-0.91, .. at 16384; both less the longer K.
+inline bool mx4_skinny_wins(int m, int rows, int k, bool a8) {
+  if (m > kMx4SkinnyM) return false;
+  if (k <= 4096) return m <= 16 || rows <= 20480;
+  if (m > 16) return rows <= 4096 && k <= (a8 ? 6144 : 8192);
+  if (m > 8) return rows <= 4096 || (rows <= 8192 && k <= 8192);
+  return rows <= (a8 ? 8192 : 16384);
+}
+
+// A plan's estimated time in us: a launch, more for each further wave of workgroups, a time a 256-K unit
+// and wave and one for its share of the memory's traffic, and where it goes through fp32 shares their
+// sum's launch and their round trip. Fitted to 1092 timed plans (M 33-4096, N 512-24576, K 512-12288,
+// weights past the cache): medians 0.99-1.01 of the times, 0.82-0.90 and 1.08-1.14 at the tenths; the
+// plans it picks take 1.03 times the best one's on average. Waves: whole ones where a workgroup has its
+// CU alone (the quadrant kernel, 128 x 128 tiles of an 8-bit A), 0.83 of their number past one where two
+// share it. A C of odd columns or alignment goes through shares on the quadrant kernel always (stored from
+// its registers two bytes at a time 3000 x 1001 took 25 us more).
+inline double mx4_cost(int kernel, int m, int n, int k, bool a8, bool pair, bool vec, int splits, int cus) {
+  static const double kC[2][3][6] = {
+      // launch, wave, unit, unit x filled, sum, share bytes
+      {{3.6, 4.7, 0.454, 0.418, 2.6, 0.64}, {4.7, 3.1, 0.713, 0.284, 2.5, 0.83}, {10.4, 7.1, 1.369, 0.375, 5.1, 0.64}},
+      {{3.8, 4.9, 0.565, 0.391, 2.8, 0.58}, {4.6, 1.6, 1.062, 0.180, 2.5, 0.88}, {10.1, 6.1, 2.070, 0.454, 5.0, 0.65}}};
+  const double* c = kC[a8][kernel - 1];
+  const int bm = mx4_rows(kernel), bn = mx4_cols(kernel, pair);
+  const int per = mx4_split_units(kernel, (k + 255) / 256, splits);
+  const double w = (double)((m + bm - 1) / bm) * ((n + bn - 1) / bn) * splits / cus;
+  const bool alone = kernel == kMx4Quad || (kernel == kMx4Tile128 && a8);
+  const double waves = w <= 1 ? 1.0 : alone ? (double)(int64_t)(w + 0.9999) : std::max(1.0, 0.83 * w);
+  double t = c[0] + c[1] * (waves - 1) + c[2] * per * waves + c[3] * per * std::min(w, 1.0);
+  if (splits > 1 || (kernel == kMx4Quad && !vec)) t += c[4] + c[5] * splits * m * (pair ? 2.0 : 1.0) * n * 8.0 / 5e6;
+  return t;
+}
+
+// quad_ok: the quadrant kernel takes the call; vec: C's rows are whole 16-byte pieces.
+inline Mx4Plan mx4_plan(int m, int n, int k, bool a8, bool pair, bool quad_ok, bool vec, int cus) {
+  if (mx4_skinny_wins(m, pair ? 2 * n : n, k, a8)) return {kMx4Skinny, 1};
+  const int units = (k + 255) / 256;
+  Mx4Plan best{kMx4Tile64, 1};
+  double t = 1e30;
+  for (int kernel = kMx4Tile64; kernel <= kMx4Quad; ++kernel) {
+    if ((kernel == kMx4Quad && (!quad_ok || m <= 128)) || (kernel == kMx4Tile128 && m <= 64)) continue;
+    for (int s = 1; s <= 8; s *= 2) {
+      if (s > 1 && (units < 2 * s || mx4_splits(kernel, units, s) != s)) continue;
+      const double e = mx4_cost(kernel, m, n, k, a8, pair, vec, s, cus);
+      if (e < t) t = e, best = {kernel, s};
+    }
+  }
+  return best;
+}
+
+}  // namespace hkx

@@ -20,6 +20,7 @@
 #pragma once
 
 #include "hkx_mx4.hpp"
+#include "hkx_mx4_rules.hpp"
 #include "hkx_skinny.hpp"
 
 namespace hkx {
@@ -38,8 +39,6 @@ struct Mx4SkinnyArgs {
   int32_t bias_dt;
   int32_t c_vec;  // C's rows 8-byte aligned and N a multiple of 4: 8-byte stores
 };
-
-constexpr int kMx4SkinnyM = 32;
 
 // Workgroups a CU, as the registers allow: three where a round's X is few, one where four are in flight
 // and many.

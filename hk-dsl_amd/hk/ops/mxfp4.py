@@ -230,7 +230,8 @@ def _gemm(a, b, sa, sb, bias, silu_mul, out, key):
     g.lda, g.ldb = _ld(a, a.shape[1]), _ld(b, k // 2)
     up4 = (k // 32 + 3) // 4 * 4
     g.sa_ld, g.sb_ld, g.ldc = _ld(sa, up4), _ld(sb, up4), _ld(c, n)
-    g.sa, g.sb = sa.data_ptr(), sb.data_ptr()  # (the workspace goes by their alignment)
+    # (the workspace goes by the scales' alignment, and by C's: a new C's is 16 bytes or more)
+    g.sa, g.sb, g.c = sa.data_ptr(), sb.data_ptr(), c.data_ptr()
     g.m, g.n, g.k, g.silu_mul = m, n, k, 1 if silu_mul else 0
     if bias is not None:
         g.bias_dtype = nat.dtype_code(bias.dtype)
