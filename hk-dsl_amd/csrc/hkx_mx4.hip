@@ -41,28 +41,6 @@ __global__ void __launch_bounds__(256) mx4_reduce_kernel(const Mx4ReduceArgs p) 
   }
 }
 
-// Scale rows at any alignment as rows of whole dwords (the 4-wave tiles' DMA takes no less): a thread a
-// dword of a row, A's rows, then B's. The last one's bytes past the row are whatever follows it: the
-// product masks them.
-struct Mx4AlignArgs {
-  const uint8_t* s[2];
-  uint32_t* out[2];
-  uint32_t ld[2], rows[2], bytes[2];
-  int32_t words, k32;
-};
-__global__ void __launch_bounds__(256) mx4_align_kernel(const Mx4AlignArgs p) {
-  const int i = blockIdx.x * 256 + threadIdx.x;
-  const int row = i / p.words, w = i - row * p.words;
-  const bool b = row >= (int)p.rows[0];
-  const uint32_t r = (uint32_t)row - (b ? p.rows[0] : 0u);
-  if (r >= p.rows[b]) return;
-  const uint32_t off = (uint32_t)((uintptr_t)p.s[b] & 3), at = off + r * p.ld[b] + 4u * (uint32_t)w;
-  const __amdgpu_buffer_rsrc_t rs = make_rsrc((const void*)((uintptr_t)p.s[b] & ~(uintptr_t)3), p.bytes[b]);
-  const uint32_t lo = __builtin_amdgcn_raw_buffer_load_b32(rs, at & ~3u, 0, 0);
-  const uint32_t hi = __builtin_amdgcn_raw_buffer_load_b32(rs, (at & ~3u) + 4u, 0, 0);
-  p.out[b][(int64_t)r * p.words + w] = __builtin_amdgcn_alignbyte(hi, lo, at & 3);
-}
-
 hipError_t launch_mx4_reduce(const Mx4ReduceArgs& r, hipStream_t s) {
   const dim3 grid((unsigned)(((r.N + 3) / 4 + 255) / 256), (unsigned)std::min(r.M, 65535));
   hipLaunchKernelGGL(mx4_reduce_kernel, grid, dim3(256), 0, s, r);
@@ -101,14 +79,7 @@ int64_t share_ld(const HkxMx4GemmArgs& g, int& up) {
   return g.silu_mul ? 2 * (int64_t)up : up;
 }
 
-// The 4-wave tiles read scales in place where their rows start at multiples of 4 bytes.
-bool scales_ok(const HkxMx4GemmArgs& g) {
-  return api_aligned(g.sa, 4) && api_aligned(g.sb, 4) && g.sa_ld % 4 == 0 && g.sb_ld % 4 == 0;
-}
-
-// The workspace: a split's shares, then A's and B's scales, packed for the quadrant kernel or as
-// aligned rows for the tiles (by the rows' strides: an unaligned address of aligned rows needs no more
-// than the room asked for it here either).
+// The workspace: a split's shares, then A's and B's scales packed for the quadrant kernel.
 struct Room {
   size_t shares, sa, sb;
   size_t all() const { return shares + sa + sb; }
@@ -122,12 +93,6 @@ Room room(const HkxMx4GemmArgs& g, const Mx4Plan& q) {
     const size_t chunks = (size_t)(g.k + 511) / 512;
     r.sa = (size_t)((g.m + 255) / 256) * chunks * 4096;
     r.sb = (size_t)((g.n + mx4_cols(q.kernel, g.silu_mul) - 1) / mx4_cols(q.kernel, g.silu_mul)) * chunks * 4096;
-  }
-  if (q.kernel == HKX_MX4_TILE64 || q.kernel == HKX_MX4_TILE128) {
-    const size_t row = (size_t)(g.k / 32 + 3) / 4 * 4;
-    r.sa = ((size_t)g.m * row + 15) / 16 * 16;
-    r.sb = ((size_t)g.n * (g.silu_mul ? 2 : 1) * row + 15) / 16 * 16;
-    if (scales_ok(g)) r.sa = r.sb = 0;
   }
   return r;
 }
@@ -172,8 +137,6 @@ int hkx_mx4_gemm(const HkxMx4GemmArgs* args, void* stream) {
     return api_fail(HKX_ERR_ARG, "mx4_gemm: kernel %d, splits %d", g.kernel, g.splits);
   if (g.bias && !api_aligned(g.bias, 16)) return api_fail(HKX_ERR_SHAPE, "mx4_gemm: the bias needs 16-byte alignment");
   if (g.kernel == HKX_MX4_QUAD && !quad_ok(g)) return api_fail(HKX_ERR_SHAPE, "mx4_gemm: the quadrant kernel does not take this call");
-  if (g.kernel == HKX_MX4_SKINNY && g.m > kMx4SkinnyM)
-    return api_fail(HKX_ERR_SHAPE, "mx4_gemm: the decode kernel takes M <= %d, got %d", kMx4SkinnyM, g.m);
   const Mx4Plan q = plan(g);
   const Room rm = room(g, q);
   const size_t need = rm.all();
@@ -231,30 +194,6 @@ int hkx_mx4_gemm(const HkxMx4GemmArgs* args, void* stream) {
   const int bm = mx4_rows(q.kernel), bn = mx4_cols(q.kernel, pair);
   t.tiles_m = (g.m + bm - 1) / bm;
   t.tiles_n = (g.n + bn - 1) / bn;
-  if (q.kernel != HKX_MX4_QUAD && !scales_ok(g)) {
-    Mx4AlignArgs l{};
-    const uint32_t rows[2] = {(uint32_t)g.m, (uint32_t)brows}, ld[2] = {t.sa_ld, t.sb_ld};
-    const uint8_t* from[2] = {g.sa, g.sb};
-    uint8_t* to = (uint8_t*)g.ws + rm.shares;
-    l.words = (int)(sbytes + 3) / 4;
-    l.k32 = (int)sbytes;
-    for (int i = 0; i < 2; ++i) {
-      l.s[i] = from[i];
-      l.out[i] = (uint32_t*)(to + (i ? rm.sa : 0));
-      l.ld[i] = ld[i];
-      l.rows[i] = rows[i];
-      l.bytes[i] = (uint32_t)(((uintptr_t)from[i] & 3) + (rows[i] - 1) * (uint64_t)ld[i] + sbytes + 3) / 4 * 4;
-    }
-    const int64_t all = ((int64_t)rows[0] + rows[1]) * l.words;
-    if (all > INT32_MAX - 256) return api_fail(HKX_ERR_SHAPE, "mx4_gemm: scales of %lld dwords", (long long)all);
-    hipLaunchKernelGGL(mx4_align_kernel, dim3((unsigned)((all + 255) / 256)), dim3(256), 0, s, l);
-    if (int rc = api_launched(hipGetLastError(), "mx4 GEMM (scales)")) return rc;
-    t.sa = (const uint8_t*)l.out[0];
-    t.sb = (const uint8_t*)l.out[1];
-    t.sa_ld = t.sb_ld = (uint32_t)l.words * 4;
-    t.sa_bytes = (uint32_t)g.m * t.sa_ld;
-    t.sb_bytes = (uint32_t)brows * t.sb_ld;
-  }
   if (q.kernel == HKX_MX4_QUAD) {
     Mx4PackArgs pa{}, pb{};
     pa.s = g.sa;

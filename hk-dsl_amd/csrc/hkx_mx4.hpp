@@ -51,7 +51,11 @@ HKX_DEV uint32_t mx4_mask(int left) { return left >= 4 ? 0xffffffffu : left <= 0
 //   row's eight 16-byte pieces XOR-swizzled (piece c of row r at c ^ swz(r % 16)) so that the
 //   fragment reads of 16 rows hit distinct banks; filled by 16-byte DMA of whole lines, the swizzle
 //   applied on the global side.
-// * A unit's scales: the 16 bytes of two units of every row by DMA, into one of two buffers.
+// * Scales, a row a thread: the dwords that hold the 16 bytes of two units (at any alignment) into
+//   registers three units ahead, joined, those past K masked, and written to one of two LDS buffers a
+//   unit ahead. (By DMA, rows off a multiple of 4 bytes took a launch that aligned them; a unit at a time
+//   they were half as many cache lines as the operands, and a wait for them one unit on held the fills to
+//   that: 15% slower each.)
 // * Fragment reads run a k-step of 64 K ahead of their MFMAs, the next unit's first ones under the last
 //   k-step, after the unit's one barrier (read just before them, 4096 x 4096 of 4-bit K = 12288 at M =
 //   777 took 39.6 us). After that barrier the unit's stage takes the fills of unit t + NST; a wave
@@ -67,7 +71,7 @@ __global__ void __launch_bounds__(256, RES) mx4_tile_kernel(const Mx4Args p) {
   constexpr int NA = BM * AL / 32;     // of which A's
   constexpr int STAGE = LINES * 128;
   constexpr int ROWS = BM + BN;
-  constexpr int NSC = (ROWS + 255) / 256;  // scale fills a wave
+  static_assert(ROWS <= 256, "a row's scales a thread");
   constexpr int OUTW = PAIR ? BN / 2 : BN;
   constexpr int RS = OUTW * 2 + 16;  // staging row stride
   constexpr int BESIDE = BN * 4 + 2 * ROWS * 16;
@@ -126,19 +130,34 @@ __global__ void __launch_bounds__(256, RES) mx4_tile_kernel(const Mx4Args p) {
       }
     }
   };
-  // the scales of units 2 c and 2 c + 1 of this split: 64 rows a wave and fill
-  auto scale_fill = [&](int c) {
+  // this thread's row of scales: A's, then B's
+  const bool row_a = tid < BM;  // (BM is a multiple of 64: whole waves)
+  const uint32_t s0 = (uint32_t)((uintptr_t)(row_a ? p.sa : p.sb) & 3);
+  const uint32_t k32 = (uint32_t)p.K / 32, srows = row_a ? (uint32_t)p.M : (uint32_t)((PAIR ? 2 : 1) * p.N);
+  const uint32_t sld = row_a ? p.sa_ld : p.sb_ld;
+  const __amdgpu_buffer_rsrc_t rs = make_rsrc((const void*)((uintptr_t)(row_a ? p.sa : p.sb) & ~(uintptr_t)3),
+                                              tid < ROWS ? (s0 + (srows - 1) * sld + k32 + 3) & ~3u : 0u);
+  const uint32_t sat = s0 + (uint32_t)(row_a ? m0 + tid : brow(tid - BM)) * sld + (uint32_t)kt0 * 8u;
+  struct Scales {  // of a chunk of two units: four dwords and, off a multiple of 4 bytes, a fifth
+    i32x4 d;
+    uint32_t e;
+  };
+  const uint32_t fifth = ((sld | s0) & 3) ? 16u : kMx4Out;
+  auto load_scales = [&](int c) {
+    const uint32_t at = (sat + (uint32_t)c * 16u) & ~3u;
+    Scales s;
+    s.d = buf_load16(rs, at, 0);
+    s.e = __builtin_amdgcn_raw_buffer_load_b32(rs, at + fifth, 0, 0);
+    return s;
+  };
+  auto write_scales = [&](int c, const Scales& s) {
+    const int left = (int)k32 - 8 * kt0 - 16 * c;
+    i32x4 v;
 #pragma unroll
-    for (int i = 0; i < NSC; ++i) {
-      const int r0 = wave * 64 + 256 * i;
-      if (r0 >= ROWS) break;
-      const bool isa = r0 < BM;
-      const uint32_t row = (uint32_t)(isa ? m0 + r0 + lane : brow(r0 - BM + lane));
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(
-          make_rsrc(isa ? p.sa : p.sb, isa ? p.sa_bytes : p.sb_bytes),
-          (__attribute__((address_space(3))) void*)(smem + SCO + (c & 1) * ROWS * 16 + r0 * 16), 16,
-          row * (isa ? p.sa_ld : p.sb_ld) + (uint32_t)(kt0 + 2 * c) * 8u, 0, 0, 0);
-    }
+    for (int i = 0; i < 4; ++i)
+      v[i] = (int)(__builtin_amdgcn_alignbyte(i < 3 ? (uint32_t)s.d[(i + 1) & 3] : s.e, (uint32_t)s.d[i], sat & 3) &
+                   mx4_mask(left - 4 * i));
+    if (tid < ROWS) *(i32x4*)(smem + SCO + (c & 1) * ROWS * 16 + tid * 16) = v;
   };
 
   const int rf = lane & 31, h = lane >> 5, sw = swz(rf & 15);
@@ -167,19 +186,17 @@ __global__ void __launch_bounds__(256, RES) mx4_tile_kernel(const Mx4Args p) {
   using ScaleB = uint32_t[FN][2];
   auto read_scales = [&](int kt, ScaleA& sca, ScaleB& scb) {
     const uint8_t* sc = smem + SCO + ((kt >> 1) & 1) * ROWS * 16 + (kt & 1) * 8 + rf * 16;
-    const int left = p.K / 32 - 8 * (kt0 + kt);
-    const uint32_t k0 = mx4_mask(left), k1 = mx4_mask(left - 4);
 #pragma unroll
     for (int i = 0; i < FM; ++i) {
       const u32x2 v = *(const u32x2*)(sc + (wm * TM + 32 * i) * 16);
-      sca[i][0] = (v.x & k0) >> (8 * h);
-      sca[i][1] = (v.y & k1) >> (8 * h);
+      sca[i][0] = v.x >> (8 * h);
+      sca[i][1] = v.y >> (8 * h);
     }
 #pragma unroll
     for (int j = 0; j < FN; ++j) {
       const u32x2 v = *(const u32x2*)(sc + (BM + wn * TN + 32 * j) * 16);
-      scb[j][0] = (v.x & k0) >> (8 * h);
-      scb[j][1] = (v.y & k1) >> (8 * h);
+      scb[j][0] = v.x >> (8 * h);
+      scb[j][1] = v.y >> (8 * h);
     }
   };
   f32x16 acc[FM][FN];
@@ -231,10 +248,11 @@ __global__ void __launch_bounds__(256, RES) mx4_tile_kernel(const Mx4Args p) {
     }
   };
   // all stages; unit 0 landed. (A fill past the last unit fetches that unit again.)
-  scale_fill(0);
-  scale_fill(1);
+  const Scales scales0 = load_scales(0);
+  Scales scales = load_scales(1);
 #pragma unroll
   for (int s = 0; s < NST; ++s) fill(min(s, nkt - 1), s);
+  write_scales(0, scales0);
   __builtin_amdgcn_s_waitcnt((((NST - 1) * NCH) & 15) | ((((NST - 1) * NCH) >> 4) << 14) | (7 << 4));
   __builtin_amdgcn_s_barrier();
   __builtin_amdgcn_sched_barrier(0);
@@ -242,8 +260,12 @@ __global__ void __launch_bounds__(256, RES) mx4_tile_kernel(const Mx4Args p) {
   i32x4 b0[FN], b1[FN];
   read(0, 0, a0, b0);
   read_scales(0, sca, scb);
-  for (int kt = 0; kt < nkt; ++kt) {
+  auto unit = [&](int kt, bool odd) {
     const int s = kt % NST;
+    if (odd) {
+      write_scales((kt + 1) >> 1, scales);  // (its buffer's last reads were two barriers ago)
+      scales = load_scales((kt + 3) >> 1);  // (past the last unit: masked, or another row's, never used)
+    }
     read(s, 1, a1, b1);
     mma(a0, b0, 0);
     interleave();
@@ -256,8 +278,6 @@ __global__ void __launch_bounds__(256, RES) mx4_tile_kernel(const Mx4Args p) {
     mma(a0, b0, 2);
     interleave();
     sync();  // every wave is past stage s, and unit kt + 1 landed
-    // (a buffer of scales: its last reads were a barrier ago, its next are two units on)
-    if ((kt & 1) && kt + 3 < nkt) scale_fill((kt + 3) >> 1);
     fill(min(kt + NST, nkt - 1), s);
     read((kt + 1) % NST, 0, a0, b0);  // (past the last unit: never used)
     read_scales(kt + 1, nsca, nscb);
@@ -268,6 +288,12 @@ __global__ void __launch_bounds__(256, RES) mx4_tile_kernel(const Mx4Args p) {
     for (int i = 0; i < FM; ++i) sca[i][0] = nsca[i][0], sca[i][1] = nsca[i][1];
 #pragma unroll
     for (int j = 0; j < FN; ++j) scb[j][0] = nscb[j][0], scb[j][1] = nscb[j][1];
+  };
+  for (int kt = 0;; kt += 2) {
+    unit(kt, false);
+    if (kt + 1 >= nkt) break;
+    unit(kt + 1, true);
+    if (kt + 2 >= nkt) break;
   }
   __builtin_amdgcn_s_waitcnt(0x3f70);  // the last fills land before LDS is reused
   __syncthreads();

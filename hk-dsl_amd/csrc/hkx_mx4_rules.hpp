@@ -7,8 +7,6 @@
 
 namespace hkx {
 
-constexpr int kMx4SkinnyM = 32;  // the decode kernel's rows
-
 // The kernels (HKX_MX4_* of hkx.h).
 constexpr int kMx4Tile64 = 1, kMx4Tile128 = 2, kMx4Quad = 3, kMx4Skinny = 4;
 
@@ -30,16 +28,24 @@ inline int mx4_splits(int kernel, int units, int s) {
   return (units + per - 1) / per;
 }
 
-// Whether up to 32 rows run on the decode kernel; its rate over the 64 x 128 tiles' of the best split,
-// cold weights (rows of B: twice the columns in the paired form), M = 1-8, 16, 24, 32:
-// * K to 4096: any up to M = 16; past it 1.13-1.8 to 16384 rows, 0.58-0.83 at 28672;
-// * past it X is streamed with every 16 rows of B: 4-bit X 1.36-1.63, 1.24-1.45, 1.01-1.33, 0.92-1.28 to
-//   4096 rows, 1.06-1.10, 0.93-1.03, 0.87-1.01, 0.8-0.96 at 8192, 0.98-1.08, 0.86-0.93, .. at 16384;
-//   8-bit X 1.26-1.52, 1.11-1.41, 0.86-1.15, 0.8-1.09 to 4096, 1.04-1.14, 0.89-1.05, 0.72-0.81, .. at 8192,
-//   0.92-1.02, 0.78-0.91, .. at 16384; both less the longer K.
-inline bool mx4_skinny_wins(int m, int rows, int k, bool a8) {
-  if (m > kMx4SkinnyM) return false;
+// Whether a call runs on the decode kernel (workgroups of 16 rows of B and up to 64 of A); its rate over
+// the other kernels' best plan, cold weights (rows of B: twice the columns in the paired form):
+// * up to 32 rows of A, M = 1-8, 16, 24, 32. K to 4096: any up to M = 16; past it 1.13-1.8 to 16384 rows,
+//   0.58-0.83 at 28672. Past it A is streamed with every 16 rows of B: 4-bit A 1.36-1.63, 1.24-1.45,
+//   1.01-1.33, 0.92-1.28 to 4096 rows, 1.06-1.10, 0.93-1.03, 0.87-1.01, 0.8-0.96 at 8192, 0.98-1.08,
+//   0.86-0.93, .. at 16384; 8-bit A 1.26-1.52, 1.11-1.41, 0.86-1.15, 0.8-1.09 to 4096, 1.04-1.14, 0.89-1.05,
+//   0.72-0.81, .. at 8192, 0.92-1.02, 0.78-0.91, .. at 16384; both less the longer K;
+// * 33 to 64: K to 4096 1.17-1.96 to 16384 rows; past it 4-bit A 1.02-1.23 at K = 8192 and 0.96-1.17 at 12288
+//   to 4096 rows, 8-bit A 0.78-0.98;
+// * 65 to 512: K to 4096 1.17-2.0 to two workgroups a CU (8-bit A past 256 rows of A: 0.83-0.97, and to one
+//   a CU 1.2-1.37), 0.58-1.24 past that; K = 8192 4-bit A 1.15-1.23 to one a CU and 256 rows of A, 0.78 past
+//   them, 8-bit A 0.92-0.95.
+inline bool mx4_skinny_wins(int m, int rows, int k, bool a8, int cus) {
+  const int64_t wgs = (int64_t)((m + 63) / 64) * ((rows + 15) / 16);
+  if (m > 64 && k <= 4096) return m <= 512 && wgs <= (a8 && m > 256 ? cus : 2 * cus);
+  if (m > 64) return !a8 && m <= 256 && wgs <= cus && k <= 8192;
   if (k <= 4096) return m <= 16 || rows <= 20480;
+  if (m > 32) return !a8 && rows <= 4096 && k <= 8192;
   if (m > 16) return rows <= 4096 && k <= (a8 ? 6144 : 8192);
   if (m > 8) return rows <= 4096 || (rows <= 8192 && k <= 8192);
   return rows <= (a8 ? 8192 : 16384);
@@ -71,7 +77,7 @@ inline double mx4_cost(int kernel, int m, int n, int k, bool a8, bool pair, bool
 
 // quad_ok: the quadrant kernel takes the call; vec: C's rows are whole 16-byte pieces.
 inline Mx4Plan mx4_plan(int m, int n, int k, bool a8, bool pair, bool quad_ok, bool vec, int cus) {
-  if (mx4_skinny_wins(m, pair ? 2 * n : n, k, a8)) return {kMx4Skinny, 1};
+  if (mx4_skinny_wins(m, pair ? 2 * n : n, k, a8, cus)) return {kMx4Skinny, 1};
   const int units = (k + 255) / 256;
   Mx4Plan best{kMx4Tile64, 1};
   double t = 1e30;

@@ -1,4 +1,6 @@
 // The MXFP4 decode kernel's forms (hkx_mx4_skinny.hpp).
+#include <algorithm>
+
 #include "hkx_mx4_skinny.hpp"
 
 namespace hkx {
@@ -24,18 +26,26 @@ static hipError_t launch_form(const Mx4SkinnyArgs& a, bool a8, bool pair, dim3 g
 }
 
 hipError_t launch_mx4_skinny(Mx4SkinnyArgs a, bool a8, bool pair, int cus, hipStream_t s) {
+  const int chunks = (a.M + 63) / 64;  // of 64 rows, each its own workgroups
+  cus = std::max(1, cus / chunks);
   // the most blocks a workgroup, up to 4, that leave the CUs full and the blocks as even over them as
   // one each
   const int nq = a.units <= 8 ? 1 : a.units <= 16 ? 2 : 0;
-  const int resident = mx4_skinny_resident(a.M <= 16 ? 1 : 2, a8, pair, nq);
+  const int mf = chunks > 1 ? 4 : (a.M + 15) / 16;
+  const int resident = mx4_skinny_resident(mf, a8, pair, nq);
   const int blocks = (a.N + (pair ? 7 : 15)) / (pair ? 8 : 16), least = (blocks + cus - 1) / cus;
   a.nb = 1;
   for (int nb = 2; nb <= 4; ++nb) {
     const int wgs = (blocks + nb - 1) / nb;
     if (wgs >= resident * cus && nb * ((wgs + cus - 1) / cus) <= least) a.nb = nb;
   }
-  const dim3 grid((unsigned)((blocks + a.nb - 1) / a.nb));
-  return a.M <= 16 ? launch_form<1>(a, a8, pair, grid, s) : launch_form<2>(a, a8, pair, grid, s);
+  const dim3 grid((unsigned)((blocks + a.nb - 1) / a.nb), (unsigned)chunks);
+  switch (mf) {
+    case 1: return launch_form<1>(a, a8, pair, grid, s);
+    case 2: return launch_form<2>(a, a8, pair, grid, s);
+    case 3: return launch_form<3>(a, a8, pair, grid, s);
+    default: return launch_form<4>(a, a8, pair, grid, s);
+  }
 }
 
 }  // namespace hkx

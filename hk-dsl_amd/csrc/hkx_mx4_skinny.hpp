@@ -1,4 +1,4 @@
-// The MXFP4 product at decode sizes: C (M <= 32, N) from X . W^T with W read once, in the 8-bit decode
+// The MXFP4 product at decode sizes (64 rows of C a workgroup, more by blockIdx.y): C (M, N) from X . W^T with W read once, in the 8-bit decode
 // kernel's plan (hkx_skinny.hpp): short workgroups whose 8 waves cut K, each wave's share of W by
 // non-temporal DMA of whole lines into slots of its own, X in registers.
 //
@@ -40,10 +40,10 @@ struct Mx4SkinnyArgs {
   int32_t c_vec;  // C's rows 8-byte aligned and N a multiple of 4: 8-byte stores
 };
 
-// Workgroups a CU, as the registers allow: three where a round's X is few, one where four are in flight
-// and many.
+// Workgroups a CU, as the registers allow: three where a round's X is few, one where it is many.
 constexpr int mx4_skinny_resident(int mf, bool a8, bool pair, int nq) {
-  return mf == 1 && nq > 0 && (!a8 || nq == 1 || !pair) ? 3 : (a8 || mf == 2) && nq == 0 ? 1 : 2;
+  if (mf == 1) return nq > 0 && (!a8 || nq == 1 || !pair) ? 3 : a8 && nq == 0 ? 1 : 2;
+  return mf == 2 && nq > 0 ? 2 : 1;
 }
 
 template <int MF, bool A8, bool PAIR, int NQ>
@@ -51,7 +51,7 @@ __global__ void __launch_bounds__(512, 2 * mx4_skinny_resident(MF, A8, PAIR, NQ)
   constexpr int NW = 8;
   constexpr int NL = A8 ? 2 : 1;          // lines of a row of X a unit
   constexpr int SLOT = 16 * 128;          // 16 rows of W, or of X as a line is turned
-  constexpr int NS = NQ ? 2 : 4;          // rounds in flight, a slot each
+  constexpr int NS = NQ || MF > 2 ? 2 : 4;  // rounds in flight, a slot each
   constexpr int RED = NW * NS * SLOT;     // then the waves' sums of a block: [wave][fragment][lane]
   constexpr int BC = PAIR ? 8 : 16;       // columns a block
   __shared__ __attribute__((aligned(16))) uint8_t lds[RED + NW * MF * 1024];
@@ -60,17 +60,20 @@ __global__ void __launch_bounds__(512, 2 * mx4_skinny_resident(MF, A8, PAIR, NQ)
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int rf = lane & 15, g = lane >> 4;
   const int n0 = blockIdx.x * BC * p.nb;
+  // blockIdx.y: 64 rows of X and C (all of them where M is no more)
+  const int mb = blockIdx.y * 64, rows = min(p.M - mb, 16 * MF);
   const int nb = min(p.nb, (p.N - n0 + BC - 1) / BC);
   const int nq = NQ ? NQ : (p.units + NW - 1) / NW;
   const int nu = nb * nq;  // steps: (block, round)
   uint8_t* own = lds + wave * NS * SLOT;
 
-  const __amdgpu_buffer_rsrc_t rw = make_rsrc(p.b, p.b_bytes), rx = make_rsrc(p.a, p.a_bytes);
+  const __amdgpu_buffer_rsrc_t rw = make_rsrc(p.b, p.b_bytes), rx = make_rsrc(p.a + (int64_t)mb * p.lda, p.a_bytes - (uint32_t)mb * p.lda);
   // the scales' buffers begin at an aligned dword and end with the one that holds the last byte
-  const uint32_t sx0 = (uint32_t)((uintptr_t)p.sa & 3), sw0 = (uint32_t)((uintptr_t)p.sb & 3);
+  const uint8_t* const sa = p.sa + (int64_t)mb * p.sa_ld;
+  const uint32_t sx0 = (uint32_t)((uintptr_t)sa & 3), sw0 = (uint32_t)((uintptr_t)p.sb & 3);
   const uint32_t k32 = (uint32_t)p.K / 32;
   const __amdgpu_buffer_rsrc_t rsx =
-      make_rsrc((const void*)((uintptr_t)p.sa & ~(uintptr_t)3), (sx0 + (uint32_t)(p.M - 1) * p.sa_ld + k32 + 3) & ~3u);
+      make_rsrc((const void*)((uintptr_t)sa & ~(uintptr_t)3), (sx0 + (uint32_t)(rows - 1) * p.sa_ld + k32 + 3) & ~3u);
   const __amdgpu_buffer_rsrc_t rsw = make_rsrc((const void*)((uintptr_t)p.sb & ~(uintptr_t)3),
                                                (sw0 + (uint32_t)((PAIR ? 2 : 1) * p.N - 1) * p.sb_ld + k32 + 3) & ~3u);
 
@@ -236,9 +239,9 @@ __global__ void __launch_bounds__(512, 2 * mx4_skinny_resident(MF, A8, PAIR, NQ)
       v = silu_mul4(v, up);
       if (g > 1) n = p.N;
     }
-    if (m_out >= p.M || n >= p.N) return;
+    if (m_out >= rows || n >= p.N) return;
     const u32x2 o = pack4<2>(HKX_BF16, v);
-    uint16_t* dst = (uint16_t*)p.c + (int64_t)m_out * p.ldc + n;
+    uint16_t* dst = (uint16_t*)p.c + (int64_t)(mb + m_out) * p.ldc + n;
     if (p.c_vec) {
       *(u32x2*)dst = o;
     } else {
@@ -311,42 +314,46 @@ __global__ void __launch_bounds__(512, 2 * mx4_skinny_resident(MF, A8, PAIR, NQ)
       finish(NQ == 1 ? 1 : 0);
     }
   } else {
-    Scales s2{}, s3{};
-    XRegs x2, x3;
+    [[maybe_unused]] Scales s2{}, s3{};
+    [[maybe_unused]] XRegs x2, x3;
     auto round_of = [&](int u) { return u < nq ? u : u % nq; };
     issue_x(0, x0);
     issue_w(0, s0);
     issue_x(round_of(1), x1);
     issue_w(1, s1);
-    issue_x(round_of(2), x2);
-    issue_w(2, s2);
-    issue_x(round_of(3), x3);
-    issue_w(3, s3);
+    if constexpr (NS == 4) {
+      issue_x(round_of(2), x2);
+      issue_w(2, s2);
+      issue_x(round_of(3), x3);
+      issue_w(3, s3);
+    }
     int j = 0, q = 0;      // step u's block and round
-    int qx = round_of(4);  // round of step u + 4
+    int qx = round_of(NS);  // round of step u + NS
     auto step = [&](int u, XRegs& x, Scales& sw) {
-      HKX_SKINNY_WAIT(3 * (WLOADS + XLOADS));
+      HKX_SKINNY_WAIT((NS - 1) * (WLOADS + XLOADS));
       read_w(u);
       turn_x(u, x);
       mma(q, x, sw);
       __builtin_amdgcn_s_waitcnt(0xc07f);
       issue_x(qx, x);
-      issue_w(u + 4, sw);
+      issue_w(u + NS, sw);
       if (++qx == nq) qx = 0;
       if (++q == nq) {
         finish(j++);
         q = 0;
       }
     };
-    for (int u = 0;; u += 4) {  // (each exit leaves the loop: a step the compiler sees skipped costs waits)
+    for (int u = 0;; u += NS) {  // (each exit leaves the loop: a step the compiler sees skipped costs waits)
       step(u, x0, s0);
       if (u + 1 >= nu) break;
       step(u + 1, x1, s1);
       if (u + 2 >= nu) break;
-      step(u + 2, x2, s2);
-      if (u + 3 >= nu) break;
-      step(u + 3, x3, s3);
-      if (u + 4 >= nu) break;
+      if constexpr (NS == 4) {
+        step(u + 2, x2, s2);
+        if (u + 3 >= nu) break;
+        step(u + 3, x3, s3);
+        if (u + 4 >= nu) break;
+      }
     }
   }
 #undef HKX_SKINNY_WAIT

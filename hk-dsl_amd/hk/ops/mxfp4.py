@@ -132,8 +132,7 @@ def dequant(q, s, dtype=None):
     return _dequant("mxfp4.dequant", _packed(q, "mxfp4.dequant", "q"), s, dtype, nat.FP4E2M1, 2)
 
 
-#: Layouts of gemm's operands: (arguments filled in but for their addresses, workspace bytes, C's shape,
-#: the scales' alignment that the workspace is for).
+#: Layouts of gemm's operands: (arguments filled in but for their addresses, workspace bytes, C's shape).
 _GEMM: dict = {}
 
 
@@ -147,10 +146,10 @@ def gemm(a, b, sa, sb, *, bias=None, silu_mul=False, out=None):
     plan = _GEMM.get(key)
     if plan is None or out is not None:
         return _gemm(a, b, sa, sb, bias, silu_mul, out, key)
-    args, need, shape, align = plan
+    args, need, shape = plan
     pa, pb, ps, pt = a.data_ptr(), b.data_ptr(), sa.data_ptr(), sb.data_ptr()
     d = a.get_device()
-    if ((pa | pb) & 15 or (ps | pt) & 3 != align or d < 0 or b.get_device() != d or sa.get_device() != d
+    if ((pa | pb) & 15 or d < 0 or b.get_device() != d or sa.get_device() != d
             or sb.get_device() != d
             or (bias is not None and (bias.get_device() != d or bias.data_ptr() & 15))):
         return _gemm(a, b, sa, sb, bias, silu_mul, out, None)
@@ -230,8 +229,7 @@ def _gemm(a, b, sa, sb, bias, silu_mul, out, key):
     g.lda, g.ldb = _ld(a, a.shape[1]), _ld(b, k // 2)
     up4 = (k // 32 + 3) // 4 * 4
     g.sa_ld, g.sb_ld, g.ldc = _ld(sa, up4), _ld(sb, up4), _ld(c, n)
-    # (the workspace goes by the scales' alignment, and by C's: a new C's is 16 bytes or more)
-    g.sa, g.sb, g.c = sa.data_ptr(), sb.data_ptr(), c.data_ptr()
+    g.c = c.data_ptr()  # (the workspace goes by its alignment: a new C's is 16 bytes or more)
     g.m, g.n, g.k, g.silu_mul = m, n, k, 1 if silu_mul else 0
     if bias is not None:
         g.bias_dtype = nat.dtype_code(bias.dtype)
@@ -239,7 +237,7 @@ def _gemm(a, b, sa, sb, bias, silu_mul, out, key):
     # (a template only where every operand was read where it is, and C is a plain new tensor)
     if key is not None and g.ldc == n and all(
             x is None or x.data_ptr() == y.data_ptr() for x, y in zip((a, b, sa, sb, bias), given)):
-        nat.remember(_GEMM, key, (bytes(g), need, (*lead, n), (g.sa | g.sb) & 3), 4096)
+        nat.remember(_GEMM, key, (bytes(g), need, (*lead, n)), 4096)
     _launch(g, need, a, a.data_ptr(), b.data_ptr(), sa.data_ptr(), sb.data_ptr(), bias, c)
     return out
 

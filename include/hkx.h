@@ -341,7 +341,7 @@ int hkx_mx_dequant(const void* q, int64_t ldq, int32_t q_dtype, const uint8_t* s
 #define HKX_MX4_AUTO 0
 #define HKX_MX4_TILE64 1  /* 64 x 128 tiles, 4 waves */
 #define HKX_MX4_TILE128 2 /* 128 x 128 tiles, 4 waves */
-#define HKX_MX4_SKINNY 4  /* the decode kernel: M up to 32; no splits */
+#define HKX_MX4_SKINNY 4  /* the decode kernel, 64 rows of C a workgroup; no splits */
 #define HKX_MX4_QUAD 3    /* 256 x 256 tiles, 8 waves, persistent; C under 4 GiB */
 typedef struct {
   int32_t size; /* sizeof(HkxMx4GemmArgs): the library refuses another layout */
