@@ -341,8 +341,8 @@ int hkx_mx_dequant(const void* q, int64_t ldq, int32_t q_dtype, const uint8_t* s
 #define HKX_MX4_AUTO 0
 #define HKX_MX4_TILE64 1  /* 64 x 128 tiles, 4 waves */
 #define HKX_MX4_TILE128 2 /* 128 x 128 tiles, 4 waves */
-#define HKX_MX4_SKINNY 4  /* the decode kernel, 64 rows of C a workgroup; no splits */
 #define HKX_MX4_QUAD 3    /* 256 x 256 tiles, 8 waves, persistent; C under 4 GiB */
+#define HKX_MX4_SKINNY 4  /* the decode kernel, 64 rows of C a workgroup; no splits */
 typedef struct {
   int32_t size; /* sizeof(HkxMx4GemmArgs): the library refuses another layout */
   int32_t a_dtype;
@@ -363,6 +363,7 @@ typedef struct {
   size_t ws_bytes;
 } HkxMx4GemmArgs;
 int hkx_mx4_gemm(const HkxMx4GemmArgs* args, void* stream);
+/* (goes by every size, stride and c's alignment, so these are set first) */
 size_t hkx_mx4_gemm_workspace(const HkxMx4GemmArgs* args);
 
 /* Between two blocks, a row at a time: u = x rsqrt(mean x^2 + eps) post (u = x without post), h =
