@@ -53,23 +53,23 @@ inline bool mx4_skinny_wins(int m, int rows, int k, bool a8, int cus) {
 
 // A plan's estimated time in us: a launch, more for each further wave of workgroups, a time a 256-K unit
 // and wave and one for its share of the memory's traffic, and where it goes through fp32 shares their
-// sum's launch and their round trip. Fitted to 1092 timed plans (M 33-4096, N 512-24576, K 512-12288,
-// weights past the cache): medians 0.99-1.01 of the times, 0.82-0.90 and 1.08-1.14 at the tenths; the
-// plans it picks take 1.03 times the best one's on average. Waves: whole ones where a workgroup has its
-// CU alone (the quadrant kernel, 128 x 128 tiles of an 8-bit A), 0.83 of their number past one where two
-// share it. A C of odd columns or alignment goes through shares on the quadrant kernel always (stored from
-// its registers two bytes at a time 3000 x 1001 took 25 us more).
+// sum's launch and their round trip. Fitted to 1740 timed plans (M 33-4096, N 512-24576, K 512-12288,
+// weights past the cache): medians 0.98-1.00 of the times, 0.84-0.91 and 1.06-1.14 at the tenths; the
+// plans it picks take 1.01 times the best one's on average. Waves are whole ones also where two workgroups
+// share a CU (0.83 of their number past one, as fitted before, picked plans of 1.02 times: 777 x 4096 x
+// 12288 of 4 bits as 448 workgroups 45.1 us, as 224 38.7). A C of odd columns or alignment goes through
+// shares on the quadrant kernel always (stored from its registers two bytes at a time 3000 x 1001 took 25
+// us more).
 inline double mx4_cost(int kernel, int m, int n, int k, bool a8, bool pair, bool vec, int splits, int cus) {
   static const double kC[2][3][6] = {
       // launch, wave, unit, unit x filled, sum, share bytes
-      {{3.6, 4.7, 0.454, 0.418, 2.6, 0.64}, {4.7, 3.1, 0.713, 0.284, 2.5, 0.83}, {10.4, 7.1, 1.369, 0.375, 5.1, 0.64}},
-      {{3.8, 4.9, 0.565, 0.391, 2.8, 0.58}, {4.6, 1.6, 1.062, 0.180, 2.5, 0.88}, {10.1, 6.1, 2.070, 0.454, 5.0, 0.65}}};
+      {{4.2, 0.32, 0.497, 0.234, 2.0, 1.05}, {5.3, 0.05, 0.720, 0.083, 2.2, 0.92}, {10.3, 6.7, 1.297, 0.425, 5.6, 0.62}},
+      {{4.4, 0.19, 0.604, 0.247, 2.0, 1.02}, {5.2, 2.6, 1.029, 0.133, 2.4, 0.93}, {10.0, 6.0, 1.979, 0.532, 5.6, 0.64}}};
   const double* c = kC[a8][kernel - 1];
   const int bm = mx4_rows(kernel), bn = mx4_cols(kernel, pair);
   const int per = mx4_split_units(kernel, (k + 255) / 256, splits);
   const double w = (double)((m + bm - 1) / bm) * ((n + bn - 1) / bn) * splits / cus;
-  const bool alone = kernel == kMx4Quad || (kernel == kMx4Tile128 && a8);
-  const double waves = w <= 1 ? 1.0 : alone ? (double)(int64_t)(w + 0.9999) : std::max(1.0, 0.83 * w);
+  const double waves = w <= 1 ? 1.0 : (double)(int64_t)(w + 0.9999);
   double t = c[0] + c[1] * (waves - 1) + c[2] * per * waves + c[3] * per * std::min(w, 1.0);
   if (splits > 1 || (kernel == kMx4Quad && !vec)) t += c[4] + c[5] * splits * m * (pair ? 2.0 : 1.0) * n * 8.0 / 5e6;
   return t;
