@@ -60,6 +60,10 @@ HKX_DEV uint32_t mx4_mask(int left) { return left >= 4 ? 0xffffffffu : left <= 0
 //   k-step, after the unit's one barrier (read just before them, 4096 x 4096 of 4-bit K = 12288 at M =
 //   777 took 39.6 us). After that barrier the unit's stage takes the fills of unit t + NST; a wave
 //   waits for its own fills of the next unit only (buffer loads land in order).
+// * Measured: 777 x 4096 x 12288 of 4 bits 38.5 us (2.0 PFLOP/s), 128 x 4096 x 12288 in four splits 19.3;
+//   bound by the fills, some 48 bytes a ns and CU at any number of CUs (32 KB a unit of 128 x 128), and the
+//   lines of the scales beside them: without the scales' loads 128 x 4096 x 12288 unsplit takes 26.1 us
+//   instead of 36.6, 777 rows on 64 x 128 tiles 43.4 instead of 53.1, on 128 x 128 ones 43.1 instead of 43.8.
 // * RES = 2: two workgroups a CU, for grids of more than one a CU, in half the LDS.
 template <int BM, int BN, bool A8, bool PAIR, bool SHARE, int RES>
 __global__ void __launch_bounds__(256, RES) mx4_tile_kernel(const Mx4Args p) {

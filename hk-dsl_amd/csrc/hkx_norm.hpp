@@ -9,6 +9,11 @@
 //
 // A row is held by T threads (a wave, or a workgroup of up to 16), 8 C elements a thread: C pieces of
 // 8 (16-byte loads), or single ones T apart where D or a row's address is no multiple of 8.
+//
+// Measured, 8192 rows of 4096 bf16 with fp32 weights and a gate a sequence: forward 54 us (268 MB, 5.0
+// TB/s; a copy of 1 GiB reaches 5.25), backward 83-86 (403 MB, 4.8) and the sum of its partial sums 5.1;
+// 4096 rows with an fp32 stream, y as MXFP8, 37 (185 MB, 5.0); 16 rows 4; 999 rows of 1111 fp32 (single
+// elements) 6.6, 14.5 and 3.9.
 #pragma once
 
 #include "hkx_api.hpp"
