@@ -51,19 +51,19 @@ HKX_DEV uint32_t mx4_mask(int left) { return left >= 4 ? 0xffffffffu : left <= 0
 //   row's eight 16-byte pieces XOR-swizzled (piece c of row r at c ^ swz(r % 16)) so that the
 //   fragment reads of 16 rows hit distinct banks; filled by 16-byte DMA of whole lines, the swizzle
 //   applied on the global side.
-// * Scales, a row a thread: the dwords that hold the 16 bytes of two units (at any alignment) into
-//   registers three units ahead, joined, those past K masked, and written to one of two LDS buffers a
-//   unit ahead. (By DMA, rows off a multiple of 4 bytes took a launch that aligned them; a unit at a time
-//   they were half as many cache lines as the operands, and a wait for them one unit on held the fills to
-//   that: 15% slower each.)
+// * Scales: four threads a row, 64 bytes of it (eight units) at a time into registers, as aligned dwords,
+//   one more where rows are off a multiple of 4 bytes; a chunk of two units goes to one of two LDS buffers a
+//   unit ahead, joined and masked past K where it needs it. (A thread a row, 16 bytes every two units, asked
+//   for a line a row and piece, half as many as the fills, and with joins and masks always, 128 x 4096 x
+//   12288 of 4 bits unsplit took 37.0 us on 64 x 128 tiles against 28.6, and on 128 x 128 ones 44.6 against
+//   38.4.)
 // * Fragment reads run a k-step of 64 K ahead of their MFMAs, the next unit's first ones under the last
 //   k-step, after the unit's one barrier (read just before them, 4096 x 4096 of 4-bit K = 12288 at M =
 //   777 took 39.6 us). After that barrier the unit's stage takes the fills of unit t + NST; a wave
 //   waits for its own fills of the next unit only (buffer loads land in order).
-// * Measured: 777 x 4096 x 12288 of 4 bits 38.5 us (2.0 PFLOP/s), 128 x 4096 x 12288 in four splits 19.3;
-//   bound by the fills, some 48 bytes a ns and CU at any number of CUs (32 KB a unit of 128 x 128), and the
-//   lines of the scales beside them: without the scales' loads 128 x 4096 x 12288 unsplit takes 26.1 us
-//   instead of 36.6, 777 rows on 64 x 128 tiles 43.4 instead of 53.1, on 128 x 128 ones 43.1 instead of 43.8.
+// * Measured: 777 x 4096 x 12288 of 4 bits 39-41 us on 128 x 128 tiles (2.0 PFLOP/s), 128 x 4096 x 12288 in
+//   four splits 17.4; bound by the fills, some 48 bytes a ns and CU whether all CUs run or 32 (32 KB a unit
+//   of 128 x 128): without them 777 rows took 36 us, on 64 x 128 tiles 28.
 // * RES = 2: two workgroups a CU, for grids of more than one a CU, in half the LDS.
 template <int BM, int BN, bool A8, bool PAIR, bool SHARE, int RES>
 __global__ void __launch_bounds__(256, RES) mx4_tile_kernel(const Mx4Args p) {
@@ -75,7 +75,7 @@ __global__ void __launch_bounds__(256, RES) mx4_tile_kernel(const Mx4Args p) {
   constexpr int NA = BM * AL / 32;     // of which A's
   constexpr int STAGE = LINES * 128;
   constexpr int ROWS = BM + BN;
-  static_assert(ROWS <= 256, "a row's scales a thread");
+  static_assert(BM % 64 == 0 && BN % 64 == 0, "64 rows of scales a load");
   constexpr int OUTW = PAIR ? BN / 2 : BN;
   constexpr int RS = OUTW * 2 + 16;  // staging row stride
   constexpr int BESIDE = BN * 4 + 2 * ROWS * 16;
@@ -134,34 +134,54 @@ __global__ void __launch_bounds__(256, RES) mx4_tile_kernel(const Mx4Args p) {
       }
     }
   };
-  // this thread's row of scales: A's, then B's
-  const bool row_a = tid < BM;  // (BM is a multiple of 64: whole waves)
-  const uint32_t s0 = (uint32_t)((uintptr_t)(row_a ? p.sa : p.sb) & 3);
-  const uint32_t k32 = (uint32_t)p.K / 32, srows = row_a ? (uint32_t)p.M : (uint32_t)((PAIR ? 2 : 1) * p.N);
-  const uint32_t sld = row_a ? p.sa_ld : p.sb_ld;
-  const __amdgpu_buffer_rsrc_t rs = make_rsrc((const void*)((uintptr_t)(row_a ? p.sa : p.sb) & ~(uintptr_t)3),
-                                              tid < ROWS ? (s0 + (srows - 1) * sld + k32 + 3) & ~3u : 0u);
-  const uint32_t sat = s0 + (uint32_t)(row_a ? m0 + tid : brow(tid - BM)) * sld + (uint32_t)kt0 * 8u;
-  struct Scales {  // of a chunk of two units: four dwords and, off a multiple of 4 bytes, a fifth
-    i32x4 d;
-    uint32_t e;
+  // scales: thread t's piece t % 4 (of a chunk of two units) of rows t / 4 + 64 i, A's and then B's
+  constexpr int NS = ROWS / 64;
+  const uint32_t k32 = (uint32_t)p.K / 32;
+  const uint32_t s0a = (uint32_t)((uintptr_t)p.sa & 3), s0b = (uint32_t)((uintptr_t)p.sb & 3);
+  const __amdgpu_buffer_rsrc_t rsa = make_rsrc((const void*)((uintptr_t)p.sa & ~(uintptr_t)3),
+                                               (s0a + (uint32_t)(p.M - 1) * p.sa_ld + k32 + 3) & ~3u);
+  const __amdgpu_buffer_rsrc_t rsb = make_rsrc((const void*)((uintptr_t)p.sb & ~(uintptr_t)3),
+                                               (s0b + (uint32_t)((PAIR ? 2 : 1) * p.N - 1) * p.sb_ld + k32 + 3) & ~3u);
+  const uint32_t fifth_a = ((p.sa_ld | s0a) & 3) ? 0u : kMx4Out, fifth_b = ((p.sb_ld | s0b) & 3) ? 0u : kMx4Out;
+  uint32_t sat[NS];
+#pragma unroll
+  for (int i = 0; i < NS; ++i) {
+    const int r = 64 * i + (tid >> 2);
+    sat[i] = (64 * i < BM ? s0a + (uint32_t)(m0 + r) * p.sa_ld : s0b + (uint32_t)brow(r - BM) * p.sb_ld) +
+             (uint32_t)kt0 * 8u + (uint32_t)(tid & 3) * 16u;
+  }
+  struct Scales {  // of four chunks: four dwords a piece and, off a multiple of 4 bytes, a fifth
+    i32x4 d[NS];
+    uint32_t e[NS];
   };
-  const uint32_t fifth = ((sld | s0) & 3) ? 16u : kMx4Out;
-  auto load_scales = [&](int c) {
-    const uint32_t at = (sat + (uint32_t)c * 16u) & ~3u;
-    Scales s;
-    s.d = buf_load16(rs, at, 0);
-    s.e = __builtin_amdgcn_raw_buffer_load_b32(rs, at + fifth, 0, 0);
-    return s;
+  auto load_scales = [&](int c, Scales& s) {  // chunks c to c + 3
+#pragma unroll
+    for (int i = 0; i < NS; ++i) {
+      const uint32_t at = (sat[i] + (uint32_t)c * 16u) & ~3u;
+      s.d[i] = buf_load16(64 * i < BM ? rsa : rsb, at, 0);
+      s.e[i] = __builtin_amdgcn_raw_buffer_load_b32(64 * i < BM ? rsa : rsb, (at + 16u) | (64 * i < BM ? fifth_a : fifth_b), 0, 0);
+    }
   };
   auto write_scales = [&](int c, const Scales& s) {
     const int left = (int)k32 - 8 * kt0 - 16 * c;
-    i32x4 v;
+    uint8_t* at = smem + SCO + (c & 1) * ROWS * 16 + (tid >> 2) * 16;
+    if ((fifth_a & fifth_b) && left >= 16) {  // nothing to join or mask
+      if ((tid & 3) == (c & 3)) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      v[i] = (int)(__builtin_amdgcn_alignbyte(i < 3 ? (uint32_t)s.d[(i + 1) & 3] : s.e, (uint32_t)s.d[i], sat & 3) &
-                   mx4_mask(left - 4 * i));
-    if (tid < ROWS) *(i32x4*)(smem + SCO + (c & 1) * ROWS * 16 + tid * 16) = v;
+        for (int i = 0; i < NS; ++i) *(i32x4*)(at + 1024 * i) = s.d[i];
+      }
+      return;
+    }
+    if ((tid & 3) != (c & 3)) return;
+#pragma unroll
+    for (int i = 0; i < NS; ++i) {
+      i32x4 v;
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        v[j] = (int)(__builtin_amdgcn_alignbyte(j < 3 ? (uint32_t)s.d[i][(j + 1) & 3] : s.e[i], (uint32_t)s.d[i][j], sat[i] & 3) &
+                     mx4_mask(left - 4 * j));
+      *(i32x4*)(at + 1024 * i) = v;
+    }
   };
 
   const int rf = lane & 31, h = lane >> 5, sw = swz(rf & 15);
@@ -252,11 +272,11 @@ __global__ void __launch_bounds__(256, RES) mx4_tile_kernel(const Mx4Args p) {
     }
   };
   // all stages; unit 0 landed. (A fill past the last unit fetches that unit again.)
-  const Scales scales0 = load_scales(0);
-  Scales scales = load_scales(1);
+  Scales scales;
+  load_scales(0, scales);
 #pragma unroll
   for (int s = 0; s < NST; ++s) fill(min(s, nkt - 1), s);
-  write_scales(0, scales0);
+  write_scales(0, scales);
   __builtin_amdgcn_s_waitcnt((((NST - 1) * NCH) & 15) | ((((NST - 1) * NCH) >> 4) << 14) | (7 << 4));
   __builtin_amdgcn_s_barrier();
   __builtin_amdgcn_sched_barrier(0);
@@ -267,8 +287,9 @@ __global__ void __launch_bounds__(256, RES) mx4_tile_kernel(const Mx4Args p) {
   auto unit = [&](int kt, bool odd) {
     const int s = kt % NST;
     if (odd) {
-      write_scales((kt + 1) >> 1, scales);  // (its buffer's last reads were two barriers ago)
-      scales = load_scales((kt + 3) >> 1);  // (past the last unit: masked, or another row's, never used)
+      const int c = (kt + 1) >> 1;
+      write_scales(c, scales);  // (its buffer's last reads were two barriers ago)
+      if ((c & 3) == 3) load_scales(c + 1, scales);  // (past the last unit: masked, or another row's, never used)
     }
     read(s, 1, a1, b1);
     mma(a0, b0, 0);

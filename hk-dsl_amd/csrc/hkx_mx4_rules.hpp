@@ -30,21 +30,21 @@ inline int mx4_splits(int kernel, int units, int s) {
 
 // Whether a call runs on the decode kernel (workgroups of 16 rows of B and up to 64 of A); its rate over
 // the other kernels' best plan, cold weights (rows of B: twice the columns in the paired form):
-// * up to 32 rows of A, M = 1-8, 16, 24, 32. K to 4096: any up to M = 16; past it 1.13-1.8 to 16384 rows,
-//   0.58-0.83 at 28672. Past it A is streamed with every 16 rows of B: 4-bit A 1.36-1.63, 1.24-1.45,
+// * up to 32 rows of A, M = 1-8, 16, 24, 32. K to 4096: any up to M = 16; past it 1.10-1.8 to 16384 rows,
+//   0.77 at 20480, 0.58-0.83 at 28672. Past it A is streamed with every 16 rows of B: 4-bit A 1.36-1.63, 1.24-1.45,
 //   1.01-1.33, 0.92-1.28 to 4096 rows, 1.06-1.10, 0.93-1.03, 0.87-1.01, 0.8-0.96 at 8192, 0.98-1.08,
 //   0.86-0.93, .. at 16384; 8-bit A 1.26-1.52, 1.11-1.41, 0.86-1.15, 0.8-1.09 to 4096, 1.04-1.14, 0.89-1.05,
 //   0.72-0.81, .. at 8192, 0.92-1.02, 0.78-0.91, .. at 16384; both less the longer K;
-// * 33 to 64: K to 4096 1.17-1.96 to 16384 rows; past it 4-bit A 1.02-1.23 at K = 8192 and 0.96-1.17 at 12288
-//   to 4096 rows, 8-bit A 0.78-0.98;
-// * 65 to 512: K to 4096 1.17-2.0 to two workgroups a CU (8-bit A past 256 rows of A: 0.83-0.97, and to one
-//   a CU 1.2-1.37), 0.58-1.24 past that; K = 8192 4-bit A 1.15-1.23 to one a CU and 256 rows of A, 0.78 past
+// * 33 to 64: K to 4096 1.10-1.96 to 16384 rows, 0.67 at 20480; past it 4-bit A 0.98-1.29 at K = 8192 to 4096
+//   rows and less at 12288, 8-bit A 0.78-0.98;
+// * 65 to 512: K to 4096 0.96-2.0 to two workgroups a CU (8-bit A past 256 rows of A: 0.83-0.97, and to one
+//   a CU 1.2-1.46), 0.58-1.24 past that; K = 8192 4-bit A 1.06-1.15 to one a CU and 256 rows of A, 0.78 past
 //   them, 8-bit A 0.92-0.95.
 inline bool mx4_skinny_wins(int m, int rows, int k, bool a8, int cus) {
   const int64_t wgs = (int64_t)((m + 63) / 64) * ((rows + 15) / 16);
   if (m > 64 && k <= 4096) return m <= 512 && wgs <= (a8 && m > 256 ? cus : 2 * cus);
   if (m > 64) return !a8 && m <= 256 && wgs <= cus && k <= 8192;
-  if (k <= 4096) return m <= 16 || rows <= 20480;
+  if (k <= 4096) return m <= 16 || rows <= 16384;
   if (m > 32) return !a8 && rows <= 4096 && k <= 8192;
   if (m > 16) return rows <= 4096 && k <= (a8 ? 6144 : 8192);
   if (m > 8) return rows <= 4096 || (rows <= 8192 && k <= 8192);
@@ -54,8 +54,8 @@ inline bool mx4_skinny_wins(int m, int rows, int k, bool a8, int cus) {
 // A plan's estimated time in us: a launch, more for each further wave of workgroups, a time a 256-K unit
 // and wave and one for its share of the memory's traffic, and where it goes through fp32 shares their
 // sum's launch and their round trip. Fitted to 1740 timed plans (M 33-4096, N 512-24576, K 512-12288,
-// weights past the cache): medians 0.98-1.00 of the times, 0.84-0.91 and 1.06-1.14 at the tenths; the
-// plans it picks take 1.01 times the best one's on average. Waves are whole ones also where two workgroups
+// weights past the cache): medians 0.98-1.00 of the times, 0.85-0.92 and 1.06-1.12 at the tenths; the
+// plans it picks take 1.008 times the best one's on average. Waves are whole ones also where two workgroups
 // share a CU (0.83 of their number past one, as fitted before, picked plans of 1.02 times: 777 x 4096 x
 // 12288 of 4 bits as 448 workgroups 45.1 us, as 224 38.7). A C of odd columns or alignment goes through
 // shares on the quadrant kernel always (stored from its registers two bytes at a time 3000 x 1001 took 25
@@ -63,8 +63,8 @@ inline bool mx4_skinny_wins(int m, int rows, int k, bool a8, int cus) {
 inline double mx4_cost(int kernel, int m, int n, int k, bool a8, bool pair, bool vec, int splits, int cus) {
   static const double kC[2][3][6] = {
       // launch, wave, unit, unit x filled, sum, share bytes
-      {{4.2, 0.32, 0.497, 0.234, 2.0, 1.05}, {5.3, 0.05, 0.720, 0.083, 2.2, 0.92}, {10.3, 6.7, 1.297, 0.425, 5.6, 0.62}},
-      {{4.4, 0.19, 0.604, 0.247, 2.0, 1.02}, {5.2, 2.6, 1.029, 0.133, 2.4, 0.93}, {10.0, 6.0, 1.979, 0.532, 5.6, 0.64}}};
+      {{4.3, 0.0, 0.437, 0.155, 2.1, 1.10}, {5.5, 0.2, 0.646, 0.116, 2.3, 0.88}, {10.3, 8.2, 1.296, 0.539, 5.5, 0.64}},
+      {{4.5, 0.0, 0.552, 0.194, 2.0, 1.00}, {5.4, 2.8, 0.977, 0.172, 2.5, 0.86}, {10.0, 7.7, 1.980, 0.638, 5.5, 0.63}}};
   const double* c = kC[a8][kernel - 1];
   const int bm = mx4_rows(kernel), bn = mx4_cols(kernel, pair);
   const int per = mx4_split_units(kernel, (k + 255) / 256, splits);
