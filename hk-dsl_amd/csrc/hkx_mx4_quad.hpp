@@ -462,10 +462,11 @@ __global__ void __launch_bounds__(512, 1) mx4_quad_kernel(const Mx4Args p) {
   __builtin_amdgcn_s_waitcnt(wait_vm(0));  // no fill lands in LDS after the exit
 }
 
-// The quadrant kernel's scales (4.8-5.3 us for 4096 + 12288 rows of 128 bytes, a launch's latency), from E8M0 rows (any alignment) to [tile of 256 rows][chunk of two
+// The quadrant kernel's scales, from E8M0 rows (any alignment) to [tile of 256 rows][chunk of two
 // units][4 KB]: A's [unit][row group][lane][16 bytes], byte 8 h + 4 i + f of lane (rf, q) the scale of
 // row 128 i + 64 grp + 16 f + rf, block 8 unit + 4 h + q; B's [unit][column group][lane][8 bytes], byte
 // 4 h + 2 j + g that of tile row 128 j + 32 c + 16 g + rf. Rows past the last and blocks past K are 0.
+// (4096 + 12288 rows of 128 bytes take 4.8-5.3 us, half of it a launch's latency.)
 struct Mx4PackArgs {
   const uint8_t* s;
   uint8_t* out;
