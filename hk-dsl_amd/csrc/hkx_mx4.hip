@@ -52,12 +52,11 @@ namespace {
 static_assert(kMx4Tile64 == HKX_MX4_TILE64 && kMx4Tile128 == HKX_MX4_TILE128 && kMx4Quad == HKX_MX4_QUAD &&
                   kMx4Skinny == HKX_MX4_SKINNY, "kernels");
 
-// The quadrant kernel's epilogue: 32-bit offsets into C or the shares, and a paired bias whose up half
-// starts at a multiple of 4 bytes.
+// The quadrant kernel's epilogue: 32-bit offsets into C or the shares. (Any bias: C of odd columns leaves through
+// shares, whose sum adds it.)
 bool quad_ok(const HkxMx4GemmArgs& g) {
   const int64_t rows = ((int64_t)g.m + 255) / 256 * 256;
-  return rows * std::max(g.ldc * 2, ((int64_t)g.n + 3) / 4 * 4 * (g.silu_mul ? 8 : 4)) < ((int64_t)1 << 32) - 65536 &&
-         (!g.bias || !g.silu_mul || g.bias_dtype == HKX_FP32 || g.n % 2 == 0);
+  return rows * std::max(g.ldc * 2, ((int64_t)g.n + 3) / 4 * 4 * (g.silu_mul ? 8 : 4)) < ((int64_t)1 << 32) - 65536;
 }
 
 // C's rows are 16-byte aligned and N a multiple of 8. (By the row stride where C is not there yet: the

@@ -232,7 +232,7 @@ def _gemm(a, b, sa, sb, bias, silu_mul, out, key):
     g.c = c.data_ptr()  # (the workspace goes by its alignment: a new C's is 16 bytes or more)
     g.m, g.n, g.k, g.silu_mul = m, n, k, 1 if silu_mul else 0
     if bias is not None:
-        g.bias_dtype = nat.dtype_code(bias.dtype)
+        g.bias, g.bias_dtype = bias.data_ptr(), nat.dtype_code(bias.dtype)
     need = nat.lib().hkx_mx4_gemm_workspace(ctypes.byref(g))
     # (a template only where every operand was read where it is, and C is a plain new tensor)
     if key is not None and g.ldc == n and all(

@@ -1,0 +1,66 @@
+"""What hk.ops.mxfp4.gemm passes to the library, without a GPU: its tensors stand on the CPU and say
+they are on one, and the launch is recorded instead of made."""
+
+import ctypes
+import types
+
+import pytest
+import torch
+
+from hk import _native as nat
+from hk.ops import mxfp4
+
+BF16, F16, F32 = torch.bfloat16, torch.float16, torch.float32
+
+
+class OnGpu(torch.Tensor):
+    is_cuda = True
+
+    def get_device(self):
+        return 0
+
+
+def _empty(*size, dtype=torch.uint8):
+    return torch.empty(size, dtype=dtype).as_subclass(OnGpu)
+
+
+@pytest.fixture
+def launches(monkeypatch):
+    """The arguments of each product that would have been launched, as the library's own struct."""
+    real, seen = nat.lib(), []
+
+    def product(ref, _stream):
+        seen.append(nat.HkxMx4GemmArgs.from_buffer_copy(ref._obj))
+        return nat.OK
+
+    monkeypatch.setattr(nat, "lib", lambda: types.SimpleNamespace(
+        hkx_mx4_gemm=product, hkx_mx4_gemm_workspace=real.hkx_mx4_gemm_workspace))
+    monkeypatch.setattr(nat, "stream_of", lambda device: 0)
+    monkeypatch.setattr(nat, "workspace", lambda device, need: types.SimpleNamespace(data_ptr=lambda: 1 << 20))
+    monkeypatch.setattr(mxfp4, "_GEMM", {})
+    return seen
+
+
+def _operands(m, n, k, wide, pair):
+    rows = 2 * n if pair else n
+    a = _empty(m, k, dtype=torch.float8_e4m3fn) if wide else _empty(m, k // 2)
+    return a, _empty(rows, k // 2), _empty(m, k // 32), _empty(rows, k // 32)
+
+
+def _asked(args):
+    """The bytes that the library wants for exactly this launch."""
+    return nat.lib().hkx_mx4_gemm_workspace(ctypes.byref(args))
+
+
+@pytest.mark.parametrize("bias", [None, BF16, F16, F32])
+@pytest.mark.parametrize("pair", [False, True], ids=["plain", "paired"])
+@pytest.mark.parametrize("wide", [False, True], ids=["a4", "a8"])
+@pytest.mark.parametrize("m,n,k", [(129, 8219, 20480), (458, 4131, 15360), (532, 3743, 16384), (136, 11029, 13312),
+                                   (300, 1001, 4096), (1024, 4096, 4096), (2048, 12288, 4096), (4096, 513, 2048)])
+def test_the_workspace_is_what_the_launch_needs(launches, m, n, k, wide, pair, bias):
+    """Also where the plan would go by the bias: odd columns, a paired product, 16-bit bias."""
+    a, b, sa, sb = _operands(m, n, k, wide, pair)
+    bias = None if bias is None else _empty(b.shape[0], dtype=bias)
+    for _ in range(2):  # the first call of the layout, and one that knows it
+        mxfp4.gemm(a, b, sa, sb, bias=bias, silu_mul=pair)
+    assert [_asked(g) for g in launches] == [g.ws_bytes for g in launches], (m, n, k)

@@ -1,0 +1,53 @@
+"""Calls of hk.ops.mxfp4 on the GPU by the way they are made -- outputs given, kept layouts, bias and scale
+forms on each kernel -- against the float64 oracle."""
+
+import ctypes
+
+import pytest
+import torch
+
+from hk import _native as nat
+from hk.ops import mxfp4
+from oracle import mxfp4_oracle as O
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+BF16, F16, F32 = torch.bfloat16, torch.float16, torch.float32
+KERNELS = [nat.MX4_TILE64, nat.MX4_TILE128, nat.MX4_QUAD, nat.MX4_SKINNY]
+
+
+def _gen(*seed):
+    return torch.Generator().manual_seed(hash(seed) % (1 << 31))
+
+
+def _operand(rows, k, wide, g, spread=2):
+    s = torch.randint(127 - spread, 128 + spread, (rows, k // 32), generator=g).to(torch.uint8)
+    if wide:
+        return torch.randn(rows, k, generator=g).to(torch.float8_e4m3fn), s
+    return torch.randint(0, 256, (rows, k // 2), generator=g).to(torch.uint8), s
+
+
+def _operands(m, n, k, wide, pair, *seed):
+    g = _gen(m, n, k, *seed)
+    a, sa = _operand(m, k, wide, g)
+    b, sb = _operand(2 * n if pair else n, k, False, g)
+    return g, a, b, sa, sb - (6 if pair else 0)
+
+
+def _within(c, ref, err):
+    bad = ~((c.cpu().double() - ref).abs() <= err)
+    assert not bad.any(), f"{int(bad.sum())} of {bad.numel()} off, first at {bad.nonzero()[0].tolist()}"
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("wide", [False, True], ids=["a4", "a8"])
+@pytest.mark.parametrize("m,n,k", [(129, 1035, 8224), (300, 1001, 4096), (520, 999, 1056)])
+def test_gemm_silu_mul_of_odd_columns_with_a_bias(m, n, k, wide, dtype):
+    """2N bias values of which the up half starts at an odd element."""
+    print(f"case {m}x{n}x{k} wide={wide} {dtype}", flush=True)
+    g, a, b, sa, sb = _operands(m, n, k, wide, True)
+    bias = torch.randn(2 * n, generator=g).to(dtype)
+    ref, err = O.gemm(a, b, sa, sb, bias, True)
+    dev = [t.to(DEV) for t in (a, b, sa, sb)]
+    for _ in range(2):
+        _within(mxfp4.gemm(*dev, bias=bias.to(DEV), silu_mul=True), ref, err)
