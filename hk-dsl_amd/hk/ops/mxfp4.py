@@ -145,7 +145,7 @@ def gemm(a, b, sa, sb, *, bias=None, silu_mul=False, out=None):
            sb.shape, sb.stride(), sb.dtype, bias is None or (bias.shape, bias.stride(), bias.dtype), silu_mul)
     plan = _GEMM.get(key)
     if plan is None or out is not None:
-        return _gemm(a, b, sa, sb, bias, silu_mul, out, key)
+        return _gemm(a, b, sa, sb, bias, silu_mul, out, key if out is None else None)
     args, need, shape = plan
     pa, pb, ps, pt = a.data_ptr(), b.data_ptr(), sa.data_ptr(), sb.data_ptr()
     d = a.get_device()
@@ -229,13 +229,14 @@ def _gemm(a, b, sa, sb, bias, silu_mul, out, key):
     g.lda, g.ldb = _ld(a, a.shape[1]), _ld(b, k // 2)
     up4 = (k // 32 + 3) // 4 * 4
     g.sa_ld, g.sb_ld, g.ldc = _ld(sa, up4), _ld(sb, up4), _ld(c, n)
-    g.c = c.data_ptr()  # (the workspace goes by its alignment: a new C's is 16 bytes or more)
+    g.c = c.data_ptr()
     g.m, g.n, g.k, g.silu_mul = m, n, k, 1 if silu_mul else 0
     if bias is not None:
         g.bias, g.bias_dtype = bias.data_ptr(), nat.dtype_code(bias.dtype)
     need = nat.lib().hkx_mx4_gemm_workspace(ctypes.byref(g))
-    # (a template only where every operand was read where it is, and C is a plain new tensor)
-    if key is not None and g.ldc == n and all(
+    # (a template only where every operand was read where it is and C is new: the plan and its workspace
+    # go by C's alignment, which a given one has of its own)
+    if key is not None and all(
             x is None or x.data_ptr() == y.data_ptr() for x, y in zip((a, b, sa, sb, bias), given)):
         nat.remember(_GEMM, key, (bytes(g), need, (*lead, n)), 4096)
     _launch(g, need, a, a.data_ptr(), b.data_ptr(), sa.data_ptr(), sb.data_ptr(), bias, c)

@@ -64,3 +64,16 @@ def test_the_workspace_is_what_the_launch_needs(launches, m, n, k, wide, pair, b
     for _ in range(2):  # the first call of the layout, and one that knows it
         mxfp4.gemm(a, b, sa, sb, bias=bias, silu_mul=pair)
     assert [_asked(g) for g in launches] == [g.ws_bytes for g in launches], (m, n, k)
+
+
+@pytest.mark.parametrize("m,n,k", [(1024, 12288, 4096), (2048, 12288, 4096), (4096, 12288, 4096)])
+def test_an_out_leaves_the_layouts_template_alone(launches, m, n, k):
+    """C 8 bytes off 16 takes another plan than a new C: neither's workspace is the other's."""
+    a, b, sa, sb = _operands(m, n, k, False, False)
+    off = _empty(m * n + 4, dtype=BF16)[4:].view(m, n)
+    assert off.data_ptr() % 16 == 8 and off.is_contiguous()
+    for out in (off, None, None, off, None):
+        mxfp4.gemm(a, b, sa, sb, out=out)
+    assert [_asked(g) for g in launches] == [g.ws_bytes for g in launches]
+    assert launches[0].ws_bytes != launches[1].ws_bytes == launches[2].ws_bytes == launches[4].ws_bytes
+    assert launches[0].c % 16 == 8 and launches[1].c % 16 == 0

@@ -51,3 +51,22 @@ def test_gemm_silu_mul_of_odd_columns_with_a_bias(m, n, k, wide, dtype):
     dev = [t.to(DEV) for t in (a, b, sa, sb)]
     for _ in range(2):
         _within(mxfp4.gemm(*dev, bias=bias.to(DEV), silu_mul=True), ref, err)
+
+
+@pytest.mark.parametrize("m,n,k", [(1024, 12288, 4096), (300, 264, 1056)])
+def test_gemm_after_an_out_8_bytes_off(m, n, k):
+    """A contiguous out that is not 16-byte aligned, then calls of the same layout without one."""
+    print(f"case {m}x{n}x{k}", flush=True)
+    g = torch.Generator(device=DEV).manual_seed(n)
+    a, b = (torch.randint(0, 256, (r, k // 2), generator=g, device=DEV, dtype=torch.uint8) for r in (m, n))
+    sa, sb = (torch.randint(127, 129, (r, k // 32), generator=g, device=DEV, dtype=torch.uint8) for r in (m, n))
+    out = torch.empty(m * n + 4, dtype=BF16, device=DEV)[4:].view(m, n)
+    assert out.data_ptr() % 16 == 8
+    given = mxfp4.gemm(a, b, sa, sb, out=out)
+    first, again = mxfp4.gemm(a, b, sa, sb), mxfp4.gemm(a, b, sa, sb)
+    assert given.data_ptr() == out.data_ptr()
+    # (a product of codes is a multiple of 1/4 up to 36, of scales 1 to 4: sums of 4096 are exact in fp32)
+    assert torch.equal(first, out) and torch.equal(first, again)
+    p = slice(0, 40)
+    ref, err = O.gemm(a[p].cpu(), b.cpu(), sa[p].cpu(), sb.cpu())
+    _within(first[p], ref, err)
