@@ -112,7 +112,7 @@ Grad grad_plan(const HkxBlockNormGradArgs& g, bool vec) {
   auto pad = [](size_t n) { return (n + 3) / 4 * 4; };
   q.post = f.post && g.dpost ? pad((size_t)q.workers * f.d) : 0;
   q.pre = f.pre && g.dpre ? pad((size_t)q.workers * f.d) : 0;
-  q.gate = f.gate && g.dgate && f.gate_rows > 1 ? pad((size_t)q.groups * q.parts * (f.gate_col ? f.d : 1)) : 0;
+  q.gate = f.gate && g.dgate && q.parts > 1 ? pad((size_t)q.workers * (f.gate_col ? f.d : 1)) : 0;
   return q;
 }
 
@@ -210,7 +210,7 @@ int hkx_block_norm_backward(const HkxBlockNormGradArgs* args, void* stream) {
   a.ppost = q.post ? ws : nullptr;
   a.ppre = q.pre ? ws + q.post : nullptr;
   a.pgate = q.gate ? ws + q.post + q.pre : nullptr;
-  a.dgate = f.gate && f.gate_rows == 1 ? g.dgate : nullptr;
+  a.dgate = f.gate && q.parts == 1 ? g.dgate : nullptr;
   const hipStream_t s = (hipStream_t)stream;
   const bool r32 = f.r_dtype == HKX_FP32, w32 = (f.post || f.pre) && f.w_dtype == HKX_FP32;
   int rc = api_launched(f.x_dtype == HKX_BF16   ? launch_norm_grad_bf16(a, r32, w32, s)
@@ -228,7 +228,7 @@ int hkx_block_norm_backward(const HkxBlockNormGradArgs* args, void* stream) {
   if (q.post) add(a.ppost, g.dpost, f.w_dtype, q.workers, f.d, 1);
   if (q.pre) add(a.ppre, g.dpre, f.w_dtype, q.workers, f.d, 1);
   if (q.gate) add(a.pgate, g.dgate, f.gate_dtype, q.parts, f.gate_col ? f.d : 1, q.groups);
-  if (groups > 65535) return api_fail(HKX_ERR_SHAPE, "block_norm_backward: %d gates", q.groups);
+  // (no more groups than workers: where there are more, each worker has whole ones)
   hipLaunchKernelGGL(norm_sum_kernel, dim3((width + 63) / 64, groups), dim3(1024), 0, s, j);
   return api_launched(hipGetLastError(), "block norm backward (sums)");
 }

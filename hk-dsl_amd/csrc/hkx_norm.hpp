@@ -53,10 +53,10 @@ struct NormGradArgs {
   const void* dy;    // nullptr: zero
   void* dx;
   void* dr;
-  void* dgate;       // written here where every row has its own (gate_rows 1), else summed from pgate
+  void* dgate;       // written here where a worker has whole groups (parts 1), else summed from pgate
   float* ppost;      // [workers][d] partial sums (nullptr: not wanted), likewise ppre
   float* ppre;
-  float* pgate;      // [groups][parts][d or 1]
+  float* pgate;      // [groups][parts][d or 1] (parts past 1)
   int64_t lddh, lddy, lddx, lddr;
   int32_t workers;
   int32_t parts;     // workers a group of gate_rows rows (groups <= workers), or 1
@@ -372,18 +372,27 @@ __global__ void __launch_bounds__(WAVE ? 256 : TM) norm_grad_kernel(const NormGr
     end = min((worker + 1) * per, p.groups) * rpg;
   }
   const bool own_gate = f.gate && f.gate_rows == 1;  // every row its own: written row by row
+  const bool group_gate = p.pgate || (f.gate && p.dgate && !own_gate);
   auto flush = [&](int grp) {  // the gate's sums of a group (or of this worker's part of it)
-    const int64_t slot = p.parts > 1 ? worker : grp;
     if (f.gate_col) {
-      store_sum(2, p.pgate, slot * f.d);
+      if (p.pgate) {
+        store_sum(2, p.pgate, (int64_t)worker * f.d);
+      } else {
+        Row o;
+#pragma unroll
+        for (int i = 0; i < E; ++i) o.v[i] = sum(2, i);
+        if (f.gate_dt == XT) cols.template store<XT>(p.dgate, (int64_t)grp * f.d, o);
+        else cols.template store<HKX_FP32>(p.dgate, (int64_t)grp * f.d, o);
+      }
     } else if (cols.t == 0) {
-      p.pgate[slot] = ags;
+      if (p.pgate) p.pgate[worker] = ags;
+      else store_one(p.dgate, f.gate_dt, grp, ags);
     }
 #pragma unroll
     for (int i = 0; i < E; ++i) sum(2, i) = 0.0f;
     ags = 0.0f;
   };
-  if (p.pgate && row >= end && p.parts > 1) flush(0);  // an empty part: zeros
+  if (p.pgate && row >= end) flush(0);  // an empty part: zeros
   int held = -1;  // the group whose gate is in g
   for (; row < end; ++row) {
     Row x = cols.template load<XT>(f.x, row * f.ldx);
@@ -444,7 +453,7 @@ __global__ void __launch_bounds__(WAVE ? 256 : TM) norm_grad_kernel(const NormGr
       for (int i = 0; i < E; ++i) dh.v[i] = rx * (dh.v[i] - x.v[i] * s2);
     }
     cols.template store<XT>(p.dx, row * p.lddx, dh);
-    if (p.pgate && (row + 1 == end || (row + 1) % rpg == 0)) flush(row / rpg);
+    if (group_gate && (row + 1 == end || (row + 1) % rpg == 0)) flush(row / rpg);
     if (!WAVE) __syncthreads();  // (the sums' slots are free for the next row)
   }
   if (p.ppost) store_sum(0, p.ppost, (int64_t)worker * f.d);
