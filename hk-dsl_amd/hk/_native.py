@@ -251,7 +251,10 @@ def remember(store: dict, key, value, cap: int) -> None:
     store[key] = value
 
 
+#: The main thread's workspaces; other threads' are attributes of _WS_OF_THREAD, which end with their thread.
 _WS: dict = {}
+_WS_OF_THREAD = threading.local()
+_MAIN_THREAD = threading.main_thread().ident
 
 
 def capturing(device) -> bool:
@@ -262,9 +265,11 @@ def capturing(device) -> bool:
 
 
 def workspace(device, nbytes: int):
-    """A cached fp32 workspace of at least `nbytes` for (device, current stream): the
-    reference's module-owned scratch (python/hk/ops/gemm_cdna_dp.py:330-338). Calls on
-    one stream run in order, so they can share it.
+    """A cached fp32 workspace of at least `nbytes` for (device, current stream) and the calling
+    thread: the reference's module-owned scratch (python/hk/ops/gemm_cdna_dp.py:330-338). A
+    thread's calls on one stream run in order, so they can share it. Two threads' on one stream do
+    not: a call may be several launches over its workspace, and the library runs without the GIL, so
+    that another thread's launches can come between them.
 
     Under CUDA-graph capture a graph bakes the buffer's address in, so a captured call gets
     a buffer of its own, allocated in the capture -- i.e. from the graph's private memory
@@ -283,10 +288,11 @@ def workspace(device, nbytes: int):
     if capturing(device):
         return torch.empty((nbytes + 3) // 4, dtype=torch.float32, device=device)
     key = (device, stream_of(device))
-    buf = _WS.get(key)
+    kept = _WS if threading.get_ident() == _MAIN_THREAD else _WS_OF_THREAD.__dict__
+    buf = kept.get(key)
     if buf is None or buf.numel() * 4 < nbytes:
         buf = torch.empty((nbytes + 3) // 4, dtype=torch.float32, device=device)
-        _WS[key] = buf
+        kept[key] = buf
     return buf
 
 

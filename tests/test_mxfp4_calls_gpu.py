@@ -70,3 +70,32 @@ def test_gemm_after_an_out_8_bytes_off(m, n, k):
     p = slice(0, 40)
     ref, err = O.gemm(a[p].cpu(), b.cpu(), sa[p].cpu(), sb.cpu())
     _within(first[p], ref, err)
+
+
+@pytest.mark.parametrize("shapes", [((512, 4096, 4096), (768, 2048, 8192)), ((1024, 1001, 2048), (300, 512, 8192))])
+def test_threads_on_one_stream(shapes):
+    """Calls of several launches (packed scales, a split's shares) by two threads at a time."""
+    import threading
+
+    g = torch.Generator(device=DEV).manual_seed(3)
+    cases = []
+    for m, n, k in shapes:
+        a, b = (torch.randint(0, 256, (r, k // 2), generator=g, device=DEV, dtype=torch.uint8) for r in (m, n))
+        sa, sb = (torch.randint(125, 130, (r, k // 32), generator=g, device=DEV, dtype=torch.uint8) for r in (m, n))
+        cases.append((a, b, sa, sb))
+    want = [mxfp4.gemm(*c) for c in cases]
+    torch.cuda.synchronize()
+    got = [[], []]
+
+    def work(i):
+        for _ in range(40):
+            got[i].append(mxfp4.gemm(*cases[i]))
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert len(got[i]) == 40 and all(torch.equal(want[i], c) for c in got[i])
