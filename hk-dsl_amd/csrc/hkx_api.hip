@@ -950,8 +950,8 @@ int hkx_mx_gemm(const void* a, int64_t lda, const void* b, int64_t ldb, const ui
   return launched(hkx::launch_reduce(r, none, false, rg, s), "mx GEMM (sum of the splits)");
 }
 
-int hkx_mx_quant(const void* x, int64_t ldx, void* q, int64_t ldq, uint8_t* s, int64_t lds,
-                 int32_t m, int32_t k, void* stream) {
+static int mx_quant(const void* x, int64_t ldx, void* q, int64_t ldq, uint8_t* s, int64_t lds,
+                    int32_t m, int32_t k, bool nans, void* stream) {
   g_err.clear();
   if (!x || !q || !s) return fail(HKX_ERR_ARG, "mx_quant: a null pointer");
   if (m < 0 || k < 0 || k % 32) return fail(HKX_ERR_SHAPE, "mx_quant: K=%d, a multiple of 32", k);
@@ -959,8 +959,18 @@ int hkx_mx_quant(const void* x, int64_t ldx, void* q, int64_t ldq, uint8_t* s, i
   if (!aligned(x, 16) || ldx % 8 || !aligned(q, 8) || ldq % 8)
     return fail(HKX_ERR_SHAPE, "mx_quant: x needs 16-byte and q 8-byte aligned rows");
   if (m == 0 || k == 0) return HKX_OK;
-  return launched(hkx::launch_mx_quant(x, ldx, q, ldq, s, lds, m, k, (hipStream_t)stream),
+  return launched(hkx::launch_mx_quant(x, ldx, q, ldq, s, lds, m, k, nans, (hipStream_t)stream),
                   "mx quant");
+}
+
+int hkx_mx_quant(const void* x, int64_t ldx, void* q, int64_t ldq, uint8_t* s, int64_t lds,
+                 int32_t m, int32_t k, void* stream) {
+  return mx_quant(x, ldx, q, ldq, s, lds, m, k, false, stream);
+}
+
+int hkx_mx_quant_nan(const void* x, int64_t ldx, void* q, int64_t ldq, uint8_t* s, int64_t lds,
+                     int32_t m, int32_t k, void* stream) {
+  return mx_quant(x, ldx, q, ldq, s, lds, m, k, true, stream);
 }
 
 int hkx_scaled_mm(const void* a, int64_t lda, const void* b, int64_t ldb, const float* scale_a,

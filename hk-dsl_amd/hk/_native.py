@@ -109,7 +109,7 @@ class HkxBlockNormGradArgs(Structure):
 SYMBOLS = ("hkx_abi_version", "hkx_abi_sizes", "hkx_last_error", "hkx_gemm_workspace",
            "hkx_gemm_counters",
            "hkx_gemm_check", "hkx_gemm", "hkx_scaled_mm", "hkx_mx_gemm", "hkx_mx_gemm_workspace",
-           "hkx_mx_quant", "hkx_gemm_noalloc", "hkx_mx4_quant", "hkx_mx_dequant", "hkx_mx4_gemm",
+           "hkx_mx_quant", "hkx_mx_quant_nan", "hkx_gemm_noalloc", "hkx_mx4_quant", "hkx_mx_dequant", "hkx_mx4_gemm",
            "hkx_mx4_gemm_workspace", "hkx_block_norm", "hkx_block_norm_backward",
            "hkx_block_norm_backward_workspace")
 
@@ -158,8 +158,9 @@ def lib() -> ctypes.CDLL:
                                   c_int32, c_void_p, c_size_t, c_void_p]
         L.hkx_mx_gemm_workspace.argtypes = [c_int32, c_int32, c_int32]
         L.hkx_mx_gemm_workspace.restype = c_size_t
-        L.hkx_mx_quant.argtypes = [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64,
-                                   c_int32, c_int32, c_void_p]
+        for quant in (L.hkx_mx_quant, L.hkx_mx_quant_nan):
+            quant.argtypes = [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64,
+                              c_int32, c_int32, c_void_p]
         L.hkx_scaled_mm.argtypes = [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64,
                                     c_void_p, c_int32, c_void_p, c_void_p, c_int64, c_int32,
                                     c_int32, c_int32, c_void_p, c_size_t, c_void_p]

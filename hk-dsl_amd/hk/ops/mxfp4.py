@@ -245,10 +245,11 @@ def _gemm(a, b, sa, sb, bias, silu_mul, out, key):
 
 def linear(x, w, ws, *, bias=None, silu_mul=False, act="mxfp8"):
     """x (M, K) @ (ws . w)^T, w packed codes (N, K/2) with scales ws: the activation quantized to
-    `act` ("mxfp8": bf16 x; "mxfp4": bf16, fp16 or fp32), then `gemm`."""
+    `act` ("mxfp8": bf16 x; "mxfp4": bf16, fp16 or fp32), then `gemm`. A row of x with an infinity or a
+    NaN gives a row of NaN."""
     if act not in ("mxfp8", "mxfp4"):
         raise ValueError(f"mxfp4.linear: act is 'mxfp8' or 'mxfp4', got {act!r}")
-    xq, xs = _quant8(x) if act == "mxfp8" else quant(x)
+    xq, xs = _quant8(x, nan_blocks=True) if act == "mxfp8" else quant(x)
     return gemm(xq, w, xs, ws, bias=bias, silu_mul=silu_mul)
 
 

@@ -96,9 +96,11 @@ def gemm(a, b, sa, sb, out=None):
     return out
 
 
-def quant(x, out=None):
+def quant(x, out=None, *, nan_blocks=False):
     """(q, s) for bf16 x [M, K], K a multiple of 32: q float8_e4m3fn [M, K], s uint8
-    [M, K/32] (OCP layout), by AITER's per_1x32 rule."""
+    [M, K/32] (OCP layout), by AITER's per_1x32 rule, which makes an infinity or a NaN
+    +-448. `nan_blocks`: its block is NaN instead (scale 255, codes 0), as in
+    `hk.ops.mxfp4.quant` and `hk.ops.block_norm`."""
     import torch  # noqa: PLC0415
 
     if x.dtype != torch.bfloat16 or x.dim() != 2:
@@ -119,9 +121,9 @@ def quant(x, out=None):
         s = x.new_empty((m, k // 32), dtype=torch.uint8)
     else:
         q, s = nat.empty(x, (m, k), torch.float8_e4m3fn), nat.empty(x, (m, k // 32), torch.uint8)
-    nat.check(nat.lib().hkx_mx_quant(x.data_ptr(), x.stride(0), q.data_ptr(), q.stride(0),
-                                     s.data_ptr(), s.stride(0), m, k,
-                                     nat.stream_of(x.device)))
+    f = nat.lib().hkx_mx_quant_nan if nan_blocks else nat.lib().hkx_mx_quant
+    nat.check(f(x.data_ptr(), x.stride(0), q.data_ptr(), q.stride(0), s.data_ptr(), s.stride(0),
+                m, k, nat.stream_of(x.device)))
     return q, s
 
 

@@ -316,6 +316,11 @@ size_t hkx_mx_gemm_workspace(int32_t m, int32_t n, int32_t k);
 int hkx_mx_quant(const void* x, int64_t ldx, void* q, int64_t ldq, uint8_t* s, int64_t lds,
                  int32_t m, int32_t k, void* stream);
 
+/* The same, but for a block with an infinity or a NaN: s = 255 (E8M0's NaN) and codes 0, as
+ * hkx_mx4_quant's and hkx_block_norm's. (hkx_mx_quant makes them +-448.) */
+int hkx_mx_quant_nan(const void* x, int64_t ldx, void* q, int64_t ldq, uint8_t* s, int64_t lds,
+                     int32_t m, int32_t k, void* stream);
+
 /* ---------------------------------------------------------------- MXFP4, and the block norm */
 
 /* x (M, K) of x_dtype (bf16, fp16, fp32) -> q (M, K/2 bytes) packed e2m1 and s (M, K/32) E8M0

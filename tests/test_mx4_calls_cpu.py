@@ -77,3 +77,14 @@ def test_an_out_leaves_the_layouts_template_alone(launches, m, n, k):
     assert [_asked(g) for g in launches] == [g.ws_bytes for g in launches]
     assert launches[0].ws_bytes != launches[1].ws_bytes == launches[2].ws_bytes == launches[4].ws_bytes
     assert launches[0].c % 16 == 8 and launches[1].c % 16 == 0
+
+
+@pytest.mark.parametrize("args,code,says", [
+    ((None, 64, 1 << 20, 64, 1 << 20, 2, 4, 64), nat.ERR_ARG, "null"),
+    ((1 << 20, 64, 1 << 20, 64, 1 << 20, 2, 4, 40), nat.ERR_SHAPE, "multiple of 32"),
+    ((1 << 20, 64, 1 << 20, 32, 1 << 20, 2, 4, 64), nat.ERR_SHAPE, "row strides"),
+    (((1 << 20) + 2, 64, 1 << 20, 64, 1 << 20, 2, 4, 64), nat.ERR_SHAPE, "aligned"),
+])
+def test_both_mxfp8_quantizations_refuse_the_same(args, code, says):
+    for f in (nat.lib().hkx_mx_quant, nat.lib().hkx_mx_quant_nan):
+        assert f(*args, None) == code and says in nat.last_error(), nat.last_error()

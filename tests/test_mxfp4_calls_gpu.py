@@ -7,7 +7,7 @@ import pytest
 import torch
 
 from hk import _native as nat
-from hk.ops import mxfp4
+from hk.ops import mxfp4, mxfp8
 from oracle import mxfp4_oracle as O
 
 pytestmark = pytest.mark.gpu
@@ -99,3 +99,32 @@ def test_threads_on_one_stream(shapes):
     torch.cuda.synchronize()
     for i in range(2):
         assert len(got[i]) == 40 and all(torch.equal(want[i], c) for c in got[i])
+
+
+@pytest.mark.parametrize("act", ["mxfp8", "mxfp4"])
+@pytest.mark.parametrize("m", [5, 700])
+def test_linear_of_a_row_that_is_not_finite_is_nan(m, act):
+    """On either path of the activation, and the other rows as without it; block_norm's quantized y, which
+    linear's activation stands for, is NaN there too."""
+    g = _gen(m, 12)
+    x = torch.randn(m, 512, generator=g).to(BF16)
+    w, ws = mxfp4.quant((torch.randn(96, 512, generator=g) * 0.05).to(DEV))
+    clean = mxfp4.linear(x.to(DEV), w, ws, act=act).cpu()
+    bad = {0: float("nan"), 2: float("inf"), m - 1: float("-inf")}
+    for row, v in bad.items():
+        x[row, 37 * (row % 13)] = v
+    y = mxfp4.linear(x.to(DEV), w, ws, act=act).cpu()
+    rows = torch.tensor(sorted(bad))
+    assert torch.isnan(y[rows]).all()
+    rest = torch.tensor([r for r in range(m) if r not in bad])
+    assert torch.equal(y[rest], clean[rest])
+    if act == "mxfp8":
+        q, s = mxfp8.quant(x.to(DEV), nan_blocks=True)
+        block = torch.zeros(m, 16, dtype=torch.bool)
+        for row in bad:
+            block[row, 37 * (row % 13) // 32] = True
+        assert torch.equal(s.cpu() == 255, block)
+        assert not q.cpu().view(torch.uint8).view(m, 16, 32)[block].any()
+        q0, s0 = mxfp8.quant(x.to(DEV))  # (the other blocks are that rule's, and it leaves no NaN)
+        assert torch.equal(q.cpu().view(torch.uint8).view(m, 16, 32)[~block], q0.cpu().view(torch.uint8).view(m, 16, 32)[~block])
+        assert torch.equal(s.cpu()[~block], s0.cpu()[~block]) and (s0 < 255).all()
