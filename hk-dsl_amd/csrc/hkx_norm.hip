@@ -88,6 +88,7 @@ int forward_args(const HkxBlockNormArgs& g, const char* what, NormArgs& a) {
   a.bs = g.branch_scale;
   a.rs = g.residual_scale;
   a.eps = g.eps;
+  a.inv_d = 1.0 / g.d;
   return HKX_OK;
 }
 

@@ -38,6 +38,7 @@ struct NormArgs {
   int32_t gate_col;   // 1: a gate a column, 0: one a row
   int32_t quant;      // 0: y as x's type, 1: MXFP8, 2: MXFP4
   float bs, rs, eps;
+  double inv_d;  // 1 / d
 };
 
 // The elements a thread (8 c, in pieces of 8 where vec), and the row's threads (64: a wave a row, else
@@ -186,6 +187,16 @@ HKX_DEV float row_sum(float x, float* red) {
   return x;
 }
 
+// A norm's factor 1 / sqrt(sum / d + eps), rounded once. v_rsq_f32 alone is up to 0.72 of a step off, for every
+// value of the row alike, and takes a subnormal mean for 0. A Newton step leaves 3/2 of the square of
+// v_rsq_f64's error (some 2^-26); of a mean of 0 or infinity the step is NaN and the seed is exact.
+HKX_DEV float row_factor(float sum, const NormArgs& p) {
+  const double m = (double)sum * p.inv_d + (double)p.eps;
+  const double y = __builtin_amdgcn_rsq(m);
+  const double e = __builtin_fma(-m * y, y, 1.0);
+  return (float)(e == e ? __builtin_fma(0.5 * e, y, y) : y);
+}
+
 // ---------------------------------------------------------------- quantized stores (whole quads of 8-value pieces)
 
 template <int CTRL>
@@ -264,13 +275,12 @@ __global__ void __launch_bounds__(WAVE ? 256 : 1024) norm_kernel(const NormArgs 
   if (p.post) w1 = cols.template load<WT>(p.post, 0);
   if (p.pre) w2 = cols.template load<WT>(p.pre, 0);
   if (p.gate) g = load_gate<XT>(p, cols, row);
-  const float inv_d = 1.0f / (float)p.d;
   float rx = 1.0f;
   if (p.post) {
     float s = 0.0f;
 #pragma unroll
     for (int i = 0; i < E; ++i) s += x.v[i] * x.v[i];
-    rx = __builtin_amdgcn_rsqf(row_sum<WAVE>(s, red[0]) * inv_d + p.eps);
+    rx = row_factor(row_sum<WAVE>(s, red[0]), p);
 #pragma unroll
     for (int i = 0; i < E; ++i) x.v[i] *= rx * w1.v[i];
   }
@@ -286,7 +296,7 @@ __global__ void __launch_bounds__(WAVE ? 256 : 1024) norm_kernel(const NormArgs 
     float s = 0.0f;
 #pragma unroll
     for (int i = 0; i < E; ++i) s += r.v[i] * r.v[i];
-    rh = __builtin_amdgcn_rsqf(row_sum<WAVE>(s, red[1]) * inv_d + p.eps);
+    rh = row_factor(row_sum<WAVE>(s, red[1]), p);
 #pragma unroll
     for (int i = 0; i < E; ++i) r.v[i] *= rh * w2.v[i];
     if (VEC && p.quant) {

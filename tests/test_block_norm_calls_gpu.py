@@ -23,3 +23,35 @@ def test_gradients_of_more_gates_than_workers(shape, one, gate_dtype):
     if one:
         a["gate"] = a["gate"][..., :1].clone()
     T._check_grads(a, 22, **T.SCALES)
+
+
+@pytest.mark.parametrize("exponent", [0, -70, 40])
+@pytest.mark.parametrize("d", [64, 333, 1000, 4096, 16384])
+def test_a_norms_factor_is_rounded_once(d, exponent):
+    """Rows of small whole numbers (times 2^exponent: squares that are subnormal, or large), whose sums of
+    squares fp32 holds exactly in any order: 1 / sqrt(sum / d) of 64 bits to half a step of fp32, and 2^-20
+    of one."""
+    from hk.ops import norm
+
+    g = torch.Generator().manual_seed(d)
+    rows = 2000
+    x = torch.randint(-9, 10, (rows, d), generator=g).float()
+    x *= (torch.arange(rows) % 3 + 1)[:, None]  # (27^2 16384 < 2^24)
+    x[:, 0] = 1 + torch.arange(rows) % 7        # (no row of zeros)
+    exact = (x.double().square().sum(-1) / d).rsqrt() * 2.0 ** -exponent
+    x = torch.ldexp(x, torch.tensor(exponent)).to(DEV)
+    step = torch.exp2(torch.floor(torch.log2(exact)) - 23)
+    w, zero = torch.ones(d, device=DEV), torch.zeros_like(x)
+    # after the block (a backward pass is to follow, so the factors are kept; D to 8192 there), and before
+    # the next: with no norm after the block h is x
+    for post, pre, at in ((w, None, 0), (None, w, 1)):
+        (_, _, rstd), *_ = norm._forward(x, zero, post, pre, None, (1.0, 1.0, 0.0), None, True)
+        off = (rstd[:, at].cpu().double() - exact).abs() / step
+        assert (off <= 0.5 + 2.0 ** -20).all(), f"{float(off.max()):.4f} of a step"
+
+
+def test_a_norm_of_zeros_without_eps_is_nan_and_of_infinity_zero():
+    x = torch.zeros(3, 64, device=DEV)
+    x[1], x[2] = 1e30, 1.0  # (squares past fp32)
+    h, _ = hk.ops.block_norm(x, torch.zeros_like(x), post=torch.ones(64, device=DEV), eps=0.0)
+    assert torch.isnan(h[0]).all() and (h[1] == 0).all() and (h[2] == 1).all()
