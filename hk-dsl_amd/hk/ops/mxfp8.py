@@ -121,6 +121,8 @@ def quant(x, out=None, *, nan_blocks=False):
         s = x.new_empty((m, k // 32), dtype=torch.uint8)
     else:
         q, s = nat.empty(x, (m, k), torch.float8_e4m3fn), nat.empty(x, (m, k // 32), torch.uint8)
+    if m == 0:  # (an empty tensor has no address)
+        return q, s
     f = nat.lib().hkx_mx_quant_nan if nan_blocks else nat.lib().hkx_mx_quant
     nat.check(f(x.data_ptr(), x.stride(0), q.data_ptr(), q.stride(0), s.data_ptr(), s.stride(0),
                 m, k, nat.stream_of(x.device)))

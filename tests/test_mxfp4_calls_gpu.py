@@ -128,3 +128,12 @@ def test_linear_of_a_row_that_is_not_finite_is_nan(m, act):
         q0, s0 = mxfp8.quant(x.to(DEV))  # (the other blocks are that rule's, and it leaves no NaN)
         assert torch.equal(q.cpu().view(torch.uint8).view(m, 16, 32)[~block], q0.cpu().view(torch.uint8).view(m, 16, 32)[~block])
         assert torch.equal(s.cpu()[~block], s0.cpu()[~block]) and (s0 < 255).all()
+
+
+@pytest.mark.parametrize("act", ["mxfp8", "mxfp4"])
+def test_linear_of_no_rows(act):
+    w, ws = mxfp4.quant(torch.randn(24, 416, generator=_gen(16)).to(DEV))
+    x = torch.empty(0, 416, dtype=BF16, device=DEV)
+    assert mxfp4.linear(x, w, ws, act=act).shape == (0, 24)
+    q, s = mxfp8.quant(x)
+    assert q.shape == (0, 416) and s.shape == (0, 13)
