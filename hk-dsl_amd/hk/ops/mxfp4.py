@@ -64,13 +64,23 @@ def _ld(t, least):
     return t.stride(0) if t.shape[0] > 1 else least
 
 
-#: What quant knows of a layout of x: (M, K, x's type code, x's row stride, the scales' row stride).
+#: What quant knows of a layout of x: (rows, K, x's type code, x's row stride, the scales' row stride, the
+#: shapes of q and s, s's strides).
 _QUANT: dict = {}
 
 
+def _padded(lead, n):
+    """(shape, strides) of scales (*lead, n) with rows of whole dwords."""
+    strides, step = [1], (n + 3) // 4 * 4
+    for size in reversed(lead):
+        strides.insert(0, step)
+        step *= size
+    return (*lead, n), tuple(strides)
+
+
 def quant(x, out=None):
-    """(q, s) for x (M, K) bf16, fp16 or fp32, K a multiple of 32: q uint8 (M, K/2) of packed codes, s
-    uint8 (M, K/32). A block's scale is 2^ceil(log2(amax / 6)) (nothing is clamped), its codes x over
+    """(q, s) for x (..., K) bf16, fp16 or fp32, K a multiple of 32: q uint8 (..., K/2) of packed codes, s
+    uint8 (..., K/32). A block's scale is 2^ceil(log2(amax / 6)) (nothing is clamped), its codes x over
     that rounded to the nearest, ties to even; a block with an infinity or a NaN is NaN (scale 255).
     `out`: (q, s) to write into."""
     key = (x.shape, x.stride(), x.dtype)
@@ -79,13 +89,13 @@ def quant(x, out=None):
         return _quant(x, out, key)
     import torch  # noqa: PLC0415
 
-    m, k, code, ldx, lds = plan
+    m, k, code, ldx, lds, q_shape, s_shape, s_strides = plan
     if type(x) is torch.Tensor:
-        q = x.new_empty((m, k >> 1), dtype=torch.uint8)
-        s = x.new_empty_strided((m, k >> 5), (lds, 1), dtype=torch.uint8)
+        q = x.new_empty(q_shape, dtype=torch.uint8)
+        s = x.new_empty_strided(s_shape, s_strides, dtype=torch.uint8)
     else:
-        q = nat.empty(x, (m, k >> 1), torch.uint8)
-        s = torch.empty_strided((m, k >> 5), (lds, 1), dtype=torch.uint8, device=x.device)
+        q = nat.empty(x, q_shape, torch.uint8)
+        s = torch.empty_strided(s_shape, s_strides, dtype=torch.uint8, device=x.device)
     nat.check(nat.lib().hkx_mx4_quant(x.data_ptr(), ldx, code, q.data_ptr(), k >> 1, s.data_ptr(), lds,
                                       m, k, nat.stream_of(x.device)))
     return q, s
@@ -94,32 +104,43 @@ def quant(x, out=None):
 def _quant(x, out, key):
     import torch  # noqa: PLC0415
 
-    if x.dtype not in (torch.bfloat16, torch.float16, torch.float32) or x.dim() != 2:
-        raise TypeError(f"mxfp4.quant: x is bf16, fp16 or fp32 (M, K), got {x.dtype} {tuple(x.shape)}")
-    m, k = x.shape
+    if x.dtype not in (torch.bfloat16, torch.float16, torch.float32) or x.dim() < 1:
+        raise TypeError(f"mxfp4.quant: x is bf16, fp16 or fp32 (..., K), got {x.dtype} {tuple(x.shape)}")
+    lead, k = tuple(x.shape[:-1]), x.shape[-1]
     if k % 32 or k == 0:
         raise ValueError(f"mxfp4.quant: K={k}, a multiple of 32")
     if not x.is_cuda:
         raise ValueError(f"mxfp4.quant: x is on a GPU, got {x.device}")
+    m, given = x.numel() // k, x
+    if x.dim() != 2:
+        x = x.reshape(m, k)
     per, ldx = 16 // x.element_size(), _ld(x, k)
+    q_shape, (s_shape, s_strides) = (*lead, k // 2), _padded(lead, k // 32)
+    lds = (k // 32 + 3) // 4 * 4
     if x.stride(1) != 1 or ldx % per or ldx < k or x.data_ptr() % 16:
         x, ldx = x.clone(memory_format=torch.contiguous_format), k
-    elif m:
-        nat.remember(_QUANT, key, (m, k, nat.dtype_code(x.dtype), ldx, (k // 32 + 3) // 4 * 4), 4096)
+    elif m and x.data_ptr() == given.data_ptr():
+        nat.remember(_QUANT, key, (m, k, nat.dtype_code(x.dtype), ldx, lds, q_shape, s_shape, s_strides), 4096)
     if out is not None:
         q, s = out
         q = _packed(q, "mxfp4.quant", "out")
-        ldq, lds = _ld(q, k // 2), _ld(s, k // 32)
-        if (tuple(q.shape) != (m, k // 2) or tuple(s.shape) != (m, k // 32) or s.dtype != torch.uint8
-                or q.stride(1) != 1 or s.stride(1) != 1 or ldq % 4 or q.data_ptr() % 4
-                or ldq < k // 2 or lds < k // 32):
-            raise ValueError(f"mxfp4.quant: out is uint8 ({m}, {k // 2}) with 4-byte aligned rows and "
-                             f"uint8 ({m}, {k // 32})")
         _on(x.device, "mxfp4.quant", q=q, s=s)
+        ok = tuple(q.shape) == q_shape and tuple(s.shape) == s_shape and s.dtype == torch.uint8
+        if ok:
+            try:
+                q2, s2 = q.view(m, k // 2), s.view(m, k // 32)
+            except RuntimeError:  # leading sizes that are no rows of one stride
+                ok = False
+            else:
+                ldq, lds = _ld(q2, k // 2), _ld(s2, k // 32)
+                ok = not (q2.stride(1) != 1 or s2.stride(1) != 1 or ldq % 4 or q.data_ptr() % 4
+                          or ldq < k // 2 or lds < k // 32)
+        if not ok:
+            raise ValueError(f"mxfp4.quant: out is uint8 {q_shape} with 4-byte aligned rows and uint8 {s_shape}")
     else:
-        ldq, lds = k // 2, (k // 32 + 3) // 4 * 4
-        q = nat.empty(x, (m, k // 2), torch.uint8)
-        s = torch.empty_strided((m, k // 32), (lds, 1), dtype=torch.uint8, device=x.device)
+        ldq = k // 2
+        q = nat.empty(x, q_shape, torch.uint8)
+        s = torch.empty_strided(s_shape, s_strides, dtype=torch.uint8, device=x.device)
     if m:
         nat.check(nat.lib().hkx_mx4_quant(x.data_ptr(), ldx, nat.dtype_code(x.dtype), q.data_ptr(), ldq,
                                           s.data_ptr(), lds, m, k, nat.stream_of(x.device)))
@@ -244,13 +265,23 @@ def _gemm(a, b, sa, sb, bias, silu_mul, out, key):
 
 
 def linear(x, w, ws, *, bias=None, silu_mul=False, act="mxfp8"):
-    """x (M, K) @ (ws . w)^T, w packed codes (N, K/2) with scales ws: the activation quantized to
+    """x (..., K) @ (ws . w)^T, w packed codes (N, K/2) with scales ws: the activation quantized to
     `act` ("mxfp8": bf16 x; "mxfp4": bf16, fp16 or fp32), then `gemm`. A row of x with an infinity or a
     NaN gives a row of NaN."""
     if act not in ("mxfp8", "mxfp4"):
         raise ValueError(f"mxfp4.linear: act is 'mxfp8' or 'mxfp4', got {act!r}")
-    xq, xs = _quant8(x, nan_blocks=True) if act == "mxfp8" else quant(x)
-    return gemm(xq, w, xs, ws, bias=bias, silu_mul=silu_mul)
+    if act == "mxfp4":
+        xq, xs = quant(x)
+        return gemm(xq, w, xs, ws, bias=bias, silu_mul=silu_mul)
+    lead = None
+    if x.dim() != 2:
+        if x.dim() < 1:
+            raise ValueError("mxfp4.linear: x is (..., K), got a single value")
+        lead, k = x.shape[:-1], x.shape[-1]
+        x = x.reshape(lead.numel(), k)
+    xq, xs = _quant8(x, nan_blocks=True)
+    y = gemm(xq, w, xs, ws, bias=bias, silu_mul=silu_mul)
+    return y if lead is None else y.view(*lead, y.shape[1])
 
 
 __all__ = ["quant", "dequant", "gemm", "linear"]

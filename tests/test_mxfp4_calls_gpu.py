@@ -130,6 +130,56 @@ def test_linear_of_a_row_that_is_not_finite_is_nan(m, act):
         assert torch.equal(s.cpu()[~block], s0.cpu()[~block]) and (s0 < 255).all()
 
 
+@pytest.mark.parametrize("lead", [(), (1,), (30,), (2, 3, 5), (0,), (4, 0, 2)])
+def test_quant_and_linear_of_any_leading_sizes(lead):
+    g = _gen(len(lead), 13)
+    rows = torch.Size(lead).numel()
+    x = torch.randn(*lead, 416, generator=g).to(BF16).to(DEV)
+    flat = x.reshape(rows, 416)
+    w, ws = mxfp4.quant((torch.randn(24, 416, generator=g) * 0.05).to(DEV))
+    bias = torch.randn(24, generator=g).to(BF16).to(DEV)
+    q0, s0 = mxfp4.quant(flat)
+    for _ in range(2):  # the first call of a layout, and one that knows it
+        q, s = mxfp4.quant(x)
+        assert q.shape == (*lead, 208) and s.shape == (*lead, 13)
+        assert torch.equal(q.reshape(rows, 208), q0) and torch.equal(s.reshape(rows, 13), s0)
+        for act in ("mxfp8", "mxfp4"):
+            y = mxfp4.linear(x, w, ws, bias=bias, act=act)
+            assert y.shape == (*lead, 24) and y.dtype == BF16
+            assert torch.equal(y.reshape(rows, 24), mxfp4.linear(flat, w, ws, bias=bias, act=act))
+    y = mxfp4.linear(x, w, ws, silu_mul=True)
+    assert y.shape == (*lead, 12)
+    out = (torch.empty(*lead, 208, dtype=torch.uint8, device=DEV), torch.empty(*lead, 13, dtype=torch.uint8, device=DEV))
+    mxfp4.quant(x, out=out)
+    assert torch.equal(out[0].reshape(rows, 208), q0) and torch.equal(out[1].reshape(rows, 13), s0)
+
+
+def test_quant_of_leading_sizes_of_any_strides():
+    x = torch.randn(6, 5, 96, generator=_gen(14)).to(BF16).to(DEV)
+    q0, s0 = mxfp4.quant(x.reshape(30, 96))
+    w, ws = mxfp4.quant(torch.randn(8, 96, generator=_gen(15)).to(DEV))
+    for v in (x.transpose(0, 1), x[::2], x[:, 1:4], x[..., :64], x.new_empty(6, 5, 104)[..., 3:99].copy_(x)):
+        flat = v.reshape(-1, v.shape[-1]).contiguous()
+        for _ in range(2):
+            q, s = mxfp4.quant(v)
+            qf, sf = mxfp4.quant(flat)
+            assert torch.equal(q.reshape(qf.shape), qf) and torch.equal(s.reshape(sf.shape), sf)
+        k = v.shape[-1]
+        for act in ("mxfp8", "mxfp4"):
+            y = mxfp4.linear(v, w[:, :k // 2], ws[:, :k // 32], act=act)
+            assert torch.equal(y.reshape(-1, 8), mxfp4.linear(flat, w[:, :k // 2].clone(), ws[:, :k // 32].clone(), act=act))
+    wide = torch.zeros(5, 6, 64, dtype=torch.uint8, device=DEV)
+    with pytest.raises(ValueError):  # (rows of two strides)
+        mxfp4.quant(x, out=(wide.transpose(0, 1)[..., :48], torch.empty(6, 5, 3, dtype=torch.uint8, device=DEV)))
+    q, s = wide.view(6, 5, 64)[..., :48], torch.empty(6, 5, 3, dtype=torch.uint8, device=DEV)
+    mxfp4.quant(x, out=(q, s))
+    assert torch.equal(q.reshape(30, 48), q0) and torch.equal(s.reshape(30, 3), s0)
+    with pytest.raises(TypeError):
+        mxfp4.quant(x[0, 0, 0])
+    with pytest.raises(ValueError):
+        mxfp4.linear(x[0, 0, 0], w, ws)
+
+
 @pytest.mark.parametrize("act", ["mxfp8", "mxfp4"])
 def test_linear_of_no_rows(act):
     w, ws = mxfp4.quant(torch.randn(24, 416, generator=_gen(16)).to(DEV))
