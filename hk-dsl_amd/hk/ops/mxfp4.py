@@ -82,7 +82,7 @@ def quant(x, out=None):
     """(q, s) for x (..., K) bf16, fp16 or fp32, K a multiple of 32: q uint8 (..., K/2) of packed codes, s
     uint8 (..., K/32). A block's scale is 2^ceil(log2(amax / 6)) (nothing is clamped), its codes x over
     that rounded to the nearest, ties to even; a block with an infinity or a NaN is NaN (scale 255).
-    `out`: (q, s) to write into."""
+    `out`: (q, s) to write into (also as float4_e2m1fn_x2 and float8_e8m0fnu); their bytes are the result."""
     key = (x.shape, x.stride(), x.dtype)
     plan = _QUANT.get(key)
     if plan is None or out is not None or x.data_ptr() & 15 or x.get_device() < 0:
@@ -124,6 +124,8 @@ def _quant(x, out, key):
     if out is not None:
         q, s = out
         q = _packed(q, "mxfp4.quant", "out")
+        if s.dtype == torch.float8_e8m0fnu:
+            s = s.view(torch.uint8)
         _on(x.device, "mxfp4.quant", q=q, s=s)
         ok = tuple(q.shape) == q_shape and tuple(s.shape) == s_shape and s.dtype == torch.uint8
         if ok:

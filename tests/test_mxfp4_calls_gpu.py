@@ -187,3 +187,19 @@ def test_linear_of_no_rows(act):
     assert mxfp4.linear(x, w, ws, act=act).shape == (0, 24)
     q, s = mxfp8.quant(x)
     assert q.shape == (0, 416) and s.shape == (0, 13)
+
+
+def test_scales_as_e8m0_wherever_they_are_taken():
+    x = torch.randn(7, 96, generator=_gen(17)).to(BF16).to(DEV)
+    e8m0, fp4 = torch.float8_e8m0fnu, torch.float4_e2m1fn_x2
+    q, s = mxfp4.quant(x)
+    assert torch.equal(mxfp4.dequant(q, s.view(e8m0)), mxfp4.dequant(q, s))
+    assert torch.equal(mxfp4.dequant(q.view(fp4), s.view(e8m0), F32), mxfp4.dequant(q, s, F32))
+    out = torch.zeros(7, 48, dtype=torch.uint8, device=DEV).view(fp4), torch.zeros(7, 3, dtype=torch.uint8, device=DEV).view(e8m0)
+    got = mxfp4.quant(x, out=out)
+    for o in (out, got):
+        assert torch.equal(o[0].view(torch.uint8), q) and torch.equal(o[1].view(torch.uint8), s)
+    q8, s8 = mxfp8.quant(x)
+    assert torch.equal(mxfp8.dequant(q8, s8.view(e8m0)), mxfp8.dequant(q8, s8))
+    with pytest.raises(ValueError):
+        mxfp4.dequant(q, s.int())
