@@ -8,6 +8,9 @@
 The OCP MX layout: two e2m1 codes a byte, the even column in the low bits (uint8, or torch's
 float4_e2m1fn_x2), and one E8M0 byte (2^(s - 127); 255 is NaN) a row and 32 columns.
 
+There is no gradient through quantized values: an activation or a bias that requires one is refused where
+gradients are taken.
+
 A call's checks and layout are kept by the shapes, strides and types they depend on, as a template of
 the library's arguments; a call of known layout fills in its addresses.
 """
@@ -30,6 +33,14 @@ def _packed(t, call, name):
     if t.dtype == getattr(torch, "float4_e2m1fn_x2", None):
         return t.view(torch.uint8)
     raise TypeError(f"{call}: {name} holds packed 4-bit codes (uint8 or float4_e2m1fn_x2), got {t.dtype}")
+
+
+def _no_gradient(call):
+    """For a call of which a tensor requires a gradient: there is none through quantized values."""
+    import torch  # noqa: PLC0415
+
+    if torch.is_grad_enabled():
+        raise ValueError(f"{call}: no gradient through quantized values (detach, or torch.no_grad())")
 
 
 def _e8m0(s, shape, name):
@@ -83,6 +94,8 @@ def quant(x, out=None):
     uint8 (..., K/32). A block's scale is 2^ceil(log2(amax / 6)) (nothing is clamped), its codes x over
     that rounded to the nearest, ties to even; a block with an infinity or a NaN is NaN (scale 255).
     `out`: (q, s) to write into (also as float4_e2m1fn_x2 and float8_e8m0fnu); their bytes are the result."""
+    if x.requires_grad:
+        _no_gradient("mxfp4.quant")
     key = (x.shape, x.stride(), x.dtype)
     plan = _QUANT.get(key)
     if plan is None or out is not None or x.data_ptr() & 15 or x.get_device() < 0:
@@ -164,6 +177,8 @@ def gemm(a, b, sa, sb, *, bias=None, silu_mul=False, out=None):
     float8_e4m3fn, b (N, K/2) packed codes, sa and sb their E8M0 scales (..., K/32), bias (N,) bf16, fp16
     or fp32. With silu_mul, b (2N, K/2) holds gate rows, then up rows: silu(z[..., :N]) * z[..., N:] of z
     (..., 2N) with its bias. Any sizes, K a multiple of 32; sums in fp32, rounded once."""
+    if a.requires_grad or (bias is not None and bias.requires_grad):
+        _no_gradient("mxfp4.gemm")
     key = (a.shape, a.stride(), a.dtype, b.shape, b.stride(), b.dtype, sa.shape, sa.stride(), sa.dtype,
            sb.shape, sb.stride(), sb.dtype, bias is None or (bias.shape, bias.stride(), bias.dtype), silu_mul)
     plan = _GEMM.get(key)
@@ -272,6 +287,8 @@ def linear(x, w, ws, *, bias=None, silu_mul=False, act="mxfp8"):
     NaN gives a row of NaN."""
     if act not in ("mxfp8", "mxfp4"):
         raise ValueError(f"mxfp4.linear: act is 'mxfp8' or 'mxfp4', got {act!r}")
+    if x.requires_grad or (bias is not None and bias.requires_grad):
+        _no_gradient("mxfp4.linear")
     if act == "mxfp4":
         xq, xs = quant(x)
         return gemm(xq, w, xs, ws, bias=bias, silu_mul=silu_mul)

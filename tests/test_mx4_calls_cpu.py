@@ -88,3 +88,23 @@ def test_an_out_leaves_the_layouts_template_alone(launches, m, n, k):
 def test_both_mxfp8_quantizations_refuse_the_same(args, code, says):
     for f in (nat.lib().hkx_mx_quant, nat.lib().hkx_mx_quant_nan):
         assert f(*args, None) == code and says in nat.last_error(), nat.last_error()
+
+
+def test_a_gradient_is_refused_and_not_dropped(launches):
+    a, b, sa, sb = _operands(64, 128, 256, False, False)
+    x = _empty(64, 256, dtype=BF16).requires_grad_()
+    bias = _empty(128, dtype=F32).requires_grad_()
+    for name, f in (("quant", lambda: mxfp4.quant(x)), ("linear", lambda: mxfp4.linear(x, b, sb)),
+                    ("linear", lambda: mxfp4.linear(x, b, sb, act="mxfp4")),
+                    ("linear", lambda: mxfp4.linear(x.detach(), b, sb, bias=bias)),
+                    ("gemm", lambda: mxfp4.gemm(a, b, sa, sb, bias=bias)),
+                    ("gemm", lambda: mxfp4.gemm(x.detach().to(torch.float8_e4m3fn).requires_grad_(), b, sa, sb))):
+        with pytest.raises(ValueError, match=f"mxfp4.{name}: no gradient"):
+            f()
+    assert not launches
+    with torch.no_grad():
+        mxfp4.gemm(a, b, sa, sb, bias=bias)
+    with torch.inference_mode():
+        mxfp4.gemm(a, b, sa, sb, bias=bias)
+    mxfp4.gemm(a, b, sa, sb, bias=bias.detach())
+    assert len(launches) == 3
