@@ -5,8 +5,8 @@
 // floor(log2 amax) - 8, plus one where amax > 448 * 2^e --, q = x / 2^e clamped to +-448 and
 // rounded to the nearest even e4m3, scale byte clamp(e + 127, 0, 254). The block's largest
 // value lands at or below 448, so nothing is clamped but a rounding at the top. An infinity or a
-// NaN becomes +-448; in the NANS form its block is NaN (scale 255, codes 0), as in MXFP4's
-// quantization and block_norm's, and every other block is the same.
+// NaN becomes +-448. The NANS form is block_norm's (hkx_mx_block.hpp): such a block is NaN, and e is at
+// least -127 in the codes too; every other block is the same.
 //
 // A workgroup 512 consecutive 16-byte pieces (8 values) of the row-major piece index, each
 // thread two of them 256 apart, both loaded before either is quantized; a piece's row is a
@@ -22,17 +22,13 @@
 // 2.23 us, 4096 x 4096 15.7 -> 11.3 (4.5 TB/s), 16384 x 5120 59.5 -> 43.5 (5.8 TB/s).
 #include "hkx_device.hpp"
 #include "hkx_launch.hpp"
+#include "hkx_mx_block.hpp"
 
 namespace hkx {
 
 template <int CTRL>
 HKX_DEV float quad_xor(float x) {
   return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), CTRL, 0xf, 0xf, true));
-}
-
-template <int CTRL>
-HKX_DEV uint32_t quad_xor_bits(uint32_t x) {
-  return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, CTRL, 0xf, 0xf, true);
 }
 
 template <typename IDX, bool NANS>
@@ -62,31 +58,31 @@ __global__ void __launch_bounds__(256) mx_quant_kernel(const uint16_t* x, int64_
       v[2 * i] = __builtin_bit_cast(float, ws[i] << 16);
       v[2 * i + 1] = __builtin_bit_cast(float, ws[i] & 0xffff0000u);
     }
+    if constexpr (NANS) {
+      const uint32_t top = mx_block_top(v);
+      if (g[u] >= k8) continue;
+      u32x2 codes;
+      const uint32_t scale = mx8_block(v, top, codes);
+      *(u32x2*)(q + (int64_t)row[u] * ldq + 8 * g[u]) = codes;
+      if ((g[u] & 3) == 0) sc[(int64_t)row[u] * lds + g[u] / 4] = (uint8_t)scale;
+      continue;
+    }
     float amax = 0.0f;
 #pragma unroll
     for (int i = 0; i < 8; ++i) amax = __builtin_fmaxf(amax, __builtin_fabsf(v[i]));
     amax = __builtin_fmaxf(amax, quad_xor<0xb1>(amax));  // quad_perm [1, 0, 3, 2]
     amax = __builtin_fmaxf(amax, quad_xor<0x4e>(amax));  // quad_perm [2, 3, 0, 1]
-    bool bad = false;
-    if constexpr (NANS) {  // (fmaxf leaves a NaN out)
-      uint32_t top = 0;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) top = max(top, __builtin_bit_cast(uint32_t, v[i]) & 0x7fffffffu);
-      top = max(top, quad_xor_bits<0xb1>(top));
-      top = max(top, quad_xor_bits<0x4e>(top));
-      bad = top >= 0x7f800000u;
-    }
     if (g[u] >= k8) continue;
     amax = __builtin_fmaxf(amax, 0x1p-126f);
     int e = (int)((__builtin_bit_cast(uint32_t, amax) >> 23) & 0xff) - 127 - 8;
     if (amax > __builtin_ldexpf(448.0f, e)) e += 1;
 #pragma unroll
     for (int i = 0; i < 8; ++i)
-      v[i] = bad ? 0.0f : __builtin_fminf(__builtin_fmaxf(__builtin_ldexpf(v[i], -e), -448.0f), 448.0f);
+      v[i] = __builtin_fminf(__builtin_fmaxf(__builtin_ldexpf(v[i], -e), -448.0f), 448.0f);
     *(u32x2*)(q + (int64_t)row[u] * ldq + 8 * g[u]) =
         u32x2{cvt_e4m3x4(v[0], v[1], v[2], v[3]), cvt_e4m3x4(v[4], v[5], v[6], v[7])};
     if ((g[u] & 3) == 0)
-      sc[(int64_t)row[u] * lds + g[u] / 4] = (uint8_t)(bad ? 255 : min(max(e + 127, 0), 254));
+      sc[(int64_t)row[u] * lds + g[u] / 4] = (uint8_t)min(max(e + 127, 0), 254);
   }
 }
 

@@ -4,21 +4,15 @@
 // 2^e rounded to the nearest e2m1 value (ties to the even code), scale byte e + 127. 6 is e2m1's
 // largest value, so nothing is clamped (the same choice as MXFP8's quantization here: rounding amax
 // up to the next scale costs a bit of resolution where the floor rule would clip values up to 25%).
-// On the bits of amax: its exponent field less 2, plus one where its mantissa is above 1.5, i.e.
-// ((bits + 0x3fffff) >> 23) - 2, at least 0. A block with an infinity or a NaN (the largest bits
-// of a block are then 0x7f800000 or more) gets the scale 255, E8M0's NaN, and codes 0.
+// A block with an infinity or a NaN gets the scale 255, E8M0's NaN, and codes 0 (hkx_mx_block.hpp).
 //
 // Both bound by HBM, a thread 8 values so that a wave reads and writes whole lines: fp32 12288 x 4096 46 us
 // (229 MB, 5.0 TB/s; a copy of 1 GiB 5.25), back to bf16 20 (129 MB, the codes from the cache).
 #include "hkx_api.hpp"
 #include "hkx_device.hpp"
+#include "hkx_mx_block.hpp"
 
 namespace hkx {
-
-template <int CTRL>
-HKX_DEV uint32_t quad_swap(uint32_t x) {
-  return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, CTRL, 0xf, 0xf, true);
-}
 
 // 8 consecutive values of row type DT as fp32
 template <int DT>
@@ -47,21 +41,8 @@ __global__ void __launch_bounds__(256) mx4_quant_kernel(const void* x, int64_t l
   const int g = (int)(p - row * (IDX)k8);
   float v[8];
   load8<DT>(x, (int64_t)row * ldx + 8 * g, v);
-  uint32_t amax = 0;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) amax = max(amax, __builtin_bit_cast(uint32_t, v[i]) & 0x7fffffffu);
-  amax = max(amax, quad_swap<0xb1>(amax));  // quad_perm [1, 0, 3, 2]
-  amax = max(amax, quad_swap<0x4e>(amax));  // quad_perm [2, 3, 0, 1]
-  const bool bad = amax >= 0x7f800000u;
-  const uint32_t s = bad ? 255u : (uint32_t)max((int)((amax + 0x3fffffu) >> 23) - 2, 0);
-  uint32_t w = 0;
-  if (!bad) {
-    const float f = __builtin_bit_cast(float, s << 23);  // (byte 0, 2^-127, too: the exponent field alone counts)
-    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, v[0], v[1], f, 0);
-    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, v[2], v[3], f, 1);
-    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, v[4], v[5], f, 2);
-    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, v[6], v[7], f, 3);
-  }
+  uint32_t w;
+  const uint32_t s = mx4_block(v, mx_block_top(v), w);
   *(uint32_t*)(q + (int64_t)row * ldq + 4 * g) = w;
   if ((g & 3) == 0) sc[(int64_t)row * lds + g / 4] = (uint8_t)s;
 }

@@ -18,6 +18,7 @@
 
 #include "hkx_api.hpp"
 #include "hkx_device.hpp"
+#include "hkx_mx_block.hpp"
 
 namespace hkx {
 
@@ -199,40 +200,17 @@ HKX_DEV float row_factor(float sum, const NormArgs& p) {
 
 // ---------------------------------------------------------------- quantized stores (whole quads of 8-value pieces)
 
-template <int CTRL>
-HKX_DEV uint32_t max_dpp(uint32_t x) {
-  return max(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, CTRL, 0xf, 0xf, true));
-}
-
-// 8 values of a row at column i (a multiple of 8) and their block's scale byte. MXFP8: e =
-// ceil(log2(amax / 448)), amax at least 2^-126 (448 = 1.75 2^8); MXFP4: ceil(log2(amax / 6)) at
-// least -127. A block with an infinity or a NaN is NaN (scale 255).
+// 8 values of a row at column i (a multiple of 8) and their block's scale byte: MXFP8, or MXFP4.
 HKX_DEV void store_quant(int quant, uint8_t* q, uint8_t* s, int i, const float (&v)[8]) {
-  uint32_t amax = 0;
-#pragma unroll
-  for (int j = 0; j < 8; ++j) amax = max(amax, __builtin_bit_cast(uint32_t, v[j]) & 0x7fffffffu);
-  amax = max_dpp<0x4e>(max_dpp<0xb1>(amax));
-  const bool bad = amax >= 0x7f800000u;
+  const uint32_t top = mx_block_top(v);
   uint32_t sc;
   if (quant == 1) {
-    amax = max(amax, 0x00800000u);
-    const int e = max((int)((amax + 0x1fffffu) >> 23) - 8, 0) - 127;
-    sc = bad ? 255u : (uint32_t)(e + 127);
-    float t[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j)
-      t[j] = bad ? 0.0f : __builtin_fminf(__builtin_fmaxf(__builtin_ldexpf(v[j], -e), -448.0f), 448.0f);
-    *(u32x2*)(q + i) = u32x2{cvt_e4m3x4(t[0], t[1], t[2], t[3]), cvt_e4m3x4(t[4], t[5], t[6], t[7])};
+    u32x2 w;
+    sc = mx8_block(v, top, w);
+    *(u32x2*)(q + i) = w;
   } else {
-    sc = bad ? 255u : (uint32_t)max((int)((amax + 0x3fffffu) >> 23) - 2, 0);
-    uint32_t w = 0;
-    if (!bad) {
-      const float f = __builtin_bit_cast(float, sc << 23);
-      w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, v[0], v[1], f, 0);
-      w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, v[2], v[3], f, 1);
-      w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, v[4], v[5], f, 2);
-      w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, v[6], v[7], f, 3);
-    }
+    uint32_t w;
+    sc = mx4_block(v, top, w);
     *(uint32_t*)(q + i / 2) = w;
   }
   if ((i & 31) == 0) s[i / 32] = (uint8_t)sc;

@@ -99,8 +99,9 @@ def gemm(a, b, sa, sb, out=None):
 def quant(x, out=None, *, nan_blocks=False):
     """(q, s) for bf16 x [M, K], K a multiple of 32: q float8_e4m3fn [M, K], s uint8
     [M, K/32] (OCP layout), by AITER's per_1x32 rule, which makes an infinity or a NaN
-    +-448. `nan_blocks`: its block is NaN instead (scale 255, codes 0), as in
-    `hk.ops.mxfp4.quant` and `hk.ops.block_norm`."""
+    +-448. `nan_blocks`: as `hk.ops.block_norm` quantizes, its block is NaN (scale 255,
+    codes 0), and blocks below 2^-119 keep their size (there the rule clamps the scale
+    byte alone)."""
     import torch  # noqa: PLC0415
 
     if x.dtype != torch.bfloat16 or x.dim() != 2:

@@ -316,8 +316,9 @@ size_t hkx_mx_gemm_workspace(int32_t m, int32_t n, int32_t k);
 int hkx_mx_quant(const void* x, int64_t ldx, void* q, int64_t ldq, uint8_t* s, int64_t lds,
                  int32_t m, int32_t k, void* stream);
 
-/* The same, but for a block with an infinity or a NaN: s = 255 (E8M0's NaN) and codes 0, as
- * hkx_mx4_quant's and hkx_block_norm's. (hkx_mx_quant makes them +-448.) */
+/* The same as hkx_block_norm quantizes y: for a block with an infinity or a NaN s = 255 (E8M0's NaN)
+ * and codes 0 (hkx_mx_quant makes them +-448), and of a block below 2^-119 e is -127, which is what s
+ * stands for (there e is less than the s it is clamped to). */
 int hkx_mx_quant_nan(const void* x, int64_t ldx, void* q, int64_t ldq, uint8_t* s, int64_t lds,
                      int32_t m, int32_t k, void* stream);
 

@@ -203,3 +203,17 @@ def test_scales_as_e8m0_wherever_they_are_taken():
     assert torch.equal(mxfp8.dequant(q8, s8.view(e8m0)), mxfp8.dequant(q8, s8))
     with pytest.raises(ValueError):
         mxfp4.dequant(q, s.int())
+
+
+@pytest.mark.parametrize("exponent", [-134, -126, -122, -119, -117, -100, 0, 110])
+def test_the_activations_quantization_keeps_a_blocks_size(exponent):
+    """linear's MXFP8 quantization: within half a step of e4m3 (2^-4 of
+    the value, 2^-10 of the scale where it is subnormal) of x, down to the least scale's blocks, where x
+    itself is subnormal."""
+    x = torch.ldexp(torch.randn(9, 96, generator=_gen(exponent)), torch.tensor(exponent)).to(BF16)
+    q, s = mxfp8.quant(x.to(DEV), nan_blocks=True)
+    v = O.values(q.cpu(), s.cpu())
+    scale = torch.ldexp(torch.ones(9, 3, dtype=torch.float64), s.cpu().int() - 127).repeat_interleave(32, 1)
+    assert (s < 255).all() and ((v - x.double()).abs() <= 2.0 ** -4 * x.double().abs() + 2.0 ** -10 * scale).all()
+    top = x.double().abs().view(9, 3, 32).amax(-1)
+    assert (448 * scale[:, ::32] >= top).all() and ((224 * scale[:, ::32] < top) | (s.cpu() == 0)).all()
