@@ -10,7 +10,7 @@
 //
 // A workgroup 512 consecutive 16-byte pieces (8 values) of the row-major piece index, each
 // thread two of them 256 apart, both loaded before either is quantized; a piece's row is a
-// 32-bit division wherever the index fits in 32 bits. The 4 threads of a 32-column block are
+// 32-bit division. The 4 threads of a 32-column block are
 // the lanes of a quad and meet with two DPP quad permutes. x / 2^e is an exact power-of-two
 // scaling (ldexp), which the division also is, so the result is bit for bit the same.
 //
@@ -31,21 +31,21 @@ HKX_DEV float quad_xor(float x) {
   return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), CTRL, 0xf, 0xf, true));
 }
 
-template <typename IDX, bool NANS>
+template <bool NANS>
 __global__ void __launch_bounds__(256) mx_quant_kernel(const uint16_t* x, int64_t ldx, uint8_t* q,
                                                        int64_t ldq, uint8_t* sc, int64_t lds,
                                                        int m, int k8) {
-  const IDX total = (IDX)m * (IDX)k8;
-  const IDX p0 = (IDX)blockIdx.x * 512 + threadIdx.x;
+  const uint32_t total = (uint32_t)m * (uint32_t)k8;
+  const uint32_t p0 = blockIdx.x * 512 + threadIdx.x;
   i32x4 w[2];
-  IDX row[2];
+  uint32_t row[2];
   int g[2];
 #pragma unroll
   for (int u = 0; u < 2; ++u) {  // whole 4-thread groups are in or out (k8 % 4 == 0)
-    const IDX p = p0 + 256 * u;
+    const uint32_t p = p0 + 256 * u;
     const bool ok = p < total;
-    row[u] = ok ? p / (IDX)k8 : 0;
-    g[u] = ok ? (int)(p - row[u] * (IDX)k8) : k8;
+    row[u] = ok ? p / (uint32_t)k8 : 0;
+    g[u] = ok ? (int)(p - row[u] * (uint32_t)k8) : k8;
     w[u] = ok ? __builtin_nontemporal_load((const i32x4*)(x + (int64_t)row[u] * ldx + 8 * g[u]))
               : i32x4{0, 0, 0, 0};
   }
@@ -90,15 +90,17 @@ template <bool NANS>
 static hipError_t launch(const void* x, int64_t ldx, void* q, int64_t ldq, uint8_t* sc, int64_t lds,
                          int m, int k, hipStream_t s) {
   const int k8 = k / 8;
-  const int64_t total = (int64_t)m * k8;
-  const dim3 grid((unsigned)((total + 511) / 512));
-  if (total + 512 < (int64_t)1 << 32)  // a 32-bit row division wherever the index fits
-    hipLaunchKernelGGL((mx_quant_kernel<uint32_t, NANS>), grid, dim3(256), 0, s, (const uint16_t*)x,
-                       ldx, (uint8_t*)q, ldq, sc, lds, m, k8);
-  else
-    hipLaunchKernelGGL((mx_quant_kernel<uint64_t, NANS>), grid, dim3(256), 0, s, (const uint16_t*)x,
-                       ldx, (uint8_t*)q, ldq, sc, lds, m, k8);
-  return hipGetLastError();
+  // (32-bit piece indices, and a grid of threads past 2^32 is cut short with no error: more rows go
+  // launch by launch)
+  const int64_t most = (((int64_t)1 << 32) - 512) / k8;
+  for (int64_t r = 0; r < m; r += most) {
+    const int rows = (int)(m - r < most ? m - r : most);
+    const dim3 grid((unsigned)(((int64_t)rows * k8 + 511) / 512));
+    hipLaunchKernelGGL(mx_quant_kernel<NANS>, grid, dim3(256), 0, s, (const uint16_t*)x + r * ldx, ldx,
+                       (uint8_t*)q + r * ldq, ldq, sc + r * lds, lds, rows, k8);
+    if (hipError_t e = hipGetLastError()) return e;
+  }
+  return hipSuccess;
 }
 
 hipError_t launch_mx_quant(const void* x, int64_t ldx, void* q, int64_t ldq, uint8_t* sc,

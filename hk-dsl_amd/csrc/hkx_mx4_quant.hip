@@ -8,6 +8,8 @@
 //
 // Both bound by HBM, a thread 8 values so that a wave reads and writes whole lines: fp32 12288 x 4096 46 us
 // (229 MB, 5.0 TB/s; a copy of 1 GiB 5.25), back to bf16 20 (129 MB, the codes from the cache).
+#include <algorithm>
+
 #include "hkx_api.hpp"
 #include "hkx_device.hpp"
 #include "hkx_mx_block.hpp"
@@ -32,13 +34,13 @@ HKX_DEV void load8(const void* p, int64_t idx, float (&v)[8]) {
 }
 
 // A thread a piece of 8 values, the 4 threads of a block a quad.
-template <int DT, typename IDX>
+template <int DT>
 __global__ void __launch_bounds__(256) mx4_quant_kernel(const void* x, int64_t ldx, uint8_t* q, int64_t ldq,
                                                         uint8_t* sc, int64_t lds, int m, int k8) {
-  const IDX p = (IDX)blockIdx.x * 256 + threadIdx.x;
-  if (p >= (IDX)m * (IDX)k8) return;  // (k8 is a multiple of 4: whole quads)
-  const IDX row = p / (IDX)k8;
-  const int g = (int)(p - row * (IDX)k8);
+  const uint32_t p = blockIdx.x * 256 + threadIdx.x;
+  if (p >= (uint32_t)m * (uint32_t)k8) return;  // (k8 is a multiple of 4: whole quads)
+  const uint32_t row = p / (uint32_t)k8;
+  const int g = (int)(p - row * (uint32_t)k8);
   float v[8];
   load8<DT>(x, (int64_t)row * ldx + 8 * g, v);
   uint32_t w;
@@ -49,13 +51,13 @@ __global__ void __launch_bounds__(256) mx4_quant_kernel(const void* x, int64_t l
 
 // MX values as numbers: a thread 8 of them, each an exact power-of-two scaling, rounded once to
 // the output's type.
-template <bool FP8, int DT, typename IDX>
+template <bool FP8, int DT>
 __global__ void __launch_bounds__(256) mx_dequant_kernel(const uint8_t* q, int64_t ldq, const uint8_t* sc, int64_t lds,
                                                          void* y, int64_t ldy, int m, int k8) {
-  const IDX p = (IDX)blockIdx.x * 256 + threadIdx.x;
-  if (p >= (IDX)m * (IDX)k8) return;
-  const IDX row = p / (IDX)k8;
-  const int g = (int)(p - row * (IDX)k8);
+  const uint32_t p = blockIdx.x * 256 + threadIdx.x;
+  if (p >= (uint32_t)m * (uint32_t)k8) return;
+  const uint32_t row = p / (uint32_t)k8;
+  const int g = (int)(p - row * (uint32_t)k8);
   const int s = sc[(int64_t)row * lds + g / 4];
   float v[8];
   if constexpr (FP8) {
@@ -89,26 +91,34 @@ __global__ void __launch_bounds__(256) mx_dequant_kernel(const uint8_t* q, int64
 
 namespace {
 
+// A launch's threads, a piece each, stay under 2^32 (a grid past that is cut short, with no error): more rows
+// go launch by launch.
+int64_t rows_a_launch(int k) { return (((int64_t)1 << 32) - 256) / (k / 8); }
+
 template <int DT>
 hipError_t quant(const void* x, int64_t ldx, void* q, int64_t ldq, uint8_t* s, int64_t lds, int m, int k, hipStream_t st) {
-  const int64_t total = (int64_t)m * (k / 8);
-  const dim3 grid((unsigned)((total + 255) / 256));
-  if (total + 256 < (int64_t)1 << 32)  // a 32-bit row division wherever the index fits
-    hipLaunchKernelGGL((hkx::mx4_quant_kernel<DT, uint32_t>), grid, dim3(256), 0, st, x, ldx, (uint8_t*)q, ldq, s, lds, m, k / 8);
-  else
-    hipLaunchKernelGGL((hkx::mx4_quant_kernel<DT, uint64_t>), grid, dim3(256), 0, st, x, ldx, (uint8_t*)q, ldq, s, lds, m, k / 8);
-  return hipGetLastError();
+  constexpr int es = DT == HKX_FP32 ? 4 : 2;
+  for (int64_t r = 0, most = rows_a_launch(k); r < m; r += most) {
+    const int rows = (int)std::min(most, m - r);
+    const dim3 grid((unsigned)(((int64_t)rows * (k / 8) + 255) / 256));
+    hipLaunchKernelGGL((hkx::mx4_quant_kernel<DT>), grid, dim3(256), 0, st, (const uint8_t*)x + r * ldx * es, ldx,
+                       (uint8_t*)q + r * ldq, ldq, s + r * lds, lds, rows, k / 8);
+    if (hipError_t e = hipGetLastError()) return e;
+  }
+  return hipSuccess;
 }
 
 template <bool FP8, int DT>
 hipError_t dequant(const void* q, int64_t ldq, const uint8_t* s, int64_t lds, void* y, int64_t ldy, int m, int k, hipStream_t st) {
-  const int64_t total = (int64_t)m * (k / 8);
-  const dim3 grid((unsigned)((total + 255) / 256));
-  if (total + 256 < (int64_t)1 << 32)
-    hipLaunchKernelGGL((hkx::mx_dequant_kernel<FP8, DT, uint32_t>), grid, dim3(256), 0, st, (const uint8_t*)q, ldq, s, lds, y, ldy, m, k / 8);
-  else
-    hipLaunchKernelGGL((hkx::mx_dequant_kernel<FP8, DT, uint64_t>), grid, dim3(256), 0, st, (const uint8_t*)q, ldq, s, lds, y, ldy, m, k / 8);
-  return hipGetLastError();
+  constexpr int es = DT == HKX_FP32 ? 4 : 2;
+  for (int64_t r = 0, most = rows_a_launch(k); r < m; r += most) {
+    const int rows = (int)std::min(most, m - r);
+    const dim3 grid((unsigned)(((int64_t)rows * (k / 8) + 255) / 256));
+    hipLaunchKernelGGL((hkx::mx_dequant_kernel<FP8, DT>), grid, dim3(256), 0, st, (const uint8_t*)q + r * ldq, ldq,
+                       s + r * lds, lds, (uint8_t*)y + r * ldy * es, ldy, rows, k / 8);
+    if (hipError_t e = hipGetLastError()) return e;
+  }
+  return hipSuccess;
 }
 
 }  // namespace
@@ -127,7 +137,6 @@ int hkx_mx4_quant(const void* x, int64_t ldx, int32_t x_dtype, void* q, int64_t 
   const int64_t es = x_dtype == HKX_FP32 ? 4 : 2;
   if (!api_aligned(x, 16) || ldx * es % 16 || !api_aligned(q, 4) || ldq % 4)
     return api_fail(HKX_ERR_SHAPE, "mx4_quant: x needs 16-byte and q 4-byte aligned rows");
-  if ((int64_t)m * (k / 8) / 256 >= (int64_t)1 << 31) return api_fail(HKX_ERR_SHAPE, "mx4_quant: M=%d K=%d too large", m, k);
   if (m == 0 || k == 0) return HKX_OK;
   const hipStream_t st = (hipStream_t)stream;
   return api_launched(x_dtype == HKX_BF16   ? quant<HKX_BF16>(x, ldx, q, ldq, s, lds, m, k, st)
@@ -150,7 +159,6 @@ int hkx_mx_dequant(const void* q, int64_t ldq, int32_t q_dtype, const uint8_t* s
   const int64_t es = y_dtype == HKX_FP32 ? 4 : 2, qa = fp8 ? 8 : 4;
   if (!api_aligned(y, 16) || ldy * es % 16 || !api_aligned(q, qa) || ldq % qa)
     return api_fail(HKX_ERR_SHAPE, "mx_dequant: y needs 16-byte and q %d-byte aligned rows", (int)qa);
-  if ((int64_t)m * (k / 8) / 256 >= (int64_t)1 << 31) return api_fail(HKX_ERR_SHAPE, "mx_dequant: M=%d K=%d too large", m, k);
   if (m == 0 || k == 0) return HKX_OK;
   const hipStream_t st = (hipStream_t)stream;
   hipError_t e;
