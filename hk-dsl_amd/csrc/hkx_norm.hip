@@ -55,7 +55,9 @@ bool floating(int dt) { return dt == HKX_BF16 || dt == HKX_FP16 || dt == HKX_FP3
 // What forward and backward check alike; the kernels' arguments.
 int forward_args(const HkxBlockNormArgs& g, const char* what, NormArgs& a) {
   if (!g.x || !g.residual) return api_fail(HKX_ERR_ARG, "%s: a null pointer", what);
-  if (g.rows < 0 || g.d < 1) return api_fail(HKX_ERR_SHAPE, "%s: rows=%d d=%d", what, g.rows, g.d);
+  // (row numbers, and a worker's past the last, are 32-bit)
+  if (g.rows < 0 || g.rows > INT32_MAX - 65536 || g.d < 1)
+    return api_fail(HKX_ERR_SHAPE, "%s: rows=%d d=%d", what, g.rows, g.d);
   if (!floating(g.x_dtype) || (g.r_dtype != g.x_dtype && g.r_dtype != HKX_FP32))
     return api_fail(HKX_ERR_DTYPE, "%s: x is bf16, fp16 or fp32, the residual the same or fp32", what);
   if ((g.post || g.pre) && g.w_dtype != g.x_dtype && g.w_dtype != HKX_FP32)

@@ -16,6 +16,8 @@
 // elements) 6.6, 14.5 and 3.9.
 #pragma once
 
+#include <algorithm>
+
 #include "hkx_api.hpp"
 #include "hkx_device.hpp"
 #include "hkx_mx_block.hpp"
@@ -40,6 +42,7 @@ struct NormArgs {
   int32_t quant;      // 0: y as x's type, 1: MXFP8, 2: MXFP4
   float bs, rs, eps;
   double inv_d;  // 1 / d
+  int32_t row0;  // the launch's first row (forward)
 };
 
 // The elements a thread (8 c, in pieces of 8 where vec), and the row's threads (64: a wave a row, else
@@ -243,7 +246,7 @@ __global__ void __launch_bounds__(WAVE ? 256 : 1024) norm_kernel(const NormArgs 
   constexpr int E = Cols<C, VEC>::E;
   __shared__ float red[2][16];
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-  const int row = WAVE ? (int)blockIdx.x * 4 + wave : (int)blockIdx.x;
+  const int row = p.row0 + (WAVE ? (int)blockIdx.x * 4 + wave : (int)blockIdx.x);
   if (row >= p.rows) return;
   const Cols<C, VEC> cols{WAVE ? (int)(threadIdx.x & 63) : (int)threadIdx.x, WAVE ? 64 : (int)blockDim.x, p.d};
   using Row = typename Cols<C, VEC>::Row;
@@ -474,24 +477,32 @@ inline NormShape norm_shape(int d, bool vec) {
 constexpr int kNormMaxD = 16384;     // 16 waves of 64 x 16 elements
 constexpr int kNormGradMaxD = 8192;  // 8 waves of 64 x 16: ten registers an element
 
+// A launch's threads stay under 2^32 (a grid past that is cut short, with no error): more rows go launch by
+// launch, whole workgroups each.
 template <int XT, int RT, int WT>
-hipError_t launch_norm_typed(const NormArgs& a, hipStream_t s) {
+hipError_t launch_norm_typed(NormArgs a, hipStream_t s) {
   auto es = [](int dt) { return dt == HKX_FP32 ? 4 : 2; };
   const NormShape f = norm_shape(a.d, norm_vec_ok(a, es(XT), es(RT), es(WT), es(a.gate_dt)));
   const bool wave = f.threads == 64;
-  const dim3 grid(wave ? (a.rows + 3) / 4 : a.rows), block(wave ? 256 : f.threads);
+  const int most = (int)((((int64_t)1 << 32) - 1) / f.threads) & ~3;
+  for (int64_t r = 0; r < a.rows; r += most) {
+    const int rows = (int)std::min<int64_t>(most, a.rows - r);
+    a.row0 = (int)r;
+    const dim3 grid(wave ? (rows + 3) / 4 : rows), block(wave ? 256 : f.threads);
 #define HKX_NORM(C, V, W) hipLaunchKernelGGL((norm_kernel<XT, RT, WT, C, V, W>), grid, block, 0, s, a)
-  if (f.vec) {
-    if (!wave) HKX_NORM(2, true, false);
-    else if (f.c == 1) HKX_NORM(1, true, true);
-    else HKX_NORM(2, true, true);
-  } else {
-    if (!wave) HKX_NORM(2, false, false);
-    else if (f.c == 1) HKX_NORM(1, false, true);
-    else HKX_NORM(2, false, true);
-  }
+    if (f.vec) {
+      if (!wave) HKX_NORM(2, true, false);
+      else if (f.c == 1) HKX_NORM(1, true, true);
+      else HKX_NORM(2, true, true);
+    } else {
+      if (!wave) HKX_NORM(2, false, false);
+      else if (f.c == 1) HKX_NORM(1, false, true);
+      else HKX_NORM(2, false, true);
+    }
 #undef HKX_NORM
-  return hipGetLastError();
+    if (hipError_t e = hipGetLastError()) return e;
+  }
+  return hipSuccess;
 }
 
 template <int XT, int RT, int WT>

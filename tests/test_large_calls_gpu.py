@@ -34,3 +34,27 @@ def test_quantization_and_numbers_back():
             assert torch.equal(q[p].view(torch.uint8), q1.view(torch.uint8)) and torch.equal(s[p], s1)
             assert torch.equal(back[p], dequant(q1, s1)) and back[p].any()
         del q, s, back
+
+
+@pytest.mark.parametrize("rows,d", [((1 << 26) + 37, 8), ((1 << 26) + 6, 3)])
+def test_block_norm_of_many_rows(rows, d):
+    """A wave a row: 2^26 rows are 2^32 threads. Forward (two launches), a gate a row of each, and backward."""
+    _free(40)
+    x = torch.empty(rows, d, device=DEV, dtype=BF16)
+    x[:] = torch.randn(1, d, device=DEV).to(BF16)
+    x *= torch.linspace(0.5, 2, 1024, device=DEV).to(BF16).repeat(rows // 1024 + 1)[:rows, None]
+    gate = torch.linspace(0.25, 1, 999, device=DEV).to(BF16).repeat(rows // 999 + 1)[:rows, None]
+    w = torch.linspace(0.9, 1.1, d, device=DEV).to(BF16)
+    h, y = hk.ops.block_norm(x, x, post=w, pre=w, gate=gate)
+    edge = (1 << 26) - 4
+    ends = [slice(0, 40), slice(edge - 40, edge + 4), slice(rows - 40, rows)]
+    for p in ends:
+        h1, y1 = hk.ops.block_norm(x[p].clone(), x[p].clone(), post=w, pre=w, gate=gate[p].clone())
+        assert torch.equal(h[p], h1) and torch.equal(y[p], y1)
+    a = x.detach().requires_grad_()
+    _, y2 = hk.ops.block_norm(a, x, post=w, pre=w, gate=gate)
+    dx, = torch.autograd.grad(y2, a, y)
+    for p in ends:
+        a1 = x[p].clone().requires_grad_()
+        _, y1 = hk.ops.block_norm(a1, x[p].clone(), post=w, pre=w, gate=gate[p].clone())
+        assert torch.equal(dx[p], torch.autograd.grad(y1, a1, y[p].clone())[0])
