@@ -53,9 +53,10 @@ static_assert(kMx4Tile64 == HKX_MX4_TILE64 && kMx4Tile128 == HKX_MX4_TILE128 && 
                   kMx4Skinny == HKX_MX4_SKINNY, "kernels");
 
 // The quadrant kernel's epilogue: 32-bit offsets into C or the shares. (Any bias: C of odd columns leaves through
-// shares, whose sum adds it.)
+// shares, whose sum adds it.) And the scales' packing: a tile each of A and B along a grid's y.
 bool quad_ok(const HkxMx4GemmArgs& g) {
   const int64_t rows = ((int64_t)g.m + 255) / 256 * 256;
+  if (rows / 256 + g.n / mx4_cols(HKX_MX4_QUAD, g.silu_mul) >= 65535) return false;
   return rows * std::max(g.ldc * 2, ((int64_t)g.n + 3) / 4 * 4 * (g.silu_mul ? 8 : 4)) < ((int64_t)1 << 32) - 65536;
 }
 
@@ -193,6 +194,9 @@ int hkx_mx4_gemm(const HkxMx4GemmArgs* args, void* stream) {
   const int bm = mx4_rows(q.kernel), bn = mx4_cols(q.kernel, pair);
   t.tiles_m = (g.m + bm - 1) / bm;
   t.tiles_n = (g.n + bn - 1) / bn;
+  // (a grid past 2^32 threads is cut short, with no error)
+  if (q.kernel != HKX_MX4_QUAD && (int64_t)t.tiles_m * t.tiles_n >= (1 << 24) - 1)
+    return api_fail(HKX_ERR_SHAPE, "mx4_gemm: M=%d N=%d is more tiles than a launch takes; split the call", g.m, g.n);
   if (q.kernel == HKX_MX4_QUAD) {
     Mx4PackArgs pa{}, pb{};
     pa.s = g.sa;

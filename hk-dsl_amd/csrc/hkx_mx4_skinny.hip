@@ -39,6 +39,8 @@ hipError_t launch_mx4_skinny(Mx4SkinnyArgs a, bool a8, bool pair, int cus, hipSt
     const int wgs = (blocks + nb - 1) / nb;
     if (wgs >= resident * cus && nb * ((wgs + cus - 1) / cus) <= least) a.nb = nb;
   }
+  // (a grid past 2^32 threads is cut short, with no error; 2^28 rows of W, the most of 4 GiB, are 2^24 blocks)
+  while ((int64_t)((blocks + a.nb - 1) / a.nb) * 512 >= (int64_t)1 << 32) ++a.nb;
   const dim3 grid((unsigned)((blocks + a.nb - 1) / a.nb), (unsigned)chunks);
   switch (mf) {
     case 1: return launch_form<1>(a, a8, pair, grid, s);

@@ -58,3 +58,22 @@ def test_block_norm_of_many_rows(rows, d):
         a1 = x[p].clone().requires_grad_()
         _, y1 = hk.ops.block_norm(a1, x[p].clone(), post=w, pre=w, gate=gate[p].clone())
         assert torch.equal(dx[p], torch.autograd.grad(y1, a1, y[p].clone())[0])
+
+
+@pytest.mark.parametrize("m,n,k,pair", [(1, 32770 * 4096 + 16, 32, False), (3, 32770 * 2048 + 8, 32, True),
+                                        ((1 << 24) + 300, 64, 32, False)])
+def test_products_of_many_columns_or_rows(m, n, k, pair):
+    """The decode kernel's blocks of 16 columns (8 paired), 512 threads each, and 65536 tiles of 256 rows."""
+    _free(20)
+    rows = 2 * n if pair else n
+    g = torch.Generator(device=DEV).manual_seed(n)
+    a, b = (torch.randint(0, 256, (r, k // 2), generator=g, device=DEV, dtype=torch.uint8) for r in (m, rows))
+    sa, sb = (torch.randint(125, 129, (r, k // 32), generator=g, device=DEV, dtype=torch.uint8) for r in (m, rows))
+    c = mxfp4.gemm(a, b, sa, sb, silu_mul=pair)
+    torch.cuda.synchronize()
+    for p in (slice(0, 48), slice(n // 2, n // 2 + 48), slice(n - 48, n)) if m < 100 else (slice(0, n),):
+        w = torch.cat([b[:n][p], b[n:][p]]) if pair else b[p].clone()
+        ws = torch.cat([sb[:n][p], sb[n:][p]]) if pair else sb[p].clone()
+        for r in (slice(0, 40), slice(m - 40, m)) if m > 100 else (slice(0, m),):
+            # (32 products: exact in fp32 in any order)
+            assert torch.equal(c[r, p], mxfp4.gemm(a[r].clone(), w, sa[r].clone(), ws, silu_mul=pair))
