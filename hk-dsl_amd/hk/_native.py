@@ -194,6 +194,13 @@ def check(code: int) -> None:
         raise HkxError(code, last_error())
 
 
+def int32(call: str, **sizes) -> None:
+    """The library's sizes are 32-bit: ctypes would cut a larger one short, and the call be another."""
+    for name, n in sizes.items():
+        if n > 0x7fffffff:
+            raise ValueError(f"{call}: {name}={n}, at most 2^31 - 1; split the call")
+
+
 # ---- torch glue
 
 _CODES: dict = {}

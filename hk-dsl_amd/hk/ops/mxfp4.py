@@ -125,6 +125,7 @@ def _quant(x, out, key):
     if not x.is_cuda:
         raise ValueError(f"mxfp4.quant: x is on a GPU, got {x.device}")
     m, given = x.numel() // k, x
+    nat.int32("mxfp4.quant", M=m, K=k)
     if x.dim() != 2:
         x = x.reshape(m, k)
     per, ldx = 16 // x.element_size(), _ld(x, k)
@@ -238,6 +239,8 @@ def _gemm(a, b, sa, sb, bias, silu_mul, out, key):
         n = rows // 2
     if not a.is_cuda or b.device != a.device:
         raise ValueError("mxfp4.gemm: a and b are on one GPU")
+    m = a.numel() // a.shape[-1]
+    nat.int32("mxfp4.gemm", M=m, N=rows, K=k)
     _on(a.device, "mxfp4.gemm", sa=sa, sb=sb, bias=bias, out=out)
     sa = _e8m0(sa, (*lead, k // 32), "sa")
     sb = _e8m0(sb, (rows, k // 32), "sb")
@@ -249,7 +252,6 @@ def _gemm(a, b, sa, sb, bias, silu_mul, out, key):
         out = nat.empty(a, (*lead, n), torch.bfloat16)
     elif out.dtype != torch.bfloat16 or tuple(out.shape) != (*lead, n):
         raise ValueError(f"mxfp4.gemm: out is bf16 {(*lead, n)}, got {out.dtype} {tuple(out.shape)}")
-    m = a.numel() // a.shape[-1]
     if m == 0 or n == 0:
         return out
     a, sa = a.reshape(m, a.shape[-1]), sa.reshape(m, k // 32)

@@ -109,6 +109,8 @@ def quant(x, out=None, *, nan_blocks=False):
     m, k = x.shape
     if k % 32:
         raise ValueError(f"mxfp8.quant: K={k}, a multiple of 32")
+    if (m | k) >> 31:
+        nat.int32("mxfp8.quant", M=m, K=k)
     if not x.is_cuda:
         raise ValueError(f"mxfp8.quant: x is on a GPU, got {x.device}")
     if out is not None:
@@ -162,8 +164,10 @@ def _dequant(call, q, s, dtype, code, per):
         raise ValueError(f"{call}: q is on a GPU, got {q.device}")
     if s.get_device() != d:
         _on(q.device, call, s=s)
-    y = nat.empty(q, (*lead, k), dtype)
     m = q.numel() // kb
+    if (m | k) >> 31:
+        nat.int32(call, M=m, K=k)
+    y = nat.empty(q, (*lead, k), dtype)
     if m == 0:
         return y
     if q.dim() != 2:

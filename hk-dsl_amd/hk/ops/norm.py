@@ -312,6 +312,7 @@ def _checked(x, residual, post, pre, gate, quant, grad):
     if not x.is_cuda:
         raise ValueError(f"block_norm: x is on a GPU, got {x.device}")
     d = x.shape[-1]
+    nat.int32("block_norm", rows=x.numel() // d)
     for name, t in (("residual", residual), ("post", post), ("pre", pre), ("gate", gate)):
         if t is None:
             continue

@@ -108,3 +108,22 @@ def test_a_gradient_is_refused_and_not_dropped(launches):
         mxfp4.gemm(a, b, sa, sb, bias=bias)
     mxfp4.gemm(a, b, sa, sb, bias=bias.detach())
     assert len(launches) == 3
+
+
+@pytest.mark.parametrize("rows", [2 ** 31, 2 ** 32 + 16])
+def test_sizes_past_32_bits_are_refused_and_not_cut_short(launches, rows):
+    """(A row that stands for all of them: nothing of that size is made.)"""
+    from hk.ops import block_norm, mxfp8
+
+    def wide(n, dtype=torch.uint8):
+        return torch.empty(1, n, dtype=dtype).expand(rows, n).as_subclass(OnGpu)
+
+    a, b, sa, sb = wide(16), _empty(8, 16), wide(1), _empty(8, 1)
+    x = wide(32, BF16)
+    for f in (lambda: mxfp4.quant(x), lambda: mxfp8.quant(x), lambda: mxfp4.linear(x, b, sb),
+              lambda: mxfp4.linear(x, b, sb, act="mxfp4"), lambda: mxfp4.gemm(a, b, sa, sb),
+              lambda: mxfp4.gemm(b, a, sb, sa), lambda: mxfp4.dequant(a, sa),
+              lambda: mxfp8.dequant(wide(32, torch.float8_e4m3fn), sa), lambda: block_norm(x, x)):
+        with pytest.raises(ValueError, match=f"={rows}, at most 2"):
+            f()
+    assert not launches
