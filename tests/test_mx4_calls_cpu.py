@@ -127,3 +127,20 @@ def test_sizes_past_32_bits_are_refused_and_not_cut_short(launches, rows):
         with pytest.raises(ValueError, match=f"={rows}, at most 2"):
             f()
     assert not launches
+
+
+#: Calls of hk.ops.mxfp4.gemm whose plan is each kernel: (M, N, K, 8-bit A, paired) and (kernel, splits).
+PLANS = [((40, 512, 2048, True, False), (nat.MX4_SKINNY, 1)), ((300, 200, 2048, False, True), (nat.MX4_SKINNY, 1)),
+         ((640, 512, 1024, False, False), (nat.MX4_TILE64, 1)), ((600, 1024, 4096, True, False), (nat.MX4_TILE64, 2)),
+         ((1024, 2048, 2080, False, True), (nat.MX4_TILE128, 1)), ((520, 1024, 8192, False, False), (nat.MX4_TILE128, 4)),
+         ((2300, 6144, 1056, False, False), (nat.MX4_QUAD, 1)), ((1100, 4099, 12320, False, False), (nat.MX4_QUAD, 2)),
+         ((777, 8192, 1056, False, True), (nat.MX4_QUAD, 1)), ((1100, 2051, 12320, False, True), (nat.MX4_QUAD, 2)),
+         ((2300, 6152, 1056, True, False), (nat.MX4_QUAD, 1)), ((2300, 1024, 12320, True, False), (nat.MX4_QUAD, 4)),
+         ((777, 8192, 1056, True, True), (nat.MX4_QUAD, 1)), ((1100, 2051, 12320, True, True), (nat.MX4_QUAD, 2))]
+
+
+def test_the_plans_of_the_calls_that_the_gpu_tests_make():
+    import test_mx4_cpu as R
+
+    got = [(call, R._plan(*call[:3], call[3], call[4], vec=call[1] % 8 == 0)) for call, _ in PLANS]
+    assert got == PLANS

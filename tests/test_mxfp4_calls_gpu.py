@@ -9,6 +9,7 @@ import torch
 from hk import _native as nat
 from hk.ops import mxfp4, mxfp8
 from oracle import mxfp4_oracle as O
+from test_mx4_calls_cpu import PLANS
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda:0"
@@ -217,3 +218,113 @@ def test_the_activations_quantization_keeps_a_blocks_size(exponent):
     assert (s < 255).all() and ((v - x.double()).abs() <= 2.0 ** -4 * x.double().abs() + 2.0 ** -10 * scale).all()
     top = x.double().abs().view(9, 3, 32).amax(-1)
     assert (448 * scale[:, ::32] >= top).all() and ((224 * scale[:, ::32] < top) | (s.cpu() == 0)).all()
+
+
+@pytest.mark.parametrize("call,plan", PLANS)
+def test_gemm_by_each_plan(call, plan):
+    """hk.ops.mxfp4.gemm where its plan is each kernel (test_mx4_calls_cpu.py holds that it is), with a 16-bit
+    bias; the layout's second call takes the kept template, on operands of other values."""
+    print(f"case {call} {plan}", flush=True)
+    m, n, k, wide, pair = call
+    for seed, dtype in enumerate((BF16, BF16, F16)):
+        g, a, b, sa, sb = _operands(m, n, k, wide, pair, seed)
+        bias = torch.randn(b.shape[0], generator=g).to(dtype)
+        c = mxfp4.gemm(*(t.to(DEV) for t in (a, b, sa, sb)), bias=bias.to(DEV), silu_mul=pair)
+        rows = torch.cat([torch.arange(0, 70), torch.arange(m // 2, m // 2 + 40), torch.arange(m - 70, m)]) if m > 200 else torch.arange(m)
+        _within(c[rows.to(DEV)], *O.gemm(a[rows], b, sa[rows], sb, bias, pair))
+
+
+def _forced(kernel, splits, a, b, sa, sb, n, k, bias=None, pair=False):
+    """A product on a kernel and split given, of operands as they stand (row strides, any scale address)."""
+    m = a.shape[0]
+    g = nat.HkxMx4GemmArgs()
+    g.size = ctypes.sizeof(g)
+    g.a_dtype = nat.FP8E4M3 if a.dtype == torch.float8_e4m3fn else nat.FP4E2M1
+    out = torch.full((m + 1, n + 8), 7.0, dtype=BF16, device=DEV)
+    g.a, g.b, g.sa, g.sb, g.c = (t.data_ptr() for t in (a, b, sa, sb, out))
+    g.lda, g.ldb, g.sa_ld, g.sb_ld, g.ldc = (t.stride(0) for t in (a, b, sa, sb, out))
+    g.m, g.n, g.k, g.silu_mul, g.kernel, g.splits = m, n, k, int(pair), kernel, splits
+    if bias is not None:
+        g.bias, g.bias_dtype = bias.data_ptr(), nat.dtype_code(bias.dtype)
+    need = nat.lib().hkx_mx4_gemm_workspace(g)
+    ws = torch.full((need // 4 + 4,), float("nan"), device=DEV)
+    g.ws, g.ws_bytes = ws.data_ptr(), need
+    nat.check(nat.lib().hkx_mx4_gemm(g, nat.stream_of(a.device)))
+    torch.cuda.synchronize()
+    assert (out[m] == 7.0).all() and (out[:, n:] == 7.0).all()  # (nothing stored past M and N)
+    return out[:m, :n]
+
+
+def _inside(t, width, fill, at=0, odd=0):
+    """t's rows inside wider ones of `fill`, `at` bytes from an aligned address, `odd` bytes a row more."""
+    rows, n = t.shape
+    big = torch.full((rows * (width + odd) + at + 64,), fill, dtype=torch.uint8, device=DEV)
+    v = big[at:at + rows * (width + odd)].view(rows, width + odd)[:, :n]
+    v.copy_(t.view(torch.uint8).to(DEV))
+    return v.view(t.dtype)
+
+
+@pytest.mark.parametrize("kernel", KERNELS)
+@pytest.mark.parametrize("wide", [False, True], ids=["a4", "a8"])
+@pytest.mark.parametrize("m,n,k,splits,pair", [(70, 264, 352, 1, False), (300, 520, 1056, 3, False), (13, 40, 96, 1, True),
+                                               (270, 264, 2208, 2, True), (300, 77, 4128, 1, False)])
+def test_every_kernel_reads_nothing_past_k(m, n, k, splits, pair, wide, kernel):
+    """Rows wider than K, NaN bytes and NaN scales past it, scale rows off a dword by their base and by their
+    stride; then a row of NaNs on each side: its own outputs alone are NaN."""
+    print(f"case past k {kernel} {m}x{n}x{k}/{splits} pair={pair} wide={wide}", flush=True)
+    g, a, b, sa, sb = _operands(m, n, k, wide, pair, 31)
+    rows = b.shape[0]
+    bias = torch.randn(rows, generator=g).to(F16).to(DEV)
+    ref, err = O.gemm(a, b, sa, sb, bias.cpu(), pair)
+    up16 = lambda x: (x + 47) // 16 * 16  # noqa: E731
+    at, odd = (1, 0) if m % 2 else (3, 1)
+    va, vb = _inside(a, up16(a.shape[1]), 0x7f), _inside(b, up16(k // 2), 0x7f)
+    vsa, vsb = _inside(sa, k // 32 + 4, 255, at, odd), _inside(sb, k // 32 + 4, 255, 4 - at, odd + 1)
+    if kernel == nat.MX4_SKINNY:
+        splits = 1
+    c = _forced(kernel, splits, va, vb, vsa, vsb, n, k, bias, pair)
+    _within(c, ref, err)
+    row, col = m // 2, n // 3
+    vsa[row] = 255
+    if wide:
+        va.view(torch.uint8)[row] = 0x7f
+    vsb[col] = 255
+    c = _forced(kernel, splits, va, vb, vsa, vsb, n, k, bias, pair).cpu().double()
+    nan = torch.zeros(m, n, dtype=torch.bool)
+    nan[row], nan[:, col] = True, True
+    assert torch.equal(torch.isnan(c), nan)
+    assert ((c - ref).abs() <= err)[~nan].all()
+
+
+@pytest.mark.parametrize("kernel", KERNELS)
+@pytest.mark.parametrize("wide", [False, True], ids=["a4", "a8"])
+def test_every_kernel_takes_extreme_scales_and_those_of_one_block(wide, kernel):
+    """Scale bytes 0 and 254 on opposite sides (their product is taken before fp32), and one block of one row
+    of each side scaled by 32, in every 32-K place of a unit."""
+    m, n, k = 270, 264, 800
+    g, a, b, sa, sb = _operands(m, n, k, wide, False, 32)
+    dev = [a.to(DEV), b.to(DEV)]
+    for lo, hi in ((0, 254), (254, 0)):
+        ta, tb = torch.full_like(sa, lo), torch.full_like(sb, hi)
+        _within(_forced(kernel, 1, *dev, ta.to(DEV), tb.to(DEV), n, k), *O.gemm(a, b, ta, tb))
+    for block in range(0, 25, 3):
+        ta, tb = sa.clone(), sb.clone()
+        ta[(37 * block) % m, block] += 5
+        tb[(53 * block) % n, 24 - block] += 5
+        _within(_forced(kernel, 1, *dev, ta.to(DEV), tb.to(DEV), n, k), *O.gemm(a, b, ta, tb))
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("kernel", KERNELS)
+@pytest.mark.parametrize("m,n,splits,pair", [(300, 264, 1, False), (300, 264, 2, False), (300, 263, 1, False),
+                                             (300, 136, 1, True), (300, 136, 2, True), (300, 135, 1, True)])
+def test_every_kernel_takes_every_bias(m, n, splits, pair, kernel, dtype):
+    """By its own epilogue and through shares: N a multiple of 8 or odd, where the up half's bias starts off
+    a dword."""
+    k = 1056
+    g, a, b, sa, sb = _operands(m, n, k, False, pair, 33)
+    bias = torch.randn(b.shape[0], generator=g).to(dtype)
+    if kernel == nat.MX4_SKINNY:
+        splits = 1
+    c = _forced(kernel, splits, *(t.to(DEV) for t in (a, b, sa, sb)), n, k, bias.to(DEV), pair)
+    _within(c, *O.gemm(a, b, sa, sb, bias, pair))
