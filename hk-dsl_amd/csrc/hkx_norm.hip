@@ -6,7 +6,8 @@
 namespace hkx {
 namespace {
 
-// Sums of rows of fp32 partial sums: out[g][c] = sum over i < count of src[g][i][c], in order.
+// Sums of rows of fp32 partial sums: out[g][c] = sum over i < count of src[g][i][c], in order and in 64 bits (in 32
+// dpost and dpre of 999 rows were 1.4e-7 off of their norm, so 7e-8; the same time).
 struct SumJob {
   const float* src;
   void* dst;
@@ -18,7 +19,7 @@ struct SumArgs {
 
 // A workgroup 64 columns of one sum, 16 waves a sixteenth of the rows each, joined in wave order.
 __global__ void __launch_bounds__(1024) norm_sum_kernel(const SumArgs p) {
-  __shared__ float part[16][64];
+  __shared__ double part[16][64];
   int y = blockIdx.y, k = 0;
   while (k < 2 && y >= p.job[k].groups) y -= p.job[k++].groups;
   const SumJob& j = p.job[k];
@@ -26,7 +27,7 @@ __global__ void __launch_bounds__(1024) norm_sum_kernel(const SumArgs p) {
   if ((int)blockIdx.x * 64 >= j.width || y >= j.groups) return;
   const int per = (j.count + 15) / 16, lo = min(wave * per, j.count), hi = min(lo + per, j.count);
   const float* src = j.src + (int64_t)y * j.count * j.width + col;
-  float s = 0.0f;
+  double s = 0.0;
   if (col < j.width) {
     int i = lo;
     for (; i + 8 <= hi; i += 8) {
@@ -43,10 +44,7 @@ __global__ void __launch_bounds__(1024) norm_sum_kernel(const SumArgs p) {
   if (wave || col >= j.width) return;
 #pragma unroll
   for (int w = 1; w < 16; ++w) s += part[w][lane];
-  const int64_t at = (int64_t)y * j.width + col;
-  if (j.dst_dt == HKX_FP32) ((float*)j.dst)[at] = s;
-  else if (j.dst_dt == HKX_BF16) ((uint16_t*)j.dst)[at] = (uint16_t)pack_bf16x2(s, 0.0f);
-  else ((uint16_t*)j.dst)[at] = (uint16_t)pack_f16x2(s, 0.0f);
+  store_one(j.dst, j.dst_dt, (int64_t)y * j.width + col, (float)s);
 }
 
 int es(int dt) { return dt == HKX_FP32 ? 4 : 2; }

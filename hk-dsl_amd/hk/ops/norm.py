@@ -17,7 +17,8 @@ quant="mxfp8" or "mxfp4" gives y as (q, s), the operand of an MX product (hk.ops
 another pass: q (..., D) float8_e4m3fn, or (..., D/2) packed codes, and s (..., D/32); D a multiple of 32.
 
 Differentiable in x, residual, post, pre and gate (not through a quantized y): one backward pass over the
-same bytes, with the gradients of post, pre and a broadcast gate summed in fp32 in a fixed order.
+same bytes, with the gradients of post, pre and a broadcast gate summed in a fixed order, a run of rows in
+fp32 and the runs in 64 bits.
 
 A call's checks and layout are kept by the shapes, strides and types they depend on, as a template of
 the library's arguments; a call of known layout fills in its addresses.

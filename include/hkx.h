@@ -404,7 +404,8 @@ int hkx_block_norm(const HkxBlockNormArgs* args, void* stream);
 /* Its gradients from dh and dy (NULL: zero): dx (x's type), dresidual (its type), dpost and dpre
  * (w_dtype), dgate (the gate's shape and type, summed over the rows and columns it is broadcast
  * over); dpost, dpre and dgate may be NULL. f as in the forward call, with its rstd; f's h, y and
- * y_scales are not used. Sums in fp32 in a fixed order: the same bits every call. */
+ * y_scales are not used. A run of rows is summed in fp32 and the runs in 64 bits, in a fixed
+ * order: the same bits every call. */
 typedef struct {
   int32_t size; /* sizeof(HkxBlockNormGradArgs) */
   int32_t reserved;

@@ -55,3 +55,19 @@ def test_a_norm_of_zeros_without_eps_is_nan_and_of_infinity_zero():
     x[1], x[2] = 1e30, 1.0  # (squares past fp32)
     h, _ = hk.ops.block_norm(x, torch.zeros_like(x), post=torch.ones(64, device=DEV), eps=0.0)
     assert torch.isnan(h[0]).all() and (h[1] == 0).all() and (h[2] == 1).all()
+
+
+@pytest.mark.parametrize("rows,d", [(400, 64), (4096, 200), (999, 1111), (16384, 40)])
+def test_sums_over_workers_lose_nothing(rows, d):
+    """A channel gate's gradient sums dh x over the rows: 2^24 from one row, 1 from each after the second,
+    which an fp32 sum of the workers' would drop one by one. The whole is rounded once."""
+    x = torch.ones(rows, d, device=DEV)
+    x[0], x[1] = 2.0 ** 12, 0.0
+    gate = torch.ones(d, device=DEV, requires_grad=True)
+    h, _ = hk.ops.block_norm(x, torch.zeros_like(x), gate=gate)
+    grad, = torch.autograd.grad(h, gate, x)
+    per = -(-rows // min(2048, (rows + 1) // 2))
+    if per <= 2:  # (a worker's own sum is of fp32)
+        assert (grad == torch.tensor(2.0 ** 24 + rows - 2, dtype=torch.float64).float().item()).all()
+    else:         # (those of the first worker's rows alone)
+        assert ((grad.double() - 2.0 ** 24 - rows + 2).abs() <= per).all()
