@@ -6,7 +6,7 @@
 // rounded to the nearest even e4m3, scale byte clamp(e + 127, 0, 254). The block's largest
 // value lands at or below 448, so nothing is clamped but a rounding at the top. An infinity or a
 // NaN becomes +-448. The NANS form is block_norm's (hkx_mx_block.hpp): such a block is NaN, and e is at
-// least -127 in the codes too; every other block is the same.
+// least -127 in the codes too; every other block is the same (4096 x 4096 12.3 us, 11.9 without).
 //
 // A workgroup 512 consecutive 16-byte pieces (8 values) of the row-major piece index, each
 // thread two of them 256 apart, both loaded before either is quantized; a piece's row is a

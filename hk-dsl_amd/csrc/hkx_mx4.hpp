@@ -61,9 +61,11 @@ HKX_DEV uint32_t mx4_mask(int left) { return left >= 4 ? 0xffffffffu : left <= 0
 //   k-step, after the unit's one barrier (read just before them, 4096 x 4096 of 4-bit K = 12288 at M =
 //   777 took 39.6 us). After that barrier the unit's stage takes the fills of unit t + NST; a wave
 //   waits for its own fills of the next unit only (buffer loads land in order).
-// * Measured: 777 x 4096 x 12288 of 4 bits 39-41 us on 128 x 128 tiles (2.0 PFLOP/s), 128 x 4096 x 12288 in
-//   four splits 17.4; bound by the fills, some 48 bytes a ns and CU whether all CUs run or 32 (32 KB a unit
-//   of 128 x 128): without them 777 rows took 36 us, on 64 x 128 tiles 28.
+// * Measured: 777 x 4096 x 12288 of 4 bits 38.0 us on 128 x 128 tiles (2.1 PFLOP/s), 128 x 4096 x 12288 in
+//   four splits on 64 x 128 ones 16.9. Bound by what a unit's fills and scales take beside its MFMAs, a SIMD
+//   having one wave and nothing else to run: copies with work left out, where the whole took 44.8 (64 x 128
+//   tiles 46.2): no fills 30.7 (31.0), no scales 33.9 (41.0), neither 25.3 (24.4), no fragment reads 39.8
+//   (43.9), the MFMAs alone 20.5 (20.2).
 // * RES = 2: two workgroups a CU, for grids of more than one a CU, in half the LDS.
 template <int BM, int BN, bool A8, bool PAIR, bool SHARE, int RES>
 __global__ void __launch_bounds__(256, RES) mx4_tile_kernel(const Mx4Args p) {

@@ -28,8 +28,9 @@
 //
 // Measured: 4096 x 12288 x 4096 of 4 bits 102-110 us (3.8-4.0 PFLOP/s; 8192 cubed 261, 4.2), 2048 x 12288 x
 // 4096 paired with an 8-bit A 138 (3.0). Register-only loops of these MFMAs on random operands reach 6.97
-// and 4.26 PFLOP/s. What bounds it is the power-limited clock: 8192 cubed with operands of zeros takes 205
-// us; without its MFMAs 183, without its fills 218 (zeros: 161), without either 101.
+// and 4.26 PFLOP/s. Two bounds lie close together: the power-limited clock (8192 cubed with operands of zeros
+// takes 205 us) and fills with LDS reads (without its MFMAs 183-185, zeros or not, where the MFMAs alone need
+// 158 at that rate); without its fills 218 (zeros: 161), without fills and MFMAs 101.
 //
 // K past its end: as in hkx_mx4.hpp (scales of 0, an 8-bit A's pieces out of range); an 8-bit A
 // takes two steps of a unit even where K ends in its first.

@@ -28,18 +28,22 @@ inline int mx4_splits(int kernel, int units, int s) {
   return (units + per - 1) / per;
 }
 
-// Whether a call runs on the decode kernel (workgroups of 16 rows of B and up to 64 of A); its rate over
-// the other kernels' best plan, cold weights (rows of B: twice the columns in the paired form):
-// * up to 32 rows of A, M = 1-8, 16, 24, 32. K to 4096: any up to M = 16; past it 1.10-1.8 to 16384 rows,
-//   0.77 at 20480, 0.58-0.83 at 28672. Past it A is streamed with every 16 rows of B: 4-bit A 1.36-1.63, 1.24-1.45,
-//   1.01-1.33, 0.92-1.28 to 4096 rows, 1.06-1.10, 0.93-1.03, 0.87-1.01, 0.8-0.96 at 8192, 0.98-1.08,
-//   0.86-0.93, .. at 16384; 8-bit A 1.26-1.52, 1.11-1.41, 0.86-1.15, 0.8-1.09 to 4096, 1.04-1.14, 0.89-1.05,
-//   0.72-0.81, .. at 8192, 0.92-1.02, 0.78-0.91, .. at 16384; both less the longer K;
-// * 33 to 64: K to 4096 1.10-1.96 to 16384 rows, 0.67 at 20480; past it 4-bit A 0.98-1.29 at K = 8192 to 4096
-//   rows and less at 12288, 8-bit A 0.78-0.98;
-// * 65 to 512: K to 4096 0.96-2.0 to two workgroups a CU (8-bit A past 256 rows of A: 0.83-0.97, and to one
-//   a CU 1.2-1.46), 0.58-1.24 past that; K = 8192 4-bit A 1.06-1.15 to one a CU and 256 rows of A, 0.78 past
-//   them, 8-bit A 0.92-0.95.
+// Whether a call runs on the decode kernel (workgroups of 16 rows of B and up to 64 of A). How many times its
+// time the plan takes that mx4_cost picks among the other kernels, from the least to the most of 1772 shapes
+// (512-28672 rows of B, K 1024-14336, cold weights; rows of B are twice the columns in the paired form):
+// * to 64 rows of A, K to 4096: 1.08-2.46 to 16384 rows of B; 20480 and 28672 rows 1.05-1.86 and 0.87-1.82
+//   (medians 1.1, 1.0) to M = 16, 0.38-0.99 past it;
+// * K past 4096, where A is streamed with every 16 rows of B, M to 8: 4-bit A 1.03-1.72 to 16384 rows, 0.65-1.23
+//   past them, 8-bit A 1.06-1.56 to 8192, 0.57-1.36 past; M = 9-16: 0.99-1.71 to 4096 rows, at 8192 0.97-1.15 to
+//   K = 8192 and 0.90-1.16 past it, 0.51-1.31 from 12288 on; M = 17-32 to 4096 rows: 4-bit A 1.06-1.48 to K =
+//   8192, 0.82-1.21 past it, 8-bit A 0.91-1.17 to 6144, 0.69-1.12 past it; more rows 0.30-1.25; M = 33-64: 4-bit
+//   A 0.99-1.51 to 4096 rows and K = 8192, else 0.36-1.10; 8-bit A 0.28-1.21. Where it is above 1 and not
+//   taken it is mostly the pick's split: the best other plan of 12288 rows and more takes 1.15 at most;
+// * 65 to 512 rows of A, K to 4096: to one workgroup a CU 1.32-2.24, to two 1.12-1.58 (4-bit A), 0.86-1.46 (8-bit
+//   to 256 rows of A) and 0.88-1.41 (past them), past two 0.26-1.18; K 5120-8192 of 4 bits to one a CU
+//   0.95-1.35 to 256 rows of A and 1.15-1.27 past them, to two 0.67-1.02; 8-bit A 0.52-1.03.
+// Both choices together take 1.03 times the best plan's time on average, 1.22 at the 95th hundredth (1.015 and
+// 1.09 past 64 rows of A).
 inline bool mx4_skinny_wins(int m, int rows, int k, bool a8, int cus) {
   const int64_t wgs = (int64_t)((m + 63) / 64) * ((rows + 15) / 16);
   if (m > 64 && k <= 4096) return m <= 512 && wgs <= (a8 && m > 256 ? cus : 2 * cus);
@@ -54,10 +58,11 @@ inline bool mx4_skinny_wins(int m, int rows, int k, bool a8, int cus) {
 // A plan's estimated time in us: a launch, more for each further wave of workgroups, a time a 256-K unit
 // and wave and one for its share of the memory's traffic, and where it goes through fp32 shares their
 // sum's launch and their round trip. Fitted to 1740 timed plans (M 33-4096, N 512-24576, K 512-12288,
-// weights past the cache): medians 0.98-1.00 of the times, 0.85-0.92 and 1.06-1.12 at the tenths; the
-// plans it picks take 1.008 times the best one's on average. Waves are whole ones also where two workgroups
-// share a CU (0.83 of their number past one, as fitted before, picked plans of 1.02 times: 777 x 4096 x
-// 12288 of 4 bits as 448 workgroups 45.1 us, as 224 38.7). A C of odd columns or alignment goes through
+// weights past the cache); over 2168 timed since the tiles' scales come by four threads a row: medians
+// 1.00-1.02 of the times, 0.85-0.94 and 1.13-1.24 at the tenths; the plans it picks take 1.005 times the best
+// one's on average, 1.04 at the 95th hundredth (M to 32, not fitted: 1.07 and 1.33). Waves are whole ones also
+// where two workgroups share a CU (0.83 of their number past one, as fitted before, picked plans of 1.02
+// times: 777 x 4096 x 12288 of 4 bits as 448 workgroups 45.1 us, as 224 38.7). A C of odd columns or alignment goes through
 // shares on the quadrant kernel always (stored from its registers two bytes at a time 3000 x 1001 took 25
 // us more).
 inline double mx4_cost(int kernel, int m, int n, int k, bool a8, bool pair, bool vec, int splits, int cus) {

@@ -155,7 +155,7 @@ def _dequant(call, q, s, dtype, code, per):
     k = per * kb
     if k % 32 or k == 0:
         raise ValueError(f"{call}: K={k}, a multiple of 32")
-    if s.dtype == torch.float8_e8m0fnu:
+    if s.dtype != torch.uint8 and s.dtype == torch.float8_e8m0fnu:
         s = s.view(torch.uint8)
     if s.dtype != torch.uint8 or s.shape[:-1] != lead or s.dim() < 1 or s.shape[-1] != k // 32:
         raise ValueError(f"{call}: s is uint8 or float8_e8m0fnu {(*lead, k // 32)}, got {s.dtype} {tuple(s.shape)}")

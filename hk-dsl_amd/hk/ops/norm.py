@@ -10,7 +10,8 @@ scaled residual add, and the norm before the next.
 with rms(v) = sqrt(mean(v^2) + eps) over the last dimension. x (..., D) is bf16, fp16 or fp32 and y the
 same; the residual stream and h have x's type or are fp32; post and pre (D,) and the gate have x's type
 or are fp32. The gate is broadcast over x: (D,), (B, 1, D), (B, S, 1), (B, S, D) and the like -- its
-leading sizes are x's, then ones. Sums and both norms are fp32; h is rounded only as it is stored.
+leading sizes are x's, then ones. A row's sums are fp32, the norms' factors made in 64 bits and rounded once;
+h is rounded only as it is stored.
 D up to 16384 (8192 where gradients are taken).
 
 quant="mxfp8" or "mxfp4" gives y as (q, s), the operand of an MX product (hk.ops.mxfp4.gemm), without
