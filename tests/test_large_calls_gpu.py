@@ -12,6 +12,12 @@ DEV = "cuda:0"
 BF16 = torch.bfloat16
 
 
+@pytest.fixture(autouse=True)
+def _hand_the_memory_back():
+    yield
+    torch.cuda.empty_cache()
+
+
 def _free(need):
     torch.cuda.empty_cache()
     if torch.cuda.mem_get_info()[0] < need * 2 ** 30:
