@@ -1,0 +1,356 @@
+// Products of ragged groups of rows, each with its expert's matrix: rows offsets[e] .. offsets[e + 1] of R are
+// expert e's, and the counts are known to the GPU alone.
+//
+//   NT  C[r] = A[r or index[r]] . B_e^T (+ bias_e), B_e (N, K): the experts' products, silu(gate) up of B_e's two
+//       halves, fp8 operands with a scale a row of A and a row of B_e
+//   NN  C[r] = A[r] . B_e,                          B_e (K, N): the gradient of their rows
+//   TN  C_e  = sum over the group's rows of A[r]^T B[r], (M, N): the gradient of their weights
+//
+// K is the contracted size; in TN it is a group's rows. A tile of C belongs to one expert: a group's last tile
+// may be ragged, and a grid is sized for the most tiles that R rows in E groups can make; where the counts
+// make fewer, the rest end at once. The rows behind the last group are one more group, whose A reads as
+// zeros.
+//
+// Operands reach LDS by 16-byte DMA through a buffer resource a tile, made from 64-bit addresses (an operand may
+// be larger than 4 GiB) and bounded by the tile's own rows: what lies past a group's rows, past N or past K reads 0.
+// Bad offsets are clamped to 0 .. R and an index past A's rows reads 0: no access leaves an operand.
+#pragma once
+
+#include "hkx_device.hpp"
+#include "hkx_ring.hpp"
+
+namespace hkx {
+
+constexpr int kGroupNT = 0, kGroupNN = 1, kGroupTN = 2;
+constexpr int kMaxExperts = 1024;
+
+struct GroupArgs {
+  const uint8_t* a;
+  const uint8_t* b;
+  uint8_t* c;
+  uint8_t* z;              // the paired form's product before silu(gate) up (nullptr: not kept)
+  const int32_t* offsets;  // E + 1
+  const int32_t* index;    // NT: the row of A of each row (nullptr: its own)
+  const void* bias;        // (E, N), N in the paired form 2 N
+  const float* sa;         // fp8: a scale a row of A (sa_ld 1) or one (0)
+  const float* sb;         // fp8: sb[e sb_ld + n sb_col]
+  int64_t lda, ldb, ldc, ldz;  // bytes a row
+  int64_t b_group, c_group;    // bytes an expert (NT and NN: B; TN: C)
+  int64_t bias_ld, sb_ld;      // elements an expert
+  int32_t experts, rows, a_rows;
+  int32_t m, n, k;   // m: TN's rows of C; n: C's columns (paired: of silu(gate) up); k: NT's and NN's contraction
+  int32_t tail;      // 1: the rows behind the last group are written too, with zeros
+  int32_t bias_dt, sa_ld, sb_col;
+};
+
+// ---------------------------------------------------------------- which tile is whose
+//
+// LDS: the first tile row of each group (first[0 .. groups]), made once a workgroup from the offsets.
+
+struct GroupMap {
+  int first[kMaxExperts + 2];
+};
+
+// Group g's rows of R; group `experts` are the rows behind the last.
+HKX_DEV void group_rows(const GroupArgs& p, int g, int& lo, int& hi) {
+  lo = min(max(p.offsets[g], 0), p.rows);
+  hi = g < p.experts ? min(max(p.offsets[g + 1], lo), p.rows) : p.tail ? p.rows : lo;
+}
+
+// `threads` threads build the map of tiles of BM rows; ends with a barrier.
+template <int BM>
+HKX_DEV void group_map(GroupMap& s, const GroupArgs& p, int tid, int threads) {
+  const int groups = p.experts + 1;
+  for (int g = tid; g < groups; g += threads) {
+    int lo, hi;
+    group_rows(p, g, lo, hi);
+    s.first[g + 1] = (hi - lo + BM - 1) / BM;
+  }
+  if (tid == 0) s.first[0] = 0;
+  __syncthreads();
+  if (tid < 64) {
+    int sum = 0;
+    for (int g = 0; g < groups; g += 64) {
+      int v = g + tid < groups ? s.first[g + tid + 1] : 0;
+#pragma unroll
+      for (int d = 1; d < 64; d <<= 1) {
+        const int u = __shfl_up(v, d);
+        if (tid >= d) v += u;
+      }
+      if (g + tid < groups) s.first[g + tid + 1] = sum + v;
+      sum += __shfl(v, 63);
+    }
+  }
+  __syncthreads();
+}
+
+// The group of tile row i (a wave's lanes look together).
+HKX_DEV int group_of(const GroupMap& s, int groups, int i) {
+  int e = 0;
+  const int lane = threadIdx.x & 63;
+  for (int g = 0; g < groups; g += 64)
+    e += __popcll(__ballot(g + lane < groups && s.first[g + lane + 1] <= i));
+  return __builtin_amdgcn_readfirstlane(e);
+}
+
+// Consecutive tiles on one XCD (workgroup v runs on XCD v % 8): the place of v among `total` tiles, or -1.
+HKX_DEV int group_place(int v, int total) {
+  const int per = (total + 7) >> 3, at = (v & 7) * per + (v >> 3);
+  return (v >> 3) < per && at < total ? at : -1;
+}
+
+constexpr uint32_t kGroupOut = 0xfffffff0u;  // an offset past every resource: reads 0
+
+// A resource of `rows` rows of `row` bytes, `ld` apart, from a 64-bit address (0 rows: reads 0).
+HKX_DEV __amdgpu_buffer_rsrc_t group_rsrc(const uint8_t* p, int rows, int64_t ld, uint32_t row) {
+  return make_rsrc(p, rows > 0 ? (uint32_t)((rows - 1) * ld) + row : 0u);
+}
+
+// ---------------------------------------------------------------- fragments in LDS
+//
+// A K unit is 128 bytes: 64 bf16 or 128 fp8.
+// * K-contiguous rows: 128 bytes a row, its 16-byte chunk c at c ^ (row % 8). A fill instruction moves 8 rows.
+// * rows along K (NN's B, TN's A and B): 64 rows of 128 values, 256 bytes; the 32-byte pair of chunks j (16 values, a
+//   fragment's columns) at j ^ group_swz(row), so that the four rows that 16 lanes read, and those of the next
+//   16, lie in different banks. A fill instruction moves 4 rows. ds_read_tr16_b64 turns them: of 16 lanes, lane i names
+//   row i / 4, values 4 (i % 4) + [0, 4), and is given value i of the four rows.
+
+HKX_DEV uint32_t group_swz(uint32_t k) { return (k & 3) | ((k >> 1) & 4); }
+
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+
+HKX_DEV s16x4 read_turned(const uint8_t* s) {
+  return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)s);
+}
+
+// The product on BM x BN tiles, BN = 16 FN WN rows of B: WM x WN waves of BM / WM rows and 16 FN columns, S stages
+// of a K unit.
+template <int OP, bool FP8, bool PAIR, int BM, int WM, int WN, int FN, int S>
+__global__ void __launch_bounds__(64 * WM * WN) group_tile_kernel(const GroupArgs p) {
+  constexpr int NW = WM * WN, BN = 16 * FN * WN, CN = PAIR ? BN / 2 : BN;
+  constexpr int FM = BM / WM / 16;
+  constexpr bool TA = OP == kGroupTN, TB = OP != kGroupNT;
+  constexpr int ES = FP8 ? 1 : 2, KU = 128 / ES;  // values a K unit
+  constexpr int AB = BM * 128, BB = BN * 128, STAGE = AB + BB;
+  constexpr int IA = AB / 1024, IB = BB / 1024;                 // fill instructions of a stage
+  constexpr int WA = (IA + NW - 1) / NW, WB = (IB + NW - 1) / NW;  // and of a wave
+  constexpr int KH = FP8 ? 1 : 2;
+  static_assert(!FP8 || OP == kGroupNT, "8-bit operands: the forward product");
+  static_assert(!TB || BN == 128, "rows along K: 128 values");
+  static_assert(!TA || BM == 128, "rows along K: 128 values");
+  static_assert(!PAIR || (FN % 2 == 0 && OP == kGroupNT), "gate and up fragments of one wave");
+  __shared__ __attribute__((aligned(16))) uint8_t smem[S * STAGE];
+  __shared__ GroupMap map;
+
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wr = wave / WN, wc = wave % WN;
+  const int tiles_n = (p.n + CN - 1) / CN;
+
+  // ---- the tile: group e, its rows [m0, m0 + mrows) of C, columns n0 .., the contraction's length
+  int e, m0, mrows, n0, klen;
+  int64_t row0 = 0;  // the group's first row of R (TN: of the contraction; else of the tile)
+  if constexpr (TA) {
+    const int tiles_m = (p.m + BM - 1) / BM, per = tiles_m * tiles_n;
+    const int at = group_place((int)blockIdx.x, p.experts * per);
+    if (at < 0) return;
+    e = at / per;
+    m0 = (at % per) % tiles_m * BM;
+    n0 = (at % per) / tiles_m * CN;
+    mrows = min(p.m - m0, BM);
+    int lo, hi;
+    group_rows(p, e, lo, hi);
+    row0 = lo;
+    klen = hi - lo;
+  } else {
+    const int groups = p.experts + 1;
+    group_map<BM>(map, p, tid, 64 * NW);
+    const int at = group_place((int)blockIdx.x, map.first[groups] * tiles_n);
+    if (at < 0) return;
+    // (tile rows fastest: tiles that share a panel of B follow one another)
+    e = group_of(map, groups, at / tiles_n);
+    const int t0 = map.first[e], tm = map.first[e + 1] - t0, in = at - t0 * tiles_n;
+    m0 = in % tm * BM;
+    n0 = in / tm * CN;
+    int lo, hi;
+    group_rows(p, e, lo, hi);
+    row0 = lo + m0;
+    mrows = min(hi - (int)row0, BM);
+    klen = p.k;
+  }
+  const bool rest = e == p.experts;  // the rows behind the last group
+  const int nku = rest ? 0 : (klen + KU - 1) / KU;
+
+  // ---- fills
+  __amdgpu_buffer_rsrc_t ra, rb;
+  uint32_t va[WA], vb[WB], ca[WA], cb[WB];  // offsets; bytes along K of K-contiguous rows
+#pragma unroll
+  for (int i = 0; i < WA; ++i) {
+    const int ins = (wave + NW * i) % IA;
+    if constexpr (TA) {
+      const uint32_t k = 4 * ins + lane / 16, c = (lane % 16) ^ (group_swz(k) << 1);
+      va[i] = k * (uint32_t)p.lda + c * 16;
+    } else {
+      const int r = 8 * ins + lane / 8;
+      ca[i] = ((lane % 8) ^ (r % 8)) * 16;
+      int64_t at = r;
+      if (OP == kGroupNT && p.index) {
+        const int j = r < mrows ? p.index[row0 + r] : -1;
+        at = (uint32_t)j < (uint32_t)p.a_rows ? j : -1;
+      }
+      va[i] = at < 0 ? kGroupOut : (uint32_t)(at * p.lda) + ca[i];
+    }
+  }
+  if constexpr (TA) {
+    ra = make_rsrc(nullptr, 0);
+    rb = make_rsrc(nullptr, 0);
+  } else {
+    const uint32_t row = (uint32_t)p.k * ES;
+    ra = OP == kGroupNT && p.index ? group_rsrc(p.a, p.a_rows, p.lda, row) : group_rsrc(p.a + row0 * p.lda, mrows, p.lda, row);
+    if constexpr (TB) rb = make_rsrc(nullptr, 0);
+    else rb = group_rsrc(p.b + (rest ? 0 : e) * p.b_group + n0 * p.ldb, (PAIR ? p.n : 0) + min(p.n - n0, CN), p.ldb, row);
+  }
+#pragma unroll
+  for (int i = 0; i < WB; ++i) {
+    const int ins = (wave + NW * i) % IB;
+    if constexpr (TB) {
+      const uint32_t k = 4 * ins + lane / 16, c = (lane % 16) ^ (group_swz(k) << 1);
+      vb[i] = k * (uint32_t)p.ldb + c * 16;
+    } else {
+      const int r = 8 * ins + lane / 8, f = r / 16;
+      cb[i] = ((lane % 8) ^ (r % 8)) * 16;
+      // paired: fragments of gate rows and up rows by turns
+      const int at = PAIR ? 16 * (f / 2) + r % 16 + (f & 1) * p.n : r;
+      vb[i] = (uint32_t)at * (uint32_t)p.ldb + cb[i];
+    }
+  }
+  // rows along K: a resource a unit, of the rows that are left
+  auto along = [&](const uint8_t* base, int64_t first, int left, int64_t ld, int cols, int col0) {
+    return group_rsrc(base + first * ld + (int64_t)col0 * 2, min(left, 64), ld, (uint32_t)(cols - col0) * 2u);
+  };
+  auto fill = [&](int t) {
+    uint8_t* s = smem + (t % S) * STAGE;
+    const bool in = t < nku;
+    const uint32_t k0 = (uint32_t)t * 128u;  // bytes along K
+    if constexpr (TA) ra = along(p.a, row0 + 64 * (int64_t)t, in ? klen - 64 * t : 0, p.lda, p.m, m0);
+    if constexpr (TB) {
+      const int64_t first = (int64_t)64 * t;
+      rb = TA ? along(p.b, row0 + first, in ? klen - 64 * t : 0, p.ldb, p.n, n0)
+              : along(p.b + (rest ? 0 : e) * p.b_group, first, in ? klen - 64 * t : 0, p.ldb, p.n, n0);
+    }
+    const uint32_t row = (uint32_t)klen * ES;
+#pragma unroll
+    for (int i = 0; i < WA; ++i) {
+      const int ins = (wave + NW * i) % IA;
+      if constexpr (TA) buf_load16_lds(ra, s + ins * 1024, va[i], 0);
+      else buf_load16_lds(ra, s + ins * 1024, in && k0 + ca[i] < row ? va[i] : kGroupOut, in ? k0 : 0);
+    }
+#pragma unroll
+    for (int i = 0; i < WB; ++i) {
+      const int ins = (wave + NW * i) % IB;
+      if constexpr (TB) buf_load16_lds(rb, s + AB + ins * 1024, vb[i], 0);
+      else buf_load16_lds(rb, s + AB + ins * 1024, in && k0 + cb[i] < row ? vb[i] : kGroupOut, in ? k0 : 0);
+    }
+  };
+
+  // ---- fragments: lane (rf, q) row rf, K 8 q + [0, 8) of a K-half (fp8: 16 bytes of each half)
+  const int rf = lane & 15, q = lane >> 4;
+  using Frag = typename std::conditional<FP8, i32x8, bf16x8>::type;
+  auto straight = [&](const uint8_t* s, int r0, int h) -> Frag {  // r0 a multiple of 16
+    const uint8_t* row = s + (r0 + rf) * 128;
+    if constexpr (FP8) {
+      const i32x4 lo = *(const i32x4*)(row + ((q ^ (rf & 7)) << 4)), hi = *(const i32x4*)(row + (((4 + q) ^ (rf & 7)) << 4));
+      return i32x8{lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+    } else {
+      return *(const bf16x8*)(row + (((4 * h + q) ^ (rf & 7)) << 4));
+    }
+  };
+  auto turned = [&](const uint8_t* s, int r0, int h) -> Frag {
+    s16x4 v[2];
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const uint32_t k = 32 * h + 8 * q + 4 * t + rf / 4;
+      v[t] = read_turned(s + k * 256 + (((uint32_t)r0 / 16) ^ group_swz(k)) * 32 + (rf % 4) * 8);
+    }
+    typedef short s16x8 __attribute__((ext_vector_type(8)));
+    if constexpr (FP8) return Frag{};
+    else return __builtin_bit_cast(bf16x8, __builtin_shufflevector(v[0], v[1], 0, 1, 2, 3, 4, 5, 6, 7));
+  };
+
+  f32x4 acc[FM][FN] = {};
+  constexpr int NF = WA + WB;
+#pragma unroll
+  for (int t = 0; t < S - 1; ++t) fill(t);
+  for (int t = 0; t < nku; ++t) {
+    // stage t has landed in every wave, and stage t - 1 is read
+    __builtin_amdgcn_sched_barrier(0);
+    __builtin_amdgcn_s_waitcnt(wait_vm_lgkm0((S - 2) * NF));
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_sched_barrier(0);
+    fill(t + S - 1);
+    const uint8_t* s = smem + (t % S) * STAGE;
+#pragma unroll
+    for (int h = 0; h < KH; ++h) {
+      Frag af[FM], bf[FN];
+#pragma unroll
+      for (int f = 0; f < FM; ++f) af[f] = TA ? turned(s, wr * (BM / WM) + 16 * f, h) : straight(s, wr * (BM / WM) + 16 * f, h);
+#pragma unroll
+      for (int g = 0; g < FN; ++g) bf[g] = TB ? turned(s + AB, (wc * FN + g) * 16, h) : straight(s + AB, (wc * FN + g) * 16, h);
+#pragma unroll
+      for (int f = 0; f < FM; ++f)
+#pragma unroll
+        for (int g = 0; g < FN; ++g) {
+          if constexpr (FP8) acc[f][g] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(bf[g], af[f], acc[f][g], 0, 0, 0, 0, 0, 0);
+          else acc[f][g] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(bf[g], af[f], acc[f][g], 0, 0, 0);
+        }
+    }
+  }
+  __builtin_amdgcn_s_waitcnt(wait_vm(0));  // no fill lands in LDS after the exit
+
+  // ---- C: lane (rf, q) holds row rf, columns 4 q + [0, 4) of each fragment
+  const int64_t c_row = TA ? (int64_t)m0 : row0;
+  uint8_t* const c0 = p.c + (TA ? e * p.c_group : 0);
+#pragma unroll
+  for (int f = 0; f < FM; ++f) {
+    const int r = wr * (BM / WM) + 16 * f + rf;
+    if (r >= mrows) continue;
+    uint8_t* const row = c0 + (c_row + r) * p.ldc;
+    float sa = 1.0f;
+    if (FP8 && !rest) {
+      int64_t at = p.index ? p.index[row0 + r] : row0 + r;
+      const bool in = !p.index || (uint32_t)at < (uint32_t)p.a_rows;
+      sa = in ? p.sa[at * p.sa_ld] : 0.0f;
+    }
+    auto finish = [&](f32x4 v, int n) {  // n: B_e's row
+      if (FP8 && !rest) {
+        const float* sb = p.sb + e * p.sb_ld;
+        if (p.sb_col) v *= *(const f32x4*)(sb + n) * sa;
+        else v *= sb[0] * sa;
+      }
+      if (OP == kGroupNT && p.bias && !rest) v += ld4(p.bias, p.bias_dt, e * p.bias_ld + n);
+      return v;
+    };
+#pragma unroll
+    for (int g = 0; g < FN; g += PAIR ? 2 : 1) {
+      const int n = n0 + (PAIR ? (wc * FN + g) / 2 * 16 : (wc * FN + g) * 16) + 4 * q;
+      if (n >= p.n) continue;
+      f32x4 v = finish(acc[f][g], n);
+      if constexpr (PAIR) {
+        const f32x4 u = finish(acc[f][g + 1], n + p.n);
+        if (p.z) {
+          store4(p.z + (c_row + r) * p.ldz, HKX_BF16, n, v);
+          store4(p.z + (c_row + r) * p.ldz, HKX_BF16, n + p.n, u);
+        }
+        v = silu_mul4(v, u);
+      }
+      store4(row, HKX_BF16, n, v);
+    }
+  }
+}
+
+// The tiles that R rows in E groups can make at most, of bm rows (and the rows behind them).
+inline int64_t group_tiles(int64_t rows, int64_t experts, int64_t bm) {
+  return rows / bm + (rows < experts ? rows : experts) + 1;
+}
+
+}  // namespace hkx

@@ -1,0 +1,34 @@
+// Host-side launchers of the experts' products, one translation unit a kind of tile.
+#pragma once
+
+#include "hkx_group.hpp"
+
+namespace hkx {
+
+// hipErrorInvalidConfiguration: more tiles than a launch takes.
+hipError_t launch_group(const GroupArgs& a, int op, bool fp8, bool pair, int kernel, int cus, hipStream_t s);
+
+// bm: 16, 64 or 128 rows (TN: 128)
+hipError_t launch_group_nt(const GroupArgs& a, bool fp8, bool pair, int bm, hipStream_t s);
+hipError_t launch_group_grad(const GroupArgs& a, int op, int bm, hipStream_t s);
+
+// A grid of `tiles` workgroups and the places that their order over the XCDs leaves open.
+inline bool group_grid(int64_t tiles, int threads, dim3& grid) {
+  const int64_t n = (tiles + 7) / 8 * 8;
+  if (n * threads >= ((int64_t)1 << 32) || n > INT32_MAX) return false;
+  grid = dim3((unsigned)n);
+  return true;
+}
+
+template <int OP, bool FP8, bool PAIR, int BM, int WM, int WN, int FN, int S>
+hipError_t launch_group_tile(const GroupArgs& a, hipStream_t s) {
+  constexpr int CN = 16 * FN * WN / (PAIR ? 2 : 1);
+  const int64_t tn = (a.n + CN - 1) / CN;
+  dim3 grid;
+  const int64_t tiles = OP == kGroupTN ? (int64_t)a.experts * ((a.m + BM - 1) / BM) * tn : group_tiles(a.rows, a.experts, BM) * tn;
+  if (!group_grid(tiles, 64 * WM * WN, grid)) return hipErrorInvalidConfiguration;
+  hipLaunchKernelGGL((group_tile_kernel<OP, FP8, PAIR, BM, WM, WN, FN, S>), grid, dim3(64 * WM * WN), 0, s, a);
+  return hipGetLastError();
+}
+
+}  // namespace hkx

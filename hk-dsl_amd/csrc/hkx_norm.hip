@@ -145,16 +145,17 @@ int hkx_block_norm(const HkxBlockNormArgs* args, void* stream) {
   if (int rc = forward_args(g, "block_norm", a)) return rc;
   if (g.d > kNormMaxD) return api_fail(HKX_ERR_SHAPE, "block_norm: d=%d, at most %d", g.d, kNormMaxD);
   if (!g.h || (g.pre && !g.y)) return api_fail(HKX_ERR_ARG, "block_norm: a null output");
-  if (g.quant < 0 || g.quant > 2) return api_fail(HKX_ERR_ARG, "block_norm: quant=%d", g.quant);
+  if (g.quant < 0 || g.quant > 4 || g.quant == 3) return api_fail(HKX_ERR_ARG, "block_norm: quant=%d", g.quant);
   if (g.quant && (!g.pre || !g.y_scales)) return api_fail(HKX_ERR_ARG, "block_norm: a quantized y needs pre and its scales");
   const int64_t ybytes = g.quant == 2 ? g.d / 2 : g.d;
-  if (g.ldh < g.d || (g.pre && g.ldy < ybytes) || (g.quant && g.ldys < g.d / 32))
+  if (g.ldh < g.d || (g.pre && g.ldy < ybytes) || ((g.quant == 1 || g.quant == 2) && g.ldys < g.d / 32))
     return api_fail(HKX_ERR_SHAPE, "block_norm: row strides below d");
   if (g.rows == 0) return HKX_OK;
   if (g.quant) {
-    if (g.d % 32) return api_fail(HKX_ERR_SHAPE, "block_norm: d=%d, a multiple of 32 where y is quantized", g.d);
+    if (g.quant != 4 && g.d % 32) return api_fail(HKX_ERR_SHAPE, "block_norm: d=%d, a multiple of 32 where y is quantized", g.d);
+    if (g.quant == 4 && !api_aligned(g.y_scales, 4)) return api_fail(HKX_ERR_SHAPE, "block_norm: the rows' scales need 4-byte alignment");
     const int64_t al = g.quant == 2 ? 4 : 8;
-    if (!norm_vec_ok(a, es(g.x_dtype), es(g.r_dtype), es(g.w_dtype), es(g.gate_dtype)) || !api_aligned(g.y, al) || g.ldy % al)
+    if (g.quant != 4 && (!norm_vec_ok(a, es(g.x_dtype), es(g.r_dtype), es(g.w_dtype), es(g.gate_dtype)) || !api_aligned(g.y, al) || g.ldy % al))
       return api_fail(HKX_ERR_SHAPE, "block_norm: a quantized y needs 16-byte aligned rows of every other operand");
   }
   const hipStream_t s = (hipStream_t)stream;

@@ -39,7 +39,7 @@ struct NormArgs {
   int32_t gate_dt;
   int32_t gate_rows;  // rows that share a gate's row
   int32_t gate_col;   // 1: a gate a column, 0: one a row
-  int32_t quant;      // 0: y as x's type, 1: MXFP8, 2: MXFP4
+  int32_t quant;      // 0: y as x's type, 1: MXFP8, 2: MXFP4, 4: e4m3 with a scale a row
   float bs, rs, eps;
   double inv_d;  // 1 / d
   int32_t row0;  // the launch's first row (forward)
@@ -69,6 +69,23 @@ struct NormGradArgs {
   int32_t group_rows;  // gate_rows (rows without a gate)
   NormShape shape;
 };
+
+// ---------------------------------------------------------------- a row in 8 bits under one scale
+//
+// s = max |v| / 448, rounded once, at least 2^-126 (v / s stays finite), 1 for a row of zeros and NaN for one that has an
+// infinity or a NaN; the codes are v / s, the quotient rounded to fp32 and then to e4m3.
+
+// top: the bits of the row's largest |v| (a NaN's above an infinity's).
+HKX_DEV float fp8_row_scale(uint32_t top) {
+  if (top >= 0x7f800000u) return __builtin_nanf("");
+  if (top == 0) return 1.0f;
+  return __builtin_fmaxf(__builtin_bit_cast(float, top) / 448.0f, 1.17549435e-38f);
+}
+
+HKX_DEV u32x2 fp8_row_codes(const float* v, float s) {
+  if (s != s) return u32x2{0u, 0u};
+  return u32x2{cvt_e4m3x4(v[0] / s, v[1] / s, v[2] / s, v[3] / s), cvt_e4m3x4(v[4] / s, v[5] / s, v[6] / s, v[7] / s)};
+}
 
 // ---------------------------------------------------------------- loads and stores of a thread's elements
 //
@@ -121,6 +138,20 @@ struct Cols {
       }
     }
     return o;
+  }
+  // piece c's 8 elements of a row of codes from column c0 on, under scale s
+  HKX_DEV void store8(uint8_t* q, int c0, const float* v, int c, float s) const {
+    if constexpr (VEC) {
+      const int i = 8 * (t + T * c);
+      if (i < d) *(u32x2*)(q + c0 + i) = fp8_row_codes(v, s);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        __builtin_amdgcn_sched_barrier(0);  // (one quotient at a time: all at once spilled)
+        const int i = t + T * (8 * c + j);
+        if (i < d) q[c0 + i] = s != s ? 0 : (uint8_t)cvt_e4m3x4(v[j] / s, 0.0f, 0.0f, 0.0f);
+      }
+    }
   }
   template <int DT>
   HKX_DEV void store(void* p, int64_t at, const Row& o) const {
@@ -176,6 +207,21 @@ HKX_DEV float wave_sum(float x) {
   return __builtin_bit_cast(float, (uint32_t)b[0]) + __builtin_bit_cast(float, (uint32_t)b[1]);
 }
 
+template <int CTRL>
+HKX_DEV uint32_t max_dpp(uint32_t x) {
+  return max(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, CTRL, 0xf, 0xf, true));
+}
+HKX_DEV uint32_t wave_max(uint32_t x) {
+  x = max_dpp<0xb1>(x);
+  x = max_dpp<0x4e>(x);
+  x = max_dpp<0x141>(x);
+  x = max_dpp<0x140>(x);
+  const auto a = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+  x = max((uint32_t)a[0], (uint32_t)a[1]);
+  const auto b = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+  return max((uint32_t)b[0], (uint32_t)b[1]);
+}
+
 // A sum over the row's threads, the same bits on each; `red`: 16 floats that no other sum uses
 // until a barrier has passed (unused where a row is a wave).
 template <bool WAVE>
@@ -219,6 +265,20 @@ HKX_DEV void store_quant(int quant, uint8_t* q, uint8_t* s, int i, const float (
   if ((i & 31) == 0) s[i / 32] = (uint8_t)sc;
 }
 
+// The largest of a row's threads' `top`; `red`: 16 words of its own.
+template <bool WAVE>
+HKX_DEV uint32_t row_top(uint32_t x, uint32_t* red) {
+  x = wave_max(x);
+  if constexpr (!WAVE) {
+    const int w = threadIdx.x >> 6, n = blockDim.x >> 6;
+    if ((threadIdx.x & 63) == 0) red[w] = x;
+    __syncthreads();
+    x = 0;
+    for (int i = 0; i < n; ++i) x = max(x, red[i]);
+  }
+  return x;
+}
+
 // The gate's values of a row: a column each, or one for all.
 template <int XT, int C, bool VEC>
 HKX_DEV typename Cols<C, VEC>::Row load_gate(const NormArgs& p, const Cols<C, VEC>& cols, int row) {
@@ -241,7 +301,8 @@ HKX_DEV void store_one(void* p, int dt, int64_t i, float v) {
 
 // ---------------------------------------------------------------- forward
 
-template <int XT, int RT, int WT, int C, bool VEC, bool WAVE>
+// Q8: y in 8 bits under one scale, of single elements (an instantiation of its own: beside the plain store it spilled).
+template <int XT, int RT, int WT, int C, bool VEC, bool WAVE, bool Q8 = false>
 __global__ void __launch_bounds__(WAVE ? 256 : 1024) norm_kernel(const NormArgs p) {
   constexpr int E = Cols<C, VEC>::E;
   __shared__ float red[2][16];
@@ -280,7 +341,16 @@ __global__ void __launch_bounds__(WAVE ? 256 : 1024) norm_kernel(const NormArgs 
     rh = row_factor(row_sum<WAVE>(s, red[1]), p);
 #pragma unroll
     for (int i = 0; i < E; ++i) r.v[i] *= rh * w2.v[i];
-    if (VEC && p.quant) {
+    if (VEC ? p.quant == 4 : Q8) {
+      __shared__ uint32_t most[16];
+      uint32_t top = 0;
+#pragma unroll
+      for (int i = 0; i < E; ++i) top = max(top, __builtin_bit_cast(uint32_t, r.v[i]) & 0x7fffffffu);
+      const float sc = fp8_row_scale(row_top<WAVE>(top, most));
+#pragma unroll
+      for (int c = 0; c < E / 8; ++c) cols.store8((uint8_t*)p.y + row * p.ldy, 0, &r.v[8 * c], c, sc);
+      if (cols.t == 0) ((float*)p.ys)[row] = sc;
+    } else if (VEC && p.quant) {
 #pragma unroll
       for (int c = 0; c < E / 8; ++c) {
         float v[8];
@@ -464,7 +534,7 @@ hipError_t launch_norm_grad_fp32(const NormGradArgs& a, hipStream_t s);
 inline bool norm_vec_ok(const NormArgs& a, int xs, int rs, int ws, int gs) {
   auto ok = [](const void* p, int64_t ld, int es) { return !p || (api_aligned(p, 16) && ld * es % 16 == 0); };
   return a.d % 8 == 0 && ok(a.x, a.ldx, xs) && ok(a.res, a.ldr, rs) && ok(a.h, a.ldh, rs) &&
-         (a.quant || ok(a.y, a.ldy, xs)) && ok(a.post, 0, ws) && ok(a.pre, 0, ws) &&
+         (a.quant ? a.quant != 4 || (api_aligned(a.y, 8) && a.ldy % 8 == 0) : ok(a.y, a.ldy, xs)) && ok(a.post, 0, ws) && ok(a.pre, 0, ws) &&
          (!a.gate || !a.gate_col || ok(a.gate, a.d, gs));
 }
 
@@ -489,13 +559,17 @@ hipError_t launch_norm_typed(NormArgs a, hipStream_t s) {
     const int rows = (int)std::min<int64_t>(most, a.rows - r);
     a.row0 = (int)r;
     const dim3 grid(wave ? (rows + 3) / 4 : rows), block(wave ? 256 : f.threads);
-#define HKX_NORM(C, V, W) hipLaunchKernelGGL((norm_kernel<XT, RT, WT, C, V, W>), grid, block, 0, s, a)
+#define HKX_NORM(...) hipLaunchKernelGGL((norm_kernel<XT, RT, WT, __VA_ARGS__>), grid, block, 0, s, a)
     if (f.vec) {
       if (!wave) HKX_NORM(2, true, false);
       else if (f.c == 1) HKX_NORM(1, true, true);
       else HKX_NORM(2, true, true);
     } else {
-      if (!wave) HKX_NORM(2, false, false);
+      if (a.quant == 4) {
+        if (!wave) HKX_NORM(2, false, false, true);
+        else if (f.c == 1) HKX_NORM(1, false, true, true);
+        else HKX_NORM(2, false, true, true);
+      } else if (!wave) HKX_NORM(2, false, false);
       else if (f.c == 1) HKX_NORM(1, false, true);
       else HKX_NORM(2, false, true);
     }

@@ -11,6 +11,7 @@ There is no fallback: if the library is not built, `lib()` raises and nothing ru
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import os
 import threading
@@ -105,13 +106,35 @@ class HkxBlockNormGradArgs(Structure):
                 ("ws_bytes", c_size_t)]
 
 
+class HkxExpertsGemmArgs(Structure):
+    _fields_ = [("size", c_int32), ("op", c_int32), ("ab_dtype", c_int32), ("experts", c_int32),
+                ("rows", c_int32), ("a_rows", c_int32), ("m", c_int32), ("n", c_int32),
+                ("k", c_int32), ("silu_mul", c_int32), ("zero_rest", c_int32),
+                ("bias_dtype", c_int32), ("sa_ld", c_int32), ("sb_col", c_int32),
+                ("kernel", c_int32), ("reserved", c_int32), ("a", c_void_p), ("b", c_void_p),
+                ("c", c_void_p), ("z", c_void_p), ("offsets", c_void_p), ("index", c_void_p),
+                ("bias", c_void_p), ("sa", c_void_p), ("sb", c_void_p), ("lda", c_int64),
+                ("ldb", c_int64), ("ldc", c_int64), ("ldz", c_int64), ("b_expert", c_int64),
+                ("c_expert", c_int64), ("bias_ld", c_int64), ("sb_ld", c_int64)]
+
+
+class HkxExpertsRouteArgs(Structure):
+    _fields_ = [("size", c_int32), ("dtype", c_int32), ("t", c_int32), ("e", c_int32),
+                ("k", c_int32), ("renormalize", c_int32), ("logits", c_void_p), ("ld", c_int64),
+                ("weights", c_void_p), ("chosen", c_void_p), ("offsets", c_void_p),
+                ("rows", c_void_p), ("slots", c_void_p), ("ws", c_void_p), ("ws_bytes", c_size_t)]
+
+
 #: Every function include/hkx.h declares.
 SYMBOLS = ("hkx_abi_version", "hkx_abi_sizes", "hkx_last_error", "hkx_gemm_workspace",
            "hkx_gemm_counters",
            "hkx_gemm_check", "hkx_gemm", "hkx_scaled_mm", "hkx_mx_gemm", "hkx_mx_gemm_workspace",
            "hkx_mx_quant", "hkx_mx_quant_nan", "hkx_gemm_noalloc", "hkx_mx4_quant", "hkx_mx_dequant", "hkx_mx4_gemm",
            "hkx_mx4_gemm_workspace", "hkx_block_norm", "hkx_block_norm_backward",
-           "hkx_block_norm_backward_workspace")
+           "hkx_block_norm_backward_workspace", "hkx_experts_gemm", "hkx_experts_silu_grad",
+           "hkx_experts_bias_grad", "hkx_experts_gather", "hkx_experts_route",
+           "hkx_experts_route_workspace", "hkx_experts_route_backward", "hkx_experts_combine",
+           "hkx_experts_combine_backward", "hkx_fp8_quant")
 
 _LIB = None
 _LOCK = threading.Lock()
@@ -175,6 +198,27 @@ def lib() -> ctypes.CDLL:
         L.hkx_block_norm_backward.argtypes = [POINTER(HkxBlockNormGradArgs), c_void_p]
         L.hkx_block_norm_backward_workspace.argtypes = [POINTER(HkxBlockNormGradArgs)]
         L.hkx_block_norm_backward_workspace.restype = c_size_t
+        L.hkx_experts_gemm.argtypes = [POINTER(HkxExpertsGemmArgs), c_void_p]
+        L.hkx_experts_silu_grad.argtypes = [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64,
+                                            c_void_p, c_int32, c_int32, c_int32, c_void_p]
+        L.hkx_experts_bias_grad.argtypes = [c_void_p, c_int64, c_void_p, c_void_p, c_int32, c_int32,
+                                            c_int32, c_int32, c_void_p]
+        L.hkx_experts_gather.argtypes = [c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_int32,
+                                         c_int32, c_int32, c_void_p]
+        L.hkx_experts_route.argtypes = [POINTER(HkxExpertsRouteArgs), c_void_p]
+        L.hkx_experts_route_workspace.argtypes = [POINTER(HkxExpertsRouteArgs)]
+        L.hkx_experts_route_workspace.restype = c_size_t
+        L.hkx_experts_route_backward.argtypes = [c_void_p, c_int64, c_int32, c_void_p, c_void_p,
+                                                 c_void_p, c_void_p, c_int64, c_int32, c_int32,
+                                                 c_int32, c_int32, c_void_p]
+        L.hkx_experts_combine.argtypes = [c_void_p, c_int64, c_int32, c_void_p, c_void_p, c_void_p,
+                                          c_int64, c_int32, c_int32, c_int32, c_int32, c_void_p]
+        L.hkx_experts_combine_backward.argtypes = [c_void_p, c_int64, c_void_p, c_int64, c_int32,
+                                                   c_void_p, c_void_p, c_int32, c_void_p, c_void_p,
+                                                   c_int64, c_void_p, c_int32, c_int32, c_int32,
+                                                   c_int32, c_void_p]
+        L.hkx_fp8_quant.argtypes = [c_void_p, c_int64, c_int32, c_void_p, c_int64, c_void_p,
+                                    c_int32, c_int32, c_void_p]
         sizes = (c_size_t * 4)()
         L.hkx_abi_sizes(sizes)
         want = [ctypes.sizeof(t) for t in (HkxOperand, HkxInstr, HkxEpilogue, HkxGemmArgs)]
@@ -232,6 +276,20 @@ def stream_of(device) -> int:
         _RAW_STREAM[:] = [torch._C._cuda_getCurrentRawStream]
         return torch.cuda.current_stream(device).cuda_stream
     return _RAW_STREAM[0](index)
+
+
+_DEVICE: list = []
+_HERE = contextlib.nullcontext()
+
+
+def current(device):
+    """A context in which `device` is the current one: kernels are launched on the current device. (No
+    context at all where it is that already, which costs the host 0.1 us.)"""
+    if not _DEVICE:
+        import torch  # noqa: PLC0415
+
+        _DEVICE[:] = [torch._C._cuda_getDevice, torch.cuda.device]
+    return _HERE if device.index == _DEVICE[0]() else _DEVICE[1](device)
 
 
 _PLAIN: list = []

@@ -15,7 +15,9 @@ h is rounded only as it is stored.
 D up to 16384 (8192 where gradients are taken).
 
 quant="mxfp8" or "mxfp4" gives y as (q, s), the operand of an MX product (hk.ops.mxfp4.gemm), without
-another pass: q (..., D) float8_e4m3fn, or (..., D/2) packed codes, and s (..., D/32); D a multiple of 32.
+another pass: q (..., D) float8_e4m3fn, or (..., D/2) packed codes, and s (..., D/32); D a multiple of 32. quant="fp8" gives the operands of hk.ops.scaled_mm and
+hk.ops.experts.gemm: q (..., D) float8_e4m3fn and s (..., 1) fp32, as hk.ops.fp8.quant makes them of the fp32 y;
+any D.
 
 Differentiable in x, residual, post, pre and gate (not through a quantized y): one backward pass over the
 same bytes, with the gradients of post, pre and a broadcast gate summed in a fixed order, a run of rows in
@@ -31,7 +33,7 @@ import ctypes
 
 from .. import _native as nat
 
-QUANT = {None: 0, "mxfp8": 1, "mxfp4": 2}
+QUANT = {None: 0, "mxfp8": 1, "mxfp4": 2, "fp8": 4}
 
 
 def _rows(t, d):
@@ -111,8 +113,11 @@ def _forward(x, residual, post, pre, gate, scales, quant, keep_rstd):
         g.quant = QUANT[quant]
         y_shape, y_type = tuple(x.shape), x.dtype
         if quant is not None:
-            y_type = torch.float8_e4m3fn if quant == "mxfp8" else torch.uint8
-            y_shape = (*x.shape[:-1], d if quant == "mxfp8" else d // 2)
+            y_type = torch.uint8 if quant == "mxfp4" else torch.float8_e4m3fn
+            y_shape = (*x.shape[:-1], d // 2 if quant == "mxfp4" else d)
+        if quant == "fp8":
+            s_shape = (*x.shape[:-1], 1)
+        elif quant is not None:
             s_shape = (*x.shape[:-1], d // 32)
             s_stride, step = [1], (d // 32 + 3) // 4 * 4
             for n in reversed(s_shape[:-1]):
@@ -137,7 +142,10 @@ def _run(g, plan, x, residual, keep_rstd):
         if s_shape is not None:
             import torch  # noqa: PLC0415
 
-            s = torch.empty_strided(s_shape, s_stride, dtype=torch.uint8, device=x.device)
+            if s_stride is None:
+                s = nat.empty(x, s_shape, torch.float32)
+            else:
+                s = torch.empty_strided(s_shape, s_stride, dtype=torch.uint8, device=x.device)
             g.y_scales = s.data_ptr()
             y = (y, s)
     if keep_rstd:
@@ -329,8 +337,8 @@ def _checked(x, residual, post, pre, gate, quant, grad):
     if gate is not None:
         _gate_shape(gate, x)
     if quant not in QUANT:
-        raise ValueError(f"block_norm: quant is None, 'mxfp8' or 'mxfp4', got {quant!r}")
-    if quant is not None and (pre is None or d % 32):
+        raise ValueError(f"block_norm: quant is None, 'mxfp8', 'mxfp4' or 'fp8', got {quant!r}")
+    if quant is not None and (pre is None or (d % 32 and quant != "fp8")):
         raise ValueError(f"block_norm: a quantized y needs pre and D={d} a multiple of 32")
     limit = 8192 if grad else 16384
     if d > limit:

@@ -377,7 +377,8 @@ size_t hkx_mx4_gemm_workspace(const HkxMx4GemmArgs* args);
  * x and y of x_dtype (bf16, fp16, fp32), residual and h of r_dtype (the same or fp32), post and pre
  * (d,) of w_dtype and gate of gate_dtype (x's or fp32). The gate's rows, d long (gate_col 1) or one
  * value (0), stand one after another, each for gate_rows rows of x. quant 1: y as MXFP8 (e4m3, ldy
- * bytes a row) with y_scales, 2: as MXFP4; d then a multiple of 32 and every row 16-byte aligned.
+ * bytes a row) with y_scales, 2: as MXFP4, 4: as e4m3 with one fp32 scale a row, as hkx_fp8_quant's
+ * (y_scales: rows of float; ldys is not used); d then a multiple of 32 and every row 16-byte aligned (1 and 2).
  * rstd (rows, 2) fp32 keeps the two norms' factors for the backward pass (NULL: not kept). d at most
  * 16384, in the backward pass 8192. Strides in elements. */
 typedef struct {
@@ -423,6 +424,107 @@ typedef struct {
 } HkxBlockNormGradArgs;
 int hkx_block_norm_backward(const HkxBlockNormGradArgs* args, void* stream);
 size_t hkx_block_norm_backward_workspace(const HkxBlockNormGradArgs* args);
+
+/* ---------------------------------------------------------------- experts: rows in groups
+ *
+ * R rows stand in the order of their experts: rows offsets[e] .. offsets[e + 1] are expert e's (offsets of
+ * experts + 1 int32 on the GPU, from 0, at most rows), those behind offsets[experts] are nobody's. A host need not
+ * know them: grids are sized for any. Offsets out of order or past the rows are clamped, an index out of range reads
+ * zeros: nothing outside the operands is touched. At most 1024 experts. */
+
+#define HKX_EXPERTS_NT 0 /* C[r] = A[r or index[r]] . B_e^T, B_e (n, k) */
+#define HKX_EXPERTS_NN 1 /* C[r] = A[r] . B_e, B_e (k, n) */
+#define HKX_EXPERTS_TN 2 /* C_e = sum of its rows A[r]^T B[r], (m, n) an expert */
+typedef struct {
+  int32_t size; /* sizeof(HkxExpertsGemmArgs) */
+  int32_t op;
+  int32_t ab_dtype; /* HKX_BF16; HKX_FP8E4M3 with scales (NT) */
+  int32_t experts, rows;
+  int32_t a_rows;    /* A's rows, where index names them */
+  int32_t m, n, k;   /* n: C's columns; k: the contraction (not TN); m: C's rows an expert (TN) */
+  int32_t silu_mul;  /* NT: B_e has n gate rows, then n up rows: C = silu(gate) * up */
+  int32_t zero_rest; /* NT, NN: C's rows behind the last group are zeroed, otherwise left */
+  int32_t bias_dtype, sa_ld, sb_col; /* sa_ld: 1 a scale a row of A, 0 one; sb_col: 1 a scale a row of B, 0 one an expert */
+  int32_t kernel;                    /* HKX_EXPERTS_AUTO, or the kernel to run (tuning, tests) */
+  int32_t reserved;
+  const void* a;
+  const void* b;
+  void* c; /* bf16 */
+  void* z; /* NT with silu_mul: the 2 n columns before it, bf16 (NULL: not kept) */
+  const int32_t* offsets;
+  const int32_t* index; /* NT: each row's row of A (NULL: its own) */
+  const void* bias;     /* NT: (experts, n), 2 n with silu_mul (NULL: none) */
+  const float* sa;
+  const float* sb;
+  int64_t lda, ldb, ldc, ldz;        /* row strides, elements */
+  int64_t b_expert, c_expert;        /* strides of an expert, elements (NT, NN: B's; TN: C's) */
+  int64_t bias_ld, sb_ld;            /* of the bias and the scales */
+} HkxExpertsGemmArgs;
+#define HKX_EXPERTS_AUTO 0
+#define HKX_EXPERTS_TILE16 1  /* tiles of 16, 64 or 128 rows */
+#define HKX_EXPERTS_TILE64 2
+#define HKX_EXPERTS_TILE128 3
+/* bf16 C from bf16 or fp8 operands, sums in fp32, rounded once. n and k multiples of 8 (m too; an fp8 k of 16), rows
+ * and experts of A and B 16-byte aligned, of C, z and the bias 8-byte, scales (a row of B each) 16-byte. */
+int hkx_experts_gemm(const HkxExpertsGemmArgs* args, void* stream);
+
+/* dz from dy (rows, n) and z (rows, 2 n), bf16: the gradient of silu(z[:n]) * z[n:]. Rows behind
+ * offsets[experts] are left. Rows 16-byte aligned, n a multiple of 8. */
+int hkx_experts_silu_grad(const void* z, int64_t ldz, const void* dy, int64_t lddy, void* dz, int64_t lddz,
+                          const int32_t* offsets, int32_t experts, int32_t rows, int32_t n, void* stream);
+
+/* db[e] (experts, n) of db_dtype = the sum of its rows of dz (bf16), in 64 bits. */
+int hkx_experts_bias_grad(const void* dz, int64_t lddz, const int32_t* offsets, void* db, int32_t db_dtype,
+                          int32_t experts, int32_t rows, int32_t n, void* stream);
+
+/* out[r] = x[index[r]] (a_rows rows of k bf16; zeros where index is out of range). */
+int hkx_experts_gather(const void* x, int64_t ldx, const int32_t* index, void* out, int64_t ldo, int32_t rows,
+                       int32_t a_rows, int32_t k, void* stream);
+
+/* The k largest of each token's logits (t, e), a tie to the lower expert, NaN above all, -inf never chosen:
+ * chosen (t, k) int32 in falling order (-1: none left) and weights (t, k) fp32, their softmax over the token's
+ * experts, or with renormalize over the chosen. And the rows of the chosen in order of (expert, token):
+ * offsets (e + 1), rows (t k) each row's token (-1 behind the last), slots (t, k) each choice's row (-1: none).
+ * e at most 1024, k at most 64 and e. */
+typedef struct {
+  int32_t size; /* sizeof(HkxExpertsRouteArgs) */
+  int32_t dtype; /* the logits' */
+  int32_t t, e, k, renormalize;
+  const void* logits;
+  int64_t ld;
+  float* weights;
+  int32_t* chosen;
+  int32_t* offsets;
+  int32_t* rows;
+  int32_t* slots;
+  void* ws; /* hkx_experts_route_workspace() bytes, 16-byte aligned */
+  size_t ws_bytes;
+} HkxExpertsRouteArgs;
+int hkx_experts_route(const HkxExpertsRouteArgs* args, void* stream);
+size_t hkx_experts_route_workspace(const HkxExpertsRouteArgs* args);
+
+/* The logits' gradient (t, e) of `dtype` from dweights (t, k) fp32 and the forward call's chosen and weights. */
+int hkx_experts_route_backward(const void* logits, int64_t ld, int32_t dtype, const float* weights,
+                               const int32_t* chosen, const float* dweights, void* dlogits, int64_t lddl, int32_t t,
+                               int32_t e, int32_t k, int32_t renormalize, void* stream);
+
+/* out[i] = sum over j of weights[i, j] y[slots[i, j]] (weights NULL: ones; a slot outside y's `rows`: nothing), in fp32,
+ * in order of j; out (t, d) and y of `dtype`. */
+int hkx_experts_combine(const void* y, int64_t ldy, int32_t dtype, const int32_t* slots, const float* weights,
+                        void* out, int64_t ldo, int32_t t, int32_t k, int32_t rows, int32_t d, void* stream);
+
+/* dy[slots[i, j]] = weights[i, j] dout[i], zeros behind offsets[experts], and dweights[i, j] = <dout[i], y[slots[i, j]]>
+ * (NULL: not wanted; then y may be NULL). rows = t k. */
+int hkx_experts_combine_backward(const void* y, int64_t ldy, const void* dout, int64_t lddo, int32_t dtype,
+                                 const int32_t* slots, const int32_t* offsets, int32_t experts, const float* weights,
+                                 void* dy, int64_t lddy, float* dweights, int32_t t, int32_t k, int32_t rows,
+                                 int32_t d, void* stream);
+
+/* x (m, k) of x_dtype -> q (m, k) e4m3 and s (m) fp32: s = max |x| / 448 of the row (at least 2^-126; 1 for a row of
+ * zeros), q = x / s rounded to nearest even. A row with an infinity or a NaN has s = NaN and codes 0. Any k and
+ * alignment of whole elements (16 bytes of x, 8 of q and k a multiple of 8: pieces of 8). */
+int hkx_fp8_quant(const void* x, int64_t ldx, int32_t x_dtype, void* q, int64_t ldq, float* s, int32_t m, int32_t k,
+                  void* stream);
 
 #ifdef __cplusplus
 }

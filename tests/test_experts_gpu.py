@@ -1,0 +1,536 @@
+"""hk.ops.experts on the GPU against the float64 oracle (oracle/experts_oracle.py): the products over every kernel,
+layout and type, the router, the combination, their gradients against float64 autograd and against differences, a layer
+as it is used, graphs, streams and what lies outside the groups.
+
+Tolerances. A bf16 result is one rounding (2^-8 of it) of an fp32 sum, whose own error is at most 2^-23 a term and addition
+of the terms' magnitudes (K of them); what a gradient is made of is rounded to bf16 first (2^-8 of each), and its errors go
+through the next product by the magnitudes of what they meet."""
+
+import math
+
+import pytest
+import torch
+
+import hk
+from hk import _native as nat
+from hk.ops import experts, fp8
+from oracle import experts_oracle as O
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+BF16, F16, F32, E4M3 = torch.bfloat16, torch.float16, torch.float32, torch.float8_e4m3fn
+HALF = {BF16: 2.0 ** -8, F16: 2.0 ** -11, F32: 2.0 ** -24}
+
+
+@pytest.fixture(params=[0, 1, 2, 3], ids=["auto", "tile16", "tile64", "tile128"])
+def kernel(request, monkeypatch):
+    """Each product on the kernel named."""
+    real = experts._run
+
+    def run(g, device):
+        g.kernel = request.param
+        real(g, device)
+
+    monkeypatch.setattr(experts, "_run", run)
+    return request.param
+
+
+def _plan(t, e, k, seed, dead=0):
+    """Tokens' experts with favourites; the last `dead` tokens have none. (plan on the GPU, the same in int64 here)"""
+    g = torch.Generator().manual_seed(seed)
+    logits = torch.randn(t, e, generator=g) + torch.randn(e, generator=g)
+    logits[t - dead:] = -math.inf
+    _, _, offsets, rows, slots = O.route(logits, k)
+    return experts.Plan(*(v.int().to(DEV) for v in (offsets, rows, slots))), (offsets, rows, slots)
+
+
+def _within(got, ref, tol):
+    assert got.shape == ref.shape
+    off = (got.cpu().double() - ref).abs()
+    bad = ~(off <= tol)
+    assert not bad.any(), f"{int(bad.sum())} off, at most {float((off / (tol + 1e-300)).max()):.3g} times the tolerance"
+
+
+def _sum_error(x, w, offsets, rows=None, bias=None):
+    """What fp32 sums of the products may be off by: 2^-23 a term of their magnitudes."""
+    mag = O.gemm(x.double().abs(), w.double().abs(), offsets, rows, None if bias is None else bias.abs())[0]
+    return (x.shape[1] + 2) * 2.0 ** -23 * mag
+
+
+def _silu_mul_error(z, err):
+    """silu(g) u from g and u off by `err`: |silu'| <= 1.1; exp, the reciprocal and the products 2^-20 in all."""
+    g, u = z.chunk(2, dim=1)
+    eg, eu = err.chunk(2, dim=1)
+    s = torch.nn.functional.silu(g)
+    return 1.1 * eg * (u.abs() + eu) + s.abs() * eu + 2.0 ** -20 * (s * u).abs()
+
+
+SIZES = [  # t, e, k, n, d, dead
+    (1, 4, 2, 8, 8, 0), (7, 3, 1, 24, 40, 0), (64, 8, 2, 136, 72, 0), (150, 5, 2, 264, 200, 9),
+    (40, 200, 3, 72, 128, 1), (300, 2, 1, 16, 1112, 0), (5, 6, 6, 520, 64, 5), (700, 4, 2, 128, 64, 33)]
+
+
+@pytest.mark.parametrize("gather", [False, True], ids=["sorted", "gather"])
+@pytest.mark.parametrize("silu_mul", [False, True], ids=["plain", "paired"])
+@pytest.mark.parametrize("size", SIZES, ids=str)
+def test_products(size, silu_mul, gather, kernel):
+    t, e, k, n, d, dead = size
+    plan, (offsets, rows, _) = _plan(t, e, k, seed=t + n, dead=dead)
+    g = torch.Generator().manual_seed(n)
+    x = torch.randn(t if gather else t * k, d, generator=g).to(BF16)
+    w = (torch.randn(e, 2 * n if silu_mul else n, d, generator=g) * d ** -0.5).to(BF16)
+    bias = torch.randn(w.shape[:2], generator=g).to(F32) if t % 2 else None
+    ref, z = O.gemm(x, w, offsets, rows if gather else None, bias, silu_mul)
+    err = _sum_error(x, w, offsets, rows if gather else None, bias)
+    if silu_mul:
+        err = _silu_mul_error(z, err)
+    y = experts.gemm(x.to(DEV), w.to(DEV), plan, gather=gather, silu_mul=silu_mul,
+                     bias=None if bias is None else bias.to(DEV))
+    assert y.dtype == BF16
+    _within(y, ref, err + HALF[BF16] * (ref.abs() + err))
+
+
+@pytest.mark.parametrize("silu_mul", [False, True], ids=["plain", "paired"])
+@pytest.mark.parametrize("size", [(1, 4, 2, 8, 16, 0), (70, 5, 2, 136, 144, 9), (40, 100, 3, 72, 128, 0),
+                                  (300, 2, 1, 16, 1040, 3)], ids=str)
+def test_products_of_8_bits(size, silu_mul, kernel):
+    t, e, k, n, d, dead = size
+    plan, (offsets, rows, _) = _plan(t, e, k, seed=t, dead=dead)
+    g = torch.Generator().manual_seed(n)
+    rows_b = 2 * n if silu_mul else n
+    x, w = torch.randn(t, d, generator=g).to(E4M3), torch.randn(e, rows_b, d, generator=g).to(E4M3)
+    for sa, sb in ((torch.rand(t, 1, generator=g) + 0.5, torch.rand(e, rows_b, generator=g) / d),
+                   (torch.rand(1, generator=g), torch.rand(e, generator=g) / d),
+                   (torch.rand(t, generator=g), torch.rand(e, 1, generator=g) / d)):
+        bias = torch.randn(e, rows_b, generator=g).to(BF16)
+        xs, ws = x.double() * sa.double().reshape(-1, 1), w.double() * sb.double().reshape(e, -1, 1)
+        ref, z = O.gemm(xs, ws, offsets, rows, bias, silu_mul)
+        err = _sum_error(xs, ws, offsets, rows, bias) + 2.0 ** -22 * (z.abs())  # (the two scales' products)
+        if silu_mul:
+            err = _silu_mul_error(z, err)
+        y = experts.gemm(x.to(DEV), w.to(DEV), plan, gather=True, silu_mul=silu_mul, bias=bias.to(DEV),
+                         scale_a=sa.to(DEV), scale_b=sb.to(DEV))
+        _within(y, ref, err + HALF[BF16] * (ref.abs() + err))
+
+
+@pytest.mark.parametrize("gather", [False, True], ids=["sorted", "gather"])
+@pytest.mark.parametrize("silu_mul", [False, True], ids=["plain", "paired"])
+@pytest.mark.parametrize("size", [(3, 4, 2, 8, 8, 0), (64, 8, 2, 136, 72, 0), (150, 5, 2, 264, 200, 9),
+                                  (40, 100, 3, 72, 128, 1), (700, 3, 2, 128, 64, 33)], ids=str)
+def test_gradients(size, silu_mul, gather, kernel):
+    t, e, k, n, d, dead = size
+    plan, (offsets, rows, slots) = _plan(t, e, k, seed=t + n, dead=dead)
+    g = torch.Generator().manual_seed(n)
+    x = torch.randn(t if gather else t * k, d, generator=g).to(BF16)
+    w = (torch.randn(e, 2 * n if silu_mul else n, d, generator=g) * d ** -0.5).to(BF16)
+    bias = torch.randn(w.shape[:2], generator=g).to(BF16)
+    dy = torch.randn(t * k, n, generator=g).to(BF16)
+    leaf = [v.to(DEV).requires_grad_() for v in (x, w, bias)]
+    y = experts.gemm(leaf[0], leaf[1], plan, gather=gather, silu_mul=silu_mul, bias=leaf[2])
+    assert torch.equal(y, experts.gemm(leaf[0].detach(), leaf[1].detach(), plan, gather=gather, silu_mul=silu_mul,
+                                       bias=leaf[2].detach()))
+    got = torch.autograd.grad(y, leaf, dy.to(DEV))
+
+    ref = [v.double().requires_grad_() for v in (x, w, bias)]
+    out, z = O.gemm(ref[0], ref[1], offsets, rows if gather else None, ref[2], silu_mul)
+    want = torch.autograd.grad(out, ref, dy.double())
+    live = int(offsets[-1])
+    z, dyd = z.detach()[:live], dy.double()[:live]
+    dz, edz = dyd, torch.zeros_like(dyd)
+    if silu_mul:
+        a, u = z.chunk(2, dim=1)
+        ea, eu = (2.0 ** -8 * z.abs() + _sum_error(x, w, offsets, rows if gather else None, bias)[:live]).chunk(2, dim=1)
+        s = torch.sigmoid(a)
+        slope = s * (1 + a * (1 - s))
+        dz = torch.cat((dyd * u * slope, dyd * a * s), 1)
+        # |silu'| <= 1.1 and |silu''| <= 0.5; what z's rounding does to both, and dz's own
+        edz = torch.cat((dyd.abs() * (1.1 * eu + 0.5 * ea * (u.abs() + eu)), dyd.abs() * 1.1 * ea), 1)
+        edz = edz + (2.0 ** -8 + 2.0 ** -19) * (dz.abs() + edz)
+    xr = (x[rows[:live]] if gather else x[:live]).double()
+    wd = w.double()
+    terms = edz + (dz.shape[1] + 2) * 2.0 ** -23 * (dz.abs() + edz)
+    e_rows, edw, edb = [], torch.zeros_like(want[1]), torch.zeros_like(want[2])
+    for i, (lo, hi) in enumerate(zip(offsets[:-1].tolist(), offsets[1:].tolist())):
+        e_rows.append(terms[lo:hi] @ wd[i].abs())
+        t2 = edz[lo:hi] + (hi - lo + 2) * 2.0 ** -23 * (dz[lo:hi].abs() + edz[lo:hi])
+        edw[i] = t2.t() @ xr[lo:hi].abs()
+        edb[i] = t2.sum(0)
+    e_rows = torch.cat([*e_rows, torch.zeros(t * k - live, d, dtype=torch.float64)])
+    if gather:
+        # a token's rows are rounded to bf16 each, then added
+        dxr = torch.cat([*(dz[lo:hi] @ wd[i] for i, (lo, hi) in enumerate(zip(offsets[:-1].tolist(), offsets[1:].tolist()))),
+                         torch.zeros(t * k - live, d, dtype=torch.float64)])
+        e_rows = O.combine(e_rows + 2.0 ** -8 * (dxr.abs() + e_rows), slots)
+    for name, a, b, err in zip("xwb", got, want, (e_rows, edw, edb)):
+        assert a.dtype == BF16, name
+        _within(a, b, err + 2.0 ** -8 * (b.abs() + err))
+
+
+def test_gradient_by_differences():
+    """The weight's and the activation's gradient along a direction, against the forward's own differences."""
+    plan, _ = _plan(96, 4, 2, seed=5)
+    g = torch.Generator().manual_seed(1)
+    x = torch.randn(96, 64, generator=g).to(BF16).to(DEV)
+    w = (torch.randn(4, 96, 64, generator=g) / 8).to(BF16).to(DEV)
+    dy = torch.randn(192, 48, generator=g).to(BF16).to(DEV)
+    a, b = x.clone().requires_grad_(), w.clone().requires_grad_()
+    dx, dw = torch.autograd.grad(experts.gemm(a, b, plan, gather=True, silu_mul=True), (a, b), dy)
+
+    def loss(x, w):
+        return float((experts.gemm(x, w, plan, gather=True, silu_mul=True).double() * dy.double()).sum())
+
+    for leaf, grad, step in ((x, dx, 0.125), (w, dw, 0.03125)):
+        # (a direction and a step that bf16 holds: the two points are exact)
+        way = torch.where(grad >= 0, 1.0, -1.0).double()
+        hi, lo = (leaf.double() + step * way).to(BF16), (leaf.double() - step * way).to(BF16)
+        args = [(hi, w), (lo, w)] if leaf is x else [(x, hi), (x, lo)]
+        change = loss(*args[0]) - loss(*args[1])
+        along = float((grad.double() * (hi.double() - lo.double())).sum())
+        # the curve's own part: the third derivative over a step of this size, measured at twice the step, is 8 times it
+        hi2, lo2 = (leaf.double() + 2 * step * way).to(BF16), (leaf.double() - 2 * step * way).to(BF16)
+        args = [(hi2, w), (lo2, w)] if leaf is x else [(x, hi2), (x, lo2)]
+        wide = loss(*args[0]) - loss(*args[1])
+        along2 = float((grad.double() * (hi2.double() - lo2.double())).sum())
+        # Richardson: (8 D(h) - D(2h)) / 6 has no cubic part; both estimate the same slope, a fifth-order rest and roundings stay
+        assert abs((8 * change - wide) / (8 * along - along2) - 1) < 0.05
+
+
+@pytest.mark.parametrize("renormalize", [True, False])
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("t,e,k,dead", [(1, 1, 1, 0), (1, 64, 8, 0), (64, 7, 3, 5), (65, 64, 8, 1), (300, 128, 6, 40),
+                                        (130, 1024, 64, 2), (1000, 33, 33, 0), (200, 500, 1, 200), (4097, 16, 2, 7)])
+def test_route(t, e, k, dead, dtype, renormalize):
+    g = torch.Generator().manual_seed(t + e)
+    logits = torch.randn(t, e, generator=g)
+    logits[::3] = (logits[::3] * 2).round()           # ties
+    logits[torch.rand(t, e, generator=g) < 0.1] = -math.inf
+    logits[t - dead:] = -math.inf
+    logits = logits.to(dtype)
+    if t > 60 and e > 8:
+        logits[3, 5] = math.nan
+        logits[4, 2] = math.inf
+        logits[5, 1:4] = torch.tensor([-0.0, 0.0, -0.0])
+    want = O.route(logits, k, renormalize)
+    weights, chosen, plan = experts.route(logits.to(DEV), k, renormalize=renormalize)
+    for a, b in zip((chosen, plan.offsets, plan.rows, plan.slots), want[1:]):
+        assert a.dtype == torch.int32 and torch.equal(a.cpu().long(), b)
+    w, ref = weights.cpu().double(), want[0]
+    assert weights.dtype == F32 and torch.equal(torch.isnan(w), torch.isnan(ref))
+    live = ~torch.isnan(ref)
+    # exp to two steps (of an argument rounded by 2^-24 of up to 16), E additions, a division
+    tol = (20 + e) * 2.0 ** -23 * ref + 1e-37
+    assert ((w - ref).abs() <= tol)[live].all()
+
+
+@pytest.mark.parametrize("renormalize", [True, False])
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("t,e,k,dead", [(1, 3, 1, 0), (70, 64, 8, 3), (33, 1000, 5, 0), (9, 130, 64, 1)])
+def test_route_gradient(t, e, k, dead, dtype, renormalize):
+    g = torch.Generator().manual_seed(e)
+    logits = torch.randn(t, e, generator=g).to(dtype)
+    logits[t - dead:] = -math.inf
+    dw = torch.randn(t, k, generator=g)
+    leaf = logits.to(DEV).requires_grad_()
+    weights, chosen, plan = experts.route(leaf, k, renormalize=renormalize)
+    assert not chosen.requires_grad and not plan.offsets.requires_grad
+    (got,) = torch.autograd.grad(weights, leaf, dw.to(DEV))
+    l = logits.double().requires_grad_()
+    c = chosen.cpu().long()
+    p = torch.softmax(torch.where(torch.isinf(l).all(1, keepdim=True), torch.zeros_like(l), l), 1)
+    w = torch.where(c >= 0, torch.gather(p, 1, c.clamp(min=0)), torch.zeros((), dtype=torch.float64))
+    if renormalize:
+        w = w / w.sum(1, keepdim=True).clamp(min=1e-300)
+    (ref,) = torch.autograd.grad(w, l, dw.double())
+    top = (w.detach() * dw.abs()).sum(1, keepdim=True) + dw.abs().amax(1, keepdim=True)
+    least = 2.0 ** -25 if dtype == F16 else 0.0
+    assert got.dtype == dtype
+    _within(got, ref, HALF[dtype] * ref.abs() + least + (20 + e) * 2.0 ** -22 * top * p.detach())
+
+
+@pytest.mark.parametrize("weighted", [True, False])
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("t,e,k,d,dead", [(1, 2, 1, 1, 0), (5, 4, 2, 8, 1), (33, 8, 3, 515, 2), (7, 64, 7, 2056, 7),
+                                          (20, 9, 9, 4104, 3)])
+def test_combine(t, e, k, d, dead, dtype, weighted):
+    plan, (offsets, _, slots) = _plan(t, e, k, seed=d, dead=dead)
+    g = torch.Generator().manual_seed(d)
+    y, dout = torch.randn(t * k, d, generator=g).to(dtype), torch.randn(t, d, generator=g).to(dtype)
+    w = torch.rand(t, k, generator=g) if weighted else None
+    leaf = [y.to(DEV).requires_grad_()] + ([w.to(DEV).requires_grad_()] if weighted else [])
+    out = experts.combine(leaf[0], plan, leaf[1] if weighted else None)
+    got = torch.autograd.grad(out, leaf, dout.to(DEV))
+    ref = [y.double().requires_grad_()] + ([w.double().requires_grad_()] if weighted else [])
+    want = O.combine(ref[0], slots, ref[1] if weighted else None)
+    grads = torch.autograd.grad(want, ref, dout.double())
+    mag = O.combine(y.double().abs(), slots, w)
+    least = 2.0 ** -25 if dtype == F16 else 0.0
+    assert out.dtype == dtype and torch.equal(out, experts.combine(leaf[0].detach(), plan, leaf[1].detach() if weighted else None))
+    _within(out, want.detach(), HALF[dtype] * want.abs().detach() + (k + 2) * 2.0 ** -23 * mag + least)
+    _within(got[0], grads[0], (HALF[dtype] + 2.0 ** -24) * grads[0].abs() + least)
+    if weighted:
+        at = slots.clamp(min=0)
+        size = (y.double().abs()[at] * dout.double().abs().unsqueeze(1)).sum(2)
+        _within(got[1], grads[1], (d + 2) * 2.0 ** -24 * size)
+
+
+def test_what_lies_outside_the_groups():
+    """Rows behind the last expert's: zeros in a new output, left in a given one; NaN there goes nowhere; experts without
+    rows; and the rows behind in the gradients."""
+    e, n, d, r = 5, 40, 72, 90
+    offsets = torch.tensor([0, 30, 30, 30, 61, 61], dtype=torch.int32)
+    plan = experts.Plan(offsets.to(DEV))
+    g = torch.Generator().manual_seed(0)
+    x, w = torch.randn(r, d, generator=g).to(BF16), torch.randn(e, n, d, generator=g).to(BF16)
+    clean = experts.gemm(x.to(DEV), w.to(DEV), plan)
+    assert not clean[61:].any() and clean[:61].any(1).all()
+    x[61:] = math.nan
+    w[[1, 2, 4]] = math.nan
+    a, b = x.to(DEV).requires_grad_(), w.to(DEV).requires_grad_()
+    y = experts.gemm(a, b, plan)
+    assert torch.equal(y, clean)
+    given = torch.full((r, n), 7.0, dtype=BF16, device=DEV)
+    assert experts.gemm(x.to(DEV), w.to(DEV), plan, out=given) is given
+    assert torch.equal(given[:61], clean[:61]) and (given[61:] == 7).all()
+    dy = torch.randn(r, n, generator=g).to(BF16).to(DEV)
+    dy[61:] = math.nan
+    dx, dw = torch.autograd.grad(y, (a, b), dy)
+    assert torch.isfinite(dx).all() and not dx[61:].any() and dx[:61].any(1).all()
+    assert torch.isfinite(dw).all() and not dw[[1, 2, 4]].any() and dw[0].any() and dw[3].any()
+
+
+def test_offsets_and_indices_out_of_range_touch_nothing_else():
+    """Clamped, as documented: offsets past the rows or out of order, row numbers outside x."""
+    e, n, d, r = 4, 24, 40, 64
+    g = torch.Generator().manual_seed(0)
+    x, w = torch.randn(r, d, generator=g).to(BF16).to(DEV), torch.randn(e, n, d, generator=g).to(BF16).to(DEV)
+    want = torch.cat((x[:20] @ w[0].t(), x[20:] @ w[1].t()))
+    y = experts.gemm(x, w, experts.Plan(torch.tensor([-5, 20, 1000, 900, 2 ** 31 - 1], dtype=torch.int32, device=DEV)))
+    torch.testing.assert_close(y, want, rtol=2 ** -7, atol=0.05)
+    rows = torch.arange(r, dtype=torch.int32, device=DEV)
+    rows[::7] = torch.tensor([-1, r, 2 ** 31 - 1, -2 ** 31, -7, r + 1, 99, -1, 64, 65], dtype=torch.int32, device=DEV)
+    even = torch.tensor([0, 16, 32, 48, 64], dtype=torch.int32, device=DEV)
+    y = experts.gemm(x, w, experts.Plan(even, rows), gather=True)
+    assert not y[::7].any() and torch.equal(y[1::7], experts.gemm(x, w, experts.Plan(even))[1::7])
+    slots = torch.arange(r, dtype=torch.int32, device=DEV).reshape(32, 2).clone()
+    slots[:, 1] = torch.where(torch.arange(32, device=DEV) % 2 == 0, -9, 2 ** 30)
+    assert torch.equal(experts.combine(y, experts.Plan(even, None, slots)), y[::2])
+
+
+def test_strided_operands():
+    plan, (offsets, rows, _) = _plan(50, 3, 2, seed=3)
+    g = torch.Generator().manual_seed(0)
+    big, wide = torch.randn(50, 200, generator=g).to(BF16).to(DEV), torch.randn(6, 50, 160, generator=g).to(BF16).to(DEV)
+    bias = torch.randn(3, 80, generator=g).to(BF16).to(DEV)
+    for x, w, b in ((big[:, 8:80], wide[::2, 2:42, 16:88], bias[:, 8:48]), (big[:, 3:75], wide[::2, 1:41, 5:77], bias[:, 1:41]),
+                    (big.t()[:72, :50].t(), wide.transpose(1, 2)[:3, :40, :48].contiguous().transpose(1, 2)[:, :, :].repeat(1, 1, 2)[:, :40, :72], bias[:, 40:])):
+        y = experts.gemm(x, w, plan, gather=True, bias=b)
+        assert torch.equal(y, experts.gemm(x.contiguous(), w.contiguous(), plan, gather=True, bias=b.contiguous()))
+        pad = torch.full((100, 64), 3.0, dtype=BF16, device=DEV)
+        experts.gemm(x, w, plan, gather=True, bias=b, out=pad[:, 4:44])
+        assert torch.equal(pad[:, 4:44], y) and (pad[:, :4] == 3).all() and (pad[:, 44:] == 3).all()
+    leaf = big[:, 3:75].clone().requires_grad_()
+    w = wide[::2, 1:41, 5:77].clone().requires_grad_()
+    dy = torch.randn(100, 80, generator=g).to(BF16).to(DEV)
+    a = torch.autograd.grad(experts.gemm(leaf, w, plan, gather=True), (leaf, w), dy[:, ::2])
+    b = torch.autograd.grad(experts.gemm(leaf, w, plan, gather=True), (leaf, w), dy[:, ::2].contiguous())
+    assert all(torch.equal(p, q) for p, q in zip(a, b))
+
+
+def test_empty_calls():
+    e, n, d = 3, 16, 24
+    plan = experts.Plan(torch.zeros(e + 1, dtype=torch.int32, device=DEV),
+                        torch.empty(0, dtype=torch.int32, device=DEV), torch.empty(0, 2, dtype=torch.int32, device=DEV))
+    w = torch.ones(e, n, d, dtype=BF16, device=DEV, requires_grad=True)
+    x = torch.empty(0, d, dtype=BF16, device=DEV, requires_grad=True)
+    for gather in (False, True):
+        y = experts.gemm(x, w, plan, gather=gather)
+        assert y.shape == (0, n)
+        dx, dw = torch.autograd.grad(y, (x, w), torch.empty(0, n, dtype=BF16, device=DEV))
+        assert dx.shape == (0, d) and not dw.any()
+    assert experts.combine(torch.empty(0, d, device=DEV), plan).shape == (0, d)
+    weights, chosen, p = experts.route(torch.empty(0, e, device=DEV), 2)
+    assert weights.shape == (0, 2) and p.rows.numel() == 0 and not p.offsets.any()
+    q, s = fp8.quant(torch.empty(0, 32, device=DEV))
+    assert q.shape == (0, 32) and s.shape == (0, 1)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("m,k", [(1, 16), (5, 48), (3, 2048), (2, 2064), (4, 4112), (3, 8208), (2, 16400), (300, 512),
+                                 (1, 1), (7, 333), (3, 2049), (2, 5003), (3, 20001)])
+def test_quantized_rows(m, k, dtype):
+    g = torch.Generator().manual_seed(k)
+    x = (torch.randn(m, k, generator=g) * torch.logspace(-6, 2, m).unsqueeze(1)).to(dtype)
+    if m > 2:
+        x[1] = 0
+        x[2, k // 3] = math.nan if k % 32 else -math.inf
+    if dtype != F16 and m > 4:
+        x[4] = torch.randn(k, generator=g).to(dtype) * 2.0 ** -126
+    v, s = O.quant8(x)
+    q, scale = fp8.quant(x.to(DEV))
+    assert q.dtype == E4M3 and q.shape == x.shape and scale.shape == (m, 1)
+    assert torch.equal(torch.nan_to_num(scale.cpu().double(), nan=-1.0), torch.nan_to_num(s, nan=-1.0))
+    assert torch.equal(q.cpu().float().double(), v)
+    strided = torch.zeros(m, k + 24, dtype=dtype, device=DEV)
+    strided[:, 5:k + 5] = x.to(DEV)
+    assert torch.equal(fp8.quant(strided[:, 5:k + 5])[0].view(torch.uint8), q.view(torch.uint8))
+
+
+@pytest.mark.parametrize("dtype,rdtype", [(BF16, BF16), (BF16, F32), (F16, F16), (F32, F32)])
+@pytest.mark.parametrize("rows,d", [(1, 16), (9, 512), (5, 1040), (3, 4096), (2, 16384), (2, 1), (6, 333),
+                                    (3, 1548), (2, 7777)])
+def test_block_norm_into_8_bits(rows, d, dtype, rdtype):
+    """The codes and scales are those of the fp32 y: between the two that an error of 2^-20 of y allows."""
+    g = torch.Generator().manual_seed(d)
+    x, r = torch.randn(rows, d, generator=g).to(dtype), torch.randn(rows, d, generator=g).to(rdtype)
+    pre = (torch.randn(d, generator=g) * 0.1 + 1).to(dtype)
+    h, (q, s) = hk.ops.block_norm(x.to(DEV), r.to(DEV), pre=pre.to(DEV), branch_scale=0.5, quant="fp8")
+    h0, y0 = hk.ops.block_norm(x.to(DEV), r.to(DEV), pre=pre.to(DEV), branch_scale=0.5)
+    assert torch.equal(h, h0) and q.dtype == E4M3 and q.shape == x.shape and s.shape == (rows, 1) and s.dtype == F32
+    hd = r.double() + 0.5 * x.double()
+    y = hd / torch.sqrt((hd * hd).mean(1, keepdim=True) + 1e-6) * pre.double()
+    top = y.abs().amax(1, keepdim=True) / 448
+    assert ((s.cpu().double() - top).abs() <= 2.0 ** -19 * top).all()
+    v = q.cpu().float().double() * s.cpu().double()
+    # half a step of e4m3: 2^-4 of a value, 2^-10 of the scale below its normals
+    assert ((v - y).abs() <= 2.0 ** -4 * y.abs() * (1 + 2.0 ** -18) + 2.0 ** -10 * top * (1 + 2.0 ** -18) + 2.0 ** -18 * y.abs()).all()
+    ref = fp8.quant((hd / torch.sqrt((hd * hd).mean(1, keepdim=True) + 1e-6) * pre.double()).float().to(DEV))[0]
+    assert (ref.view(torch.uint8) != q.view(torch.uint8)).float().mean() < 1e-3  # (values next to a tie alone)
+    bad = x.clone()
+    bad[0, d // 2] = math.nan
+    _, (_, s) = hk.ops.block_norm(bad.to(DEV), r.to(DEV), pre=pre.to(DEV), quant="fp8")
+    assert torch.isnan(s[0]) and torch.isfinite(s[1:]).all()
+
+
+def _layer(t, e, k, d, inner, seed, dead=0):
+    g = torch.Generator().manual_seed(seed)
+    x = torch.randn(t, d, generator=g).to(BF16)
+    logits = torch.randn(t, e, generator=g)
+    logits[t - dead:] = -math.inf
+    up = (torch.randn(e, 2 * inner, d, generator=g) * d ** -0.5).to(BF16)
+    down = (torch.randn(e, d, inner, generator=g) * inner ** -0.5).to(BF16)
+    return x, logits, up, down
+
+
+def _layer_oracle(x, logits, k, up, down):
+    weights, _, offsets, rows, slots = O.route(logits, k)
+    a, _ = O.gemm(x, up, offsets, rows, silu_mul=True)
+    return O.combine(O.gemm(a, down, offsets)[0], slots, weights)
+
+
+@pytest.mark.parametrize("t,e,k,d,inner,dead", [(1, 8, 2, 64, 32, 0), (90, 6, 3, 128, 96, 11)])
+def test_a_layer_of_experts(t, e, k, d, inner, dead):
+    """The run of them, in bf16 (with its gradients) and in 8 bits behind block_norm: the 2-norm of what bf16 and 8-bit
+    roundings add (independent, each at most half a step: 2^-8 in bf16 three times over, 2^-4 in 8 bits for both operands
+    of two products) stays below the sum of the half steps."""
+    x, logits, up, down = _layer(t, e, k, d, inner, seed=t, dead=dead)
+    ref = _layer_oracle(x, logits, k, up, down)
+    leaf = [v.to(DEV).requires_grad_() for v in (x, logits, up, down)]
+    out = experts.mlp(leaf[0], leaf[1], k, leaf[2], leaf[3])
+    assert (out.cpu().double() - ref).norm() <= 3 * 2.0 ** -8 * ref.norm()
+    dout = torch.randn(t, d, generator=torch.Generator().manual_seed(9)).to(BF16)
+    got = torch.autograd.grad(out, leaf, dout.to(DEV))
+    # the same in float64 torch, the oracle's choices held fixed
+    p = [v.double().requires_grad_() for v in (x, logits, up, down)]
+    _, chosen, offsets, rows, slots = O.route(logits, k)
+    live = (chosen >= 0)
+    l = torch.where(torch.isinf(p[1]), torch.zeros_like(p[1]), p[1])
+    w = torch.softmax(torch.gather(l, 1, chosen.clamp(min=0)), 1) * live
+    a, _ = O.gemm(p[0], p[2], offsets, rows, silu_mul=True)
+    want = torch.autograd.grad(O.combine(O.gemm(a, p[3], offsets)[0], slots, w), p, dout.double())
+    for name, a, b in zip(("x", "logits", "up", "down"), got, want):
+        b = torch.nan_to_num(b)
+        assert (a.cpu().double() - b).norm() <= 6 * 2.0 ** -8 * b.norm() + 1e-12, name
+    if d % 16 or inner % 16:
+        return
+    qu, su = fp8.quant(up.to(DEV))
+    qd, sd = fp8.quant(down.to(DEV))
+    one = torch.ones(d, dtype=BF16, device=DEV)
+    res = torch.zeros(t, d, dtype=BF16, device=DEV)
+    _, (q, s) = hk.ops.block_norm(x.to(DEV), res, pre=one, quant="fp8")
+    scales = dict(gate_up_scale=su.squeeze(2), down_scale=sd.squeeze(2))
+    y = experts.mlp((q, s), logits.to(DEV), k, qu, qd, **scales)
+    xd = x.double()
+    ref8 = _layer_oracle(xd / torch.sqrt((xd * xd).mean(1, keepdim=True) + 1e-6), logits, k, up, down)
+    assert (y.cpu().double() - ref8).norm() <= 4 * 2.0 ** -4 * ref8.norm()
+    # on the numbers that the codes stand for, the products alone: bf16's roundings and the second quantization
+    ref8 = _layer_oracle((q.float() * s).cpu(), logits, k, (qu.float() * su).cpu(), (qd.float() * sd).cpu())
+    assert (y.cpu().double() - ref8).norm() <= (2.0 ** -4 + 3 * 2.0 ** -8) * ref8.norm()
+    z = experts.mlp((q, s), logits.to(DEV), k, qu, qd, **scales)
+    assert torch.equal(y, z)
+
+
+def test_graphs_streams_and_threads():
+    """Captured once and replayed over new inputs, with eager work between; on another stream; two threads at once."""
+    import threading
+
+    x, logits, up, down = (v.to(DEV) for v in _layer(200, 8, 2, 64, 48, seed=1))
+    calls = [v.to(DEV) for v in (torch.randn(5, 200, 64).to(BF16), torch.randn(5, 200, 8))]
+    eager = [experts.mlp(a, b, 2, up, down) for a, b in zip(*calls)]
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        graphs = []
+        for _ in range(2):
+            a, b = torch.zeros_like(x), torch.zeros_like(logits)
+            experts.mlp(a, b, 2, up, down)
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph, stream=stream):
+                out = experts.mlp(a, b, 2, up, down)
+            graphs.append((graph, a, b, out))
+        for i in range(5):
+            graph, a, b, out = graphs[i % 2]
+            a.copy_(calls[0][i])
+            b.copy_(calls[1][i])
+            graph.replay()
+            assert torch.equal(out, eager[i])
+            assert torch.equal(experts.mlp(calls[0][0], calls[1][0], 2, up, down), eager[0])
+            torch.cuda.synchronize()
+    seen = {}
+
+    def work(i):
+        s = torch.cuda.Stream()
+        with torch.cuda.stream(s):
+            seen[i] = [experts.mlp(a, b, 2, up, down) for a, b in zip(*calls) for _ in range(3)]
+        s.synchronize()
+
+    torch.cuda.synchronize()
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    [th.start() for th in threads]
+    [th.join() for th in threads]
+    for got in seen.values():
+        assert all(torch.equal(v, eager[i // 3]) for i, v in enumerate(got))
+
+
+def test_the_same_bits_every_time():
+    x, logits, up, down = (v.to(DEV) for v in _layer(1500, 16, 4, 128, 96, seed=2))
+    first = None
+    for _ in range(3):
+        leaf = [v.clone().requires_grad_() for v in (x, logits, up, down)]
+        out = experts.mlp(leaf[0], leaf[1], 4, leaf[2], leaf[3])
+        now = [out.detach(), *torch.autograd.grad(out, leaf, torch.ones_like(out))]
+        first = first or now
+        assert all(torch.equal(a, b) for a, b in zip(first, now))
+
+
+def test_gemm_refuses_a_second_derivative_and_out_with_gradients():
+    plan, _ = _plan(10, 2, 1, seed=1)
+    x = torch.randn(10, 16, device=DEV).to(BF16).requires_grad_()
+    w = torch.randn(2, 8, 16, device=DEV).to(BF16).requires_grad_()
+    (dx,) = torch.autograd.grad(experts.gemm(x, w, plan).float().square().sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError):
+        dx.sum().backward()
+    with pytest.raises(ValueError, match="out="):
+        experts.gemm(x, w, plan, out=torch.empty(10, 8, dtype=BF16, device=DEV))
+
+
+def test_a_call_of_known_layout_checks_its_tensors_again():
+    plan, _ = _plan(10, 2, 1, seed=1)
+    x, w = torch.randn(10, 16, device=DEV).to(BF16), torch.randn(2, 8, 16, device=DEV).to(BF16)
+    y = experts.gemm(x, w, plan)
+    with pytest.raises(ValueError):
+        experts.gemm(x, w.cpu(), plan)
+    with pytest.raises(ValueError):
+        experts.gemm(x, w, experts.Plan(plan.offsets.cpu()))
+    odd = torch.empty(10 * 16 + 1, dtype=BF16, device=DEV)[1:].view(10, 16).copy_(x)
+    assert odd.data_ptr() % 16 and torch.equal(experts.gemm(odd, w, plan), y)
+    assert nat.lib() is not None
