@@ -135,9 +135,9 @@ int hkx_experts_gemm(const HkxExpertsGemmArgs* args, void* stream) {
     return api_fail(HKX_ERR_SHAPE, "experts_gemm: the scales' alignment");
   // offsets in a tile, in an expert of B, and in an A that an index picks from are 32-bit
   const int64_t lim = ((int64_t)1 << 32) - 4096;
-  if (256 * g.lda * es > lim || (nt ? brows : 256) * g.ldb * es > lim || (g.index && g.a_rows * g.lda * es > lim))
+  if (256 * g.lda * es > lim || 256 * g.ldc * 2 > lim || 256 * g.ldz * 2 > lim || (nt ? brows : 256) * g.ldb * es > lim || (g.index && g.a_rows * g.lda * es > lim))
     return api_fail(HKX_ERR_SHAPE, "experts_gemm: an expert's B or an indexed A spans 4 GiB or more; split the call");
-  if (g.kernel < 0 || g.kernel > HKX_EXPERTS_TILE128) return api_fail(HKX_ERR_ARG, "experts_gemm: kernel %d", g.kernel);
+  if (g.kernel < 0 || g.kernel > HKX_EXPERTS_QUAD) return api_fail(HKX_ERR_ARG, "experts_gemm: kernel %d", g.kernel);
   if (g.rows == 0 && !tn) return HKX_OK;
   GroupArgs a{};
   a.a = (const uint8_t*)g.a;
@@ -167,6 +167,8 @@ int hkx_experts_gemm(const HkxExpertsGemmArgs* args, void* stream) {
   a.bias_dt = g.bias_dtype;
   a.sa_ld = g.sa_ld != 0;
   a.sb_col = g.sb_col != 0;
+  if (g.kernel == HKX_EXPERTS_QUAD && !group_quad_ok(a))
+    return api_fail(HKX_ERR_SHAPE, "experts_gemm: the 256-row kernel stores 16-byte aligned rows");
   const hipError_t e = launch_group(a, g.op, fp8, g.silu_mul != 0, g.kernel, api_cus(), (hipStream_t)stream);
   if (e == hipErrorInvalidConfiguration)
     return api_fail(HKX_ERR_SHAPE, "experts_gemm: rows=%d of n=%d are more tiles than a launch takes; split the call", g.rows, g.n);

@@ -99,6 +99,49 @@ HKX_DEV int group_place(int v, int total) {
   return (v >> 3) < per && at < total ? at : -1;
 }
 
+// A tile: group e, its rows (columns of A in TN) from m0 on, C's columns from n0 on, `rows` of them in C; row0: the
+// first row of R (TN: of the contraction), klen: the contraction's length.
+struct GroupTile {
+  int e, m0, n0, rows, klen;
+  int64_t row0;
+};
+
+// Tile `in` of tm x tn: eight tile rows at a time, down them first, so that the tiles in flight on an XCD share panels
+// of A and of B.
+HKX_DEV void group_raster(int in, int tm, int tn, int& tr, int& tc) {
+  const int g = in / (8 * tn), first = 8 * g, gm = min(tm - first, 8), r = in - g * 8 * tn;
+  tr = first + r % gm;
+  tc = r / gm;
+}
+
+// rows_of(e, lo, hi): group e's rows.
+template <int OP, int BM, int CN, typename Rows>
+HKX_DEV GroupTile group_tile_at(const GroupMap& map, const GroupArgs& p, int at, int tiles_n, Rows rows_of) {
+  GroupTile t;
+  int lo, hi, tr, tc;
+  if constexpr (OP == kGroupTN) {
+    const int tiles_m = (p.m + BM - 1) / BM, per = tiles_m * tiles_n;
+    t.e = at / per;
+    group_raster(at - t.e * per, tiles_m, tiles_n, tr, tc);
+    rows_of(t.e, lo, hi);
+    t.m0 = tr * BM;
+    t.rows = min(p.m - t.m0, BM);
+    t.row0 = lo;
+    t.klen = hi - lo;
+  } else {
+    t.e = group_of(map, p.experts + 1, at / tiles_n);
+    const int t0 = map.first[t.e];
+    group_raster(at - t0 * tiles_n, map.first[t.e + 1] - t0, tiles_n, tr, tc);
+    rows_of(t.e, lo, hi);
+    t.m0 = tr * BM;
+    t.row0 = lo + t.m0;
+    t.rows = min(hi - (int)t.row0, BM);
+    t.klen = t.e == p.experts ? 0 : p.k;
+  }
+  t.n0 = tc * CN;
+  return t;
+}
+
 constexpr uint32_t kGroupOut = 0xfffffff0u;  // an offset past every resource: reads 0
 
 // A resource of `rows` rows of `row` bytes, `ld` apart, from a 64-bit address (0 rows: reads 0).
@@ -112,15 +155,102 @@ HKX_DEV __amdgpu_buffer_rsrc_t group_rsrc(const uint8_t* p, int rows, int64_t ld
 // * K-contiguous rows: 128 bytes a row, its 16-byte chunk c at c ^ (row % 8). A fill instruction moves 8 rows.
 // * rows along K (NN's B, TN's A and B): 64 rows of 128 values, 256 bytes; the 32-byte pair of chunks j (16 values, a
 //   fragment's columns) at j ^ group_swz(row), so that the four rows that 16 lanes read, and those of the next
-//   16, lie in different banks. A fill instruction moves 4 rows. ds_read_tr16_b64 turns them: of 16 lanes, lane i names
+//   16, lie in different banks. A fill instruction moves 4 rows. ds_read_b64_tr_b16 turns them: of 16 lanes, lane i names
 //   row i / 4, values 4 (i % 4) + [0, 4), and is given value i of the four rows.
 
 HKX_DEV uint32_t group_swz(uint32_t k) { return (k & 3) | ((k >> 1) & 4); }
 
-typedef short s16x4 __attribute__((ext_vector_type(4)));
+// Fragments of 16 values from a quarter of rows along K: `at` their LDS addresses (turned_at, 8 KB a K-half on, 1 KB the
+// half's later rows), out[f] the K-halves of fragment f. The reads and their wait are one block: behind the compiler's own
+// instruction for them stands a wait for every fill in flight.
+template <int N>
+HKX_DEV void read_turned(const uint32_t (&at)[N], bf16x8 (&out)[N][2]) {
+  u32x2 v[4 * N];
+  static_assert(N == 2 || N == 4 || N == 6, "fragments");
+  if constexpr (N == 2) {
+    asm volatile(
+      "ds_read_b64_tr_b16 %0, %8 offset:0\n"
+      "ds_read_b64_tr_b16 %1, %8 offset:1024\n"
+      "ds_read_b64_tr_b16 %2, %8 offset:8192\n"
+      "ds_read_b64_tr_b16 %3, %8 offset:9216\n"
+      "ds_read_b64_tr_b16 %4, %9 offset:0\n"
+      "ds_read_b64_tr_b16 %5, %9 offset:1024\n"
+      "ds_read_b64_tr_b16 %6, %9 offset:8192\n"
+      "ds_read_b64_tr_b16 %7, %9 offset:9216\n"
+      "s_waitcnt lgkmcnt(0)"
+        : "=&v"(v[0]), "=&v"(v[1]), "=&v"(v[2]), "=&v"(v[3]), "=&v"(v[4]), "=&v"(v[5]), "=&v"(v[6]), "=&v"(v[7])
+        : "v"(at[0]), "v"(at[1])
+        : "memory");
+  }
+  if constexpr (N == 4) {
+    asm volatile(
+      "ds_read_b64_tr_b16 %0, %16 offset:0\n"
+      "ds_read_b64_tr_b16 %1, %16 offset:1024\n"
+      "ds_read_b64_tr_b16 %2, %16 offset:8192\n"
+      "ds_read_b64_tr_b16 %3, %16 offset:9216\n"
+      "ds_read_b64_tr_b16 %4, %17 offset:0\n"
+      "ds_read_b64_tr_b16 %5, %17 offset:1024\n"
+      "ds_read_b64_tr_b16 %6, %17 offset:8192\n"
+      "ds_read_b64_tr_b16 %7, %17 offset:9216\n"
+      "ds_read_b64_tr_b16 %8, %18 offset:0\n"
+      "ds_read_b64_tr_b16 %9, %18 offset:1024\n"
+      "ds_read_b64_tr_b16 %10, %18 offset:8192\n"
+      "ds_read_b64_tr_b16 %11, %18 offset:9216\n"
+      "ds_read_b64_tr_b16 %12, %19 offset:0\n"
+      "ds_read_b64_tr_b16 %13, %19 offset:1024\n"
+      "ds_read_b64_tr_b16 %14, %19 offset:8192\n"
+      "ds_read_b64_tr_b16 %15, %19 offset:9216\n"
+      "s_waitcnt lgkmcnt(0)"
+        : "=&v"(v[0]), "=&v"(v[1]), "=&v"(v[2]), "=&v"(v[3]), "=&v"(v[4]), "=&v"(v[5]), "=&v"(v[6]), "=&v"(v[7]), "=&v"(v[8]), "=&v"(v[9]), "=&v"(v[10]), "=&v"(v[11]), "=&v"(v[12]), "=&v"(v[13]), "=&v"(v[14]), "=&v"(v[15])
+        : "v"(at[0]), "v"(at[1]), "v"(at[2]), "v"(at[3])
+        : "memory");
+  }
+  if constexpr (N == 6) {
+    asm volatile(
+      "ds_read_b64_tr_b16 %0, %24 offset:0\n"
+      "ds_read_b64_tr_b16 %1, %24 offset:1024\n"
+      "ds_read_b64_tr_b16 %2, %24 offset:8192\n"
+      "ds_read_b64_tr_b16 %3, %24 offset:9216\n"
+      "ds_read_b64_tr_b16 %4, %25 offset:0\n"
+      "ds_read_b64_tr_b16 %5, %25 offset:1024\n"
+      "ds_read_b64_tr_b16 %6, %25 offset:8192\n"
+      "ds_read_b64_tr_b16 %7, %25 offset:9216\n"
+      "ds_read_b64_tr_b16 %8, %26 offset:0\n"
+      "ds_read_b64_tr_b16 %9, %26 offset:1024\n"
+      "ds_read_b64_tr_b16 %10, %26 offset:8192\n"
+      "ds_read_b64_tr_b16 %11, %26 offset:9216\n"
+      "ds_read_b64_tr_b16 %12, %27 offset:0\n"
+      "ds_read_b64_tr_b16 %13, %27 offset:1024\n"
+      "ds_read_b64_tr_b16 %14, %27 offset:8192\n"
+      "ds_read_b64_tr_b16 %15, %27 offset:9216\n"
+      "ds_read_b64_tr_b16 %16, %28 offset:0\n"
+      "ds_read_b64_tr_b16 %17, %28 offset:1024\n"
+      "ds_read_b64_tr_b16 %18, %28 offset:8192\n"
+      "ds_read_b64_tr_b16 %19, %28 offset:9216\n"
+      "ds_read_b64_tr_b16 %20, %29 offset:0\n"
+      "ds_read_b64_tr_b16 %21, %29 offset:1024\n"
+      "ds_read_b64_tr_b16 %22, %29 offset:8192\n"
+      "ds_read_b64_tr_b16 %23, %29 offset:9216\n"
+      "s_waitcnt lgkmcnt(0)"
+        : "=&v"(v[0]), "=&v"(v[1]), "=&v"(v[2]), "=&v"(v[3]), "=&v"(v[4]), "=&v"(v[5]), "=&v"(v[6]), "=&v"(v[7]), "=&v"(v[8]), "=&v"(v[9]), "=&v"(v[10]), "=&v"(v[11]), "=&v"(v[12]), "=&v"(v[13]), "=&v"(v[14]), "=&v"(v[15]), "=&v"(v[16]), "=&v"(v[17]), "=&v"(v[18]), "=&v"(v[19]), "=&v"(v[20]), "=&v"(v[21]), "=&v"(v[22]), "=&v"(v[23])
+        : "v"(at[0]), "v"(at[1]), "v"(at[2]), "v"(at[3]), "v"(at[4]), "v"(at[5])
+        : "memory");
+  }
+#pragma unroll
+  for (int f = 0; f < N; ++f)
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const u32x2 lo = v[4 * f + 2 * h], hi = v[4 * f + 2 * h + 1];
+      out[f][h] = __builtin_bit_cast(bf16x8, i32x4{(int)lo.x, (int)lo.y, (int)hi.x, (int)hi.y});
+    }
+}
 
-HKX_DEV s16x4 read_turned(const uint8_t* s) {
-  return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)s);
+HKX_DEV uint32_t lds_address(const uint8_t* s) { return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const uint8_t*)s; }
+
+// What a lane adds to a quarter's address for the fragment of values 16 j + [0, 16).
+HKX_DEV uint32_t turned_at(int lane, uint32_t j) {
+  const uint32_t rf = lane & 15, k = 8 * (lane >> 4) + rf / 4;
+  return k * 256 + (j ^ group_swz(k)) * 32 + (rf % 4) * 8;
 }
 
 // The product on BM x BN tiles, BN = 16 FN WN rows of B: WM x WN waves of BM / WM rows and 16 FN columns, S stages
@@ -139,47 +269,26 @@ __global__ void __launch_bounds__(64 * WM * WN) group_tile_kernel(const GroupArg
   static_assert(!TB || BN == 128, "rows along K: 128 values");
   static_assert(!TA || BM == 128, "rows along K: 128 values");
   static_assert(!PAIR || (FN % 2 == 0 && OP == kGroupNT), "gate and up fragments of one wave");
-  __shared__ __attribute__((aligned(16))) uint8_t smem[S * STAGE];
-  __shared__ GroupMap map;
+  // (one array: beside a second one the compiler waits for every fill before each LDS read)
+  __shared__ __attribute__((aligned(16))) uint8_t smem[S * STAGE + (TA ? 0 : sizeof(GroupMap))];
+  GroupMap& map = *(GroupMap*)(smem + (TA ? 0 : S * STAGE));
 
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wr = wave / WN, wc = wave % WN;
   const int tiles_n = (p.n + CN - 1) / CN;
 
-  // ---- the tile: group e, its rows [m0, m0 + mrows) of C, columns n0 .., the contraction's length
-  int e, m0, mrows, n0, klen;
-  int64_t row0 = 0;  // the group's first row of R (TN: of the contraction; else of the tile)
-  if constexpr (TA) {
-    const int tiles_m = (p.m + BM - 1) / BM, per = tiles_m * tiles_n;
-    const int at = group_place((int)blockIdx.x, p.experts * per);
-    if (at < 0) return;
-    e = at / per;
-    m0 = (at % per) % tiles_m * BM;
-    n0 = (at % per) / tiles_m * CN;
-    mrows = min(p.m - m0, BM);
-    int lo, hi;
-    group_rows(p, e, lo, hi);
-    row0 = lo;
-    klen = hi - lo;
-  } else {
-    const int groups = p.experts + 1;
-    group_map<BM>(map, p, tid, 64 * NW);
-    const int at = group_place((int)blockIdx.x, map.first[groups] * tiles_n);
-    if (at < 0) return;
-    // (tile rows fastest: tiles that share a panel of B follow one another)
-    e = group_of(map, groups, at / tiles_n);
-    const int t0 = map.first[e], tm = map.first[e + 1] - t0, in = at - t0 * tiles_n;
-    m0 = in % tm * BM;
-    n0 = in / tm * CN;
-    int lo, hi;
-    group_rows(p, e, lo, hi);
-    row0 = lo + m0;
-    mrows = min(hi - (int)row0, BM);
-    klen = p.k;
-  }
+  const int groups = p.experts + 1;
+  if constexpr (!TA) group_map<BM>(map, p, tid, 64 * NW);
+  const int total = TA ? p.experts * ((p.m + BM - 1) / BM) * tiles_n : map.first[groups] * tiles_n;
+  const int place = group_place((int)blockIdx.x, total);
+  if (place < 0) return;
+  const GroupTile tile = group_tile_at<OP, BM, CN>(
+      map, p, place, tiles_n, [&](int g, int& lo, int& hi) { group_rows(p, g, lo, hi); });
+  const int e = tile.e, m0 = tile.m0, mrows = tile.rows, n0 = tile.n0, klen = tile.klen;
+  const int64_t row0 = tile.row0;
   const bool rest = e == p.experts;  // the rows behind the last group
-  const int nku = rest ? 0 : (klen + KU - 1) / KU;
+  const int nku = (klen + KU - 1) / KU;
 
   // ---- fills
   __amdgpu_buffer_rsrc_t ra, rb;
@@ -265,16 +374,20 @@ __global__ void __launch_bounds__(64 * WM * WN) group_tile_kernel(const GroupArg
       return *(const bf16x8*)(row + (((4 * h + q) ^ (rf & 7)) << 4));
     }
   };
-  auto turned = [&](const uint8_t* s, int r0, int h) -> Frag {
-    s16x4 v[2];
+  // both K-halves of a wave's fragments: along r0 + [0, 16 N) of an operand's rows
+  auto read = [&](const uint8_t* s, int r0, auto along, auto& out) {
+    constexpr int N = sizeof(out) / sizeof(out[0]);
+    if constexpr (decltype(along)::value) {
+      uint32_t at[N];
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      const uint32_t k = 32 * h + 8 * q + 4 * t + rf / 4;
-      v[t] = read_turned(s + k * 256 + (((uint32_t)r0 / 16) ^ group_swz(k)) * 32 + (rf % 4) * 8);
+      for (int f = 0; f < N; ++f) at[f] = lds_address(s) + turned_at(lane, r0 / 16 + f);
+      read_turned<N>(at, out);
+    } else {
+#pragma unroll
+      for (int f = 0; f < N; ++f)
+#pragma unroll
+        for (int h = 0; h < KH; ++h) out[f][h] = straight(s, r0 + 16 * f, h);
     }
-    typedef short s16x8 __attribute__((ext_vector_type(8)));
-    if constexpr (FP8) return Frag{};
-    else return __builtin_bit_cast(bf16x8, __builtin_shufflevector(v[0], v[1], 0, 1, 2, 3, 4, 5, 6, 7));
   };
 
   f32x4 acc[FM][FN] = {};
@@ -289,21 +402,18 @@ __global__ void __launch_bounds__(64 * WM * WN) group_tile_kernel(const GroupArg
     __builtin_amdgcn_sched_barrier(0);
     fill(t + S - 1);
     const uint8_t* s = smem + (t % S) * STAGE;
+    Frag af[FM][2], bf[FN][2];
+    read(s, wr * (BM / WM), std::bool_constant<TA>{}, af);
+    read(s + AB, wc * FN * 16, std::bool_constant<TB>{}, bf);
 #pragma unroll
-    for (int h = 0; h < KH; ++h) {
-      Frag af[FM], bf[FN];
-#pragma unroll
-      for (int f = 0; f < FM; ++f) af[f] = TA ? turned(s, wr * (BM / WM) + 16 * f, h) : straight(s, wr * (BM / WM) + 16 * f, h);
-#pragma unroll
-      for (int g = 0; g < FN; ++g) bf[g] = TB ? turned(s + AB, (wc * FN + g) * 16, h) : straight(s + AB, (wc * FN + g) * 16, h);
+    for (int h = 0; h < KH; ++h)
 #pragma unroll
       for (int f = 0; f < FM; ++f)
 #pragma unroll
         for (int g = 0; g < FN; ++g) {
-          if constexpr (FP8) acc[f][g] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(bf[g], af[f], acc[f][g], 0, 0, 0, 0, 0, 0);
-          else acc[f][g] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(bf[g], af[f], acc[f][g], 0, 0, 0);
+          if constexpr (FP8) acc[f][g] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(bf[g][h], af[f][h], acc[f][g], 0, 0, 0, 0, 0, 0);
+          else acc[f][g] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(bf[g][h], af[f][h], acc[f][g], 0, 0, 0);
         }
-    }
   }
   __builtin_amdgcn_s_waitcnt(wait_vm(0));  // no fill lands in LDS after the exit
 

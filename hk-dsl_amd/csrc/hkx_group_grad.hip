@@ -13,6 +13,8 @@ hipError_t launch_group_grad(const GroupArgs& a, int op, int bm, hipStream_t s) 
 hipError_t launch_group(const GroupArgs& a, int op, bool fp8, bool pair, int kernel, int cus, hipStream_t s) {
   // rows an expert, were they even (the host does not know the counts)
   const int64_t each = a.rows / a.experts;
+  if (kernel == HKX_EXPERTS_QUAD || (kernel == HKX_EXPERTS_AUTO && each >= 128 && group_quad_ok(a)))
+    return op == kGroupNT ? launch_group_quad_nt(a, fp8, pair, cus, s) : launch_group_quad_grad(a, op, cus, s);
   const int bm = kernel == HKX_EXPERTS_TILE16 ? 16 : kernel == HKX_EXPERTS_TILE64 ? 64 : kernel == HKX_EXPERTS_TILE128 ? 128
                  : each <= 16 ? 16 : each <= 64 ? 64 : 128;
   return op == kGroupNT ? launch_group_nt(a, fp8, pair, bm, s) : launch_group_grad(a, op, bm, s);

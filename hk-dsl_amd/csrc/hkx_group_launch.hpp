@@ -12,6 +12,15 @@ hipError_t launch_group(const GroupArgs& a, int op, bool fp8, bool pair, int ker
 hipError_t launch_group_nt(const GroupArgs& a, bool fp8, bool pair, int bm, hipStream_t s);
 hipError_t launch_group_grad(const GroupArgs& a, int op, int bm, hipStream_t s);
 
+// 256 x 256 tiles, at most `cus` workgroups
+hipError_t launch_group_quad_nt(const GroupArgs& a, bool fp8, bool pair, int cus, hipStream_t s);
+hipError_t launch_group_quad_grad(const GroupArgs& a, int op, int cus, hipStream_t s);
+// C's rows are stored 16 bytes a lane
+inline bool group_quad_ok(const GroupArgs& a) {
+  auto whole = [](const void* p, int64_t ld) { return !p || ((uintptr_t)p % 16 == 0 && ld % 16 == 0); };
+  return whole(a.c, a.ldc) && a.c_group % 16 == 0 && whole(a.z, a.ldz) && (!a.bias || a.bias_ld * (a.bias_dt == HKX_FP32 ? 4 : 2) % 16 == 0);
+}
+
 // A grid of `tiles` workgroups and the places that their order over the XCDs leaves open.
 inline bool group_grid(int64_t tiles, int threads, dim3& grid) {
   const int64_t n = (tiles + 7) / 8 * 8;
