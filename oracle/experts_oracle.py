@@ -46,7 +46,7 @@ def gemm(x, w, offsets, rows=None, bias=None, silu_mul=False):
         xe = x[lo:hi] if rows is None else x[rows[lo:hi].long()]
         z = xe.double() @ w[e].double().t()
         parts.append(z if bias is None else z + bias[e].double())
-    z = torch.cat([*parts, torch.zeros(r - off[-1], w.shape[1], dtype=torch.float64)])
+    z = torch.cat([*parts, torch.zeros(r - off[-1], w.shape[1], dtype=torch.float64, device=w.device)])
     if not silu_mul:
         return z, z
     n = w.shape[1] // 2
