@@ -249,7 +249,16 @@ def _e4m3_rows(x):
     return (x / s).clamp(-448, 448).to(E4M3), s
 
 
+def _package():
+    if own:
+        path = str(Path(__file__).resolve().parents[1] / "hk-dsl_amd")
+        if path not in sys.path:
+            sys.path.insert(0, path)
+        import hk  # noqa: F401, PLC0415
+
+
 def prepare(case, seed):
+    _package()
     gen = torch.Generator(device="cuda").manual_seed(seed)
     kind = case["kind"]
     if kind == "norm":
@@ -288,17 +297,10 @@ def prepare(case, seed):
     return st
 
 
-def _package():
-    path = str(Path(__file__).resolve().parents[1] / "hk-dsl_amd")
-    if path not in sys.path:
-        sys.path.insert(0, path)
+def _own(st):
     import hk  # noqa: PLC0415
 
-    return hk.ops
-
-
-def _own(st):
-    ops = _package()
+    ops = hk.ops
     experts, kind = ops.experts, st["kind"]
     if kind == "norm":
         h, (q, s) = ops.block_norm(st["x"], st["residual"], pre=st["pre"], eps=EPS, quant="fp8")
