@@ -1,6 +1,8 @@
 // Host-side launchers of the experts' products, one translation unit a kind of tile.
 #pragma once
 
+#include <algorithm>
+
 #include "hkx_group.hpp"
 
 namespace hkx {
@@ -21,11 +23,18 @@ inline bool group_quad_ok(const GroupArgs& a) {
   return whole(a.c, a.ldc) && a.c_group % 16 == 0 && whole(a.z, a.ldz) && (!a.bias || a.bias_ld * (a.bias_dt == HKX_FP32 ? 4 : 2) % 16 == 0);
 }
 
-// A grid of `tiles` workgroups and the places that their order over the XCDs leaves open.
+// A grid of `tiles` workgroups and the places that their order over the XCDs leaves open (group_place).
 inline bool group_grid(int64_t tiles, int threads, dim3& grid) {
-  const int64_t n = (tiles + 7) / 8 * 8;
+  const int64_t n = (tiles + 255) / 256 * 256;
   if (n * threads >= ((int64_t)1 << 32) || n > INT32_MAX) return false;
   grid = dim3((unsigned)n);
+  return true;
+}
+
+// The persistent kernel's: a workgroup a CU, whole rounds of places.
+inline bool group_quad_grid(int64_t tiles, int cus, dim3& grid) {
+  if (tiles > INT32_MAX - 65536) return false;
+  grid = dim3((unsigned)std::max(cus / 256 * 256, 256));
   return true;
 }
 

@@ -60,13 +60,13 @@ __global__ void __launch_bounds__(512, 1) group_quad_kernel(const GroupArgs p) {
   };
   const int total = __builtin_amdgcn_readfirstlane(TA ? p.experts * ((p.m + BM - 1) / BM) * tiles_n
                                                       : map.first[p.experts + 1] * tiles_n);
-  // the workgroup's tiles: places of v, v + grid, ... (grid a multiple of 8, so all on its XCD's stretch)
-  const int per = (total + 7) >> 3, x = (int)blockIdx.x & 7, y0 = (int)blockIdx.x >> 3, step = (int)gridDim.x >> 3;
-  const int my_tiles = max(0, (min(per, total - x * per) - y0 + step - 1) / step);
+  // the workgroup's tiles: the places of its number, and of it and the grid (a multiple of 256, or one round) on and on
+  const int place = group_place((int)blockIdx.x), step = (int)gridDim.x;
+  const int my_tiles = place < total ? (total - place + step - 1) / step : 0;
   if (my_tiles == 0) return;
   auto tile_at = [&](int lt) {
     const GroupArgs& p = args_anew();
-    GroupTile t = group_tile_at<OP, BM, BN>(map, p, x * per + y0 + lt * step, tiles_n, rows_of);
+    GroupTile t = group_tile_at<OP, BM, BN>(map, p, place + lt * step, tiles_n, rows_of);
     t.e = __builtin_amdgcn_readfirstlane(t.e);
     t.m0 = __builtin_amdgcn_readfirstlane(t.m0);
     t.n0 = __builtin_amdgcn_readfirstlane(t.n0);
@@ -79,97 +79,141 @@ __global__ void __launch_bounds__(512, 1) group_quad_kernel(const GroupArgs p) {
 
   // ---- fills. Instruction k (0, 1) of wave w: K-contiguous rows 16 w + 8 k + [0, 8) of a quarter, lane l row l % 32 / 4,
   // K-half l / 32, its 16-byte piece (l % 4) ^ swz4(row); rows along K 8 w + 4 k + [0, 4), lane l row l / 16.
-  uint32_t la[2], lb[2], lch[2];
-#pragma unroll
-  for (int k = 0; k < 2; ++k) {
-    const uint32_t r = (uint32_t)(16 * wave + 8 * k + (lane & 31) / 4);
-    const uint32_t rb = PAIR ? (uint32_t)(16 * (wave >> 1) + 8 * k + (lane & 31) / 4 + ((wave & 1) ? p.n : 0)) : r;
-    lch[k] = (uint32_t)(64 * (lane >> 5) + 16 * ((lane & 3) ^ ((wave & 1) | (k << 1))));
-    const uint32_t kr = (uint32_t)(8 * wave + 4 * k + lane / 16), kc = (uint32_t)((lane % 16) ^ (group_swz(kr) << 1)) * 16u;
-    la[k] = TA ? kr * (uint32_t)p.lda + kc : r * (uint32_t)p.lda + lch[k];
-    lb[k] = TB ? kr * (uint32_t)p.ldb + kc : rb * (uint32_t)p.ldb + lch[k];
-  }
-  const uint32_t k_row = (uint32_t)p.k * ES;  // NT, NN: bytes of a K-contiguous row
-
-  // The two fill streams: s1 a unit ahead (A1), s2 two (A0, B0, B1).
-  struct Ahead {
-    int t, nkt, par;           // its unit in its tile, the tile's units, its slot
-    int left;                  // TN, NN: rows along K that are left
-    const uint8_t *a, *b;
-    uint32_t ba, bb;           // the resources' bytes; of rows along K a row's
-    uint32_t b1;               // B's second half behind the first (0: past N, the first again: it is never stored)
-    uint32_t va[2];            // offsets of A's half
+  //
+  // Two streams walk the workgroup's units: one a unit ahead (A1), one two (A0, B0, B1). A unit's fills are loads at a
+  // scalar offset from a resource made once a tile (rows along K: moved on a unit at a time) into the stream's slot; what
+  // is not every unit's, a ragged last unit, units past K and the next tile, is told by one comparison with the stream's
+  // `edge` (scalar work between two barriers is time that no MFMA covers: 140 instructions of it a phase took NT from 1380
+  // to 1100 TFLOP/s).
+  auto lane_anew = [&]() {  // (made where a tile begins: held through the K loop it would spill)
+    int l = tid & 63;
+    asm volatile("" : "+v"(l));
+    return l;
+  };
+  auto row_of = [&](int l, int k) { return 16 * wave + 8 * k + (l & 31) / 4; };
+  auto piece_of = [&](int l, int k) { return (uint32_t)(64 * (l >> 5) + 16 * ((l & 3) ^ ((wave & 1) | (k << 1)))); };
+  auto along_of = [&](int l, int k, int64_t ld) {
+    const uint32_t kr = (uint32_t)(8 * wave + 4 * k + l / 16);
+    return kr * (uint32_t)ld + (uint32_t)((l % 16) ^ (group_swz(kr) << 1)) * 16u;
+  };
+  struct Walk {
+    int t, nkt, edge;     // its unit in its tile; the tile's units; the unit at which something changes
+    uint32_t slot;        // its slot, bytes
+    uint32_t so, inc;     // K-contiguous operands: the unit's offset along K
+    int lt, klen;         // its tile, and that tile's contraction
   };
   const bool gathered = NT && p.index != nullptr;
   const int32_t* const idx_lds = (const int32_t*)(smem + IDX);
   auto rows_bytes = [](int rows, int64_t ld, uint32_t row) { return rows > 0 ? (uint32_t)((rows - 1) * ld) + row : 0u; };
-  // a lane's row of a half, instruction k (made where a tile begins: held through the K loop it would spill)
-  auto row_a = [&](int k) {
-    int l = lane;
-    asm volatile("" : "+v"(l));
-    return 16 * wave + 8 * k + (l & 31) / 4;
+  Walk w1{}, w2{};
+  __amdgpu_buffer_rsrc_t ra1 = make_rsrc(nullptr, 0), ra2 = ra1, rb = ra1;
+  uint32_t va1[2], va2[2], vb[2];
+  const uint8_t *pa1 = nullptr, *pa2 = nullptr, *pb = nullptr;  // rows along K: the unit's first
+  uint32_t na1 = 0, na2 = 0, nb = 0;                            // and the resource's bytes
+  uint32_t b1 = 0;  // B's second half behind the first (0: past N, the first again: it is never stored)
+  GroupTile cur = tile_at(0), nxt = cur;
+
+  auto load2 = [&](__amdgpu_buffer_rsrc_t r, uint32_t slot, const uint32_t (&v)[2], uint32_t so) {
+    uint8_t* s = smem + slot + wave * 2048;
+    buf_load16_lds(r, s, v[0], so);
+    buf_load16_lds(r, s + 1024, v[1], so);
   };
-  // A's offsets of half i from its row numbers
-  auto offset_of = [&](int j, int k) { return (uint32_t)j < (uint32_t)p.a_rows ? (uint32_t)j * (uint32_t)p.lda + lch[k] : kGroupOut; };
-  auto begin_a = [&](Ahead& s, const GroupTile& t, int i) {
+  auto fill_a1 = [&]() { load2(ra1, w1.slot + QB, va1, TA ? 0u : w1.so); };
+  auto fill_a0 = [&]() { load2(ra2, w2.slot, va2, TA ? 0u : w2.so); };
+  auto fill_b = [&](int j) { load2(rb, w2.slot + (2 + j) * QB, vb, (TB ? 0u : w2.so) + (j ? b1 : 0u)); };
+
+  // A's half i of tile t: offsets, and the resource of a K-contiguous A or the first rows and bytes of one along K
+  auto begin_a = [&](const GroupTile& t, int i, const int32_t* index, uint32_t (&v)[2], __amdgpu_buffer_rsrc_t& r,
+                     const uint8_t*& base, uint32_t& bytes) {
     const GroupArgs& p = args_anew();
+    const int l = lane_anew();
     if constexpr (TA) {
       const int m = t.m0 + (t.rows > 128 * i ? 128 * i : 0);  // (a half past M: the first again)
-      s.a = p.a + t.row0 * p.lda + (int64_t)m * 2;
-      s.ba = (uint32_t)(p.m - m) * 2u;
-      s.left = t.klen;
-    } else if (gathered) {
-      s.a = p.a;
-      s.ba = t.klen ? rows_bytes(p.a_rows, p.lda, k_row) : 0u;
+      base = p.a + t.row0 * p.lda + (int64_t)m * 2;
+      bytes = rows_bytes(64, p.lda, (uint32_t)(p.m - m) * 2u);
+      v[0] = along_of(l, 0, p.lda), v[1] = along_of(l, 1, p.lda);
     } else {
-      s.a = p.a + (t.row0 + 128 * i) * p.lda;
-      s.ba = t.klen ? rows_bytes(t.rows - 128 * i, p.lda, k_row) : 0u;
-    }
-  };
-  auto begin_b = [&](Ahead& s, const GroupTile& t) {
-    const GroupArgs& p = args_anew();
-    const int e = t.klen ? t.e : 0;
-    constexpr int HB = PAIR ? 64 : 128;
-    s.b1 = t.n0 + HB < p.n ? (TB ? HB * 2u : (uint32_t)HB * (uint32_t)p.ldb) : 0u;
-    s.bb = (uint32_t)(p.n - t.n0) * 2u;
-    if constexpr (TA) {
-      s.b = p.b + t.row0 * p.ldb + (int64_t)t.n0 * 2;
-    } else if constexpr (TB) {
-      s.b = p.b + e * p.b_group + (int64_t)t.n0 * 2;
-      s.left = t.klen;
-    } else {
-      s.b = p.b + e * p.b_group + t.n0 * p.ldb;
-      s.bb = t.klen ? rows_bytes((PAIR ? p.n : 0) + min(p.n - t.n0, BN), p.ldb, k_row) : 0u;
-    }
-  };
-  auto fill2 = [&](const uint8_t* base, uint32_t bytes, uint8_t* slot, const uint32_t (&v)[2], uint32_t so, bool straight, bool ends) {
-    const __amdgpu_buffer_rsrc_t r = make_rsrc(base, bytes);
+      const uint32_t k_row = (uint32_t)p.k * ES;
 #pragma unroll
-    for (int k = 0; k < 2; ++k)
-      buf_load16_lds(r, slot + wave * 2048 + k * 1024, straight && ends && so + lch[k] >= k_row ? kGroupOut : v[k], so);
-  };
-  // half i of A (B) of stream s's unit into its slot
-  auto fill_a = [&](const Ahead& s, int i) {
-    uint8_t* slot = smem + (s.par * 4 + i) * QB;
-    if constexpr (TA) {
-      fill2(s.a, rows_bytes(min(s.left, 64), p.lda, s.ba), slot, la, 0, false, false);
-    } else {
-      const uint32_t so = (uint32_t)s.t * 128u;
-      const bool in = s.ba != 0 && so < k_row;
-      const bool ends = in && so + 128u > k_row;
-      fill2(s.a, in ? s.ba : 0u, slot, NT ? s.va : la, in ? so : 0u, true, ends);
+      for (int k = 0; k < 2; ++k) {
+        const int row = row_of(l, k);
+        v[k] = (uint32_t)row * (uint32_t)p.lda + piece_of(l, k);
+        if (gathered) {
+          const int j = row + 128 * i < t.rows ? index[row + 128 * i] : -1;
+          v[k] = (uint32_t)j < (uint32_t)p.a_rows ? (uint32_t)j * (uint32_t)p.lda + piece_of(l, k) : kGroupOut;
+        }
+      }
+      r = gathered ? make_rsrc(p.a, rows_bytes(p.a_rows, p.lda, k_row))
+                   : make_rsrc(p.a + (t.row0 + 128 * i) * p.lda, rows_bytes(t.rows - 128 * i, p.lda, k_row));
+      // (no row of the half: every offset is out, as a resource of nothing is at any offset along K)
+      if (!gathered && t.rows <= 128 * i) r = make_rsrc(p.a, k_row), v[0] = v[1] = kGroupOut;
     }
   };
-  auto fill_b = [&](const Ahead& s, int j) {
-    uint8_t* slot = smem + (s.par * 4 + 2 + j) * QB;
-    const uint32_t c = j ? s.b1 : 0u;
+  auto begin_b = [&](const GroupTile& t) {
+    const GroupArgs& p = args_anew();
+    const int l = lane_anew();
+    constexpr int HB = PAIR ? 64 : 128;
+    b1 = t.n0 + HB < p.n ? (TB ? HB * 2u : (uint32_t)HB * (uint32_t)p.ldb) : 0u;
     if constexpr (TB) {
-      fill2(s.b + c, rows_bytes(min(s.left, 64), p.ldb, s.bb - c), slot, lb, 0, false, false);
+      pb = p.b + (TA ? t.row0 * p.ldb : t.e * p.b_group) + (int64_t)t.n0 * 2;
+      nb = rows_bytes(64, p.ldb, (uint32_t)(p.n - t.n0) * 2u);
+      vb[0] = along_of(l, 0, p.ldb), vb[1] = along_of(l, 1, p.ldb);
     } else {
-      const uint32_t so = (uint32_t)s.t * 128u;
-      const bool in = s.bb != 0 && so < k_row;
-      fill2(s.b + c, in ? s.bb - c : 0u, slot, lb, in ? so : 0u, true, in && so + 128u > k_row);
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const int row = PAIR ? 16 * (wave >> 1) + 8 * k + (l & 31) / 4 + ((wave & 1) ? p.n : 0) : row_of(l, k);
+        vb[k] = (uint32_t)row * (uint32_t)p.ldb + piece_of(l, k);
+      }
+      rb = make_rsrc(p.b + t.e * p.b_group + t.n0 * p.ldb, rows_bytes((PAIR ? p.n : 0) + min(p.n - t.n0, BN), p.ldb, (uint32_t)p.k * ES));
     }
+  };
+  // At unit w.t: a ragged last unit, units past K (nothing), or nothing special until the
+  // edge. out(k): what lanes past K of K-contiguous rows do; rows(n): rows along K that are left; none(): zeros.
+  auto at_edge = [&](Walk& w, auto out, auto rows, auto none) {
+    const int real = (w.klen + KU - 1) / KU, ragged = w.klen % KU;
+    if (w.t >= real) {
+      none();
+      w.so = w.inc = 0;
+      w.edge = w.nkt;
+    } else if (ragged && w.t == real - 1) {
+      if (TB) rows(ragged);
+      if (!TA) {
+        const int l = lane_anew();
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+          if (piece_of(l, k) >= (uint32_t)(ragged * ES)) out(k);
+      }
+      w.edge = real;
+    } else {
+      w.edge = ragged ? real - 1 : real;
+    }
+  };
+  auto edge1 = [&]() {
+    at_edge(w1, [&](int k) { va1[k] = kGroupOut; },
+            [&](int n) { if (TA) na1 -= (uint32_t)(64 - n) * (uint32_t)args_anew().lda; },
+            [&]() { na1 = 0; ra1 = make_rsrc(nullptr, 0); });
+  };
+  auto edge2 = [&]() {
+    at_edge(w2, [&](int k) { va2[k] = kGroupOut; if (!TB) vb[k] = kGroupOut; },
+            [&](int n) {
+              if (TA) na2 -= (uint32_t)(64 - n) * (uint32_t)args_anew().lda;
+              nb -= (uint32_t)(64 - n) * (uint32_t)args_anew().ldb;
+            },
+            [&]() { na2 = nb = b1 = 0; ra2 = rb = make_rsrc(nullptr, 0); });
+  };
+  auto begin1 = [&](const GroupTile& t, const int32_t* index) {
+    w1.t = 0, w1.so = 0, w1.inc = 128, w1.nkt = units(t), w1.klen = t.klen;
+    begin_a(t, 1, index, va1, ra1, pa1, na1);
+    edge1();
+    if (TA) ra1 = make_rsrc(pa1, na1);
+  };
+  auto begin2 = [&](const GroupTile& t, const int32_t* index) {
+    w2.t = 0, w2.so = 0, w2.inc = 128, w2.nkt = units(t), w2.klen = t.klen;
+    begin_a(t, 0, index, va2, ra2, pa2, na2);
+    begin_b(t);
+    edge2();
+    if (TA) ra2 = make_rsrc(pa2, na2);
+    if (TB) rb = make_rsrc(pb, nb);
   };
 
   // ---- a tile's vectors and row numbers
@@ -380,85 +424,60 @@ __global__ void __launch_bounds__(512, 1) group_quad_kernel(const GroupArgs p) {
     __builtin_amdgcn_s_barrier();
     __builtin_amdgcn_sched_barrier(0);
   };
-  GroupTile cur = tile_at(0), nxt = cur;
-  Ahead s1{}, s2{};
-  s1.va[0] = s2.va[0] = la[0];
-  s1.va[1] = s2.va[1] = la[1];
-  if (gathered) {
-#pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      const int r0 = row_a(k), r1 = r0 + 128;
-      s2.va[k] = r0 < cur.rows ? offset_of(p.index[cur.row0 + r0], k) : kGroupOut;
-      s1.va[k] = r1 < cur.rows ? offset_of(p.index[cur.row0 + r1], k) : kGroupOut;
-    }
-  }
-  // the row numbers of tile lt are in LDS from the tile before on; the first's are read here, for its scales
-  begin_a(s1, cur, 1);
-  begin_a(s2, cur, 0);
-  begin_b(s2, cur);
-  s1.nkt = s2.nkt = units(cur);
-  int l1 = 0, l2 = 0;
-  if constexpr (NT) fill_vectors(cur, 0, p.index ? p.index + cur.row0 : nullptr);
-  auto step_on = [&](Ahead& s) {
-    ++s.t;
-    s.par ^= 1;
-    if constexpr (TA) s.a += 64 * p.lda;
-    if constexpr (TB) s.b += 64 * p.ldb;
-    if constexpr (TB) s.left -= 64;
+  // A step: the next unit, at an edge what changes there. Past a tile's last unit the next one begins (found at the current
+  // tile's first unit); past the last tile's there is nothing.
+  auto uniform = [](uint32_t v) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)v); };  // (kept in scalar registers)
+  auto over = [](Walk& w) {
+    w.klen = w.t = 0;
+    w.nkt = 0x7fffffff;
   };
-  // Past a stream's last unit its next tile begins (found at the current tile's first unit), or nothing is left.
   auto next1 = [&]() {
-    step_on(s1);
-    if (s1.t < s1.nkt) return;
-    s1.t = 0;
-    if (++l1 >= my_tiles) {  // nothing is left: zeros
-      s1.ba = 0;
-      s1.left = 0;
-      return;
-    }
-    const GroupTile& t1 = nxt;
-    s1.nkt = units(t1);
-    if (gathered) {
-#pragma unroll
-      for (int k = 0; k < 2; ++k)
-      {
-        const int r = row_a(k) + 128;
-        s1.va[k] = r < t1.rows ? offset_of(idx_lds[(l1 & 1) * 256 + r], k) : kGroupOut;
+    w1.t = (int)uniform((uint32_t)w1.t + 1);
+    w1.slot ^= 4 * QB;
+    if constexpr (TA) pa1 += 64 * p.lda;
+    else w1.so = uniform(w1.so + w1.inc);
+    if (w1.t == w1.edge) {
+      if (w1.t == w1.nkt && ++w1.lt < my_tiles) {
+        begin1(nxt, idx_lds + (w1.lt & 1) * 256);
+      } else {
+        if (w1.t == w1.nkt) over(w1);
+        edge1();
       }
     }
-    begin_a(s1, t1, 1);
+    if constexpr (TA) ra1 = make_rsrc(pa1, na1);
   };
   auto next2 = [&]() {
-    step_on(s2);
-    if (s2.t < s2.nkt) return;
-    s2.t = 0;
-    if (++l2 >= my_tiles) {
-      s2.ba = s2.bb = s2.b1 = 0;
-      s2.left = 0;
-      return;
-    }
-    const GroupTile& t2 = nxt;
-    s2.nkt = units(t2);
-    if (gathered) {
-#pragma unroll
-      for (int k = 0; k < 2; ++k)
-      {
-        const int r = row_a(k);
-        s2.va[k] = r < t2.rows ? offset_of(idx_lds[(l2 & 1) * 256 + r], k) : kGroupOut;
+    w2.t = (int)uniform((uint32_t)w2.t + 1);
+    w2.slot ^= 4 * QB;
+    if constexpr (TA) pa2 += 64 * p.lda;
+    else w2.so = uniform(w2.so + w2.inc);
+    if constexpr (TB) pb += 64 * p.ldb;
+    if (w2.t == w2.edge) {
+      if (w2.t == w2.nkt && ++w2.lt < my_tiles) {
+        begin2(nxt, idx_lds + (w2.lt & 1) * 256);
+        if constexpr (NT) fill_vectors(nxt, w2.lt, idx_lds + (w2.lt & 1) * 256);
+      } else {
+        if (w2.t == w2.nkt) over(w2);
+        edge2();
       }
     }
-    begin_a(s2, t2, 0);
-    begin_b(s2, t2);
-    if constexpr (NT) fill_vectors(t2, l2, idx_lds + (l2 & 1) * 256);
+    if constexpr (TA) ra2 = make_rsrc(pa2, na2);
+    if constexpr (TB) rb = make_rsrc(pb, nb);
   };
+  {
+    const int32_t* const index = gathered ? p.index + cur.row0 : nullptr;
+    begin1(cur, index);
+    begin2(cur, index);
+    if constexpr (NT) fill_vectors(cur, 0, index);
+  }
   // unit 0 whole and unit 1 but A1, in the steady state's order (a tile has 5 units or more)
 #pragma unroll
   for (int r = 0; r < 2; ++r) {
-    fill_b(s2, 1);
-    fill_b(s2, 0);
-    fill_a(s2, 0);
+    fill_b(1);
+    fill_b(0);
+    fill_a0();
     if (r == 0) {
-      fill_a(s1, 1);
+      fill_a1();
       next1();
     }
     next2();
@@ -479,17 +498,17 @@ __global__ void __launch_bounds__(512, 1) group_quad_kernel(const GroupArgs p) {
       nxt = tile_at(lt + 1);
       if constexpr (NT) fill_index(nxt, lt + 1);
     }
-    fill_a(s1, 1);
+    fill_a1();
     next1();
-    fill_b(s2, 1);
+    fill_b(1);
     if constexpr (TB) read_ab(slot, 0, slot, 0, bf0);
     sync(true);
     math(0, 0, bf0);
     math(0, 1, b1);
     sync(false);
     if constexpr (!TB) read_ab(slot, 1, slot ^ 1, 1, nb1);
-    fill_b(s2, 0);
-    fill_a(s2, 0);
+    fill_b(0);
+    fill_a0();
     next2();
     if constexpr (TB) read_ab(slot, 1, slot ^ 1, 1, nb1);
     sync(true);

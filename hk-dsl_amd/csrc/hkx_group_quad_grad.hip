@@ -1,6 +1,4 @@
 // The experts' gradient products on 256 x 256 tiles (hkx_group_quad.hpp).
-#include <algorithm>
-
 #include "hkx_group_launch.hpp"
 #include "hkx_group_quad.hpp"
 
@@ -9,8 +7,9 @@ namespace hkx {
 hipError_t launch_group_quad_grad(const GroupArgs& a, int op, int cus, hipStream_t s) {
   const int64_t tn = (a.n + 255) / 256;
   const int64_t tiles = op == kGroupTN ? (int64_t)a.experts * ((a.m + 255) / 256) * tn : group_tiles(a.rows, a.experts, 256) * tn;
-  if (tiles > INT32_MAX - 65536) return hipErrorInvalidConfiguration;
-  const dim3 grid((unsigned)std::min<int64_t>((tiles + 7) / 8 * 8, cus / 8 * 8)), block(512);
+  dim3 grid;
+  if (!group_quad_grid(tiles, cus, grid)) return hipErrorInvalidConfiguration;
+  const dim3 block(512);
   if (op == kGroupTN) hipLaunchKernelGGL((group_quad_kernel<kGroupTN, false, false>), grid, block, 0, s, a);
   else hipLaunchKernelGGL((group_quad_kernel<kGroupNN, false, false>), grid, block, 0, s, a);
   return hipGetLastError();

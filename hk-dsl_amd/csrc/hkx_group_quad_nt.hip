@@ -1,6 +1,4 @@
 // The experts' forward products on 256 x 256 tiles (hkx_group_quad.hpp).
-#include <algorithm>
-
 #include "hkx_group_launch.hpp"
 #include "hkx_group_quad.hpp"
 
@@ -9,8 +7,9 @@ namespace hkx {
 hipError_t launch_group_quad_nt(const GroupArgs& a, bool fp8, bool pair, int cus, hipStream_t s) {
   const int cn = pair ? 128 : 256;
   const int64_t tiles = group_tiles(a.rows, a.experts, 256) * ((a.n + cn - 1) / cn);
-  if (tiles > INT32_MAX - 65536) return hipErrorInvalidConfiguration;
-  const dim3 grid((unsigned)std::min<int64_t>((tiles + 7) / 8 * 8, cus / 8 * 8)), block(512);
+  dim3 grid;
+  if (!group_quad_grid(tiles, cus, grid)) return hipErrorInvalidConfiguration;
+  const dim3 block(512);
   if (fp8 && pair) hipLaunchKernelGGL((group_quad_kernel<kGroupNT, true, true>), grid, block, 0, s, a);
   else if (fp8) hipLaunchKernelGGL((group_quad_kernel<kGroupNT, true, false>), grid, block, 0, s, a);
   else if (pair) hipLaunchKernelGGL((group_quad_kernel<kGroupNT, false, true>), grid, block, 0, s, a);
