@@ -11,12 +11,20 @@ hipError_t launch_group_grad(const GroupArgs& a, int op, int bm, hipStream_t s) 
 }
 
 hipError_t launch_group(const GroupArgs& a, int op, bool fp8, bool pair, int kernel, int cus, hipStream_t s) {
-  // rows an expert, were they even (the host does not know the counts)
-  const int64_t each = a.rows / a.experts;
-  if (kernel == HKX_EXPERTS_QUAD || (kernel == HKX_EXPERTS_AUTO && each >= 128 && group_quad_ok(a)))
+  // The host does not know the counts: it goes by the tiles that even groups would make. 256-row tiles where they fill
+  // most of the CUs and a group more than a quarter of one (64 groups of 64 rows, 2048 x 2048: 139 us against 119 on
+  // 64-row tiles; 16 of 100 rows, N = 4096: 58 against 68, their 128 tiles of 2048 columns with K = 4096: 97 against
+  // 50), 128-row tiles where those fill the CUs, 64-row and, where a group has few rows, 16-row ones.
+  const int64_t each = (a.rows + a.experts - 1) / a.experts;
+  auto tiles = [&](int64_t bm, int64_t cn) {
+    return op == kGroupTN ? a.experts * ((a.m + bm - 1) / bm) * ((a.n + cn - 1) / cn)
+                          : std::min<int64_t>(a.experts, a.rows) * ((each + bm - 1) / bm) * ((a.n + cn - 1) / cn);
+  };
+  const bool quad = tiles(256, pair ? 128 : 256) * 5 >= (int64_t)cus * 4 && (each > 64 || op == kGroupTN);
+  if (kernel == HKX_EXPERTS_QUAD || (kernel == HKX_EXPERTS_AUTO && quad && group_quad_ok(a)))
     return op == kGroupNT ? launch_group_quad_nt(a, fp8, pair, cus, s) : launch_group_quad_grad(a, op, cus, s);
   const int bm = kernel == HKX_EXPERTS_TILE16 ? 16 : kernel == HKX_EXPERTS_TILE64 ? 64 : kernel == HKX_EXPERTS_TILE128 ? 128
-                 : each <= 16 ? 16 : each <= 64 ? 64 : 128;
+                 : each <= 16 ? 16 : each > 64 && tiles(128, pair ? 64 : 128) >= cus ? 128 : 64;
   return op == kGroupNT ? launch_group_nt(a, fp8, pair, bm, s) : launch_group_grad(a, op, bm, s);
 }
 
