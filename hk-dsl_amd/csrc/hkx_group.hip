@@ -137,7 +137,7 @@ int hkx_experts_gemm(const HkxExpertsGemmArgs* args, void* stream) {
   const int64_t lim = ((int64_t)1 << 32) - 4096;
   if (256 * g.lda * es > lim || 256 * g.ldc * 2 > lim || 256 * g.ldz * 2 > lim || (nt ? brows : 256) * g.ldb * es > lim || (g.index && g.a_rows * g.lda * es > lim))
     return api_fail(HKX_ERR_SHAPE, "experts_gemm: an expert's B or an indexed A spans 4 GiB or more; split the call");
-  if (g.kernel < 0 || g.kernel > HKX_EXPERTS_QUAD) return api_fail(HKX_ERR_ARG, "experts_gemm: kernel %d", g.kernel);
+  if (g.kernel < 0 || g.kernel > HKX_EXPERTS_SKINNY32) return api_fail(HKX_ERR_ARG, "experts_gemm: kernel %d", g.kernel);
   if (g.rows == 0 && !tn) return HKX_OK;
   GroupArgs a{};
   a.a = (const uint8_t*)g.a;

@@ -148,6 +148,39 @@ HKX_DEV __amdgpu_buffer_rsrc_t group_rsrc(const uint8_t* p, int rows, int64_t ld
   return make_rsrc(p, rows > 0 ? (uint32_t)((rows - 1) * ld) + row : 0u);
 }
 
+// ---------------------------------------------------------------- C
+//
+// What row r of R (a tile's, not `rest`) is scaled by, and four columns n of C from the sums v (paired: gate v, up u).
+
+HKX_DEV float group_row_scale(const GroupArgs& p, int64_t r) {
+  int64_t at = p.index ? p.index[r] : r;
+  const bool in = !p.index || (uint32_t)at < (uint32_t)p.a_rows;
+  return in ? p.sa[at * p.sa_ld] : 0.0f;
+}
+
+template <bool NT, bool FP8, bool PAIR>
+HKX_DEV void group_store(const GroupArgs& p, int e, bool rest, uint8_t* c, uint8_t* z, int n, f32x4 v, f32x4 u, float sa) {
+  auto finish = [&](f32x4 v, int n) {  // n: B_e's row
+    if (FP8 && !rest) {
+      const float* sb = p.sb + e * p.sb_ld;
+      if (p.sb_col) v *= *(const f32x4*)(sb + n) * sa;
+      else v *= sb[0] * sa;
+    }
+    if (NT && p.bias && !rest) v += ld4(p.bias, p.bias_dt, e * p.bias_ld + n);
+    return v;
+  };
+  v = finish(v, n);
+  if constexpr (PAIR) {
+    u = finish(u, n + p.n);
+    if (p.z) {
+      store4(z, HKX_BF16, n, v);
+      store4(z, HKX_BF16, n + p.n, u);
+    }
+    v = silu_mul4(v, u);
+  }
+  store4(c, HKX_BF16, n, v);
+}
+
 // ---------------------------------------------------------------- fragments in LDS
 //
 // A K unit is 128 bytes: 64 bf16 or 128 fp8.
@@ -423,36 +456,13 @@ __global__ void __launch_bounds__(64 * WM * WN) group_tile_kernel(const GroupArg
   for (int f = 0; f < FM; ++f) {
     const int r = wr * (BM / WM) + 16 * f + rf;
     if (r >= mrows) continue;
-    uint8_t* const row = c0 + (c_row + r) * p.ldc;
-    float sa = 1.0f;
-    if (FP8 && !rest) {
-      int64_t at = p.index ? p.index[row0 + r] : row0 + r;
-      const bool in = !p.index || (uint32_t)at < (uint32_t)p.a_rows;
-      sa = in ? p.sa[at * p.sa_ld] : 0.0f;
-    }
-    auto finish = [&](f32x4 v, int n) {  // n: B_e's row
-      if (FP8 && !rest) {
-        const float* sb = p.sb + e * p.sb_ld;
-        if (p.sb_col) v *= *(const f32x4*)(sb + n) * sa;
-        else v *= sb[0] * sa;
-      }
-      if (OP == kGroupNT && p.bias && !rest) v += ld4(p.bias, p.bias_dt, e * p.bias_ld + n);
-      return v;
-    };
+    const float sa = FP8 && !rest ? group_row_scale(p, row0 + r) : 1.0f;
 #pragma unroll
     for (int g = 0; g < FN; g += PAIR ? 2 : 1) {
       const int n = n0 + (PAIR ? (wc * FN + g) / 2 * 16 : (wc * FN + g) * 16) + 4 * q;
-      if (n >= p.n) continue;
-      f32x4 v = finish(acc[f][g], n);
-      if constexpr (PAIR) {
-        const f32x4 u = finish(acc[f][g + 1], n + p.n);
-        if (p.z) {
-          store4(p.z + (c_row + r) * p.ldz, HKX_BF16, n, v);
-          store4(p.z + (c_row + r) * p.ldz, HKX_BF16, n + p.n, u);
-        }
-        v = silu_mul4(v, u);
-      }
-      store4(row, HKX_BF16, n, v);
+      if (n < p.n)
+        group_store<OP == kGroupNT, FP8, PAIR>(p, e, rest, c0 + (c_row + r) * p.ldc, PAIR ? p.z + (c_row + r) * p.ldz : nullptr, n,
+                                               acc[f][g], PAIR ? acc[f][g + 1] : f32x4{}, sa);
     }
   }
 }

@@ -23,6 +23,8 @@ hipError_t launch_group(const GroupArgs& a, int op, bool fp8, bool pair, int ker
   const bool quad = tiles(256, pair ? 128 : 256) * 5 >= (int64_t)cus * 4 && (each > 64 || op == kGroupTN);
   if (kernel == HKX_EXPERTS_QUAD || (kernel == HKX_EXPERTS_AUTO && quad && group_quad_ok(a)))
     return op == kGroupNT ? launch_group_quad_nt(a, fp8, pair, cus, s) : launch_group_quad_grad(a, op, cus, s);
+  if (op == kGroupNT && (kernel == HKX_EXPERTS_SKINNY16 || kernel == HKX_EXPERTS_SKINNY32 || (kernel == HKX_EXPERTS_AUTO && each <= 16)))
+    return launch_group_skinny(a, fp8, pair, kernel == HKX_EXPERTS_SKINNY16 || (kernel == HKX_EXPERTS_AUTO && each <= 4) ? 16 : 32, s);
   const int bm = kernel == HKX_EXPERTS_TILE16 ? 16 : kernel == HKX_EXPERTS_TILE64 ? 64 : kernel == HKX_EXPERTS_TILE128 ? 128
                  : each <= 16 ? 16 : each > 64 && tiles(128, pair ? 64 : 128) >= cus ? 128 : 64;
   return op == kGroupNT ? launch_group_nt(a, fp8, pair, bm, s) : launch_group_grad(a, op, bm, s);

@@ -47,6 +47,7 @@ typedef float f32x16 __attribute__((ext_vector_type(16)));
 
 // s_waitcnt operands (gfx9 encoding: vmcnt in bits 3:0 and 15:14, expcnt 6:4, lgkmcnt 11:8)
 constexpr int wait_vm(int n) { return (n & 15) | ((n >> 4) << 14) | (7 << 4) | (15 << 8); }
+constexpr int wait_lgkm0() { return 15 | (3 << 14) | (7 << 4); }
 constexpr int wait_vm_lgkm0(int n) { return (n & 15) | ((n >> 4) << 14) | (7 << 4); }
 
 // v_permlane32_swap: lanes 32-63 of a trade places with lanes 0-31 of b.

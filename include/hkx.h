@@ -464,6 +464,8 @@ typedef struct {
 #define HKX_EXPERTS_TILE16 1  /* tiles of 16, 64 or 128 rows */
 #define HKX_EXPERTS_TILE64 2
 #define HKX_EXPERTS_TILE128 3
+#define HKX_EXPERTS_SKINNY16 5 /* NT (else by size): the decode kernel, 16 or 32 rows */
+#define HKX_EXPERTS_SKINNY32 6
 #define HKX_EXPERTS_QUAD 4 /* 256 x 256 tiles, 8 waves, persistent; C, z and the bias in 16-byte aligned rows */
 /* bf16 C from bf16 or fp8 operands, sums in fp32, rounded once. n and k multiples of 8 (m too; an fp8 k of 16), rows
  * and experts of A and B 16-byte aligned, of C, z and the bias 8-byte, scales (a row of B each) 16-byte. */

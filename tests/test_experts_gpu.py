@@ -25,7 +25,7 @@ BF16, F16, F32, E4M3 = torch.bfloat16, torch.float16, torch.float32, torch.float
 HALF = {BF16: 2.0 ** -8, F16: 2.0 ** -11, F32: 2.0 ** -24}
 
 
-@pytest.fixture(params=[0, 1, 2, 3, 4], ids=["auto", "tile16", "tile64", "tile128", "quad"])
+@pytest.fixture(params=range(7), ids=["auto", "tile16", "tile64", "tile128", "quad", "skinny16", "skinny32"])
 def kernel(request, monkeypatch):
     """Each product on the kernel named."""
     real = experts._run
