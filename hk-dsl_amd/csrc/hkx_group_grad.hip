@@ -23,10 +23,15 @@ hipError_t launch_group(const GroupArgs& a, int op, bool fp8, bool pair, int ker
   const bool quad = tiles(256, pair ? 128 : 256) * 5 >= (int64_t)cus * 4 && (each > 64 || op == kGroupTN);
   if (kernel == HKX_EXPERTS_QUAD || (kernel == HKX_EXPERTS_AUTO && quad && group_quad_ok(a)))
     return op == kGroupNT ? launch_group_quad_nt(a, fp8, pair, cus, s) : launch_group_quad_grad(a, op, cus, s);
-  if (op == kGroupNT && (kernel == HKX_EXPERTS_SKINNY16 || kernel == HKX_EXPERTS_SKINNY32 || (kernel == HKX_EXPERTS_AUTO && each <= 16)))
-    return launch_group_skinny(a, fp8, pair, kernel == HKX_EXPERTS_SKINNY16 || (kernel == HKX_EXPERTS_AUTO && each <= 4) ? 16 : 32, s);
+  // The decode kernel for up to 8 rows an expert and 2048 bytes along K (64 experts, 8 rows each: 98 us against 103 on
+  // 16-row tiles; 16 each 117 against 103; 8 each over 1024 bytes 39 against 30 on 64-row tiles, which read a favoured
+  // expert's W once and, with as little to do, have fewer workgroups to start).
+  const int64_t row = (int64_t)a.k * (fp8 ? 1 : 2);
+  const bool few = kernel == HKX_EXPERTS_AUTO && each <= 8 && row >= 2048;
+  if (op == kGroupNT && (kernel == HKX_EXPERTS_SKINNY16 || kernel == HKX_EXPERTS_SKINNY32 || few))
+    return launch_group_skinny(a, fp8, pair, kernel == HKX_EXPERTS_SKINNY16 || (few && each <= 4) ? 16 : 32, cus, s);
   const int bm = kernel == HKX_EXPERTS_TILE16 ? 16 : kernel == HKX_EXPERTS_TILE64 ? 64 : kernel == HKX_EXPERTS_TILE128 ? 128
-                 : each <= 16 ? 16 : each > 64 && tiles(128, pair ? 64 : 128) >= cus ? 128 : 64;
+                 : each <= 4 || (each <= 16 && row >= 2048) ? 16 : each > 64 && tiles(128, pair ? 64 : 128) >= cus ? 128 : 64;
   return op == kGroupNT ? launch_group_nt(a, fp8, pair, bm, s) : launch_group_grad(a, op, bm, s);
 }
 
