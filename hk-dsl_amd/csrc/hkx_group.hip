@@ -90,24 +90,8 @@ __global__ void __launch_bounds__(256) gather_kernel(const uint8_t* x, int64_t l
 
 bool floating(int dt) { return dt == HKX_BF16 || dt == HKX_FP16 || dt == HKX_FP32; }
 
-// Blocks of 256 threads, a thread one of `per` pieces of a row; 0 where a launch does not take them.
-unsigned pieces(int64_t rows, int64_t per) {
-  const int64_t n = (rows * per + 255) / 256;
-  return n < ((int64_t)1 << 24) ? (unsigned)n : 0;
-}
-
-}  // namespace
-}  // namespace hkx
-
-extern "C" {
-
-int hkx_experts_gemm(const HkxExpertsGemmArgs* args, void* stream) {
-  using namespace hkx;
-  api_clear();
-  if (!args) return api_fail(HKX_ERR_ARG, "experts_gemm: null args");
-  if (args->size != sizeof *args)
-    return api_fail(HKX_ERR_ARG, "experts_gemm: args of %d bytes, the library's have %zu", args->size, sizeof *args);
-  const HkxExpertsGemmArgs& g = *args;
+// What a call asks for, refused where the kernels do not take it; the kernels' arguments.
+int gemm_args(const HkxExpertsGemmArgs& g, GroupArgs& a) {
   const bool nt = g.op == HKX_EXPERTS_NT, tn = g.op == HKX_EXPERTS_TN, fp8 = g.ab_dtype == HKX_FP8E4M3;
   if (!nt && !tn && g.op != HKX_EXPERTS_NN) return api_fail(HKX_ERR_ARG, "experts_gemm: op %d", g.op);
   if (!fp8 && g.ab_dtype != HKX_BF16) return api_fail(HKX_ERR_DTYPE, "experts_gemm: operands are bf16 or e4m3");
@@ -138,8 +122,6 @@ int hkx_experts_gemm(const HkxExpertsGemmArgs* args, void* stream) {
   if (256 * g.lda * es > lim || 256 * g.ldc * 2 > lim || 256 * g.ldz * 2 > lim || (nt ? brows : 256) * g.ldb * es > lim || (g.index && g.a_rows * g.lda * es > lim))
     return api_fail(HKX_ERR_SHAPE, "experts_gemm: an expert's B or an indexed A spans 4 GiB or more; split the call");
   if (g.kernel < 0 || g.kernel > HKX_EXPERTS_SKINNY32) return api_fail(HKX_ERR_ARG, "experts_gemm: kernel %d", g.kernel);
-  if (g.rows == 0 && !tn) return HKX_OK;
-  GroupArgs a{};
   a.a = (const uint8_t*)g.a;
   a.b = (const uint8_t*)g.b;
   a.c = (uint8_t*)g.c;
@@ -169,10 +151,46 @@ int hkx_experts_gemm(const HkxExpertsGemmArgs* args, void* stream) {
   a.sb_col = g.sb_col != 0;
   if (g.kernel == HKX_EXPERTS_QUAD && !group_quad_ok(a))
     return api_fail(HKX_ERR_SHAPE, "experts_gemm: the 256-row kernel stores 16-byte aligned rows");
-  const hipError_t e = launch_group(a, g.op, fp8, g.silu_mul != 0, g.kernel, api_cus(), (hipStream_t)stream);
+  return HKX_OK;
+}
+
+// Blocks of 256 threads, a thread one of `per` pieces of a row; 0 where a launch does not take them.
+unsigned pieces(int64_t rows, int64_t per) {
+  const int64_t n = (rows * per + 255) / 256;
+  return n < ((int64_t)1 << 24) ? (unsigned)n : 0;
+}
+
+}  // namespace
+}  // namespace hkx
+
+extern "C" {
+
+int hkx_experts_gemm(const HkxExpertsGemmArgs* args, void* stream) {
+  using namespace hkx;
+  api_clear();
+  if (!args) return api_fail(HKX_ERR_ARG, "experts_gemm: null args");
+  if (args->size != sizeof *args)
+    return api_fail(HKX_ERR_ARG, "experts_gemm: args of %d bytes, the library's have %zu", args->size, sizeof *args);
+  const HkxExpertsGemmArgs& g = *args;
+  GroupArgs a{};
+  if (int rc = gemm_args(g, a)) return rc;
+  if (g.rows == 0 && g.op != HKX_EXPERTS_TN) return HKX_OK;
+  const bool fp8 = g.ab_dtype == HKX_FP8E4M3, pair = g.silu_mul != 0;
+  const size_t need = group_ws_bytes(a, g.op, fp8, pair, g.kernel, api_cus());
+  if (need && (!g.ws || g.ws_bytes < need || !api_aligned(g.ws, 16)))
+    return api_fail(HKX_ERR_WORKSPACE, "experts_gemm: needs %zu bytes of 16-byte aligned workspace, got %zu", need, g.ws ? g.ws_bytes : (size_t)0);
+  a.ws = need ? (float*)g.ws : nullptr;
+  const hipError_t e = launch_group(a, g.op, fp8, pair, g.kernel, api_cus(), (hipStream_t)stream);
   if (e == hipErrorInvalidConfiguration)
     return api_fail(HKX_ERR_SHAPE, "experts_gemm: rows=%d of n=%d are more tiles than a launch takes; split the call", g.rows, g.n);
   return api_launched(e, "experts gemm");
+}
+
+size_t hkx_experts_gemm_workspace(const HkxExpertsGemmArgs* args) {
+  using namespace hkx;
+  GroupArgs a{};
+  if (!args || args->size != sizeof *args || gemm_args(*args, a) || args->rows == 0) return 0;
+  return group_ws_bytes(a, args->op, args->ab_dtype == HKX_FP8E4M3, args->silu_mul != 0, args->kernel, api_cus());
 }
 
 int hkx_experts_silu_grad(const void* z, int64_t ldz, const void* dy, int64_t lddy, void* dz, int64_t lddz,

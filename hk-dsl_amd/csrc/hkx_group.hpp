@@ -34,6 +34,7 @@ struct GroupArgs {
   const void* bias;        // (E, N), N in the paired form 2 N
   const float* sa;         // fp8: a scale a row of A (sa_ld 1) or one (0)
   const float* sb;         // fp8: sb[e sb_ld + n sb_col]
+  float* ws;               // the 256-row kernel's parts of tiles (nullptr: none)
   int64_t lda, ldb, ldc, ldz;  // bytes a row
   int64_t b_group, c_group;    // bytes an expert (NT and NN: B; TN: C)
   int64_t bias_ld, sb_ld;      // elements an expert

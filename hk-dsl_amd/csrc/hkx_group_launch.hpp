@@ -25,6 +25,14 @@ inline bool group_quad_ok(const GroupArgs& a) {
   return whole(a.c, a.ldc) && a.c_group % 16 == 0 && whole(a.z, a.ldz) && (!a.bias || a.bias_ld * (a.bias_dt == HKX_FP32 ? 4 : 2) % 16 == 0);
 }
 
+// Whether a call runs on 256 x 256 tiles (kernel: HKX_EXPERTS_AUTO, or the one asked for), and then may split its last
+// round along K: the bytes of workspace that takes (0: none; 24 units of K are some 36 us a round).
+bool group_quad_takes(const GroupArgs& a, int op, bool pair, int kernel, int cus);
+inline size_t group_ws_bytes(const GroupArgs& a, int op, bool fp8, bool pair, int kernel, int cus) {
+  if (op == kGroupTN || (int64_t)a.k * (fp8 ? 1 : 2) < 24 * 128 || !group_quad_takes(a, op, pair, kernel, cus)) return 0;
+  return (size_t)std::max(cus / 256 * 256, 256) * 256 * 256 * 4;
+}
+
 // A grid of `tiles` workgroups and the places that their order over the XCDs leaves open (group_place).
 inline bool group_grid(int64_t tiles, int threads, dim3& grid) {
   const int64_t n = (tiles + 255) / 256 * 256;

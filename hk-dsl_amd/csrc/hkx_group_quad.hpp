@@ -19,6 +19,24 @@
 namespace hkx {
 
 constexpr int kQuadUnits = 5;  // K units a tile at least
+constexpr int kQuadMostParts = 8, kQuadPartUnits = 8;
+constexpr size_t kQuadPartBytes = 256 * 256 * 4;
+
+// The last round of `total` tiles on `grid` workgroups, where it fills at most half of them: its `rem` tiles in `parts`
+// along K each (1: whole), a workgroup one part, the fp32 sums through memory. A round of nku units takes some 1.5 nku us, a
+// part's sums written and read 0.13 us of the whole: parts while their square times rem is below 12 nku. (Gradient of
+// 8192 rows, 36 tile rows of 8 tiles, K = 8192: 335 us, with the 32 tiles over SPLIT_US.)
+struct QuadRound {
+  int full, rem, parts;
+};
+HKX_DEV QuadRound quad_round(int total, int grid, int nku, bool ws) {
+  QuadRound r{total / grid * grid, total % grid, 1};
+  if (!ws || r.rem == 0) return r;
+  while (r.parts < kQuadMostParts && (r.parts + 1) * r.rem <= grid && (r.parts + 1) * (r.parts + 1) * r.rem <= 12 * nku &&
+         (r.parts + 1) * kQuadPartUnits <= nku)
+    ++r.parts;
+  return r;
+}
 
 // The kernel's arguments, read anew: what only a tile's beginning and end take of them is not held through the K loop
 // (held, they filled the scalar registers, and what was moved to vector lanes cost a lane's read a use).
@@ -60,22 +78,35 @@ __global__ void __launch_bounds__(512, 1) group_quad_kernel(const GroupArgs p) {
   };
   const int total = __builtin_amdgcn_readfirstlane(TA ? p.experts * ((p.m + BM - 1) / BM) * tiles_n
                                                       : map.first[p.experts + 1] * tiles_n);
-  // the workgroup's tiles: the places of its number, and of it and the grid (a multiple of 256, or one round) on and on
+  // the workgroup's tiles: one at its place in every round of the grid
   const int place = group_place((int)blockIdx.x), step = (int)gridDim.x;
-  const int my_tiles = place < total ? (total - place + step - 1) / step : 0;
+  const int nku = TA ? 0 : (p.k + KU - 1) / KU;
+  const QuadRound round = quad_round(total, step, nku, !TA && p.ws != nullptr);
+  const int whole = round.full / step;  // rounds before the last
+  const int my_tiles = whole + (place < round.rem * round.parts ? 1 : 0);
   if (my_tiles == 0) return;
+  struct Tile : GroupTile {
+    int u0, u1;  // its units (at least kQuadUnits: what is past K reads as zeros)
+    bool part;   // of a tile's units: the sums go to memory
+  };
   auto tile_at = [&](int lt) {
     const GroupArgs& p = args_anew();
-    GroupTile t = group_tile_at<OP, BM, BN>(map, p, place + lt * step, tiles_n, rows_of);
+    const bool last = lt == whole;
+    const int at = place + lt * step, part = last && round.parts > 1 ? place / round.rem : 0;
+    Tile t;
+    (GroupTile&)t = group_tile_at<OP, BM, BN>(map, p, last && round.parts > 1 ? round.full + place % round.rem : at, tiles_n, rows_of);
     t.e = __builtin_amdgcn_readfirstlane(t.e);
     t.m0 = __builtin_amdgcn_readfirstlane(t.m0);
     t.n0 = __builtin_amdgcn_readfirstlane(t.n0);
     t.rows = __builtin_amdgcn_readfirstlane(t.rows);
     t.klen = __builtin_amdgcn_readfirstlane(t.klen);
     t.row0 = (int64_t)__builtin_amdgcn_readfirstlane((int)t.row0);
+    t.part = last && round.parts > 1;
+    const int real = (t.klen + KU - 1) / KU, each = t.part ? (real + round.parts - 1) / round.parts : real;
+    t.u0 = __builtin_amdgcn_readfirstlane(part * each);
+    t.u1 = __builtin_amdgcn_readfirstlane(max(min(real, t.u0 + each), t.u0 + kQuadUnits));
     return t;
   };
-  auto units = [&](const GroupTile& t) { return max((t.klen + KU - 1) / KU, kQuadUnits); };
 
   // ---- fills. Instruction k (0, 1) of wave w: K-contiguous rows 16 w + 8 k + [0, 8) of a quarter, lane l row l % 32 / 4,
   // K-half l / 32, its 16-byte piece (l % 4) ^ swz4(row); rows along K 8 w + 4 k + [0, 4), lane l row l / 16.
@@ -111,7 +142,7 @@ __global__ void __launch_bounds__(512, 1) group_quad_kernel(const GroupArgs p) {
   const uint8_t *pa1 = nullptr, *pa2 = nullptr, *pb = nullptr;  // rows along K: the unit's first
   uint32_t na1 = 0, na2 = 0, nb = 0;                            // and the resource's bytes
   uint32_t b1 = 0;  // B's second half behind the first (0: past N, the first again: it is never stored)
-  GroupTile cur = tile_at(0), nxt = cur;
+  Tile cur = tile_at(0), nxt = cur;
 
   auto load2 = [&](__amdgpu_buffer_rsrc_t r, uint32_t slot, const uint32_t (&v)[2], uint32_t so) {
     uint8_t* s = smem + slot + wave * 2048;
@@ -123,13 +154,13 @@ __global__ void __launch_bounds__(512, 1) group_quad_kernel(const GroupArgs p) {
   auto fill_b = [&](int j) { load2(rb, w2.slot + (2 + j) * QB, vb, (TB ? 0u : w2.so) + (j ? b1 : 0u)); };
 
   // A's half i of tile t: offsets, and the resource of a K-contiguous A or the first rows and bytes of one along K
-  auto begin_a = [&](const GroupTile& t, int i, const int32_t* index, uint32_t (&v)[2], __amdgpu_buffer_rsrc_t& r,
+  auto begin_a = [&](const Tile& t, int i, const int32_t* index, uint32_t (&v)[2], __amdgpu_buffer_rsrc_t& r,
                      const uint8_t*& base, uint32_t& bytes) {
     const GroupArgs& p = args_anew();
     const int l = lane_anew();
     if constexpr (TA) {
       const int m = t.m0 + (t.rows > 128 * i ? 128 * i : 0);  // (a half past M: the first again)
-      base = p.a + t.row0 * p.lda + (int64_t)m * 2;
+      base = p.a + (t.row0 + 64 * (int64_t)t.u0) * p.lda + (int64_t)m * 2;
       bytes = rows_bytes(64, p.lda, (uint32_t)(p.m - m) * 2u);
       v[0] = along_of(l, 0, p.lda), v[1] = along_of(l, 1, p.lda);
     } else {
@@ -149,13 +180,13 @@ __global__ void __launch_bounds__(512, 1) group_quad_kernel(const GroupArgs p) {
       if (!gathered && t.rows <= 128 * i) r = make_rsrc(p.a, k_row), v[0] = v[1] = kGroupOut;
     }
   };
-  auto begin_b = [&](const GroupTile& t) {
+  auto begin_b = [&](const Tile& t) {
     const GroupArgs& p = args_anew();
     const int l = lane_anew();
     constexpr int HB = PAIR ? 64 : 128;
     b1 = t.n0 + HB < p.n ? (TB ? HB * 2u : (uint32_t)HB * (uint32_t)p.ldb) : 0u;
     if constexpr (TB) {
-      pb = p.b + (TA ? t.row0 * p.ldb : t.e * p.b_group) + (int64_t)t.n0 * 2;
+      pb = p.b + (TA ? t.row0 * p.ldb : t.e * p.b_group) + 64 * (int64_t)t.u0 * p.ldb + (int64_t)t.n0 * 2;
       nb = rows_bytes(64, p.ldb, (uint32_t)(p.n - t.n0) * 2u);
       vb[0] = along_of(l, 0, p.ldb), vb[1] = along_of(l, 1, p.ldb);
     } else {
@@ -183,9 +214,9 @@ __global__ void __launch_bounds__(512, 1) group_quad_kernel(const GroupArgs p) {
         for (int k = 0; k < 2; ++k)
           if (piece_of(l, k) >= (uint32_t)(ragged * ES)) out(k);
       }
-      w.edge = real;
+      w.edge = min(real, w.nkt);
     } else {
-      w.edge = ragged ? real - 1 : real;
+      w.edge = min(ragged ? real - 1 : real, w.nkt);
     }
   };
   auto edge1 = [&]() {
@@ -201,14 +232,14 @@ __global__ void __launch_bounds__(512, 1) group_quad_kernel(const GroupArgs p) {
             },
             [&]() { na2 = nb = b1 = 0; ra2 = rb = make_rsrc(nullptr, 0); });
   };
-  auto begin1 = [&](const GroupTile& t, const int32_t* index) {
-    w1.t = 0, w1.so = 0, w1.inc = 128, w1.nkt = units(t), w1.klen = t.klen;
+  auto begin1 = [&](const Tile& t, const int32_t* index) {
+    w1.t = t.u0, w1.so = (uint32_t)t.u0 * 128u, w1.inc = 128, w1.nkt = t.u1, w1.klen = t.klen;
     begin_a(t, 1, index, va1, ra1, pa1, na1);
     edge1();
     if (TA) ra1 = make_rsrc(pa1, na1);
   };
-  auto begin2 = [&](const GroupTile& t, const int32_t* index) {
-    w2.t = 0, w2.so = 0, w2.inc = 128, w2.nkt = units(t), w2.klen = t.klen;
+  auto begin2 = [&](const Tile& t, const int32_t* index) {
+    w2.t = t.u0, w2.so = (uint32_t)t.u0 * 128u, w2.inc = 128, w2.nkt = t.u1, w2.klen = t.klen;
     begin_a(t, 0, index, va2, ra2, pa2, na2);
     begin_b(t);
     edge2();
@@ -218,7 +249,7 @@ __global__ void __launch_bounds__(512, 1) group_quad_kernel(const GroupArgs p) {
 
   // ---- a tile's vectors and row numbers
   uint8_t* const vecs = smem + VEC;
-  [[maybe_unused]] auto fill_index = [&](const GroupTile& t, int lt) {  // wave 7
+  [[maybe_unused]] auto fill_index = [&](const Tile& t, int lt) {  // wave 7
     if (!gathered || wave != 7) return;
     const GroupArgs& p = args_anew();
     const __amdgpu_buffer_rsrc_t r = make_rsrc(p.index + t.row0, (uint32_t)t.rows * 4u);
@@ -227,7 +258,7 @@ __global__ void __launch_bounds__(512, 1) group_quad_kernel(const GroupArgs p) {
       __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void*)(smem + IDX + (lt & 1) * 1024 + i * 256), 4,
                                                (uint32_t)(64 * i + lane) * 4u, 0, 0, 0);
   };
-  [[maybe_unused]] auto fill_vectors = [&](const GroupTile& t, int lt, const int32_t* index) {
+  [[maybe_unused]] auto fill_vectors = [&](const Tile& t, int lt, const int32_t* index) {
     uint8_t* s = vecs + (lt % 3) * 4096;
     if (t.klen == 0) return;
     const GroupArgs& p = args_anew();
@@ -329,13 +360,25 @@ __global__ void __launch_bounds__(512, 1) group_quad_kernel(const GroupArgs p) {
 
   // ---- the epilogue: lane (rf, q) holds row rf, columns 4 q + [0, 4) of each fragment; two fragments trade quarters so
   // that a lane stores 16 bytes
-  auto epilogue = [&](const GroupTile& t, int lt) __attribute__((always_inline)) {
+  auto epilogue = [&](const Tile& t, int lt) __attribute__((always_inline)) {
     // (values the compiler cannot see through: what the stores need of the lane is made here, once a tile, instead of
     // held in registers through the K loop, which spilled)
     const GroupArgs& p = args_anew();
     int lane = tid & 63;
     asm volatile("" : "+v"(lane));
     const int rf = lane & 15, q = lane >> 4;
+    if (!TA && t.part) {
+      f32x4* const w = (f32x4*)p.ws + (int64_t)place * (kQuadPartBytes / 16) + 64 * wave + lane;
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+          for (int f = 0; f < NA; ++f)
+#pragma unroll
+            for (int g = 0; g < NB; ++g) w[(((i * 2 + j) * 4 + f) * 2 + g) * 512] = acc[i][j][f][g];
+      return;
+    }
     const uint8_t* ev = vecs + (lt % 3) * 4096;
     const int64_t row0 = TA ? t.m0 : t.row0;
     const __amdgpu_buffer_rsrc_t rc = make_rsrc(p.c + (TA ? t.e * p.c_group : 0) + row0 * p.ldc, rows_bytes(t.rows, p.ldc, (uint32_t)p.n * 2u));
@@ -518,7 +561,7 @@ __global__ void __launch_bounds__(512, 1) group_quad_kernel(const GroupArgs p) {
   };
   int slot = 0;
   for (int lt = 0; lt < my_tiles; ++lt) {
-    const int nkt = units(cur);
+    const int nkt = cur.u1 - cur.u0;
 #pragma unroll
     for (int i = 0; i < 2; ++i)
 #pragma unroll
@@ -548,6 +591,41 @@ __global__ void __launch_bounds__(512, 1) group_quad_kernel(const GroupArgs p) {
   }
   if (grp == 0) __builtin_amdgcn_s_barrier();
   __builtin_amdgcn_s_waitcnt(wait_vm(0));  // no fill lands in LDS after the exit
+}
+
+// The last round's parts, summed in order: a workgroup a quarter (i, j) of a tile, its threads where the product's were.
+template <int OP, bool FP8, bool PAIR>
+__global__ void __launch_bounds__(512) group_quad_join_kernel(const GroupArgs p, const int grid) {
+  constexpr int BM = 256, BN = PAIR ? 128 : 256, KU = FP8 ? 128 : 64;
+  __shared__ GroupMap map;
+  const int tiles_n = (p.n + BN - 1) / BN;
+  group_map<BM>(map, p, threadIdx.x, 512);
+  const QuadRound round = quad_round(map.first[p.experts + 1] * tiles_n, grid, (p.k + KU - 1) / KU, true);
+  const int tile = (int)blockIdx.x >> 2, i = ((int)blockIdx.x >> 1) & 1, j = (int)blockIdx.x & 1;
+  if (round.parts < 2 || tile >= round.rem) return;
+  const GroupTile t = group_tile_at<OP, BM, BN>(map, p, round.full + tile, tiles_n,
+                                                [&](int g, int& lo, int& hi) { group_rows(p, g, lo, hi); });
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, rf = lane & 15, q = lane >> 4;
+  const bool rest = t.klen == 0;
+  const f32x4* const w = (const f32x4*)p.ws + (int64_t)tile * (kQuadPartBytes / 16) + threadIdx.x;
+#pragma unroll
+  for (int f = 0; f < 4; ++f) {
+    const int r = 128 * i + 64 * (wave >> 2) + 16 * f + rf;
+    if (r >= t.rows) continue;
+    f32x4 v[2] = {};
+    for (int k = 0; k < round.parts; ++k) {
+      const f32x4* at = w + (int64_t)k * round.rem * (kQuadPartBytes / 16) + ((i * 2 + j) * 4 + f) * 2 * 512;
+      v[0] += at[0];
+      v[1] += at[512];
+    }
+    const float sa = FP8 && !rest ? group_row_scale(p, t.row0 + r) : 1.0f;
+    uint8_t *const c = p.c + (t.row0 + r) * p.ldc, *const z = PAIR ? p.z + (t.row0 + r) * p.ldz : nullptr;
+#pragma unroll
+    for (int g = 0; g < (PAIR ? 1 : 2); ++g) {
+      const int n = t.n0 + (PAIR ? 64 * j + 16 * (wave & 3) : 128 * j + 32 * (wave & 3) + 16 * g) + 4 * q;
+      if (n < p.n) group_store<OP == kGroupNT, FP8, PAIR>(p, t.e, rest, c, z, n, v[g], PAIR ? v[1] : f32x4{}, sa);
+    }
+  }
 }
 
 }  // namespace hkx

@@ -12,6 +12,8 @@ hipError_t launch_group_quad_grad(const GroupArgs& a, int op, int cus, hipStream
   const dim3 block(512);
   if (op == kGroupTN) hipLaunchKernelGGL((group_quad_kernel<kGroupTN, false, false>), grid, block, 0, s, a);
   else hipLaunchKernelGGL((group_quad_kernel<kGroupNN, false, false>), grid, block, 0, s, a);
+  if (op == kGroupNN && a.ws)
+    hipLaunchKernelGGL((group_quad_join_kernel<kGroupNN, false, false>), dim3(4 * (grid.x / 2)), block, 0, s, a, (int)grid.x);
   return hipGetLastError();
 }
 

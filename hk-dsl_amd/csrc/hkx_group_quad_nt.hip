@@ -10,10 +10,17 @@ hipError_t launch_group_quad_nt(const GroupArgs& a, bool fp8, bool pair, int cus
   dim3 grid;
   if (!group_quad_grid(tiles, cus, grid)) return hipErrorInvalidConfiguration;
   const dim3 block(512);
-  if (fp8 && pair) hipLaunchKernelGGL((group_quad_kernel<kGroupNT, true, true>), grid, block, 0, s, a);
-  else if (fp8) hipLaunchKernelGGL((group_quad_kernel<kGroupNT, true, false>), grid, block, 0, s, a);
-  else if (pair) hipLaunchKernelGGL((group_quad_kernel<kGroupNT, false, true>), grid, block, 0, s, a);
-  else hipLaunchKernelGGL((group_quad_kernel<kGroupNT, false, false>), grid, block, 0, s, a);
+#define HKX_QUAD(FP8, PAIR)                                                                                            \
+  do {                                                                                                                 \
+    hipLaunchKernelGGL((group_quad_kernel<kGroupNT, FP8, PAIR>), grid, block, 0, s, a);                                \
+    if (a.ws)                                                                                                          \
+      hipLaunchKernelGGL((group_quad_join_kernel<kGroupNT, FP8, PAIR>), dim3(4 * (grid.x / 2)), block, 0, s, a, (int)grid.x); \
+  } while (0)
+  if (fp8 && pair) HKX_QUAD(true, true);
+  else if (fp8) HKX_QUAD(true, false);
+  else if (pair) HKX_QUAD(false, true);
+  else HKX_QUAD(false, false);
+#undef HKX_QUAD
   return hipGetLastError();
 }
 

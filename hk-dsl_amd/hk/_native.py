@@ -115,7 +115,8 @@ class HkxExpertsGemmArgs(Structure):
                 ("c", c_void_p), ("z", c_void_p), ("offsets", c_void_p), ("index", c_void_p),
                 ("bias", c_void_p), ("sa", c_void_p), ("sb", c_void_p), ("lda", c_int64),
                 ("ldb", c_int64), ("ldc", c_int64), ("ldz", c_int64), ("b_expert", c_int64),
-                ("c_expert", c_int64), ("bias_ld", c_int64), ("sb_ld", c_int64)]
+                ("c_expert", c_int64), ("bias_ld", c_int64), ("sb_ld", c_int64),
+                ("ws", c_void_p), ("ws_bytes", c_size_t)]
 
 
 class HkxExpertsRouteArgs(Structure):
@@ -131,7 +132,8 @@ SYMBOLS = ("hkx_abi_version", "hkx_abi_sizes", "hkx_last_error", "hkx_gemm_works
            "hkx_gemm_check", "hkx_gemm", "hkx_scaled_mm", "hkx_mx_gemm", "hkx_mx_gemm_workspace",
            "hkx_mx_quant", "hkx_mx_quant_nan", "hkx_gemm_noalloc", "hkx_mx4_quant", "hkx_mx_dequant", "hkx_mx4_gemm",
            "hkx_mx4_gemm_workspace", "hkx_block_norm", "hkx_block_norm_backward",
-           "hkx_block_norm_backward_workspace", "hkx_experts_gemm", "hkx_experts_silu_grad",
+           "hkx_block_norm_backward_workspace", "hkx_experts_gemm", "hkx_experts_gemm_workspace",
+           "hkx_experts_silu_grad",
            "hkx_experts_bias_grad", "hkx_experts_gather", "hkx_experts_route",
            "hkx_experts_route_workspace", "hkx_experts_route_backward", "hkx_experts_combine",
            "hkx_experts_combine_backward", "hkx_fp8_quant")
@@ -199,6 +201,8 @@ def lib() -> ctypes.CDLL:
         L.hkx_block_norm_backward_workspace.argtypes = [POINTER(HkxBlockNormGradArgs)]
         L.hkx_block_norm_backward_workspace.restype = c_size_t
         L.hkx_experts_gemm.argtypes = [POINTER(HkxExpertsGemmArgs), c_void_p]
+        L.hkx_experts_gemm_workspace.argtypes = [POINTER(HkxExpertsGemmArgs)]
+        L.hkx_experts_gemm_workspace.restype = c_size_t
         L.hkx_experts_silu_grad.argtypes = [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64,
                                             c_void_p, c_int32, c_int32, c_int32, c_void_p]
         L.hkx_experts_bias_grad.argtypes = [c_void_p, c_int64, c_void_p, c_void_p, c_int32, c_int32,

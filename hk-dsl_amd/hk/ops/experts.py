@@ -92,7 +92,7 @@ def _grad(*tensors):
 # ---------------------------------------------------------------- the products
 
 
-#: Layouts of gemm's operands: (arguments filled in but for their addresses, C's shape).
+#: Layouts of gemm's operands: (arguments filled in but for their addresses, C's shape, the workspace's bytes).
 _GEMM: dict = {}
 
 
@@ -129,10 +129,10 @@ def _gemm(x, w, plan, gather, bias, silu_mul, scale_a, scale_b, out, z):
     if known is None or d < 0 or any(t is not None and t.get_device() != d for t in operands) or any(
             p is not None and p & 15 for p in (ptr[0], ptr[1], ptr[4], ptr[6])):
         return _gemm_checked(x, w, plan, gather, bias, silu_mul, scale_a, scale_b, out, z, key)
-    args, shape = known
+    args, shape, need = known
     g = nat.HkxExpertsGemmArgs.from_buffer_copy(args)
     g.a, g.b, g.offsets, g.index, g.bias, g.sa, g.sb = ptr
-    return _launch(g, x, nat.empty(x, shape, _bf16()), z)
+    return _launch(g, x, nat.empty(x, shape, _bf16()), z, need)
 
 
 _BF16: list = []
@@ -146,16 +146,22 @@ def _bf16():
     return _BF16[0]
 
 
-def _launch(g, x, out, z):
+def _launch(g, x, out, z, need=None):
     g.c = out.data_ptr()
     if z is not None:
         g.z, g.ldz = z.data_ptr(), _ld(z, z.shape[1])
-    _run(g, x.device)
+    _run(g, x.device, need)
     return out
 
 
-def _run(g, device):
+def _run(g, device, need=None):
+    """The launch; need: the workspace's bytes, where they are known."""
     with nat.current(device):
+        if need is None:
+            need = nat.lib().hkx_experts_gemm_workspace(ctypes.byref(g))
+        if need:
+            ws = nat.workspace(device, need)
+            g.ws, g.ws_bytes = ws.data_ptr(), need
         nat.check(nat.lib().hkx_experts_gemm(ctypes.byref(g), nat.stream_of(device)))
 
 
@@ -249,9 +255,16 @@ def _gemm_checked(x, w, plan, gather, bias, silu_mul, scale_a, scale_b, out, z, 
         g.sb_col = int(scale_b.dim() == 2 and scale_b.shape[1] == w.shape[1] and w.shape[1] > 1)
         g.sb_ld = w.shape[1] if g.sb_col else 1
     # (a template only where every operand was read where it is, and C is new)
-    if new and all(a is None or a.data_ptr() == b.data_ptr() for a, b in zip(given, (x, w, bias, scale_a, scale_b))):
-        nat.remember(_GEMM, key, (bytes(g), (r, n)), 4096)
-    return _launch(g, x, out, z)
+    known = bytes(g) if new and all(a is None or a.data_ptr() == b.data_ptr() for a, b in zip(
+        given, (x, w, bias, scale_a, scale_b))) else None
+    g.c = out.data_ptr()
+    if z is not None:
+        g.z, g.ldz = z.data_ptr(), _ld(z, z.shape[1])
+    with nat.current(x.device):
+        need = nat.lib().hkx_experts_gemm_workspace(ctypes.byref(g))
+    if known is not None:
+        nat.remember(_GEMM, key, (known, (r, n), need), 4096)
+    return _launch(g, x, out, z, need)
 
 
 def _product(op, a, b, plan, out):

@@ -459,17 +459,21 @@ typedef struct {
   int64_t lda, ldb, ldc, ldz;        /* row strides, elements */
   int64_t b_expert, c_expert;        /* strides of an expert, elements (NT, NN: B's; TN: C's) */
   int64_t bias_ld, sb_ld;            /* of the bias and the scales */
+  void* ws;                          /* hkx_experts_gemm_workspace() bytes, 16-byte aligned */
+  size_t ws_bytes;
 } HkxExpertsGemmArgs;
 #define HKX_EXPERTS_AUTO 0
 #define HKX_EXPERTS_TILE16 1  /* tiles of 16, 64 or 128 rows */
 #define HKX_EXPERTS_TILE64 2
 #define HKX_EXPERTS_TILE128 3
-#define HKX_EXPERTS_SKINNY16 5 /* NT (else by size): the decode kernel, 16 or 32 rows */
-#define HKX_EXPERTS_SKINNY32 6
 #define HKX_EXPERTS_QUAD 4 /* 256 x 256 tiles, 8 waves, persistent; C, z and the bias in 16-byte aligned rows */
+#define HKX_EXPERTS_SKINNY16 5 /* the decode kernel, 16 or 32 rows (NT; a gradient goes by its size) */
+#define HKX_EXPERTS_SKINNY32 6
 /* bf16 C from bf16 or fp8 operands, sums in fp32, rounded once. n and k multiples of 8 (m too; an fp8 k of 16), rows
  * and experts of A and B 16-byte aligned, of C, z and the bias 8-byte, scales (a row of B each) 16-byte. */
 int hkx_experts_gemm(const HkxExpertsGemmArgs* args, void* stream);
+/* (goes by every size, stride and address, so these are set first) */
+size_t hkx_experts_gemm_workspace(const HkxExpertsGemmArgs* args);
 
 /* dz from dy (rows, n) and z (rows, 2 n), bf16: the gradient of silu(z[:n]) * z[n:]. Rows behind
  * offsets[experts] are left. Rows 16-byte aligned, n a multiple of 8. */

@@ -30,7 +30,7 @@ def kernel(request, monkeypatch):
     """Each product on the kernel named."""
     real = experts._run
 
-    def run(g, device):
+    def run(g, device, need=None):
         g.kernel = request.param
         real(g, device)
 
@@ -599,3 +599,33 @@ def test_gradients_of_many_tiles(t, e, k, n, d, dead, kernel):
                                      (dw[i], a.t() @ c, a.abs().t() @ c.abs(), hi - lo)):
             err = (terms + 2) * 2.0 ** -23 * mag
             assert ((got.double() - ref).abs() <= err + 2.0 ** -8 * (ref.abs() + err)).all()
+
+
+@pytest.mark.parametrize("gather", [False, True], ids=["sorted", "gather"])
+@pytest.mark.parametrize("silu_mul", [False, True], ids=["plain", "paired"])
+@pytest.mark.parametrize("kind,d", [("bf16", 2088), ("bf16", 4096), ("fp8", 3216)])
+@pytest.mark.parametrize("t,e,n,dead", [(1300, 3, 520, 40), (6000, 2, 2824, 0), (300, 1, 264, 300)])
+def test_a_last_round_split_along_k(t, e, n, dead, kind, d, silu_mul, gather, monkeypatch):
+    """Few tiles behind whole rounds, or no whole round, with a long K: parts of tiles that meet in memory."""
+    monkeypatch.setattr(experts, "_run", lambda g, dev, need=None, real=experts._run: (setattr(g, "kernel", 4), real(g, dev)))
+    plan, _ = _plan(t, e, 1, seed=n, dead=dead)
+    g = torch.Generator(device=DEV).manual_seed(n)
+    x = torch.randn(t, d, generator=g, device=DEV)
+    w = torch.randn(e, 2 * n if silu_mul else n, d, generator=g, device=DEV) * d ** -0.5
+    bias = torch.randn(w.shape[:2], generator=g, device=DEV)
+    scales, xd, wd = {}, x.to(BF16), w.to(BF16)
+    if kind == "fp8":
+        (x, sa), (w, sb) = fp8.quant(x), fp8.quant(w)
+        scales = dict(scale_a=sa, scale_b=sb.squeeze(2))
+        xd, wd = x.double() * sa.double(), w.double() * sb.double()
+    else:
+        x, w = xd, wd
+    y = experts.gemm(x, w, plan, gather=gather, silu_mul=silu_mul, bias=bias, **scales)
+    ref, z = _on_gpu(plan, xd, wd, gather, bias, silu_mul)
+    err = _sum_error(xd, wd, plan.offsets, plan.rows if gather else None, bias, kind == "bf16") + 2.0 ** -22 * z.abs()
+    if silu_mul:
+        err = _silu_mul_error(z, err)
+    assert not y[int(plan.offsets[-1]):].any()
+    assert ((y.double() - ref).abs() <= err + HALF[BF16] * (ref.abs() + err)).all()
+    again = experts.gemm(x, w, plan, gather=gather, silu_mul=silu_mul, bias=bias, **scales)
+    assert torch.equal(y, again)
