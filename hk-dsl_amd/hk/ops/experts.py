@@ -35,6 +35,17 @@ from .mxfp8 import _on
 MAX_EXPERTS, MAX_CHOSEN = 1024, 64
 NT, NN, TN = range(3)  # the library's products (include/hkx.h)
 
+_TORCH: list = []
+
+
+def _torch():
+    """torch, looked up once (an import statement costs a call 0.3 us)."""
+    if not _TORCH:
+        import torch  # noqa: PLC0415
+
+        _TORCH.append(torch)
+    return _TORCH[0]
+
 
 class Plan(NamedTuple):
     """The order of rows by expert (the module's docstring)."""
@@ -84,9 +95,20 @@ def _experts16(w):
 
 
 def _grad(*tensors):
-    import torch  # noqa: PLC0415
+    for t in tensors:
+        if t is not None and t.requires_grad:
+            return _torch().is_grad_enabled()
+    return False
 
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+
+def _elsewhere(d, *tensors):
+    """Whether a tensor is not on GPU d (a device's number; below 0: none)."""
+    if d < 0:
+        return True
+    for t in tensors:
+        if t is not None and t.get_device() != d:
+            return True
+    return False
 
 
 # ---------------------------------------------------------------- the products
@@ -124,26 +146,26 @@ def _gemm(x, w, plan, gather, bias, silu_mul, scale_a, scale_b, out, z):
            _layout(scale_a), _layout(scale_b), z is None)
     known = _GEMM.get(key) if out is None else None
     d = x.get_device()
-    operands = (x, w, plan.offsets, index, bias, scale_a, scale_b)
-    ptr = [None if t is None else t.data_ptr() for t in operands]
-    if known is None or d < 0 or any(t is not None and t.get_device() != d for t in operands) or any(
-            p is not None and p & 15 for p in (ptr[0], ptr[1], ptr[4], ptr[6])):
+    offsets = plan.offsets
+    if known is None or _elsewhere(d, x, w, offsets, index, bias, scale_a, scale_b):
         return _gemm_checked(x, w, plan, gather, bias, silu_mul, scale_a, scale_b, out, z, key)
-    args, shape, need = known
-    g = nat.HkxExpertsGemmArgs.from_buffer_copy(args)
-    g.a, g.b, g.offsets, g.index, g.bias, g.sa, g.sb = ptr
-    return _launch(g, x, nat.empty(x, shape, _bf16()), z, need)
-
-
-_BF16: list = []
-
-
-def _bf16():
-    if not _BF16:
-        import torch  # noqa: PLC0415
-
-        _BF16.append(torch.bfloat16)
-    return _BF16[0]
+    pa, pb = x.data_ptr(), w.data_ptr()
+    bits = pa | pb
+    g = nat.HkxExpertsGemmArgs.from_buffer_copy(known[0])
+    g.a, g.b, g.offsets = pa, pb, offsets.data_ptr()
+    if index is not None:
+        g.index = index.data_ptr()
+    if bias is not None:
+        at = bias.data_ptr()
+        g.bias = at
+        bits |= at
+    if scale_a is not None:
+        at = scale_b.data_ptr()
+        g.sa, g.sb = scale_a.data_ptr(), at
+        bits |= at
+    if bits & 15:
+        return _gemm_checked(x, w, plan, gather, bias, silu_mul, scale_a, scale_b, out, z, key)
+    return _launch(g, x, nat.empty(x, known[1], _torch().bfloat16), z, known[2])
 
 
 def _launch(g, x, out, z, need=None):
@@ -352,13 +374,21 @@ def combine(y, plan, weights=None):
     """(T, D): out[t] = sum over j of weights[t, j] * y[plan.slots[t, j]], y (R, D) bf16, fp16 or fp32 and weights
     (T, k) fp32 (None: ones), in fp32 and in order of j, rounded once to y's type. A choice without a row (slot -1)
     adds nothing. Differentiable in y and weights (y's rows behind the last expert's get zeros)."""
-    _check_combine(y, plan, weights)
+    slots = plan.slots
+    key = (_layout(y), _layout(slots), _layout(weights))
+    if key not in _COMBINE or _elsewhere(y.get_device(), y, slots, weights):
+        _check_combine(y, plan, weights)
+        nat.remember(_COMBINE, key, True, 4096)
     if _grad(y, weights):
         if plan.offsets is None:
             raise ValueError("experts.combine: the gradient takes the plan's offsets")
         _int32("experts.combine", y.device, offsets=plan.offsets)
         return _functions()[1].apply(y, weights, plan)
-    return _combine(y, plan.slots, weights)
+    return _combine(y, slots, weights)
+
+
+#: Layouts of combine's operands that were checked.
+_COMBINE: dict = {}
 
 
 def _check_combine(y, plan, weights):
@@ -428,12 +458,16 @@ def route(logits, k, *, renormalize=True):
     without `renormalize` over all E. An expert of logit -inf is not chosen: -1, weight 0, no row. NaN counts as the
     largest and makes its token's weights NaN. E up to 1024, k up to 64. The weights are differentiable in the
     logits."""
-    _check_route(logits, k)
     if _grad(logits):
+        _check_route(logits, k)
         weights, chosen, *plan = _functions()[2].apply(logits, int(k), bool(renormalize))
-    else:
-        weights, chosen, *plan = _route(logits, k, renormalize)
-    return weights, chosen, Plan(*plan)
+        return weights, chosen, Plan(*plan)
+    weights, chosen, offsets, rows, slots = _route(logits, k, renormalize)
+    return weights, chosen, Plan(offsets, rows, slots)
+
+
+#: Layouts of route's logits: (arguments filled in but for their addresses, the workspace's bytes).
+_ROUTE: dict = {}
 
 
 def _check_route(logits, k):
@@ -451,27 +485,38 @@ def _check_route(logits, k):
 
 
 def _route(logits, k, renormalize):
-    import torch  # noqa: PLC0415
-
+    torch = _torch()
+    key = (logits.shape, logits.stride(), logits.dtype, k, renormalize)
+    known = _ROUTE.get(key)
+    device = logits.device
+    if known is None or logits.get_device() < 0:
+        _check_route(logits, k)
+        t, e = logits.shape
+        if t == 0:
+            known = None
+        else:
+            given, logits = logits, _unit(logits)
+            g = nat.HkxExpertsRouteArgs()
+            g.size, g.dtype, g.t, g.e, g.k = ctypes.sizeof(g), nat.dtype_code(logits.dtype), t, e, k
+            g.renormalize, g.ld = int(bool(renormalize)), _ld(logits, e)
+            known = (bytes(g), nat.lib().hkx_experts_route_workspace(ctypes.byref(g)))
+            if logits is given:
+                nat.remember(_ROUTE, key, known, 4096)
     t, e = logits.shape
-    weights = nat.empty(logits, (t, k), torch.float32)
-    chosen, slots = nat.empty(logits, (t, k), torch.int32), nat.empty(logits, (t, k), torch.int32)
-    offsets, rows = nat.empty(logits, (e + 1,), torch.int32), nat.empty(logits, (t * k,), torch.int32)
-    if t == 0:
+    empty, int32 = nat.empty, torch.int32
+    weights = empty(logits, (t, k), torch.float32)
+    chosen, slots = empty(logits, (t, k), int32), empty(logits, (t, k), int32)
+    offsets, rows = empty(logits, (e + 1,), int32), empty(logits, (t * k,), int32)
+    if known is None:
         return weights, chosen, offsets.zero_(), rows, slots
-    logits = _unit(logits)
-    g = nat.HkxExpertsRouteArgs()
-    g.size, g.dtype, g.t, g.e, g.k = ctypes.sizeof(g), nat.dtype_code(logits.dtype), t, e, k
-    g.renormalize, g.logits, g.ld = int(bool(renormalize)), logits.data_ptr(), _ld(logits, e)
-    g.weights, g.chosen, g.offsets = weights.data_ptr(), chosen.data_ptr(), offsets.data_ptr()
-    g.rows, g.slots = rows.data_ptr(), slots.data_ptr()
-    L = nat.lib()
-    with nat.current(logits.device):
-        need = L.hkx_experts_route_workspace(ctypes.byref(g))
-        ws = nat.workspace(logits.device, need)
-        if ws is not None:
-            g.ws, g.ws_bytes = ws.data_ptr(), need
-        nat.check(L.hkx_experts_route(ctypes.byref(g), nat.stream_of(logits.device)))
+    g = nat.HkxExpertsRouteArgs.from_buffer_copy(known[0])
+    g.logits, g.weights, g.chosen = logits.data_ptr(), weights.data_ptr(), chosen.data_ptr()
+    g.offsets, g.rows, g.slots = offsets.data_ptr(), rows.data_ptr(), slots.data_ptr()
+    with nat.current(device):
+        if known[1]:
+            ws = nat.workspace(device, known[1])
+            g.ws, g.ws_bytes = ws.data_ptr(), known[1]
+        nat.check(nat.lib().hkx_experts_route(ctypes.byref(g), nat.stream_of(device)))
     return weights, chosen, offsets, rows, slots
 
 
