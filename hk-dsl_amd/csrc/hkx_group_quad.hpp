@@ -25,7 +25,7 @@ constexpr size_t kQuadPartBytes = 256 * 256 * 4;
 // The last round of `total` tiles on `grid` workgroups, where it fills at most half of them: its `rem` tiles in `parts`
 // along K each (1: whole), a workgroup one part, the fp32 sums through memory. A round of nku units takes some 1.5 nku us, a
 // part's sums written and read 0.13 us of the whole: parts while their square times rem is below 12 nku. (Gradient of
-// 8192 rows, 36 tile rows of 8 tiles, K = 8192: 335 us, with the 32 tiles over SPLIT_US.)
+// 8192 rows, 36 tile rows of 8 tiles, K = 8192: 335 us, with the 32 tiles over in parts 236.)
 struct QuadRound {
   int full, rem, parts;
 };
@@ -144,14 +144,15 @@ __global__ void __launch_bounds__(512, 1) group_quad_kernel(const GroupArgs p) {
   uint32_t b1 = 0;  // B's second half behind the first (0: past N, the first again: it is never stored)
   Tile cur = tile_at(0), nxt = cur;
 
-  auto load2 = [&](__amdgpu_buffer_rsrc_t r, uint32_t slot, const uint32_t (&v)[2], uint32_t so) {
+  auto load = [&](__amdgpu_buffer_rsrc_t r, uint32_t slot, const uint32_t (&v)[2], uint32_t so, int k) {
     uint8_t* s = smem + slot + wave * 2048;
-    buf_load16_lds(r, s, v[0], so);
-    buf_load16_lds(r, s + 1024, v[1], so);
+    if (k != 1) buf_load16_lds(r, s, v[0], so);
+    if (k != 0) buf_load16_lds(r, s + 1024, v[1], so);
   };
-  auto fill_a1 = [&]() { load2(ra1, w1.slot + QB, va1, TA ? 0u : w1.so); };
-  auto fill_a0 = [&]() { load2(ra2, w2.slot, va2, TA ? 0u : w2.so); };
-  auto fill_b = [&](int j) { load2(rb, w2.slot + (2 + j) * QB, vb, (TB ? 0u : w2.so) + (j ? b1 : 0u)); };
+  // (k: instruction 0 or 1, or both)
+  auto fill_a1 = [&](int k = 2) { load(ra1, w1.slot + QB, va1, TA ? 0u : w1.so, k); };
+  auto fill_a0 = [&](int k = 2) { load(ra2, w2.slot, va2, TA ? 0u : w2.so, k); };
+  auto fill_b = [&](int j, int k = 2) { load(rb, w2.slot + (2 + j) * QB, vb, (TB ? 0u : w2.so) + (j ? b1 : 0u), k); };
 
   // A's half i of tile t: offsets, and the resource of a K-contiguous A or the first rows and bytes of one along K
   auto begin_a = [&](const Tile& t, int i, const int32_t* index, uint32_t (&v)[2], __amdgpu_buffer_rsrc_t& r,
@@ -293,6 +294,8 @@ __global__ void __launch_bounds__(512, 1) group_quad_kernel(const GroupArgs p) {
   constexpr int NA = 4, NB = 2;
   using Frag = typename std::conditional<FP8, i32x8, bf16x8>::type;
   Frag af[NA][2], bf0[NB][2], bf1[NB][2], bfn[NB][2];
+  // (a quarter is a multiple of 256 bytes: fragments f on are 32 f bytes away under an exclusive or, as the swizzle is)
+  const uint32_t ta = turned_at(lane, grp * 4), tb = turned_at(lane, wc * 2);
   auto straight = [&](const uint8_t* s, int r0, int h, int par) -> Frag {
     if constexpr (FP8) {
       const i32x4 lo = *(const i32x4*)(s + r0 * 128 + rdo[par]), hi = *(const i32x4*)(s + r0 * 128 + 512 + rdo[par]);
@@ -306,7 +309,7 @@ __global__ void __launch_bounds__(512, 1) group_quad_kernel(const GroupArgs p) {
     if constexpr (TB) {
       uint32_t at[NB];
 #pragma unroll
-      for (int g = 0; g < NB; ++g) at[g] = lds_address(s) + turned_at(lane, wc * 2 + g);
+      for (int g = 0; g < NB; ++g) at[g] = (lds_address(s) + tb) ^ (32u * g);
       read_turned<NB>(at, bf);
     } else {
 #pragma unroll
@@ -322,9 +325,9 @@ __global__ void __launch_bounds__(512, 1) group_quad_kernel(const GroupArgs p) {
       uint32_t at[NA + NB];
       Frag both[NA + NB][2];
 #pragma unroll
-      for (int f = 0; f < NA; ++f) at[f] = lds_address(sa) + turned_at(lane, grp * 4 + f);
+      for (int f = 0; f < NA; ++f) at[f] = (lds_address(sa) + ta) ^ (32u * f);
 #pragma unroll
-      for (int g = 0; g < NB; ++g) at[NA + g] = lds_address(s2) + turned_at(lane, wc * 2 + g);
+      for (int g = 0; g < NB; ++g) at[NA + g] = (lds_address(s2) + tb) ^ (32u * g);
       read_turned<NA + NB>(at, both);
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
@@ -343,7 +346,9 @@ __global__ void __launch_bounds__(512, 1) group_quad_kernel(const GroupArgs p) {
   };
 
   f32x4 acc[2][2][NA][NB];
-  auto math = [&](int i, int j, const Frag (&bf)[NB][2]) {
+  // TN issues its fills here, an instruction behind four MFMAs: before its reads, twice as many as the others', they held
+  // those up (8192 even rows of 8 groups, 8192 x 2048: 253 us, like this 239; NT and NN got 6-13% slower by it).
+  auto math = [&](int i, int j, const Frag (&bf)[NB][2], auto fill) {
     __builtin_amdgcn_s_setprio(1);
 #pragma unroll
     for (int h = 0; h < KH; ++h)
@@ -354,6 +359,11 @@ __global__ void __launch_bounds__(512, 1) group_quad_kernel(const GroupArgs p) {
           const f32x4 c = acc[i][j][f][g];
           if constexpr (FP8) acc[i][j][f][g] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(bf[g][h], af[f][h], c, 0, 0, 0, 0, 0, 0);
           else acc[i][j][f][g] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(bf[g][h], af[f][h], c, 0, 0, 0);
+          if (TA && g == 1 && (h * NA + f) % 4 == 1) {
+            __builtin_amdgcn_sched_barrier(0);
+            fill(h);
+            __builtin_amdgcn_sched_barrier(0);
+          }
         }
     __builtin_amdgcn_s_setprio(0);
   };
@@ -461,7 +471,8 @@ __global__ void __launch_bounds__(512, 1) group_quad_kernel(const GroupArgs p) {
   // ---- the K loop
   auto sync = [&](bool lds) {
     __builtin_amdgcn_sched_barrier(0);
-    if (lds) __builtin_amdgcn_s_waitcnt(wait_vm_lgkm0(8));
+    // (TN's own fills of the phase come after this)
+    if (lds) __builtin_amdgcn_s_waitcnt(wait_vm_lgkm0(TA ? 4 : 8));
     else __builtin_amdgcn_s_waitcnt(wait_vm(8));
     __builtin_amdgcn_sched_barrier(0);
     __builtin_amdgcn_s_barrier();
@@ -523,7 +534,7 @@ __global__ void __launch_bounds__(512, 1) group_quad_kernel(const GroupArgs p) {
       fill_a1();
       next1();
     }
-    next2();
+    if (!TA || r == 0) next2();
   }
   __builtin_amdgcn_s_waitcnt(wait_vm(8));  // A0, B0 and B1 of unit 0
   __builtin_amdgcn_s_barrier();
@@ -535,28 +546,34 @@ __global__ void __launch_bounds__(512, 1) group_quad_kernel(const GroupArgs p) {
   // unit t of tile lt: b1 holds its B1 fragments, nb1 takes the next unit's. Group 1's last barrier of a tile is after
   // its epilogue.
   auto unit = [&](int lt, int t, int nkt, int slot, Frag (&b1)[NB][2], Frag (&nb1)[NB][2]) {
-    // (rows along K are read, and waited for, behind the fills; the fills' quarters are none that is read here)
-    if constexpr (!TB) read_ab(slot, 0, slot, 0, bf0);
+    // (NN: rows along K are read, and waited for, behind the fills; the fills' quarters are none that is read here)
+    if constexpr (!TB || TA) read_ab(slot, 0, slot, 0, bf0);
+    if constexpr (TA) next2();
     if (t == 0 && lt + 1 < my_tiles) {
       nxt = tile_at(lt + 1);
       if constexpr (NT) fill_index(nxt, lt + 1);
     }
-    fill_a1();
-    next1();
-    fill_b(1);
-    if constexpr (TB) read_ab(slot, 0, slot, 0, bf0);
+    if constexpr (!TA) {
+      fill_a1();
+      next1();
+      fill_b(1);
+    }
+    if constexpr (TB && !TA) read_ab(slot, 0, slot, 0, bf0);
     sync(true);
-    math(0, 0, bf0);
-    math(0, 1, b1);
+    math(0, 0, bf0, [&](int k) { fill_a1(k); });
+    math(0, 1, b1, [&](int k) { fill_b(1, k); });
     sync(false);
-    if constexpr (!TB) read_ab(slot, 1, slot ^ 1, 1, nb1);
-    fill_b(0);
-    fill_a0();
-    next2();
-    if constexpr (TB) read_ab(slot, 1, slot ^ 1, 1, nb1);
+    if constexpr (!TB || TA) read_ab(slot, 1, slot ^ 1, 1, nb1);
+    if constexpr (TA) next1();
+    if constexpr (!TA) {
+      fill_b(0);
+      fill_a0();
+      next2();
+    }
+    if constexpr (TB && !TA) read_ab(slot, 1, slot ^ 1, 1, nb1);
     sync(true);
-    math(1, 0, bf0);
-    math(1, 1, b1);
+    math(1, 0, bf0, [&](int k) { fill_b(0, k); });
+    math(1, 1, b1, [&](int k) { fill_a0(k); });
     if (grp == 0 || t + 1 < nkt) sync(false);
   };
   int slot = 0;
