@@ -605,6 +605,8 @@ def mlp(x, logits, k, gate_up, down, *, gate_up_scale=None, down_scale=None, ren
     (E, 2 I, K) and down (E, D, I) bf16; differentiable in x, logits and both. Or gate_up and down float8_e4m3fn with
     the scales of their rows ((E, 2 I) and (E, D)), and x bf16 or quantized already, (q, s) as
     hk.ops.block_norm(quant="fp8") gives it: each product's rows are quantized by hk.ops.fp8.quant."""
+    if (gate_up_scale is None) != (down_scale is None) or (isinstance(x, tuple) and down_scale is None):
+        raise TypeError("experts.mlp: 8-bit weights come with both scales, a quantized x with 8-bit weights")
     weights, _, plan = route(logits, k, renormalize=renormalize)
     if gate_up_scale is None and down_scale is None:
         a = gemm(x, gate_up, plan, gather=True, silu_mul=True)
