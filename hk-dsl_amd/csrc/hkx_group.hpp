@@ -76,13 +76,20 @@ HKX_DEV void group_map(GroupMap& s, const GroupArgs& p, int tid, int threads) {
 #pragma unroll
       for (int d = 1; d < 64; d <<= 1) {
         const int u = __shfl_up(v, d);
-        if (tid >= d) v += u;
+        if (tid >= d) v = __builtin_elementwise_add_sat(v, u);
       }
-      if (g + tid < groups) s.first[g + tid + 1] = sum + v;
-      sum += __shfl(v, 63);
+      v = __builtin_elementwise_add_sat(v, sum);
+      if (g + tid < groups) s.first[g + tid + 1] = v;
+      sum = __shfl(v, 63);
     }
   }
   __syncthreads();
+}
+
+// All tiles of the map. (Offsets out of order can make groups that overlap, and more tiles than a launch has or an int
+// counts: what is past them is not computed.)
+HKX_DEV int group_total(const GroupMap& s, const GroupArgs& p, int tiles_n) {
+  return (int)min((int64_t)s.first[p.experts + 1] * tiles_n, (int64_t)1 << 30);
 }
 
 // The group of tile row i (a wave's lanes look together).
@@ -311,9 +318,8 @@ __global__ void __launch_bounds__(64 * WM * WN) group_tile_kernel(const GroupArg
   const int wr = wave / WN, wc = wave % WN;
   const int tiles_n = (p.n + CN - 1) / CN;
 
-  const int groups = p.experts + 1;
   if constexpr (!TA) group_map<BM>(map, p, tid, 64 * NW);
-  const int total = TA ? p.experts * ((p.m + BM - 1) / BM) * tiles_n : map.first[groups] * tiles_n;
+  const int total = TA ? p.experts * ((p.m + BM - 1) / BM) * tiles_n : group_total(map, p, tiles_n);
   const int place = group_place((int)blockIdx.x);
   if (place >= total) return;
   const GroupTile tile = group_tile_at<OP, BM, CN>(

@@ -77,7 +77,7 @@ __global__ void __launch_bounds__(512, 1) group_quad_kernel(const GroupArgs p) {
     hi = g < p.experts ? max(starts[g + 1], lo) : p.tail ? p.rows : lo;
   };
   const int total = __builtin_amdgcn_readfirstlane(TA ? p.experts * ((p.m + BM - 1) / BM) * tiles_n
-                                                      : map.first[p.experts + 1] * tiles_n);
+                                                      : group_total(map, p, tiles_n));
   // the workgroup's tiles: one at its place in every round of the grid
   const int place = group_place((int)blockIdx.x), step = (int)gridDim.x;
   const int nku = TA ? 0 : (p.k + KU - 1) / KU;
@@ -617,7 +617,7 @@ __global__ void __launch_bounds__(512) group_quad_join_kernel(const GroupArgs p,
   __shared__ GroupMap map;
   const int tiles_n = (p.n + BN - 1) / BN;
   group_map<BM>(map, p, threadIdx.x, 512);
-  const QuadRound round = quad_round(map.first[p.experts + 1] * tiles_n, grid, (p.k + KU - 1) / KU, true);
+  const QuadRound round = quad_round(group_total(map, p, tiles_n), grid, (p.k + KU - 1) / KU, true);
   const int tile = (int)blockIdx.x >> 2, i = ((int)blockIdx.x >> 1) & 1, j = (int)blockIdx.x & 1;
   if (round.parts < 2 || tile >= round.rem) return;
   const GroupTile t = group_tile_at<OP, BM, BN>(map, p, round.full + tile, tiles_n,
