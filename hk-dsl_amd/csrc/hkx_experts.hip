@@ -304,16 +304,17 @@ __global__ void __launch_bounds__(256) route_grad_kernel(const RouteGradArgs p) 
 //
 // A workgroup 2048 columns of a token, a thread 8 (pieces of 16 bytes of a 16-bit type, or single elements 256 apart).
 
+struct Named;
 struct CombineArgs {
   const void* y;
   const void* dout;
   const int32_t* slots;
-  const int32_t* offsets;
+  const Named* named;  // the gradient's
   const float* weights;
   void* out;
   float* dw;
   int64_t ldy, ldo, lddy;
-  int32_t t, k, rows, d, experts;
+  int32_t t, k, rows, d;
 };
 
 template <int DT, bool VEC>
@@ -340,22 +341,44 @@ __global__ void __launch_bounds__(256) combine_kernel(const CombineArgs p) {
   cols.template store<DT>(p.out, token * p.ldo + c0, o);
 }
 
-// A workgroup a token: dy's k rows, the k dot products, and its share of the rows behind the last.
+// The gradient: a workgroup a token, its k rows of dy and k dot products. named[r] is how many slots name row r and which is
+// the first: a row that none names gets zeros (from the token whose choices have its number), one that several name the
+// sum of theirs, in order, from the first of them.
+
+struct Named {
+  int32_t count, first;
+};
+
+__global__ void __launch_bounds__(256) combine_clear_kernel(Named* named, int rows) {
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i < rows) named[i] = {0, INT32_MAX};
+}
+__global__ void __launch_bounds__(256) combine_count_kernel(const int32_t* slots, Named* named, int rows) {
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= rows) return;
+  const int s = slots[i];
+  if ((uint32_t)s >= (uint32_t)rows) return;
+  atomicAdd(&named[s].count, 1);
+  atomicMin(&named[s].first, (int)i);
+}
+
 template <int DT, bool VEC>
 __global__ void __launch_bounds__(256) combine_grad_kernel(const CombineArgs p) {
   __shared__ float red[2][4];
   const int64_t token = blockIdx.x;
   const int32_t* slots = p.slots + token * p.k;
-  const int live = p.offsets ? min(max(p.offsets[p.experts], 0), p.rows) : p.rows;
+  auto piece = [&](int c0) { return Cols<1, VEC>{(int)threadIdx.x, 256, min(p.d - c0, 2048)}; };
   for (int j = 0; j < p.k; ++j) {
     const int s = slots[j];
     const bool in = (uint32_t)s < (uint32_t)p.rows;
     const float f = in ? (p.weights ? p.weights[token * p.k + j] : 1.0f) : 0.0f;
+    const int64_t at = token * p.k + j;
+    const Named named = p.out && in ? p.named[s] : Named{};
+    const bool mine = named.count == 1, clear = p.out && p.named[at].count == 0;
     float dot = 0.0f;
-    const int64_t rest = token * p.k + j;
-    if (in || rest >= live) {
+    if ((in && (mine || p.dw)) || clear) {
       for (int c0 = 0; c0 < p.d; c0 += 2048) {
-        const Cols<1, VEC> cols{(int)threadIdx.x, 256, min(p.d - c0, 2048)};
+        const auto cols = piece(c0);
         if (in) {
           auto g = cols.template load<DT>(p.dout, token * p.ldo + c0);
           if (p.dw) {
@@ -365,12 +388,30 @@ __global__ void __launch_bounds__(256) combine_grad_kernel(const CombineArgs p) 
           }
 #pragma unroll
           for (int i = 0; i < 8; ++i) g.v[i] *= f;
-          cols.template store<DT>(p.out, s * p.lddy + c0, g);
+          if (mine) cols.template store<DT>(p.out, s * p.lddy + c0, g);
         }
-        if (rest >= live) {
+        if (clear) {
           typename Cols<1, VEC>::Row zero{};
-          cols.template store<DT>(p.out, rest * p.lddy + c0, zero);
+          cols.template store<DT>(p.out, at * p.lddy + c0, zero);
         }
+      }
+    }
+    if (named.count > 1 && named.first == at) {
+      const int lane = threadIdx.x & 63;
+      for (int c0 = 0; c0 < p.d; c0 += 2048) {
+        const auto cols = piece(c0);
+        typename Cols<1, VEC>::Row sum{};
+        int left = named.count;
+        for (int64_t i = at; left && i < p.rows; i += 64) {
+          for (uint64_t m = __ballot(i + lane < p.rows && p.slots[min(i + lane, (int64_t)p.rows - 1)] == s); m; m &= m - 1, --left) {
+            const int64_t from = i + __builtin_ctzll(m);
+            const float w = p.weights ? p.weights[from] : 1.0f;
+            const auto g = cols.template load<DT>(p.dout, from / p.k * p.ldo + c0);
+#pragma unroll
+            for (int c = 0; c < 8; ++c) sum.v[c] += w * g.v[c];
+          }
+        }
+        cols.template store<DT>(p.out, s * p.lddy + c0, sum);
       }
     }
     if (p.dw) {
@@ -379,7 +420,7 @@ __global__ void __launch_bounds__(256) combine_grad_kernel(const CombineArgs p) 
       __syncthreads();
       if (threadIdx.x == 0) {
         const float* r = red[j & 1];
-        p.dw[token * p.k + j] = in ? r[0] + r[1] + r[2] + r[3] : 0.0f;
+        p.dw[at] = in ? r[0] + r[1] + r[2] + r[3] : 0.0f;
       }
     }
   }
@@ -590,20 +631,20 @@ int hkx_experts_combine(const void* y, int64_t ldy, int32_t dtype, const int32_t
 }
 
 int hkx_experts_combine_backward(const void* y, int64_t ldy, const void* dout, int64_t lddo, int32_t dtype, const int32_t* slots,
-                                 const int32_t* offsets, int32_t experts, const float* weights, void* dy, int64_t lddy,
-                                 float* dweights, int32_t t, int32_t k, int32_t rows, int32_t d, void* stream) {
+                                 const float* weights, void* dy, int64_t lddy, float* dweights, void* ws, int32_t t,
+                                 int32_t k, int32_t rows, int32_t d, void* stream) {
   using namespace hkx;
   api_clear();
-  if ((dweights && !y) || !dout || !slots || !offsets || !dy) return api_fail(HKX_ERR_ARG, "experts_combine_backward: a null pointer");
+  if ((dweights && !y) || !dout || !slots || (!dy && !dweights) || (dy && !ws)) return api_fail(HKX_ERR_ARG, "experts_combine_backward: a null pointer");
   if (!floating(dtype)) return api_fail(HKX_ERR_DTYPE, "experts_combine_backward: y is bf16, fp16 or fp32");
-  if (t < 0 || k < 1 || rows != (int64_t)t * k || d < 1 || (dweights && ldy < d) || lddo < d || lddy < d || experts < 1 || t >= 1 << 24)
-    return api_fail(HKX_ERR_SHAPE, "experts_combine_backward: t=%d k=%d rows=%d d=%d experts=%d", t, k, rows, d, experts);
+  if (t < 0 || k < 1 || rows != (int64_t)t * k || d < 1 || (dweights && ldy < d) || lddo < d || (dy && (lddy < d || !api_aligned(ws, 8))) || t >= 1 << 24)
+    return api_fail(HKX_ERR_SHAPE, "experts_combine_backward: t=%d k=%d rows=%d d=%d", t, k, rows, d);
   if (t == 0) return HKX_OK;
   CombineArgs a{};
   a.y = y;
   a.dout = dout;
   a.slots = slots;
-  a.offsets = offsets;
+  a.named = (const Named*)ws;
   a.weights = weights;
   a.out = dy;
   a.dw = dweights;
@@ -614,11 +655,17 @@ int hkx_experts_combine_backward(const void* y, int64_t ldy, const void* dout, i
   a.k = k;
   a.rows = rows;
   a.d = d;
-  a.experts = experts;
+  const hipStream_t st = (hipStream_t)stream;
+  if (dy) {
+    const dim3 grid((unsigned)(((int64_t)rows + 255) / 256));
+    hipLaunchKernelGGL(combine_clear_kernel, grid, dim3(256), 0, st, (Named*)ws, rows);
+    hipLaunchKernelGGL(combine_count_kernel, grid, dim3(256), 0, st, slots, (Named*)ws, rows);
+    if (hipError_t e = hipGetLastError()) return api_launched(e, "experts combine backward");
+  }
   const bool vec = d % 8 == 0 && whole(dweights ? y : nullptr, ldy, dtype) && whole(dout, lddo, dtype) && whole(dy, lddy, dtype);
   return api_launched(by_type(dtype, [&](auto dt) {
-    if (vec) hipLaunchKernelGGL((combine_grad_kernel<decltype(dt)::value, true>), dim3(t), dim3(256), 0, (hipStream_t)stream, a);
-    else hipLaunchKernelGGL((combine_grad_kernel<decltype(dt)::value, false>), dim3(t), dim3(256), 0, (hipStream_t)stream, a);
+    if (vec) hipLaunchKernelGGL((combine_grad_kernel<decltype(dt)::value, true>), dim3(t), dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((combine_grad_kernel<decltype(dt)::value, false>), dim3(t), dim3(256), 0, st, a);
     return hipGetLastError();
   }), "experts combine backward");
 }

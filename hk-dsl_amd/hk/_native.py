@@ -218,9 +218,9 @@ def lib() -> ctypes.CDLL:
         L.hkx_experts_combine.argtypes = [c_void_p, c_int64, c_int32, c_void_p, c_void_p, c_void_p,
                                           c_int64, c_int32, c_int32, c_int32, c_int32, c_void_p]
         L.hkx_experts_combine_backward.argtypes = [c_void_p, c_int64, c_void_p, c_int64, c_int32,
-                                                   c_void_p, c_void_p, c_int32, c_void_p, c_void_p,
-                                                   c_int64, c_void_p, c_int32, c_int32, c_int32,
-                                                   c_int32, c_void_p]
+                                                   c_void_p, c_void_p, c_void_p, c_int64, c_void_p,
+                                                   c_void_p, c_int32, c_int32, c_int32, c_int32,
+                                                   c_void_p]
         L.hkx_fp8_quant.argtypes = [c_void_p, c_int64, c_int32, c_void_p, c_int64, c_void_p,
                                     c_int32, c_int32, c_void_p]
         sizes = (c_size_t * 4)()

@@ -12,7 +12,7 @@ call can be captured in a graph after a first call.
 
 A `Plan` is three int32 tensors on the GPU: offsets (E + 1), of expert e the rows offsets[e] .. offsets[e + 1], from
 0; rows (R), the token of each row, -1 behind the last; slots (T, k), the row of each choice, -1 for one that has no
-expert. A token whose logits are all -inf (padding) has no rows, and its output is zero. Plans from elsewhere may
+expert. To drop a choice, set its slot to -1 (its row is then computed, and passes no gradient). A token whose logits are all -inf (padding) has no rows, and its output is zero. Plans from elsewhere may
 leave out `rows` where no call gathers, and `slots` where none combines or has a gathered gradient. Offsets out of
 order or past the rows are clamped and an index out of range stands for a row of zeros: nothing is read or written
 outside the tensors.
@@ -142,7 +142,7 @@ def gemm(x, w, plan, *, gather=False, bias=None, silu_mul=False, scale_a=None, s
 
 def _gemm(x, w, plan, gather, bias, silu_mul, scale_a, scale_b, out, z):
     index = plan.rows if gather else None
-    key = (_layout(x), _layout(w), _layout(plan.offsets), _layout(index), _layout(bias), silu_mul, gather,
+    key = (_layout(x), _layout(w), _layout(plan.offsets), _layout(plan.rows), _layout(bias), silu_mul, gather,
            _layout(scale_a), _layout(scale_b), z is None)
     known = _GEMM.get(key) if out is None else None
     d = x.get_device()
@@ -312,6 +312,8 @@ def _gemm_grad(x, w, plan, gather, bias, silu_mul, scale_a, scale_b, out):
         raise ValueError("experts.gemm: no gradient through out=")
     if x.dtype == torch.float8_e4m3fn or scale_a is not None or scale_b is not None:
         raise ValueError("experts.gemm: no gradient through quantized values (detach, or torch.no_grad())")
+    if x.dim() != 2 or w.dim() != 3:
+        _check("experts.gemm", x, w, plan, gather, bias, silu_mul, scale_a, scale_b, out)
     if gather and x.requires_grad:
         if plan.slots is None or plan.slots.dim() != 2 or plan.slots.shape[0] != x.shape[0]:
             raise ValueError("experts.gemm: a gathered x's gradient takes the plan's slots (T, k)")
@@ -373,17 +375,14 @@ def _gemm_backward(x, w, bias, z, plan, gather, need, dy):
 def combine(y, plan, weights=None):
     """(T, D): out[t] = sum over j of weights[t, j] * y[plan.slots[t, j]], y (R, D) bf16, fp16 or fp32 and weights
     (T, k) fp32 (None: ones), in fp32 and in order of j, rounded once to y's type. A choice without a row (slot -1)
-    adds nothing. Differentiable in y and weights (y's rows behind the last expert's get zeros)."""
+    adds nothing. Differentiable in y and weights (a row that no choice has gets zeros)."""
     slots = plan.slots
     key = (_layout(y), _layout(slots), _layout(weights))
     if key not in _COMBINE or _elsewhere(y.get_device(), y, slots, weights):
         _check_combine(y, plan, weights)
         nat.remember(_COMBINE, key, True, 4096)
     if _grad(y, weights):
-        if plan.offsets is None:
-            raise ValueError("experts.combine: the gradient takes the plan's offsets")
-        _int32("experts.combine", y.device, offsets=plan.offsets)
-        return _functions()[1].apply(y, weights, plan)
+        return _functions()[1].apply(y, weights, slots)
     return _combine(y, slots, weights)
 
 
@@ -430,22 +429,23 @@ def _combine(y, slots, weights):
     return out
 
 
-def _combine_backward(y, weights, plan, need, dout):
+def _combine_backward(y, weights, slots, need, dout):
     import torch  # noqa: PLC0415
 
-    t, k = plan.slots.shape
+    t, k = slots.shape
     dw = nat.empty(y, (t, k), torch.float32) if need[1] else None
-    dy = nat.empty(y, y.shape, y.dtype)
+    dy = nat.empty(y, y.shape, y.dtype) if need[0] else None
     if t == 0 or k == 0:
         return dy, dw
     y, dout = _unit(y), _unit(dout)
     w = None if weights is None else weights.contiguous()
     with nat.current(y.device):
+        ws = nat.workspace(y.device, 8 * t * k) if need[0] else None
         nat.check(nat.lib().hkx_experts_combine_backward(
             y.data_ptr(), _ld(y, y.shape[1]), dout.data_ptr(), _ld(dout, dout.shape[1]), nat.dtype_code(y.dtype),
-            plan.slots.data_ptr(), plan.offsets.data_ptr(), plan.offsets.shape[0] - 1,
-            None if w is None else w.data_ptr(), dy.data_ptr(), dy.shape[1], None if dw is None else dw.data_ptr(),
-            t, k, y.shape[0], y.shape[1], nat.stream_of(y.device)))
+            slots.data_ptr(), None if w is None else w.data_ptr(), None if dy is None else dy.data_ptr(), y.shape[1],
+            None if dw is None else dw.data_ptr(), None if ws is None else ws.data_ptr(), t, k, y.shape[0], y.shape[1],
+            nat.stream_of(y.device)))
     return dy, dw
 
 
@@ -568,15 +568,15 @@ def _functions():
 
     class ExpertsCombine(torch.autograd.Function):
         @staticmethod
-        def forward(ctx, y, weights, plan):
-            ctx.save_for_backward(y, weights, *plan)
-            return _combine(y, plan.slots, weights)
+        def forward(ctx, y, weights, slots):
+            ctx.save_for_backward(y, weights, slots)
+            return _combine(y, slots, weights)
 
         @staticmethod
         @once
         def backward(ctx, dout):
-            y, weights, *plan = ctx.saved_tensors
-            return (*_combine_backward(y, weights, Plan(*plan), ctx.needs_input_grad, dout), None)
+            y, weights, slots = ctx.saved_tensors
+            return (*_combine_backward(y, weights, slots, ctx.needs_input_grad, dout), None)
 
     class ExpertsRoute(torch.autograd.Function):
         @staticmethod

@@ -520,12 +520,12 @@ int hkx_experts_route_backward(const void* logits, int64_t ld, int32_t dtype, co
 int hkx_experts_combine(const void* y, int64_t ldy, int32_t dtype, const int32_t* slots, const float* weights,
                         void* out, int64_t ldo, int32_t t, int32_t k, int32_t rows, int32_t d, void* stream);
 
-/* dy[slots[i, j]] = weights[i, j] dout[i], zeros behind offsets[experts], and dweights[i, j] = <dout[i], y[slots[i, j]]>
- * (NULL: not wanted; then y may be NULL). rows = t k. */
+/* dy[r] = the sum of weights[i, j] dout[i] over the slots[i, j] that name row r, in fp32 and in their order (zeros where none
+ * does), and dweights[i, j] = <dout[i], y[slots[i, j]]>, 0 of no row. rows = t k. Either may be NULL: not wanted (without
+ * dweights y may be NULL, without dy `ws`, 8 bytes of 8-byte aligned scratch memory a row). */
 int hkx_experts_combine_backward(const void* y, int64_t ldy, const void* dout, int64_t lddo, int32_t dtype,
-                                 const int32_t* slots, const int32_t* offsets, int32_t experts, const float* weights,
-                                 void* dy, int64_t lddy, float* dweights, int32_t t, int32_t k, int32_t rows,
-                                 int32_t d, void* stream);
+                                 const int32_t* slots, const float* weights, void* dy, int64_t lddy, float* dweights,
+                                 void* ws, int32_t t, int32_t k, int32_t rows, int32_t d, void* stream);
 
 /* x (m, k) of x_dtype -> q (m, k) e4m3 and s (m) fp32: s = max |x| / 448 of the row (at least 2^-126; 1 for a row of
  * zeros), q = x / s rounded to nearest even. A row with an infinity or a NaN has s = NaN and codes 0. Any k and

@@ -133,7 +133,6 @@ def test_combine_and_route_refuse():
         (ValueError, "on a GPU", (torch.zeros(24, 32), plan)),
     ]:
         _refused(error, match, experts.combine, *args)
-    _refused(ValueError, "offsets", experts.combine, _t(24, 32, dtype=F32).requires_grad_(), plan._replace(offsets=None))
     for error, match, args in [
         (TypeError, "T, E", (_t(4, 3, 8), 2)), (TypeError, "T, E", (_t(4, 8, dtype=torch.int32), 2)),
         (ValueError, "k=0", (_t(4, 8), 0)), (ValueError, "k=9", (_t(4, 8), 9)), (ValueError, "k=65", (_t(4, 80), 65)),
@@ -291,8 +290,11 @@ def test_the_other_calls_refusals():
         (L.hkx_experts_combine(AT, 8, nat.INT8, AT, None, AT, 8, 4, 2, 8, 8, None), nat.ERR_DTYPE),
         (L.hkx_experts_combine(AT, 7, 0, AT, None, AT, 8, 4, 2, 8, 8, None), nat.ERR_SHAPE),
         (L.hkx_experts_combine(AT, 8, 0, AT, None, AT, 8, 1 << 24, 2, 8, 8, None), nat.ERR_SHAPE),
-        (L.hkx_experts_combine_backward(None, 8, AT, 8, 0, AT, AT, 4, None, AT, 8, AT, 4, 2, 8, 8, None), nat.ERR_ARG),
-        (L.hkx_experts_combine_backward(AT, 8, AT, 8, 0, AT, AT, 4, None, AT, 8, AT, 4, 2, 9, 8, None), nat.ERR_SHAPE),
+        (L.hkx_experts_combine_backward(None, 8, AT, 8, 0, AT, None, AT, 8, AT, AT, 4, 2, 8, 8, None), nat.ERR_ARG),
+        (L.hkx_experts_combine_backward(AT, 8, AT, 8, 0, AT, None, AT, 8, AT, None, 4, 2, 8, 8, None), nat.ERR_ARG),
+        (L.hkx_experts_combine_backward(AT, 8, AT, 8, 0, AT, None, None, 8, None, AT, 4, 2, 8, 8, None), nat.ERR_ARG),
+        (L.hkx_experts_combine_backward(AT, 8, AT, 8, 0, AT, None, AT, 8, AT, AT + 4, 4, 2, 8, 8, None), nat.ERR_SHAPE),
+        (L.hkx_experts_combine_backward(AT, 8, AT, 8, 0, AT, None, AT, 8, AT, AT, 4, 2, 9, 8, None), nat.ERR_SHAPE),
         (L.hkx_fp8_quant(AT, 16, nat.INT8, AT, 16, AT, 4, 16, None), nat.ERR_DTYPE),
         (L.hkx_fp8_quant(AT, 8, 0, AT, 16, AT, 4, 16, None), nat.ERR_SHAPE),
         (L.hkx_fp8_quant(AT + 1, 16, 0, AT, 16, AT, 4, 16, None), nat.ERR_SHAPE),

@@ -629,3 +629,131 @@ def test_a_last_round_split_along_k(t, e, n, dead, kind, d, silu_mul, gather, mo
     assert ((y.double() - ref).abs() <= err + HALF[BF16] * (ref.abs() + err)).all()
     again = experts.gemm(x, w, plan, gather=gather, silu_mul=silu_mul, bias=bias, **scales)
     assert torch.equal(y, again)
+
+
+# ---------------------------------------------------------------- plans from elsewhere, and gradients in a graph
+
+
+def _own_slots(kind, t, k, seed):
+    """Choices without rows, rows that several choices have, all choices one row."""
+    g = torch.Generator().manual_seed(seed)
+    if kind == "dropped":
+        slots = torch.randperm(t * k, generator=g).reshape(t, k)
+        slots[torch.rand(t, k, generator=g) < 0.4] = -1
+    elif kind == "shared":
+        slots = torch.randint(-1, max(t * k // 2, 1), (t, k), generator=g)
+    else:
+        slots = torch.full((t, k), t * k - 1)
+    return slots
+
+
+@pytest.mark.parametrize("weighted", [True, False])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("kind", ["dropped", "shared", "one"])
+@pytest.mark.parametrize("t,k,d", [(1, 1, 3), (40, 3, 24), (130, 2, 2051)])
+def test_combine_of_other_slots(t, k, d, kind, dtype, weighted):
+    """A row's gradient is the sum over the choices that have it (fp32, in order), zeros where none does."""
+    slots = _own_slots(kind, t, k, seed=t + d)
+    g = torch.Generator().manual_seed(d)
+    y, dout = torch.randn(t * k, d, generator=g).to(dtype), torch.randn(t, d, generator=g).to(dtype)
+    w = torch.rand(t, k, generator=g)
+    torch.full((1 << 22,), math.nan, device=DEV)  # (what a new tensor may hold)
+    leaf = [y.to(DEV).requires_grad_(), w.to(DEV).requires_grad_()][: 1 + weighted]
+    out = experts.combine(leaf[0], experts.Plan(None, None, slots.int().to(DEV)), leaf[1] if weighted else None)
+    got = torch.autograd.grad(out, leaf, dout.to(DEV))
+    again = torch.autograd.grad(experts.combine(leaf[0], experts.Plan(None, None, slots.int().to(DEV)),
+                                                leaf[1] if weighted else None), leaf, dout.to(DEV))
+    assert all(torch.equal(a, b) for a, b in zip(got, again))
+    ref = [y.double().requires_grad_(), w.double().requires_grad_()][: 1 + weighted]
+    grads = torch.autograd.grad(O.combine(ref[0], slots, ref[1] if weighted else None), ref, dout.double())
+    size = torch.zeros(t * k, d, dtype=torch.float64)
+    for i, s in enumerate(slots.flatten().tolist()):
+        if s >= 0:
+            size[s] += dout[i // k].double().abs() * (float(w.flatten()[i]) if weighted else 1.0)
+    # (a term and an addition each 2^-24 of what has been added up)
+    many = int(torch.bincount(slots.flatten() + 1, minlength=2)[1:].max())
+    _within(got[0], grads[0], HALF[dtype] * grads[0].abs() + (many + 1) * 2.0 ** -23 * size)
+    if weighted:
+        at = slots.clamp(min=0)
+        _within(got[1], grads[1], (d + 2) * 2.0 ** -24 * (y.double().abs()[at] * dout.double().abs().unsqueeze(1)).sum(2))
+
+
+def test_a_gradient_of_one_operand_alone():
+    """y's or the weights' gradient alone is what it is beside the other."""
+    plan, _ = _plan(33, 5, 2, seed=8, dead=3)
+    y, w = torch.randn(66, 40, device=DEV).to(BF16), torch.rand(33, 2, device=DEV)
+    dout = torch.randn(33, 40, device=DEV).to(BF16)
+    a, b = y.clone().requires_grad_(), w.clone().requires_grad_()
+    both = torch.autograd.grad(experts.combine(a, plan, b), (a, b), dout)
+    assert torch.equal(torch.autograd.grad(experts.combine(a, plan, w), a, dout)[0], both[0])
+    assert torch.equal(torch.autograd.grad(experts.combine(y, plan, b), b, dout)[0], both[1])
+
+
+def test_a_dropped_choice_of_the_layer():
+    """slots set to -1: the tokens' outputs without those rows, and no gradient through them."""
+    x, logits, up, down = _layer(60, 4, 2, 64, 32, seed=11)
+    weights, _, plan = experts.route(logits.to(DEV), 2)
+    drop = torch.rand(60, 2, generator=torch.Generator().manual_seed(1)) < 0.3
+    cut = plan._replace(slots=plan.slots.masked_fill(drop.to(DEV), -1))
+    got, full = [], []
+    for p, w, into in ((cut, weights, got), (plan, weights.masked_fill(drop.to(DEV), 0.0), full)):
+        leaf = [v.to(DEV).requires_grad_() for v in (x, up, down)]
+        torch.full((1 << 22,), math.nan, device=DEV)
+        out = experts.combine(experts.gemm(experts.gemm(leaf[0], leaf[1], p, gather=True, silu_mul=True), leaf[2], p), p, w)
+        into += [out, *torch.autograd.grad(out, leaf, torch.ones_like(out))]
+    for a, b in zip(got, full):
+        assert torch.equal(a, b)
+
+
+def test_a_step_captured_and_replayed():
+    """Forward and backward in one graph, replayed over new values with eager work between."""
+    t, e, k, d, inner = 300, 6, 2, 64, 48
+    given = [v.to(DEV) for v in _layer(t, e, k, d, inner, seed=4)]
+    fresh = [v.to(DEV) for v in (torch.randn(4, t, d).to(BF16), torch.randn(4, t, e))]
+
+    def step(x, logits, up, down):
+        leaf = [v.detach().requires_grad_() for v in (x, logits, up, down)]
+        out = experts.mlp(leaf[0], leaf[1], k, leaf[2], leaf[3])
+        return [out.detach(), *torch.autograd.grad(out, leaf, torch.ones_like(out))]
+
+    want = [step(a, b, *given[2:]) for a, b in zip(*fresh)]
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        step(*given)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            out = step(*given)
+        for i in range(4):
+            given[0].copy_(fresh[0][i])
+            given[1].copy_(fresh[1][i])
+            graph.replay()
+            assert all(torch.equal(a, b) for a, b in zip(out, want[i]))
+            assert torch.equal(step(fresh[0][0], fresh[1][0], *given[2:])[1], want[0][1])
+            torch.cuda.synchronize()
+
+
+def test_the_largest_counts_of_experts_and_choices():
+    """1024 experts, 64 choices each: router, products, combination."""
+    x, logits, up, down = _layer(70, 1024, 64, 16, 8, seed=9)
+    out = experts.mlp(*(v.to(DEV) for v in (x, logits)), 64, up.to(DEV), down.to(DEV))
+    ref = _layer_oracle(x, logits, 64, up, down)
+    assert (out.cpu().double() - ref).norm() <= 3 * 2.0 ** -8 * ref.norm()  # (three roundings to bf16, as above)
+
+
+def test_weights_shared_by_the_experts():
+    """w and bias expanded over the experts (stride 0): their gradient is the sum over all rows."""
+    plan, (offsets, rows, _) = _plan(40, 3, 2, seed=2)
+    g = torch.Generator().manual_seed(0)
+    x, w, b = (torch.randn(*s, generator=g).to(BF16).to(DEV) for s in ((40, 72), (1, 24, 72), (1, 24)))
+    one, bias = w.clone().requires_grad_(), b.clone().requires_grad_()
+    y = experts.gemm(x, one.expand(3, -1, -1), plan, gather=True, bias=bias.expand(3, -1))
+    assert torch.equal(y, experts.gemm(x, w.repeat(3, 1, 1), plan, gather=True, bias=b.repeat(3, 1)))
+    dy = torch.randn(80, 24, generator=g).to(BF16).to(DEV)
+    dw, db = torch.autograd.grad(y, (one, bias), dy)
+    ref = dy.double().t() @ x.double()[plan.rows.long()]
+    size = dy.double().abs().t() @ x.double().abs()[plan.rows.long()]
+    # (each expert's sum rounded to bf16, and their sum: 2^-8 of the magnitudes twice, and of the roundings)
+    assert ((dw[0].double() - ref).abs() <= 2.1 * 2.0 ** -8 * size).all()
+    assert ((db[0].double() - dy.double().sum(0)).abs() <= 2.1 * 2.0 ** -8 * dy.double().abs().sum(0)).all()
