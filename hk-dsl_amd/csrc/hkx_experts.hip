@@ -304,12 +304,12 @@ __global__ void __launch_bounds__(256) route_grad_kernel(const RouteGradArgs p) 
 //
 // A workgroup 2048 columns of a token, a thread 8 (pieces of 16 bytes of a 16-bit type, or single elements 256 apart).
 
-struct Named;
 struct CombineArgs {
   const void* y;
   const void* dout;
   const int32_t* slots;
-  const Named* named;  // the gradient's
+  const int32_t* owner;  // the gradient's
+  const int32_t* other;
   const float* weights;
   void* out;
   float* dw;
@@ -341,86 +341,109 @@ __global__ void __launch_bounds__(256) combine_kernel(const CombineArgs p) {
   cols.template store<DT>(p.out, token * p.ldo + c0, o);
 }
 
-// The gradient: a workgroup a token, its k rows of dy and k dot products. named[r] is how many slots name row r and which is
-// the first: a row that none names gets zeros (from the token whose choices have its number), one that several name the
-// sum of theirs, in order, from the first of them.
+// The gradient: a workgroup a token, its k rows of dy and k dot products. A row that no slot names gets zeros (from the
+// token whose choices have its number), one that several name the sum of theirs, in order, from one of them.
+//
+// Which is which takes one launch and no cleared memory. owner[r] ends as a choice that names r; of what stands in it
+// beforehand nothing is assumed, as slots says whether a choice names a row. A choice that finds another one that names its
+// row in its place keeps it in other[]: of several at least the last has one, and the last is the owner.
 
-struct Named {
-  int32_t count, first;
-};
-
-__global__ void __launch_bounds__(256) combine_clear_kernel(Named* named, int rows) {
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (i < rows) named[i] = {0, INT32_MAX};
-}
-__global__ void __launch_bounds__(256) combine_count_kernel(const int32_t* slots, Named* named, int rows) {
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (i >= rows) return;
-  const int s = slots[i];
-  if ((uint32_t)s >= (uint32_t)rows) return;
-  atomicAdd(&named[s].count, 1);
-  atomicMin(&named[s].first, (int)i);
+__global__ void __launch_bounds__(256) combine_owner_kernel(const int32_t* slots, int32_t* owner, int32_t* other, int rows) {
+  const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (at >= rows) return;
+  const int i = (int)at, s = slots[i];
+  int found = -1;
+  if ((uint32_t)s < (uint32_t)rows) {
+    const int before = atomicExch(&owner[s], i);
+    if ((uint32_t)before < (uint32_t)rows && before != i && slots[before] == s) found = before;
+  }
+  other[i] = found;
 }
 
 template <int DT, bool VEC>
 __global__ void __launch_bounds__(256) combine_grad_kernel(const CombineArgs p) {
-  __shared__ float red[2][4];
-  const int64_t token = blockIdx.x;
-  const int32_t* slots = p.slots + token * p.k;
+  constexpr int B = 4;
+  __shared__ float red[B][4];
+  const int64_t token = blockIdx.x, first = token * p.k;
+  const int lane = threadIdx.x & 63;
   auto piece = [&](int c0) { return Cols<1, VEC>{(int)threadIdx.x, 256, min(p.d - c0, 2048)}; };
-  for (int j = 0; j < p.k; ++j) {
-    const int s = slots[j];
-    const bool in = (uint32_t)s < (uint32_t)p.rows;
-    const float f = in ? (p.weights ? p.weights[token * p.k + j] : 1.0f) : 0.0f;
-    const int64_t at = token * p.k + j;
-    const Named named = p.out && in ? p.named[s] : Named{};
-    const bool mine = named.count == 1, clear = p.out && p.named[at].count == 0;
-    float dot = 0.0f;
-    if ((in && (mine || p.dw)) || clear) {
-      for (int c0 = 0; c0 < p.d; c0 += 2048) {
-        const auto cols = piece(c0);
-        if (in) {
-          auto g = cols.template load<DT>(p.dout, token * p.ldo + c0);
-          if (p.dw) {
-            const auto y = cols.template load<DT>(p.y, s * p.ldy + c0);
+  auto sum_all = [&](int s) {  // row s of dy: its choices, in order
+    for (int c0 = 0; c0 < p.d; c0 += 2048) {
+      const auto cols = piece(c0);
+      typename Cols<1, VEC>::Row sum{};
+      for (int64_t i = 0; i < p.rows; i += 64) {
+        for (uint64_t m = __ballot(i + lane < p.rows && p.slots[min(i + lane, (int64_t)p.rows - 1)] == s); m; m &= m - 1) {
+          const int64_t from = i + __builtin_ctzll(m);
+          const float w = p.weights ? p.weights[from] : 1.0f;
+          const auto g = cols.template load<DT>(p.dout, from / p.k * p.ldo + c0);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) dot += g.v[i] * y.v[i];
-          }
-#pragma unroll
-          for (int i = 0; i < 8; ++i) g.v[i] *= f;
-          if (mine) cols.template store<DT>(p.out, s * p.lddy + c0, g);
-        }
-        if (clear) {
-          typename Cols<1, VEC>::Row zero{};
-          cols.template store<DT>(p.out, at * p.lddy + c0, zero);
+          for (int c = 0; c < 8; ++c) sum.v[c] += w * g.v[c];
         }
       }
+      cols.template store<DT>(p.out, s * p.lddy + c0, sum);
     }
-    if (named.count > 1 && named.first == at) {
-      const int lane = threadIdx.x & 63;
+  };
+  for (int j0 = 0; j0 < p.k; j0 += 64) {
+    // a lane a choice: its row, and whose rows the choice's row and the row of its own number are
+    const int n = min(p.k - j0, 64);
+    int slot = -1, kind = 0;  // kind: 1 its row is this choice's alone, 2 others' too and this one's to write; 4 a row of zeros
+    float weight = 0.0f;
+    if (lane < n) {
+      const int i = (int)first + j0 + lane;
+      slot = p.slots[i];
+      const bool in = (uint32_t)slot < (uint32_t)p.rows;
+      if (in) weight = p.weights ? p.weights[i] : 1.0f;
+      if (p.out) {
+        const int other = p.other[i], here = p.owner[i];
+        if (in && p.owner[slot] == i) kind = other < 0 ? 1 : 2;
+        if ((uint32_t)here >= (uint32_t)p.rows || p.slots[here] != i) kind |= 4;
+      }
+      if (!in) slot = -1;
+    }
+    // B choices at a time: their rows of y are in flight together, and dout is read once
+    for (int jb = 0; jb < n; jb += B) {
+      int s[B], what[B];
+      float f[B], dot[B] = {};
+#pragma unroll
+      for (int b = 0; b < B; ++b) {  // (past n: no row)
+        s[b] = __builtin_amdgcn_readlane(slot, jb + b);
+        what[b] = __builtin_amdgcn_readlane(kind, jb + b);
+        f[b] = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, weight), jb + b));
+      }
       for (int c0 = 0; c0 < p.d; c0 += 2048) {
         const auto cols = piece(c0);
-        typename Cols<1, VEC>::Row sum{};
-        int left = named.count;
-        for (int64_t i = at; left && i < p.rows; i += 64) {
-          for (uint64_t m = __ballot(i + lane < p.rows && p.slots[min(i + lane, (int64_t)p.rows - 1)] == s); m; m &= m - 1, --left) {
-            const int64_t from = i + __builtin_ctzll(m);
-            const float w = p.weights ? p.weights[from] : 1.0f;
-            const auto g = cols.template load<DT>(p.dout, from / p.k * p.ldo + c0);
+        const auto g = cols.template load<DT>(p.dout, token * p.ldo + c0);
+        if (p.dw) {
+          typename Cols<1, VEC>::Row y[B];
 #pragma unroll
-            for (int c = 0; c < 8; ++c) sum.v[c] += w * g.v[c];
-          }
+          for (int b = 0; b < B; ++b) y[b] = cols.template load<DT>(s[b] >= 0 ? p.y : nullptr, max(s[b], 0) * p.ldy + c0);
+#pragma unroll
+          for (int b = 0; b < B; ++b)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) dot[b] += g.v[i] * y[b].v[i];
         }
-        cols.template store<DT>(p.out, s * p.lddy + c0, sum);
+#pragma unroll
+        for (int b = 0; b < B; ++b) {
+          typename Cols<1, VEC>::Row o;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) o.v[i] = g.v[i] * f[b];
+          if (what[b] & 1) cols.template store<DT>(p.out, s[b] * p.lddy + c0, o);
+          if (what[b] & 4) cols.template store<DT>(p.out, (first + j0 + jb + b) * p.lddy + c0, typename Cols<1, VEC>::Row{});
+        }
       }
-    }
-    if (p.dw) {
-      dot = wave_sum(dot);
-      if ((threadIdx.x & 63) == 0) red[j & 1][threadIdx.x >> 6] = dot;
-      __syncthreads();
-      if (threadIdx.x == 0) {
-        const float* r = red[j & 1];
-        p.dw[at] = in ? r[0] + r[1] + r[2] + r[3] : 0.0f;
+#pragma unroll
+      for (int b = 0; b < B; ++b)
+        if (what[b] & 2) sum_all(s[b]);
+      if (p.dw) {
+        __syncthreads();  // (the last ones are read)
+#pragma unroll
+        for (int b = 0; b < B; ++b) {
+          dot[b] = wave_sum(dot[b]);
+          if (lane == 0) red[b][threadIdx.x >> 6] = s[b] >= 0 ? dot[b] : 0.0f;
+        }
+        __syncthreads();
+        const int b = threadIdx.x;
+        if (b < B && jb + b < n) p.dw[first + j0 + jb + b] = red[b][0] + red[b][1] + red[b][2] + red[b][3];
       }
     }
   }
@@ -637,14 +660,15 @@ int hkx_experts_combine_backward(const void* y, int64_t ldy, const void* dout, i
   api_clear();
   if ((dweights && !y) || !dout || !slots || (!dy && !dweights) || (dy && !ws)) return api_fail(HKX_ERR_ARG, "experts_combine_backward: a null pointer");
   if (!floating(dtype)) return api_fail(HKX_ERR_DTYPE, "experts_combine_backward: y is bf16, fp16 or fp32");
-  if (t < 0 || k < 1 || rows != (int64_t)t * k || d < 1 || (dweights && ldy < d) || lddo < d || (dy && (lddy < d || !api_aligned(ws, 8))) || t >= 1 << 24)
+  if (t < 0 || k < 1 || rows != (int64_t)t * k || d < 1 || (dweights && ldy < d) || lddo < d || (dy && (lddy < d || !api_aligned(ws, 4))) || t >= 1 << 24)
     return api_fail(HKX_ERR_SHAPE, "experts_combine_backward: t=%d k=%d rows=%d d=%d", t, k, rows, d);
   if (t == 0) return HKX_OK;
   CombineArgs a{};
   a.y = y;
   a.dout = dout;
   a.slots = slots;
-  a.named = (const Named*)ws;
+  a.owner = (const int32_t*)ws;
+  a.other = a.owner + rows;
   a.weights = weights;
   a.out = dy;
   a.dw = dweights;
@@ -658,8 +682,7 @@ int hkx_experts_combine_backward(const void* y, int64_t ldy, const void* dout, i
   const hipStream_t st = (hipStream_t)stream;
   if (dy) {
     const dim3 grid((unsigned)(((int64_t)rows + 255) / 256));
-    hipLaunchKernelGGL(combine_clear_kernel, grid, dim3(256), 0, st, (Named*)ws, rows);
-    hipLaunchKernelGGL(combine_count_kernel, grid, dim3(256), 0, st, slots, (Named*)ws, rows);
+    hipLaunchKernelGGL(combine_owner_kernel, grid, dim3(256), 0, st, slots, (int32_t*)ws, (int32_t*)ws + rows, rows);
     if (hipError_t e = hipGetLastError()) return api_launched(e, "experts combine backward");
   }
   const bool vec = d % 8 == 0 && whole(dweights ? y : nullptr, ldy, dtype) && whole(dout, lddo, dtype) && whole(dy, lddy, dtype);

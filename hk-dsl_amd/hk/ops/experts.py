@@ -607,6 +607,9 @@ def mlp(x, logits, k, gate_up, down, *, gate_up_scale=None, down_scale=None, ren
     hk.ops.block_norm(quant="fp8") gives it: each product's rows are quantized by hk.ops.fp8.quant."""
     if (gate_up_scale is None) != (down_scale is None) or (isinstance(x, tuple) and down_scale is None):
         raise TypeError("experts.mlp: 8-bit weights come with both scales, a quantized x with 8-bit weights")
+    if (x[0] if isinstance(x, tuple) else x).shape[:1] != logits.shape[:1]:
+        raise ValueError(f"experts.mlp: x has {tuple((x[0] if isinstance(x, tuple) else x).shape)}, logits {tuple(logits.shape)}: "
+                         f"a row a token")
     weights, _, plan = route(logits, k, renormalize=renormalize)
     if gate_up_scale is None and down_scale is None:
         a = gemm(x, gate_up, plan, gather=True, silu_mul=True)

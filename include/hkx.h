@@ -522,7 +522,7 @@ int hkx_experts_combine(const void* y, int64_t ldy, int32_t dtype, const int32_t
 
 /* dy[r] = the sum of weights[i, j] dout[i] over the slots[i, j] that name row r, in fp32 and in their order (zeros where none
  * does), and dweights[i, j] = <dout[i], y[slots[i, j]]>, 0 of no row. rows = t k. Either may be NULL: not wanted (without
- * dweights y may be NULL, without dy `ws`, 8 bytes of 8-byte aligned scratch memory a row). */
+ * dweights y may be NULL, without dy `ws`, 8 bytes of 4-byte aligned scratch memory a row). */
 int hkx_experts_combine_backward(const void* y, int64_t ldy, const void* dout, int64_t lddo, int32_t dtype,
                                  const int32_t* slots, const float* weights, void* dy, int64_t lddy, float* dweights,
                                  void* ws, int32_t t, int32_t k, int32_t rows, int32_t d, void* stream);

@@ -154,6 +154,7 @@ def test_mlp_refuses_a_mixed_call():
     logits = _t(12, 4, dtype=F32)
     _refused(TypeError, "scales", experts.mlp, (x, _t(12, 1, dtype=F32)), logits, 2, up, down)
     _refused(TypeError, "scales", experts.mlp, x, logits, 2, up, down, gate_up_scale=_t(4, 80, dtype=F32))
+    _refused(ValueError, "a row a token", experts.mlp, x[:11], logits, 2, up, down)
 
 
 # ------------------------------------------------------------------ what a call passes on
@@ -293,7 +294,7 @@ def test_the_other_calls_refusals():
         (L.hkx_experts_combine_backward(None, 8, AT, 8, 0, AT, None, AT, 8, AT, AT, 4, 2, 8, 8, None), nat.ERR_ARG),
         (L.hkx_experts_combine_backward(AT, 8, AT, 8, 0, AT, None, AT, 8, AT, None, 4, 2, 8, 8, None), nat.ERR_ARG),
         (L.hkx_experts_combine_backward(AT, 8, AT, 8, 0, AT, None, None, 8, None, AT, 4, 2, 8, 8, None), nat.ERR_ARG),
-        (L.hkx_experts_combine_backward(AT, 8, AT, 8, 0, AT, None, AT, 8, AT, AT + 4, 4, 2, 8, 8, None), nat.ERR_SHAPE),
+        (L.hkx_experts_combine_backward(AT, 8, AT, 8, 0, AT, None, AT, 8, AT, AT + 2, 4, 2, 8, 8, None), nat.ERR_SHAPE),
         (L.hkx_experts_combine_backward(AT, 8, AT, 8, 0, AT, None, AT, 8, AT, AT, 4, 2, 9, 8, None), nat.ERR_SHAPE),
         (L.hkx_fp8_quant(AT, 16, nat.INT8, AT, 16, AT, 4, 16, None), nat.ERR_DTYPE),
         (L.hkx_fp8_quant(AT, 8, 0, AT, 16, AT, 4, 16, None), nat.ERR_SHAPE),

@@ -757,3 +757,14 @@ def test_weights_shared_by_the_experts():
     # (each expert's sum rounded to bf16, and their sum: 2^-8 of the magnitudes twice, and of the roundings)
     assert ((dw[0].double() - ref).abs() <= 2.1 * 2.0 ** -8 * size).all()
     assert ((db[0].double() - dy.double().sum(0)).abs() <= 2.1 * 2.0 ** -8 * dy.double().abs().sum(0)).all()
+
+
+def test_nan_in_the_gradient_of_a_token_without_experts():
+    """Its weights' gradient stays 0, and nobody else's sees it."""
+    plan, _ = _plan(20, 4, 3, seed=6, dead=5)
+    y, w = torch.randn(60, 24, device=DEV).to(BF16).requires_grad_(), torch.rand(20, 3, device=DEV).requires_grad_()
+    dout = torch.randn(20, 24, device=DEV).to(BF16)
+    clean = torch.autograd.grad(experts.combine(y, plan, w), (y, w), dout)
+    dout[15:] = math.nan
+    got = torch.autograd.grad(experts.combine(y, plan, w), (y, w), dout)
+    assert all(torch.equal(a, b) for a, b in zip(got, clean)) and not got[1][15:].any()
