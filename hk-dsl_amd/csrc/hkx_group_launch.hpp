@@ -25,11 +25,19 @@ inline bool group_quad_ok(const GroupArgs& a) {
   return whole(a.c, a.ldc) && a.c_group % 16 == 0 && whole(a.z, a.ldz) && (!a.bias || a.bias_ld * (a.bias_dt == HKX_FP32 ? 4 : 2) % 16 == 0);
 }
 
-// Whether a call runs on 256 x 256 tiles (kernel: HKX_EXPERTS_AUTO, or the one asked for), and then may split its last
-// round along K: the bytes of workspace that takes (0: none; 24 units of K are some 36 us a round).
-bool group_quad_takes(const GroupArgs& a, int op, bool pair, int kernel, int cus);
+// The kernel of a call: the one asked for (of the forward product's decode kernels a gradient has none, of tiles TN
+// has 128 and 256 rows), or the one that its shape picks.
+inline int group_kernel(const GroupArgs& a, int op, bool fp8, bool pair, int kernel, int cus) {
+  if (op != kGroupNT && kernel >= kGroupSkinny16) kernel = HKX_EXPERTS_AUTO;
+  if (op == kGroupTN && kernel != HKX_EXPERTS_AUTO) return kernel == kGroupQuad ? kGroupQuad : kGroupTile128;
+  if (kernel != HKX_EXPERTS_AUTO) return kernel;
+  return group_pick({op, fp8, a.experts, a.rows, a.m, pair ? 2 * (int64_t)a.n : a.n, a.k}, group_quad_ok(a), cus);
+}
+
+// The 256-row kernel may split its last round along K: the bytes of workspace that takes (0: none; 24 units of K are
+// some 36 us a round).
 inline size_t group_ws_bytes(const GroupArgs& a, int op, bool fp8, bool pair, int kernel, int cus) {
-  if (op == kGroupTN || (int64_t)a.k * (fp8 ? 1 : 2) < 24 * 128 || !group_quad_takes(a, op, pair, kernel, cus)) return 0;
+  if (op == kGroupTN || (int64_t)a.k * (fp8 ? 1 : 2) < 24 * 128 || group_kernel(a, op, fp8, pair, kernel, cus) != kGroupQuad) return 0;
   return (size_t)std::max(cus / 256 * 256, 256) * 256 * 256 * 4;
 }
 

@@ -2,6 +2,12 @@
 library, and the C calls' own refusals (nothing is launched)."""
 
 import ctypes
+import functools
+import math
+import shutil
+import subprocess
+import tempfile
+from pathlib import Path
 import math
 import types
 
@@ -305,3 +311,53 @@ def test_the_other_calls_refusals():
         (L.hkx_experts_bias_grad(AT, 16, AT, AT, nat.BF16, 0, 4, 16, None), nat.ERR_SHAPE),
     ]:
         assert rc == code, nat.last_error()
+
+
+# ------------------------------------------------------------------ the choice between the kernels
+
+SHIM = """
+#include "hkx_group_rules.hpp"
+extern "C" int pick(int op, int fp8, int experts, int rows, int m, int n, int k, int quad, int cus) {
+  return hkx::group_pick({op, fp8 != 0, experts, rows, m, n, k}, quad != 0, cus);
+}
+extern "C" double cost(int op, int fp8, int experts, int rows, int m, int n, int k, int kernel, int cus) {
+  return hkx::group_cost({op, fp8 != 0, experts, rows, m, n, k}, kernel, cus);
+}
+"""
+
+
+@functools.lru_cache(maxsize=None)
+def _rules():
+    cxx = shutil.which("g++") or shutil.which("c++") or "/opt/rocm/bin/amdclang++"
+    csrc = Path(__file__).resolve().parents[1] / "hk-dsl_amd" / "csrc"
+    with tempfile.TemporaryDirectory() as d:
+        src, so = Path(d) / "shim.cpp", Path(d) / "shim.so"
+        src.write_text(SHIM)
+        subprocess.run([cxx, "-std=c++17", "-O1", "-shared", "-fPIC", f"-I{csrc}", str(src), "-o", str(so)], check=True)
+        lib = ctypes.CDLL(str(so))
+        lib.cost.restype = ctypes.c_double
+        return lib
+
+
+def test_a_pick_is_one_that_the_product_has():
+    for op in range(3):
+        for fp8 in (0, 1) if op == 0 else (0,):
+            for e in (1, 2, 8, 64, 1024):
+                for rows in (0, 1, 7, 500, 16384, 2 ** 31 - 1):
+                    for n in (8, 2048, 2 ** 31 - 8):
+                        for k in (16, 4096, 2 ** 31 - 16):
+                            for quad in (0, 1):
+                                got = _rules().pick(op, fp8, e, rows, 4096, n, k, quad, 256)
+                                assert (3 if op == 2 else 1) <= got <= (6 if op == 0 else 4) and (quad or got != 4)
+                                kernels = range(3 if op == 2 else 1, 7 if op == 0 else 5)
+                                costs = [_rules().cost(op, fp8, e, rows, 4096, n, k, j, 256) for j in kernels]
+                                assert all(math.isfinite(c) and c > 0 for c in costs)
+
+
+@pytest.mark.parametrize("op,fp8,e,rows,m,n,k,kernels", [
+    (0, 0, 64, 8, 0, 2048, 2048, (5,)), (0, 0, 64, 512, 0, 8192, 512, (1, 2)), (0, 1, 64, 16376, 0, 2048, 4096, (4,)),
+    (0, 0, 8, 8192, 0, 14336, 4096, (4,)), (1, 0, 8, 8192, 0, 2048, 8192, (4,)), (2, 0, 8, 8192, 8192, 2048, 0, (4,)),
+    (2, 0, 5, 666, 904, 1112, 0, (3,)), (1, 0, 3, 90, 0, 512, 512, (1,))])
+def test_picks(op, fp8, e, rows, m, n, k, kernels):
+    """What measured fastest of all kernels at shapes far apart."""
+    assert _rules().pick(op, fp8, e, rows, m, n, k, 1, 256) in kernels
