@@ -18,6 +18,10 @@ constexpr int kChunk = 64;        // tokens whose places are found together: a b
 // A wave a token; lane l holds logits J l .. J l + J - 1 as keys: 32 bits that order as the numbers do (-0 as 0, NaN above
 // all; 0: no logit), so that the lowest lane of the largest key has the lowest expert. A round: each lane's largest, the
 // wave's, the first lane that has it.
+//
+// Bound by latency: k rounds, one after another, of a wave's largest. 16 tokens of 64 experts, k = 8: 5.2 us, one launch with
+// the plan behind it in LDS (up to 64 tokens: a bit of a 64-bit mask each); 16384 of 128: 18 us for the choices (4 tokens a
+// wave, 16 waves a workgroup, one after another), 5 for the sums, 5 for the places.
 
 struct RouteArgs {
   const void* logits;
@@ -244,7 +248,7 @@ __global__ void __launch_bounds__(1024) route_small_kernel(const RouteArgs p) {
 // ---------------------------------------------------------------- the logits' gradient
 //
 // A wave a token. Of the chosen alone: w (dw - sum w dw), else 0. Of a softmax over all: p_e (dw_e or 0 - sum w dw), with
-// p made again from the logits.
+// p made again from the logits. 16384 tokens of 128 experts, bf16: 6.6 us, 1.3 TB/s: four waves a workgroup, two barriers.
 
 struct RouteGradArgs {
   const void* logits;
@@ -302,7 +306,8 @@ __global__ void __launch_bounds__(256) route_grad_kernel(const RouteGradArgs p) 
 
 // ---------------------------------------------------------------- the way back
 //
-// A workgroup 2048 columns of a token, a thread 8 (pieces of 16 bytes of a 16-bit type, or single elements 256 apart).
+// A workgroup 2048 columns of a token, a thread 8 (pieces of 16 bytes of a 16-bit type, or single elements 256 apart). Bound
+// by HBM: 8192 tokens of 4 rows of 4096 bf16, 335 MB in 72 us, 4.7 TB/s; four rows in flight.
 
 struct CombineArgs {
   const void* y;
@@ -347,6 +352,9 @@ __global__ void __launch_bounds__(256) combine_kernel(const CombineArgs p) {
 // Which is which takes one launch and no cleared memory. owner[r] ends as a choice that names r; of what stands in it
 // beforehand nothing is assumed, as slots says whether a choice names a row. A choice that finds another one that names its
 // row in its place keeps it in other[]: of several at least the last has one, and the last is the owner.
+//
+// Bound by HBM: 8192 tokens of 4 rows of 4096 bf16, 604 MB in 113 us, 5.3 TB/s (one choice after another, its barriers and
+// dout again for each, 130).
 
 __global__ void __launch_bounds__(256) combine_owner_kernel(const int32_t* slots, int32_t* owner, int32_t* other, int rows) {
   const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x;
@@ -452,7 +460,8 @@ __global__ void __launch_bounds__(256) combine_grad_kernel(const CombineArgs p) 
 // ---------------------------------------------------------------- rows to 8 bits
 //
 // A workgroup a row, a thread 8 columns of every 2048; up to 16384 columns stay in registers between the largest and
-// the codes (P pieces a thread), past that they are read again.
+// the codes (P pieces a thread), past that they are read again. Bound by HBM for many rows, by a launch for few (512
+// rows of 1024 bf16: 4 us). The scale is the row's largest / 448, so that no value is clamped.
 
 struct QuantArgs {
   const void* x;

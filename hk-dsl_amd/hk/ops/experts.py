@@ -322,7 +322,9 @@ def _gemm_grad(x, w, plan, gather, bias, silu_mul, scale_a, scale_b, out):
 
 
 def _gemm_backward(x, w, bias, z, plan, gather, need, dy):
-    """(dx, dw, dbias)"""
+    """(dx, dw, dbias). Rounded to bf16 on the way: z (kept in bf16), dz (the products read bf16) and a gathered row's
+    gradient before its token's rows are added; fp32 in their place would double the traffic of the passes between the
+    products, and bf16 in separate calls has the same three."""
     import torch  # noqa: PLC0415
 
     r, e = dy.shape[0], w.shape[0]
