@@ -407,13 +407,13 @@ __global__ void __launch_bounds__(512, 1) group_quad_kernel(const GroupArgs p) {
 #pragma unroll
       for (int i = 0; i < 2; ++i)
 #pragma unroll
-        for (int f = 0; f < 4; ++f) rs[i][f] = p.sa_ld ? ((const float*)ev)[128 * i + 64 * grp + 16 * f + rf] : one;
+        for (int f = 0; f < 4; ++f) rs[i][f] = p.sa_ld && t.klen ? ((const float*)ev)[128 * i + 64 * grp + 16 * f + rf] : one;
 #pragma unroll
       for (int j = 0; j < 2; ++j)
 #pragma unroll
         for (int g = 0; g < 2; ++g) {
           const int c = PAIR ? 128 * g + 64 * j + 16 * wc + 4 * q : 128 * j + 32 * wc + 16 * g + 4 * q;
-          cs[j][g] = p.sb_col ? *(const f32x4*)(ev + 1024 + 4 * c) : f32x4{col, col, col, col};
+          cs[j][g] = p.sb_col && t.klen ? *(const f32x4*)(ev + 1024 + 4 * c) : f32x4{col, col, col, col};
         }
     }
     const bool bias = NT && p.bias && t.klen;
@@ -427,15 +427,15 @@ __global__ void __launch_bounds__(512, 1) group_quad_kernel(const GroupArgs p) {
           bv[j][g] = bias ? ld4(b, p.bias_dt, c) : f32x4{};
         }
     }
-    // (a tile without a contraction, the rows behind the last: what its vectors' slots hold is not used)
-    auto value = [&](int i, int j, int f, int g) {
+    // (a tile without a contraction, the rows behind the last: its sums and scales are 0)
+    auto value = [&](int i, int j, int f, int g, auto biased) {
       f32x4 v = acc[i][j][f][g];
-      if constexpr (FP8) v = t.klen ? v * (cs[j][g] * rs[i][f]) : f32x4{};
-      if constexpr (NT) {
-        if (bias) v += bv[j][g];
-      }
+      if constexpr (FP8) v *= cs[j][g] * rs[i][f];
+      if constexpr (NT && decltype(biased)::value) v += bv[j][g];
       return v;
     };
+    const bool z = PAIR && p.z != nullptr;
+    const __amdgpu_buffer_rsrc_t rz = make_rsrc(z ? p.z + t.row0 * p.ldz : nullptr, z ? rows_bytes(t.rows, p.ldz, (uint32_t)p.n * 4u) : 0u);
     // two fragments' values to 16 bytes a lane
     auto join = [&](f32x4 a, f32x4 b) {
       const u32x2 wa = pack4<2>(HKX_BF16, a), wb = pack4<2>(HKX_BF16, b);
@@ -444,33 +444,36 @@ __global__ void __launch_bounds__(512, 1) group_quad_kernel(const GroupArgs p) {
       swap16(y0, y1);
       return i32x4{(int)x0, (int)y0, (int)x1, (int)y1};
     };
+    auto stores = [&](auto biased) __attribute__((always_inline)) {
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
+      for (int i = 0; i < 2; ++i)
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        if constexpr (PAIR) {
-          // fragments 2 a and 2 a + 1 of the rows: a lane ends with 8 columns of a row of one of them
+        for (int j = 0; j < 2; ++j) {
+          if constexpr (PAIR) {
+            // fragments 2 a and 2 a + 1 of the rows: a lane ends with 8 columns of a row of one of them
 #pragma unroll
-          for (int a = 0; a < 2; ++a) {
-            __builtin_amdgcn_sched_barrier(0);
-            const f32x4 g0 = value(i, j, 2 * a, 0), u0 = value(i, j, 2 * a, 1), g1 = value(i, j, 2 * a + 1, 0), u1 = value(i, j, 2 * a + 1, 1);
-            const int n = t.n0 + 64 * j + 16 * wc + 8 * (lane >> 5), m = 128 * i + 64 * grp + 32 * a + 16 * (q & 1) + rf;
-            store(rc, join(silu_mul4(g0, u0), silu_mul4(g1, u1)), n, (uint32_t)m * (uint32_t)p.ldc + (uint32_t)n * 2u);
-            if (p.z) {
-              const __amdgpu_buffer_rsrc_t rz = make_rsrc(p.z + t.row0 * p.ldz, rows_bytes(t.rows, p.ldz, (uint32_t)p.n * 4u));
-              store(rz, join(g0, g1), n, (uint32_t)m * (uint32_t)p.ldz + (uint32_t)n * 2u);
-              store(rz, join(u0, u1), n, (uint32_t)m * (uint32_t)p.ldz + (uint32_t)(n + p.n) * 2u);
+            for (int a = 0; a < 2; ++a) {
+              __builtin_amdgcn_sched_barrier(0);
+              const f32x4 g0 = value(i, j, 2 * a, 0, biased), u0 = value(i, j, 2 * a, 1, biased), g1 = value(i, j, 2 * a + 1, 0, biased), u1 = value(i, j, 2 * a + 1, 1, biased);
+              const int n = t.n0 + 64 * j + 16 * wc + 8 * (lane >> 5), m = 128 * i + 64 * grp + 32 * a + 16 * (q & 1) + rf;
+              store(rc, join(silu_mul4(g0, u0), silu_mul4(g1, u1)), n, (uint32_t)m * (uint32_t)p.ldc + (uint32_t)n * 2u);
+              if (z) {
+                store(rz, join(g0, g1), n, (uint32_t)m * (uint32_t)p.ldz + (uint32_t)n * 2u);
+                store(rz, join(u0, u1), n, (uint32_t)m * (uint32_t)p.ldz + (uint32_t)(n + p.n) * 2u);
+              }
+            }
+          } else {
+#pragma unroll
+            for (int f = 0; f < 4; ++f) {
+              __builtin_amdgcn_sched_barrier(0);
+              const int n = t.n0 + 128 * j + 32 * wc + 16 * (q & 1) + 8 * (q >> 1), m = 128 * i + 64 * grp + 16 * f + rf;
+              store(rc, join(value(i, j, f, 0, biased), value(i, j, f, 1, biased)), n, (uint32_t)m * (uint32_t)p.ldc + (uint32_t)n * 2u);
             }
           }
-        } else {
-#pragma unroll
-          for (int f = 0; f < 4; ++f) {
-            __builtin_amdgcn_sched_barrier(0);
-            const int n = t.n0 + 128 * j + 32 * wc + 16 * (q & 1) + 8 * (q >> 1), m = 128 * i + 64 * grp + 16 * f + rf;
-            store(rc, join(value(i, j, f, 0), value(i, j, f, 1)), n, (uint32_t)m * (uint32_t)p.ldc + (uint32_t)n * 2u);
-          }
         }
-      }
+    };
+    if (bias) stores(std::true_type{});
+    else stores(std::false_type{});
   };
 
   // ---- the K loop
