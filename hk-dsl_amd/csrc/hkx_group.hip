@@ -181,11 +181,12 @@ int hkx_experts_gemm(const HkxExpertsGemmArgs* args, void* stream) {
   if (int rc = gemm_args(g, a)) return rc;
   if (g.rows == 0 && g.op != HKX_EXPERTS_TN) return HKX_OK;
   const bool fp8 = g.ab_dtype == HKX_FP8E4M3, pair = g.silu_mul != 0;
-  const size_t need = group_ws_bytes(a, g.op, fp8, pair, g.kernel, api_cus());
+  const int kernel = group_kernel(a, g.op, fp8, pair, g.kernel, api_cus());
+  const size_t need = group_ws_bytes(a, g.op, fp8, pair, kernel, api_cus());
   if (need && (!g.ws || g.ws_bytes < need || !api_aligned(g.ws, 16)))
     return api_fail(HKX_ERR_WORKSPACE, "experts_gemm: needs %zu bytes of 16-byte aligned workspace, got %zu", need, g.ws ? g.ws_bytes : (size_t)0);
   a.ws = need ? (float*)g.ws : nullptr;
-  const hipError_t e = launch_group(a, g.op, fp8, pair, g.kernel, api_cus(), (hipStream_t)stream);
+  const hipError_t e = launch_group(a, g.op, fp8, pair, kernel, api_cus(), (hipStream_t)stream);
   if (e == hipErrorInvalidConfiguration)
     return api_fail(HKX_ERR_SHAPE, "experts_gemm: rows=%d of n=%d are more tiles than a launch takes; split the call", g.rows, g.n);
   return api_launched(e, "experts gemm");

@@ -7,7 +7,7 @@
 
 namespace hkx {
 
-// hipErrorInvalidConfiguration: more tiles than a launch takes.
+// (kernel: group_kernel's) hipErrorInvalidConfiguration: more tiles than a launch takes.
 hipError_t launch_group(const GroupArgs& a, int op, bool fp8, bool pair, int kernel, int cus, hipStream_t s);
 
 // bm: 16, 64 or 128 rows (TN: 128)
