@@ -307,7 +307,7 @@ __global__ void __launch_bounds__(256) route_grad_kernel(const RouteGradArgs p) 
 // ---------------------------------------------------------------- the way back
 //
 // A workgroup 2048 columns of a token, a thread 8 (pieces of 16 bytes of a 16-bit type, or single elements 256 apart). Bound
-// by HBM: 8192 tokens of 4 rows of 4096 bf16, 335 MB in 72 us, 4.7 TB/s; four rows in flight.
+// by HBM: 8192 tokens of 4 rows of 4096 bf16, 335 MB in 72-79 us, 4.4 TB/s; four rows in flight.
 
 struct CombineArgs {
   const void* y;
@@ -353,7 +353,7 @@ __global__ void __launch_bounds__(256) combine_kernel(const CombineArgs p) {
 // beforehand nothing is assumed, as slots says whether a choice names a row. A choice that finds another one that names its
 // row in its place keeps it in other[]: of several at least the last has one, and the last is the owner.
 //
-// Bound by HBM: 8192 tokens of 4 rows of 4096 bf16, 604 MB in 113 us, 5.3 TB/s (one choice after another, its barriers and
+// Bound by HBM: 8192 tokens of 4 rows of 4096 bf16, 604 MB in 107 us, 5.6 TB/s (one choice after another, its barriers and
 // dout again for each, 130).
 
 __global__ void __launch_bounds__(256) combine_owner_kernel(const int32_t* slots, int32_t* owner, int32_t* other, int rows) {

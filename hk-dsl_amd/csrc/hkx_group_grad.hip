@@ -1,4 +1,4 @@
-// The experts' gradient products on tiles (hkx_group.hpp), and the choice of a kernel.
+// The experts' gradient products on tiles (hkx_group.hpp), and the launch of whichever kernel a call takes.
 #include "hkx_group_launch.hpp"
 
 namespace hkx {
