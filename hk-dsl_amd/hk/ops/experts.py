@@ -460,11 +460,9 @@ def route(logits, k, *, renormalize=True):
     without `renormalize` over all E. An expert of logit -inf is not chosen: -1, weight 0, no row. NaN counts as the
     largest and makes its token's weights NaN. E up to 1024, k up to 64. The weights are differentiable in the
     logits."""
-    if _grad(logits):
-        _check_route(logits, k)
-        weights, chosen, *plan = _functions()[2].apply(logits, int(k), bool(renormalize))
-        return weights, chosen, Plan(*plan)
     weights, chosen, offsets, rows, slots = _route(logits, k, renormalize)
+    if _grad(logits):
+        weights = _functions()[2].apply(logits, weights, chosen, bool(renormalize))
     return weights, chosen, Plan(offsets, rows, slots)
 
 
@@ -582,18 +580,16 @@ def _functions():
 
     class ExpertsRoute(torch.autograd.Function):
         @staticmethod
-        def forward(ctx, logits, k, renormalize):
-            weights, chosen, offsets, rows, slots = _route(logits, k, renormalize)
+        def forward(ctx, logits, weights, chosen, renormalize):  # (of weights made already)
             ctx.save_for_backward(logits, weights, chosen)
             ctx.renormalize = renormalize
-            ctx.mark_non_differentiable(chosen, offsets, rows, slots)
-            return weights, chosen, offsets, rows, slots
+            return weights.detach()
 
         @staticmethod
         @once
-        def backward(ctx, dw, *_):
+        def backward(ctx, dw):
             logits, weights, chosen = ctx.saved_tensors
-            return _route_backward(logits, weights, chosen, ctx.renormalize, dw), None, None
+            return _route_backward(logits, weights, chosen, ctx.renormalize, dw), None, None, None
 
     _FUNCTIONS[:] = [ExpertsGemm, ExpertsCombine, ExpertsRoute]
     return _FUNCTIONS
