@@ -249,16 +249,7 @@ def _e4m3_rows(x):
     return (x / s).clamp(-448, 448).to(E4M3), s
 
 
-def _package():
-    if own:
-        path = str(Path(__file__).resolve().parents[1] / "hk-dsl_amd")
-        if path not in sys.path:
-            sys.path.insert(0, path)
-        import hk  # noqa: F401, PLC0415
-
-
 def prepare(case, seed):
-    _package()
     gen = torch.Generator(device="cuda").manual_seed(seed)
     kind = case["kind"]
     if kind == "norm":
@@ -297,10 +288,17 @@ def prepare(case, seed):
     return st
 
 
-def _own(st):
+def _package():
+    path = str(Path(__file__).resolve().parents[1] / "hk-dsl_amd")
+    if path not in sys.path:
+        sys.path.insert(0, path)
     import hk  # noqa: PLC0415
 
-    ops = hk.ops
+    return hk.ops
+
+
+def _own(st):
+    ops = _package()
     experts, kind = ops.experts, st["kind"]
     if kind == "norm":
         h, (q, s) = ops.block_norm(st["x"], st["residual"], pre=st["pre"], eps=EPS, quant="fp8")
