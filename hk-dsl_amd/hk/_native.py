@@ -282,6 +282,23 @@ def stream_of(device) -> int:
     return _RAW_STREAM[0](index)
 
 
+_FORWARD_AD: list = []
+
+
+def no_tangents(call: str, *tensors) -> None:
+    """Refuses a tensor with a forward-mode derivative: a kernel reads its values alone, and the result would have none."""
+    if not _FORWARD_AD:
+        import torch.autograd.forward_ad as ad  # noqa: PLC0415
+
+        _FORWARD_AD.append(ad)
+    ad = _FORWARD_AD[0]
+    if ad._current_level < 0:
+        return
+    for t in tensors:
+        if t is not None and ad.unpack_dual(t).tangent is not None:
+            raise ValueError(f"{call}: no forward-mode derivative")
+
+
 _DEVICE: list = []
 _HERE = contextlib.nullcontext()
 

@@ -135,6 +135,7 @@ def gemm(x, w, plan, *, gather=False, bias=None, silu_mul=False, scale_a=None, s
     Sums are fp32, rounded once. Differentiable in x, w and bias (bf16): with silu_mul z is kept in bf16 for
     the backward pass; a gathered x's gradient adds a token's rows in fp32, in order of its choices. No atomics: the
     same bits every time."""
+    nat.no_tangents("experts.gemm", x, w, bias, scale_a, scale_b)
     if _grad(x, w, bias):
         return _gemm_grad(x, w, plan, gather, bias, silu_mul, scale_a, scale_b, out)
     return _gemm(x, w, plan, gather, bias, silu_mul, scale_a, scale_b, out, None)
@@ -378,6 +379,7 @@ def combine(y, plan, weights=None):
     """(T, D): out[t] = sum over j of weights[t, j] * y[plan.slots[t, j]], y (R, D) bf16, fp16 or fp32 and weights
     (T, k) fp32 (None: ones), in fp32 and in order of j, rounded once to y's type. A choice without a row (slot -1)
     adds nothing. Differentiable in y and weights (a row that no choice has gets zeros)."""
+    nat.no_tangents("experts.combine", y, weights)
     slots = plan.slots
     key = (_layout(y), _layout(slots), _layout(weights))
     if key not in _COMBINE or _elsewhere(y.get_device(), y, slots, weights):
@@ -460,6 +462,7 @@ def route(logits, k, *, renormalize=True):
     without `renormalize` over all E. An expert of logit -inf is not chosen: -1, weight 0, no row. NaN counts as the
     largest and makes its token's weights NaN. E up to 1024, k up to 64. The weights are differentiable in the
     logits."""
+    nat.no_tangents("experts.route", logits)
     weights, chosen, offsets, rows, slots = _route(logits, k, renormalize)
     if _grad(logits):
         weights = _functions()[2].apply(logits, weights, chosen, bool(renormalize))

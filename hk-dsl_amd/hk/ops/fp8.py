@@ -21,6 +21,7 @@ _QUANT: dict = {}
 def quant(x, out=None):
     """(q, s) of x (..., K), any K: q float8_e4m3fn (..., K), s fp32 (..., 1). `out`: (q, s) to write
     into, contiguous. There is no gradient through quantized values."""
+    nat.no_tangents("fp8.quant", x)
     known = None
     if out is None and not x.requires_grad:
         key = (x.shape, x.stride(), x.dtype)

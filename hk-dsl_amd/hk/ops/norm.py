@@ -298,6 +298,7 @@ def block_norm(x, residual, *, post=None, pre=None, gate=None, branch_scale=1.0,
     """(h, y): see the module's docstring."""
     import torch  # noqa: PLC0415
 
+    nat.no_tangents("block_norm", x, residual, post, pre, gate)
     scales = (float(branch_scale), float(residual_scale), float(eps))
     if torch.is_grad_enabled() and (x.requires_grad or residual.requires_grad or any(
             t is not None and t.requires_grad for t in (post, pre, gate))):

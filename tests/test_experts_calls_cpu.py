@@ -1,0 +1,82 @@
+"""Derivatives that hk.ops.experts, hk.ops.fp8 and hk.ops.block_norm do not take are refused, not dropped (no GPU: the
+library is a stub that launches nothing)."""
+
+import types
+
+import pytest
+import torch
+import torch.autograd.forward_ad as ad
+
+import hk  # noqa: F401
+from hk import _native as nat
+from hk.ops import block_norm, experts, fp8, norm
+
+BF16, F32, E4M3 = torch.bfloat16, torch.float32, torch.float8_e4m3fn
+
+
+class OnGpu(torch.Tensor):
+    """A CPU tensor that says it is on a GPU."""
+
+    is_cuda = True
+
+    def get_device(self):
+        return 0
+
+
+def _t(*size, dtype=BF16):
+    return torch.zeros(size, dtype=dtype).as_subclass(OnGpu)
+
+
+PLAN = experts.Plan(_t(5, dtype=torch.int32), _t(24, dtype=torch.int32), _t(12, 2, dtype=torch.int32))
+
+
+@pytest.fixture
+def stub(monkeypatch):
+    class Lib:
+        def __getattr__(self, name):
+            return lambda *a: 0
+
+    monkeypatch.setattr(nat, "lib", lambda: Lib())
+    monkeypatch.setattr(nat, "stream_of", lambda device: 0)
+    monkeypatch.setattr(nat, "current", lambda device: nat._HERE)
+    for module, stores in ((experts, ("_GEMM", "_COMBINE", "_ROUTE")), (fp8, ("_QUANT",)), (norm, ("_PLANS",))):
+        for name in stores:
+            monkeypatch.setattr(module, name, {})
+
+
+def _calls():
+    """(what is called, its arguments, the names of those that may carry a derivative)."""
+    gemm = dict(x=_t(24, 32), w=_t(4, 40, 32), bias=_t(4, 40))
+    wide = dict(x=_t(24, 32).to(E4M3), w=_t(4, 40, 32).to(E4M3), scale_a=_t(24, dtype=F32), scale_b=_t(4, 40, dtype=F32))
+    rows = dict(y=_t(24, 32), weights=_t(12, 2, dtype=F32))
+    norms = dict(x=_t(6, 64), residual=_t(6, 64), pre=_t(64), post=_t(64), gate=_t(6, 64))
+    return [
+        ("gemm", lambda x, w, **kw: experts.gemm(x, w, PLAN, **kw), gemm, ("x", "w", "bias")),
+        ("gemm", lambda x, w, **kw: experts.gemm(x, w, PLAN, **kw), wide, ("scale_a", "scale_b")),
+        ("combine", lambda y, weights: experts.combine(y, PLAN, weights), rows, ("y", "weights")),
+        ("route", lambda logits: experts.route(logits, 2), dict(logits=_t(12, 4, dtype=F32)), ("logits",)),
+        ("fp8.quant", fp8.quant, dict(x=_t(6, 64)), ("x",)),
+        ("block_norm", block_norm, norms, tuple(norms)),
+        ("block_norm", lambda **kw: block_norm(**kw, quant="fp8"), norms, tuple(norms)),
+        ("block_norm", lambda **kw: block_norm(**kw, quant="mxfp8"), norms, tuple(norms)),
+    ]
+
+
+@pytest.mark.parametrize("at", range(8))
+@pytest.mark.parametrize("known", [False, True])
+def test_a_forward_mode_derivative_is_refused(stub, at, known):
+    call, run, given, names = _calls()[at]
+    for name in names:
+        if known:
+            run(**given)  # (a call of known layout checks too)
+        with ad.dual_level():
+            run(**given)  # (a level alone is none's business)
+            dual = dict(given, **{name: ad.make_dual(given[name], torch.ones_like(given[name]))})
+            with pytest.raises(ValueError, match=f"{call}: no forward-mode"):
+                run(**dual)
+
+
+def test_a_forward_mode_derivative_beside_gradients_is_refused(stub):
+    w = _t(4, 40, 32).requires_grad_()
+    with ad.dual_level(), pytest.raises(ValueError, match="gemm: no forward-mode"):
+        experts.gemm(ad.make_dual(_t(24, 32), _t(24, 32)), w, PLAN)
