@@ -136,7 +136,7 @@ def gemm(x, w, plan, *, gather=False, bias=None, silu_mul=False, scale_a=None, s
     the backward pass; a gathered x's gradient adds a token's rows in fp32, in order of its choices. No atomics: the
     same bits every time."""
     nat.no_tangents("experts.gemm", x, w, bias, scale_a, scale_b)
-    if _grad(x, w, bias):
+    if _grad(x, w, bias, scale_a, scale_b):
         return _gemm_grad(x, w, plan, gather, bias, silu_mul, scale_a, scale_b, out)
     return _gemm(x, w, plan, gather, bias, silu_mul, scale_a, scale_b, out, None)
 

@@ -39,6 +39,7 @@ def stub(monkeypatch):
     monkeypatch.setattr(nat, "lib", lambda: Lib())
     monkeypatch.setattr(nat, "stream_of", lambda device: 0)
     monkeypatch.setattr(nat, "current", lambda device: nat._HERE)
+    monkeypatch.setattr(nat, "empty", lambda like, shape, dtype: _t(*shape, dtype=dtype))
     for module, stores in ((experts, ("_GEMM", "_COMBINE", "_ROUTE")), (fp8, ("_QUANT",)), (norm, ("_PLANS",))):
         for name in stores:
             monkeypatch.setattr(module, name, {})
@@ -80,3 +81,25 @@ def test_a_forward_mode_derivative_beside_gradients_is_refused(stub):
     w = _t(4, 40, 32).requires_grad_()
     with ad.dual_level(), pytest.raises(ValueError, match="gemm: no forward-mode"):
         experts.gemm(ad.make_dual(_t(24, 32), _t(24, 32)), w, PLAN)
+
+
+@pytest.mark.parametrize("name", ["scale_a", "scale_b"])
+@pytest.mark.parametrize("known", [False, True])
+def test_a_gradient_of_a_scale_is_refused(stub, name, known):
+    _, run, given, _ = _calls()[1]
+    if known:
+        run(**given)
+    wants = dict(given, **{name: given[name].clone().requires_grad_()})
+    with pytest.raises(ValueError, match="quantized"):
+        run(**wants)
+    with torch.no_grad():
+        run(**wants)
+
+
+def test_a_gradient_of_a_layers_scales_is_refused(stub):
+    x, up, down = _t(12, 32), _t(4, 64, 32).to(E4M3), _t(4, 32, 32).to(E4M3)
+    scales = dict(gate_up_scale=_t(4, 64, dtype=F32), down_scale=_t(4, 32, dtype=F32))
+    for name in scales:
+        wants = dict(scales, **{name: scales[name].clone().requires_grad_()})
+        with pytest.raises(ValueError, match="quantized"):
+            experts.mlp(x, _t(12, 4, dtype=F32), 2, up, down, **wants)
