@@ -154,7 +154,8 @@ def _run(g, plan, x, residual, keep_rstd):
         rstd = nat.empty(x, (rows, 2), torch.float32)
         g.rstd = rstd.data_ptr()
     if rows:
-        nat.check(nat.lib().hkx_block_norm(ctypes.byref(g), nat.stream_of(x.device)))
+        with nat.current(x.device):
+            nat.check(nat.lib().hkx_block_norm(ctypes.byref(g), nat.stream_of(x.device)))
     return h, y, rstd
 
 
@@ -229,7 +230,8 @@ def _backward(x, residual, post, pre, gate, rstd, dh, dy, scales, need):
         if nws:
             ws = nat.workspace(x.device, nws)
             q.ws, q.ws_bytes = ws.data_ptr(), nws
-        nat.check(nat.lib().hkx_block_norm_backward(ctypes.byref(q), nat.stream_of(x.device)))
+        with nat.current(x.device):
+            nat.check(nat.lib().hkx_block_norm_backward(ctypes.byref(q), nat.stream_of(x.device)))
     if dpost is not None and tpost != post.dtype:
         dpost = dpost.to(post.dtype)
     if dpre is not None and tpre != pre.dtype:

@@ -103,3 +103,36 @@ def test_a_gradient_of_a_layers_scales_is_refused(stub):
         wants = dict(scales, **{name: scales[name].clone().requires_grad_()})
         with pytest.raises(ValueError, match="quantized"):
             experts.mlp(x, _t(12, 4, dtype=F32), 2, up, down, **wants)
+
+
+@pytest.mark.parametrize("quant", [None, "fp8"])
+def test_block_norm_is_launched_on_its_tensors_device(stub, monkeypatch, quant):
+    """The stream alone does not say which: device 0's default stream and device 1's are both 0."""
+    inside, at = [], []
+
+    class Current:
+        def __init__(self, device):
+            self.device = device
+
+        def __enter__(self):
+            inside.append(self.device)
+
+        def __exit__(self, *a):
+            inside.pop()
+
+    class Lib:
+        def __getattr__(self, name):
+            return lambda *a: at.append((name, list(inside))) or 0
+
+    monkeypatch.setattr(nat, "lib", lambda: Lib())
+    monkeypatch.setattr(nat, "current", Current)
+    x, pre = _t(6, 64), _t(64)
+    for _ in range(2):  # (and of known layout)
+        block_norm(x, x, pre=pre, quant=quant)
+    want = [("hkx_block_norm", [x.device])] * 2
+    if quant is None:
+        leaf = x.clone().requires_grad_()
+        h, y = block_norm(leaf, x, pre=pre)
+        torch.autograd.grad((h, y), leaf, (x, x))
+        want += [("hkx_block_norm", [x.device]), ("hkx_block_norm_backward", [x.device])]
+    assert [(n, d) for n, d in at if not n.endswith("workspace")] == want
