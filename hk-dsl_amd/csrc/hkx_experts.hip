@@ -322,7 +322,8 @@ struct CombineArgs {
   int32_t t, k, rows, d;
 };
 
-template <int DT, bool VEC>
+// (OT: out's type)
+template <int DT, bool VEC, int OT = DT>
 __global__ void __launch_bounds__(256) combine_kernel(const CombineArgs p) {
   const int per = (p.d + 2047) / 2048;
   const int64_t token = blockIdx.x / per;
@@ -343,7 +344,7 @@ __global__ void __launch_bounds__(256) combine_kernel(const CombineArgs p) {
   typename Cols<1, VEC>::Row o;
 #pragma unroll
   for (int i = 0; i < 8; ++i) o.v[i] = sum[i];
-  cols.template store<DT>(p.out, token * p.ldo + c0, o);
+  cols.template store<OT>(p.out, token * p.ldo + c0, o);
 }
 
 // The gradient: a workgroup a token, its k rows of dy and k dot products. A row that no slot names gets zeros (from the
@@ -660,6 +661,34 @@ int hkx_experts_combine(const void* y, int64_t ldy, int32_t dtype, const int32_t
     else hipLaunchKernelGGL((combine_kernel<decltype(dt)::value, false>), dim3((unsigned)grid), dim3(256), 0, (hipStream_t)stream, a);
     return hipGetLastError();
   }), "experts combine");
+}
+
+int hkx_experts_gather_grad(const float* dr, int64_t lddr, const int32_t* slots, void* dx, int64_t lddx, int32_t t, int32_t k,
+                            int32_t rows, int32_t d, void* stream) {
+  using namespace hkx;
+  api_clear();
+  if (!dr || !slots || !dx) return api_fail(HKX_ERR_ARG, "experts_gather_grad: a null pointer");
+  if (t < 0 || k < 1 || rows < 0 || d < 1 || lddr < d || lddx < d)
+    return api_fail(HKX_ERR_SHAPE, "experts_gather_grad: t=%d k=%d rows=%d d=%d", t, k, rows, d);
+  if (!api_aligned(dr, 4) || !api_aligned(dx, 2)) return api_fail(HKX_ERR_SHAPE, "experts_gather_grad: the operands need their elements' alignment");
+  if (t == 0) return HKX_OK;
+  const int64_t grid = (int64_t)t * ((d + 2047) / 2048);
+  if (grid >= 1 << 24) return api_fail(HKX_ERR_SHAPE, "experts_gather_grad: t=%d of d=%d are more than a launch takes; split the call", t, d);
+  CombineArgs a{};
+  a.y = dr;
+  a.slots = slots;
+  a.out = dx;
+  a.ldy = lddr;
+  a.ldo = lddx;
+  a.t = t;
+  a.k = k;
+  a.rows = rows;
+  a.d = d;
+  if (d % 8 == 0 && whole(dr, lddr, HKX_FP32) && whole(dx, lddx, HKX_BF16))
+    hipLaunchKernelGGL((combine_kernel<HKX_FP32, true, HKX_BF16>), dim3((unsigned)grid), dim3(256), 0, (hipStream_t)stream, a);
+  else
+    hipLaunchKernelGGL((combine_kernel<HKX_FP32, false, HKX_BF16>), dim3((unsigned)grid), dim3(256), 0, (hipStream_t)stream, a);
+  return api_launched(hipGetLastError(), "experts gather grad");
 }
 
 int hkx_experts_combine_backward(const void* y, int64_t ldy, const void* dout, int64_t lddo, int32_t dtype, const int32_t* slots,

@@ -101,6 +101,8 @@ int gemm_args(const HkxExpertsGemmArgs& g, GroupArgs& a) {
   if (!nt && !tn && g.op != HKX_EXPERTS_NN) return api_fail(HKX_ERR_ARG, "experts_gemm: op %d", g.op);
   if (!fp8 && g.ab_dtype != HKX_BF16) return api_fail(HKX_ERR_DTYPE, "experts_gemm: operands are bf16 or e4m3");
   if (fp8 && !nt) return api_fail(HKX_ERR_DTYPE, "experts_gemm: no gradient of e4m3 operands");
+  if (g.c_dtype != HKX_BF16 && (g.c_dtype != HKX_FP32 || g.op != HKX_EXPERTS_NN))
+    return api_fail(HKX_ERR_DTYPE, "experts_gemm: C is bf16, or fp32 where op is NN");
   if (!g.a || !g.b || !g.c || !g.offsets || (fp8 && (!g.sa || !g.sb))) return api_fail(HKX_ERR_ARG, "experts_gemm: a null pointer");
   if (g.experts < 1 || g.experts > kMaxExperts || g.rows < 0 || g.n < 1 || (tn ? g.m < 1 : g.k < 1))
     return api_fail(HKX_ERR_SHAPE, "experts_gemm: experts=%d (at most %d) rows=%d m=%d n=%d k=%d", g.experts, kMaxExperts, g.rows,
@@ -109,7 +111,7 @@ int gemm_args(const HkxExpertsGemmArgs& g, GroupArgs& a) {
   if (g.z && !g.silu_mul) return api_fail(HKX_ERR_ARG, "experts_gemm: z goes with silu_mul");
   if (g.bias && !floating(g.bias_dtype)) return api_fail(HKX_ERR_DTYPE, "experts_gemm: the bias is bf16, fp16 or fp32");
   if (g.index && g.a_rows < 1) return api_fail(HKX_ERR_SHAPE, "experts_gemm: an index into %d rows", g.a_rows);
-  const int64_t es = fp8 ? 1 : 2, step = fp8 ? 16 : 8, brows = nt ? (g.silu_mul ? 2 * (int64_t)g.n : g.n) : g.k;
+  const int64_t es = fp8 ? 1 : 2, ces = g.c_dtype == HKX_FP32 ? 4 : 2, step = fp8 ? 16 : 8, brows = nt ? (g.silu_mul ? 2 * (int64_t)g.n : g.n) : g.k;
   if (g.n % 8 || (tn ? g.m % 8 : g.k % step) || brows > INT32_MAX)
     return api_fail(HKX_ERR_SHAPE, "experts_gemm: m=%d n=%d k=%d: multiples of 8, an e4m3 k of 16", g.m, g.n, g.k);
   const int64_t acols = tn ? g.m : g.k, bcols = nt ? g.k : g.n;
@@ -117,14 +119,14 @@ int gemm_args(const HkxExpertsGemmArgs& g, GroupArgs& a) {
     return api_fail(HKX_ERR_SHAPE, "experts_gemm: row strides below a row");
   if (g.lda % step || g.ldb % step || (!tn && g.b_expert % step) || !api_aligned(g.a, 16) || !api_aligned(g.b, 16))
     return api_fail(HKX_ERR_SHAPE, "experts_gemm: A's and B's rows and experts need 16-byte alignment");
-  if (g.ldc % 4 || !api_aligned(g.c, 8) || (tn && g.c_expert % 4) || (g.z && (g.ldz % 4 || !api_aligned(g.z, 8))))
-    return api_fail(HKX_ERR_SHAPE, "experts_gemm: C's and z's rows need 8-byte alignment");
+  if (g.ldc % 4 || !api_aligned(g.c, 4 * ces) || (tn && g.c_expert % 4) || (g.z && (g.ldz % 4 || !api_aligned(g.z, 8))))
+    return api_fail(HKX_ERR_SHAPE, "experts_gemm: C's and z's rows need 8-byte alignment, an fp32 C's 16");
   if (g.bias && (!api_aligned(g.bias, 16) || g.bias_ld % 4)) return api_fail(HKX_ERR_SHAPE, "experts_gemm: the bias needs 16-byte aligned rows");
   if (fp8 && (!api_aligned(g.sa, 4) || !api_aligned(g.sb, g.sb_col ? 16 : 4) || (g.sb_col && g.sb_ld % 4)))
     return api_fail(HKX_ERR_SHAPE, "experts_gemm: the scales' alignment");
   // offsets in a tile, in an expert of B, and in an A that an index picks from are 32-bit
   const int64_t lim = ((int64_t)1 << 32) - 4096;
-  if (256 * g.lda * es > lim || 256 * g.ldc * 2 > lim || 256 * g.ldz * 2 > lim || (nt ? brows : 256) * g.ldb * es > lim || (g.index && g.a_rows * g.lda * es > lim))
+  if (256 * g.lda * es > lim || 256 * g.ldc * ces > lim || 256 * g.ldz * 2 > lim || (nt ? brows : 256) * g.ldb * es > lim || (g.index && g.a_rows * g.lda * es > lim))
     return api_fail(HKX_ERR_SHAPE, "experts_gemm: an expert's B or an indexed A spans 4 GiB or more; split the call");
   if (g.kernel < 0 || g.kernel > HKX_EXPERTS_SKINNY32) return api_fail(HKX_ERR_ARG, "experts_gemm: kernel %d", g.kernel);
   a.a = (const uint8_t*)g.a;
@@ -138,7 +140,7 @@ int gemm_args(const HkxExpertsGemmArgs& g, GroupArgs& a) {
   a.sb = g.sb;
   a.lda = g.lda * es;
   a.ldb = g.ldb * es;
-  a.ldc = g.ldc * 2;
+  a.ldc = g.ldc * ces;
   a.ldz = g.ldz * 2;
   a.b_group = g.b_expert * es;
   a.c_group = g.c_expert * 2;
@@ -154,6 +156,7 @@ int gemm_args(const HkxExpertsGemmArgs& g, GroupArgs& a) {
   a.bias_dt = g.bias_dtype;
   a.sa_ld = g.sa_ld != 0;
   a.sb_col = g.sb_col != 0;
+  a.c_f32 = g.c_dtype == HKX_FP32;
   if (g.kernel == HKX_EXPERTS_QUAD && !group_quad_ok(a))
     return api_fail(HKX_ERR_SHAPE, "experts_gemm: the 256-row kernel stores 16-byte aligned rows");
   return HKX_OK;

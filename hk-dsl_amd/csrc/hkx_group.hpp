@@ -42,6 +42,7 @@ struct GroupArgs {
   int32_t m, n, k;   // m: TN's rows of C; n: C's columns (paired: of silu(gate) up); k: NT's and NN's contraction
   int32_t tail;      // 1: the rows behind the last group are written too, with zeros
   int32_t bias_dt, sa_ld, sb_col;
+  int32_t c_f32;     // NN: C is fp32
 };
 
 // ---------------------------------------------------------------- which tile is whose
@@ -186,7 +187,7 @@ HKX_DEV void group_store(const GroupArgs& p, int e, bool rest, uint8_t* c, uint8
     }
     v = silu_mul4(v, u);
   }
-  store4(c, HKX_BF16, n, v);
+  store4(c, !NT && p.c_f32 ? HKX_FP32 : HKX_BF16, n, v);
 }
 
 // ---------------------------------------------------------------- fragments in LDS

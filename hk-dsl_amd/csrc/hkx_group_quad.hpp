@@ -396,7 +396,7 @@ __global__ void __launch_bounds__(512, 1) group_quad_kernel(const GroupArgs p) {
     }
     const uint8_t* ev = vecs + (lt % 3) * 4096;
     const int64_t row0 = TA ? t.m0 : t.row0;
-    const __amdgpu_buffer_rsrc_t rc = make_rsrc(p.c + (TA ? t.e * p.c_group : 0) + row0 * p.ldc, rows_bytes(t.rows, p.ldc, (uint32_t)p.n * 2u));
+    const __amdgpu_buffer_rsrc_t rc = make_rsrc(p.c + (TA ? t.e * p.c_group : 0) + row0 * p.ldc, rows_bytes(t.rows, p.ldc, (uint32_t)p.n * (OP == kGroupNN && p.c_f32 ? 4u : 2u)));
     auto store = [&](const __amdgpu_buffer_rsrc_t& r, i32x4 v, int n, uint32_t off) {
       if (n < p.n) __builtin_amdgcn_raw_buffer_store_b128(v, r, off, 0, 0);
     };
@@ -444,6 +444,20 @@ __global__ void __launch_bounds__(512, 1) group_quad_kernel(const GroupArgs p) {
       swap16(y0, y1);
       return i32x4{(int)x0, (int)y0, (int)x1, (int)y1};
     };
+    if (OP == kGroupNN && p.c_f32) {  // (16 bytes a lane as they are)
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+          for (int f = 0; f < 4; ++f)
+#pragma unroll
+            for (int g = 0; g < 2; ++g) {
+              const int n = t.n0 + 128 * j + 32 * wc + 16 * g + 4 * q, m = 128 * i + 64 * grp + 16 * f + rf;
+              store(rc, __builtin_bit_cast(i32x4, acc[i][j][f][g]), n, (uint32_t)m * (uint32_t)p.ldc + (uint32_t)n * 4u);
+            }
+      return;
+    }
     auto stores = [&](auto biased) __attribute__((always_inline)) {
 #pragma unroll
       for (int i = 0; i < 2; ++i)

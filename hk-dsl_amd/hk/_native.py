@@ -111,7 +111,7 @@ class HkxExpertsGemmArgs(Structure):
                 ("rows", c_int32), ("a_rows", c_int32), ("m", c_int32), ("n", c_int32),
                 ("k", c_int32), ("silu_mul", c_int32), ("zero_rest", c_int32),
                 ("bias_dtype", c_int32), ("sa_ld", c_int32), ("sb_col", c_int32),
-                ("kernel", c_int32), ("reserved", c_int32), ("a", c_void_p), ("b", c_void_p),
+                ("kernel", c_int32), ("c_dtype", c_int32), ("a", c_void_p), ("b", c_void_p),
                 ("c", c_void_p), ("z", c_void_p), ("offsets", c_void_p), ("index", c_void_p),
                 ("bias", c_void_p), ("sa", c_void_p), ("sb", c_void_p), ("lda", c_int64),
                 ("ldb", c_int64), ("ldc", c_int64), ("ldz", c_int64), ("b_expert", c_int64),
@@ -134,7 +134,7 @@ SYMBOLS = ("hkx_abi_version", "hkx_abi_sizes", "hkx_last_error", "hkx_gemm_works
            "hkx_mx4_gemm_workspace", "hkx_block_norm", "hkx_block_norm_backward",
            "hkx_block_norm_backward_workspace", "hkx_experts_gemm", "hkx_experts_gemm_workspace",
            "hkx_experts_silu_grad",
-           "hkx_experts_bias_grad", "hkx_experts_gather", "hkx_experts_route",
+           "hkx_experts_bias_grad", "hkx_experts_gather", "hkx_experts_gather_grad", "hkx_experts_route",
            "hkx_experts_route_workspace", "hkx_experts_route_backward", "hkx_experts_combine",
            "hkx_experts_combine_backward", "hkx_fp8_quant")
 
@@ -209,6 +209,8 @@ def lib() -> ctypes.CDLL:
                                             c_int32, c_int32, c_void_p]
         L.hkx_experts_gather.argtypes = [c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_int32,
                                          c_int32, c_int32, c_void_p]
+        L.hkx_experts_gather_grad.argtypes = [c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_int32,
+                                              c_int32, c_int32, c_int32, c_void_p]
         L.hkx_experts_route.argtypes = [POINTER(HkxExpertsRouteArgs), c_void_p]
         L.hkx_experts_route_workspace.argtypes = [POINTER(HkxExpertsRouteArgs)]
         L.hkx_experts_route_workspace.restype = c_size_t

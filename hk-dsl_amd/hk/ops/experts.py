@@ -132,9 +132,9 @@ def gemm(x, w, plan, *, gather=False, bias=None, silu_mul=False, scale_a=None, s
     * out: bf16 (R, N) to write into (no gradient), columns next to each other.
 
     K and N multiples of 8, an 8-bit K of 16; E up to 1024; an expert's w, and an x that is gathered, under 4 GiB.
-    Sums are fp32, rounded once. Differentiable in x, w and bias (bf16): with silu_mul z is kept in bf16 for
-    the backward pass; a gathered x's gradient adds a token's rows in fp32, in order of its choices. No atomics: the
-    same bits every time."""
+    Sums are fp32, rounded once. Differentiable in x, w and bias (bf16): with silu_mul z is kept in bf16 for the backward
+    pass and its gradient, which the other products read, rounded to bf16; a gathered x's gradient adds a token's rows,
+    which stay fp32 till then, in order of its choices. No atomics: the same bits every time."""
     nat.no_tangents("experts.gemm", x, w, bias, scale_a, scale_b)
     if _grad(x, w, bias, scale_a, scale_b):
         return _gemm_grad(x, w, plan, gather, bias, silu_mul, scale_a, scale_b, out)
@@ -291,9 +291,10 @@ def _gemm_checked(x, w, plan, gather, bias, silu_mul, scale_a, scale_b, out, z, 
 
 
 def _product(op, a, b, plan, out):
-    """A gradient's product into `out`: NN dx (R, K) = dz (R, N) . w (E, N, K), TN dw (E, N, K) = dz^T x."""
+    """A gradient's product into `out`: NN dx (R, K) = dz (R, N) . w (E, N, K), bf16 or fp32, TN dw (E, N, K) = dz^T x."""
     g = nat.HkxExpertsGemmArgs()
     g.size, g.op, g.ab_dtype = ctypes.sizeof(g), op, nat.BF16
+    g.c_dtype = nat.dtype_code(out.dtype)
     g.experts, g.rows, g.n, g.zero_rest = plan.offsets.shape[0] - 1, a.shape[0], out.shape[-1], 1
     g.a, g.b, g.c, g.offsets = a.data_ptr(), b.data_ptr(), out.data_ptr(), plan.offsets.data_ptr()
     g.lda = _ld(a, a.shape[1])
@@ -323,9 +324,9 @@ def _gemm_grad(x, w, plan, gather, bias, silu_mul, scale_a, scale_b, out):
 
 
 def _gemm_backward(x, w, bias, z, plan, gather, need, dy):
-    """(dx, dw, dbias). Rounded to bf16 on the way: z (kept in bf16), dz (the products read bf16) and a gathered row's
-    gradient before its token's rows are added; fp32 in their place would double the traffic of the passes between the
-    products, and bf16 in separate calls has the same three."""
+    """(dx, dw, dbias). Rounded to bf16 on the way: dz, as the products read bf16, and z, kept in bf16 (fp32 would double
+    its write and its read, for an error of the size of dz's). A gathered row's gradient stays fp32 until its token's rows
+    are added, which may cancel."""
     import torch  # noqa: PLC0415
 
     r, e = dy.shape[0], w.shape[0]
@@ -341,11 +342,11 @@ def _gemm_backward(x, w, bias, z, plan, gather, need, dy):
                                                   plan.offsets.data_ptr(), e, r, rows16.shape[1], nat.stream_of(dev)))
     dx = dw = db = None
     if need[0]:
-        dx = nat.empty(x, (r, w.shape[2]), torch.bfloat16)
+        dx = nat.empty(x, (r, w.shape[2]), torch.float32 if gather else torch.bfloat16)
         if r:
             _product(NN, dz, _experts16(w), plan, dx)
         if gather:
-            dx = _combine(dx, plan.slots, None)
+            dx = _gather_backward(x, dx, plan.slots)
     if need[1]:
         dw = nat.empty(x, w.shape, torch.bfloat16)
         xr = _rows16(x)
@@ -370,6 +371,18 @@ def _gemm_backward(x, w, bias, z, plan, gather, need, dy):
         else:
             db.zero_()
     return dx, dw, db
+
+
+def _gather_backward(x, dr, slots):
+    """bf16 (T, K) from the rows' dr (R, K) fp32."""
+    t, k = slots.shape
+    dx = nat.empty(x, (t, dr.shape[1]), x.dtype)
+    if t == 0 or k == 0 or dr.shape[0] == 0:
+        return dx.zero_()
+    with nat.current(x.device):
+        nat.check(nat.lib().hkx_experts_gather_grad(dr.data_ptr(), dr.shape[1], slots.data_ptr(), dx.data_ptr(), dr.shape[1],
+                                                    t, k, dr.shape[0], dr.shape[1], nat.stream_of(x.device)))
+    return dx
 
 
 # ---------------------------------------------------------------- the way back

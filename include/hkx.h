@@ -446,10 +446,10 @@ typedef struct {
   int32_t zero_rest; /* NT, NN: C's rows behind the last group are zeroed, otherwise left */
   int32_t bias_dtype, sa_ld, sb_col; /* sa_ld: 1 a scale a row of A, 0 one; sb_col: 1 a scale a row of B, 0 one an expert */
   int32_t kernel;                    /* HKX_EXPERTS_AUTO, or the kernel to run (tuning, tests) */
-  int32_t reserved;
+  int32_t c_dtype;                   /* HKX_BF16; NN: or HKX_FP32 */
   const void* a;
   const void* b;
-  void* c; /* bf16 */
+  void* c;
   void* z; /* NT with silu_mul: the 2 n columns before it, bf16 (NULL: not kept) */
   const int32_t* offsets;
   const int32_t* index; /* NT: each row's row of A (NULL: its own) */
@@ -469,8 +469,9 @@ typedef struct {
 #define HKX_EXPERTS_QUAD 4 /* 256 x 256 tiles, 8 waves, persistent; C, z and the bias in 16-byte aligned rows */
 #define HKX_EXPERTS_SKINNY16 5 /* the decode kernel, 16 or 32 rows (NT; a gradient goes by its size) */
 #define HKX_EXPERTS_SKINNY32 6
-/* bf16 C from bf16 or fp8 operands, sums in fp32, rounded once. n and k multiples of 8 (m too; an fp8 k of 16), rows
- * and experts of A and B 16-byte aligned, of C, z and the bias 8-byte, scales (a row of B each) 16-byte. */
+/* C from bf16 or fp8 operands, sums in fp32, rounded once to bf16 or, in NN with an fp32 C, kept. n and k multiples of 8 (m too; an fp8 k of 16), rows
+ * and experts of A and B 16-byte aligned, of C and z 8-byte (an fp32 C 16-byte), of the bias and scales (a row of B
+ * each) 16-byte. */
 int hkx_experts_gemm(const HkxExpertsGemmArgs* args, void* stream);
 /* (goes by every size, stride and address, so these are set first) */
 size_t hkx_experts_gemm_workspace(const HkxExpertsGemmArgs* args);
@@ -487,6 +488,11 @@ int hkx_experts_bias_grad(const void* dz, int64_t lddz, const int32_t* offsets, 
 /* out[r] = x[index[r]] (a_rows rows of k bf16; zeros where index is out of range). */
 int hkx_experts_gather(const void* x, int64_t ldx, const int32_t* index, void* out, int64_t ldo, int32_t rows,
                        int32_t a_rows, int32_t k, void* stream);
+
+/* The gradient of x from that of its rows: dx[i] (bf16) = the sum over j of dr[slots[i, j]] (fp32; a slot outside dr's
+ * `rows`: nothing), in fp32, in order of j, rounded once. */
+int hkx_experts_gather_grad(const float* dr, int64_t lddr, const int32_t* slots, void* dx, int64_t lddx, int32_t t,
+                            int32_t k, int32_t rows, int32_t d, void* stream);
 
 /* The k largest of each token's logits (t, e), a tie to the lower expert, NaN above all, -inf never chosen:
  * chosen (t, k) int32 in falling order (-1: none left) and weights (t, k) fp32, their softmax over the token's

@@ -1,0 +1,36 @@
+"""Calls of hk.ops.experts on the GPU beside those of test_experts_gpu.py, with its tolerances: a bf16 result is within
+half a step (2^-8 of it) of an fp32 sum, which is within 2^-23 a term of the terms' magnitudes."""
+
+import pytest
+import torch
+
+from hk.ops import experts
+from test_experts_gpu import BF16, DEV, _plan, kernel  # noqa: F401
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("t,e,k,n,d,dead", [(9, 4, 2, 40, 24, 1), (150, 6, 4, 136, 200, 9), (700, 8, 8, 128, 64, 33),
+                                            (3000, 4, 4, 264, 520, 0), (600, 2, 2, 2824, 264, 5)])
+def test_a_gathered_rows_gradient_is_rounded_once(t, e, k, n, d, dead, kernel):  # noqa: F811
+    """Experts that nearly cancel: a token's rows are large, their sum is not, and what each row lost would show."""
+    plan, (offsets, rows, slots) = _plan(t, e, k, seed=t, dead=dead)
+    g = torch.Generator().manual_seed(n)
+    x = torch.randn(t, d, generator=g).to(BF16)
+    sign = 1.0 - 2.0 * (torch.arange(e) % 2).reshape(e, 1, 1)
+    w = (sign * torch.randn(1, n, d, generator=g) + 0.01 * torch.randn(e, n, d, generator=g)).to(BF16)
+    v = torch.randn(t, n, generator=g).to(BF16)
+    dy = torch.where((rows >= 0).unsqueeze(1), v[rows.clamp(min=0)], torch.zeros((), dtype=BF16))
+    leaf = x.to(DEV).requires_grad_()
+    y = experts.gemm(leaf, w.to(DEV), plan, gather=True)
+    (dx,) = torch.autograd.grad(y, leaf, dy.to(DEV))
+    assert dx.dtype == BF16 and dx.shape == x.shape
+    ref, mag = torch.zeros(t, d, dtype=torch.float64, device=DEV), torch.zeros(t, d, dtype=torch.float64, device=DEV)
+    off, wd, dyd = offsets.tolist(), w.to(DEV).double(), dy.to(DEV).double()
+    for i in range(e):
+        a, to = dyd[off[i]:off[i + 1]], rows[off[i]:off[i + 1]].to(DEV)
+        ref.index_add_(0, to, a @ wd[i])
+        mag.index_add_(0, to, a.abs() @ wd[i].abs())
+    # (the sums of a row, and then of k rows; the one rounding)
+    err = (n + 2 + k) * 2.0 ** -23 * mag
+    assert ((dx.double() - ref).abs() <= err + 2.0 ** -8 * (ref.abs() + err)).all()
