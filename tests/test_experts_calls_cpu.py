@@ -136,3 +136,19 @@ def test_block_norm_is_launched_on_its_tensors_device(stub, monkeypatch, quant):
         torch.autograd.grad((h, y), leaf, (x, x))
         want += [("hkx_block_norm", [x.device]), ("hkx_block_norm_backward", [x.device])]
     assert [(n, d) for n, d in at if not n.endswith("workspace")] == want
+
+
+def test_tokens_whose_plan_has_no_rows_have_a_gradient_of_zeros(stub, monkeypatch):
+    """Every choice dropped: no rows, and slots of -1. Nothing is launched (the library refuses a null address)."""
+
+    class Lib:
+        def __getattr__(self, name):
+            raise AssertionError(f"{name} of no rows")
+
+    monkeypatch.setattr(nat, "lib", lambda: Lib())
+    x, w = _t(12, 32).requires_grad_(), _t(4, 40, 32).requires_grad_()
+    slots = torch.full((12, 2), -1, dtype=torch.int32).as_subclass(OnGpu)
+    y = experts.gemm(x, w, experts.Plan(PLAN.offsets, _t(0, dtype=torch.int32), slots), gather=True)
+    assert y.shape == (0, 40)
+    dx, dw = torch.autograd.grad(y, (x, w), _t(0, 40))
+    assert dx.shape == (12, 32) and dw.shape == (4, 40, 32) and not dx.any() and not dw.any()
