@@ -12,7 +12,7 @@ hipError_t launch_group_grad(const GroupArgs& a, int op, int bm, hipStream_t s) 
 
 hipError_t launch_group(const GroupArgs& a, int op, bool fp8, bool pair, int kernel, int cus, hipStream_t s) {
   if (kernel == kGroupQuad) return op == kGroupNT ? launch_group_quad_nt(a, fp8, pair, cus, s) : launch_group_quad_grad(a, op, cus, s);
-  if (kernel >= kGroupSkinny16) return launch_group_skinny(a, fp8, pair, kernel == kGroupSkinny16 ? 16 : 32, cus, s);
+  if (kernel >= kGroupSkinny16) return launch_group_skinny(a, fp8, pair, kernel == kGroupSkinny16 ? 16 : 32, s);
   const int bm = kernel == kGroupTile16 ? 16 : kernel == kGroupTile64 ? 64 : 128;
   return op == kGroupNT ? launch_group_nt(a, fp8, pair, bm, s) : launch_group_grad(a, op, bm, s);
 }

@@ -15,7 +15,7 @@ hipError_t launch_group_nt(const GroupArgs& a, bool fp8, bool pair, int bm, hipS
 hipError_t launch_group_grad(const GroupArgs& a, int op, int bm, hipStream_t s);
 
 // the decode kernel, bm 16 or 32 rows
-hipError_t launch_group_skinny(const GroupArgs& a, bool fp8, bool pair, int bm, int cus, hipStream_t s);
+hipError_t launch_group_skinny(const GroupArgs& a, bool fp8, bool pair, int bm, hipStream_t s);
 // 256 x 256 tiles, at most `cus` workgroups
 hipError_t launch_group_quad_nt(const GroupArgs& a, bool fp8, bool pair, int cus, hipStream_t s);
 hipError_t launch_group_quad_grad(const GroupArgs& a, int op, int cus, hipStream_t s);
