@@ -93,6 +93,9 @@ __global__ void __launch_bounds__(256) gather_kernel(const uint8_t* x, int64_t l
   *(i32x4*)(out + r * ldo + c) = v;
 }
 
+// A group's rows are counted in tiles by ints: rows + 255 is one.
+constexpr int32_t kMostRows = INT32_MAX - 255;
+
 bool floating(int dt) { return dt == HKX_BF16 || dt == HKX_FP16 || dt == HKX_FP32; }
 
 // What a call asks for, refused where the kernels do not take it; the kernels' arguments.
@@ -104,7 +107,7 @@ int gemm_args(const HkxExpertsGemmArgs& g, GroupArgs& a) {
   if (g.c_dtype != HKX_BF16 && (g.c_dtype != HKX_FP32 || g.op != HKX_EXPERTS_NN))
     return api_fail(HKX_ERR_DTYPE, "experts_gemm: C is bf16, or fp32 where op is NN");
   if (!g.a || !g.b || !g.c || !g.offsets || (fp8 && (!g.sa || !g.sb))) return api_fail(HKX_ERR_ARG, "experts_gemm: a null pointer");
-  if (g.experts < 1 || g.experts > kMaxExperts || g.rows < 0 || g.n < 1 || (tn ? g.m < 1 : g.k < 1))
+  if (g.experts < 1 || g.experts > kMaxExperts || g.rows < 0 || g.rows > kMostRows || g.n < 1 || (tn ? g.m < 1 : g.k < 1))
     return api_fail(HKX_ERR_SHAPE, "experts_gemm: experts=%d (at most %d) rows=%d m=%d n=%d k=%d", g.experts, kMaxExperts, g.rows,
                     g.m, g.n, g.k);
   if (!nt && (g.silu_mul || g.z || g.index || g.bias)) return api_fail(HKX_ERR_ARG, "experts_gemm: silu_mul, z, index and bias go with NT");
@@ -226,7 +229,7 @@ int hkx_experts_bias_grad(const void* dz, int64_t lddz, const int32_t* offsets, 
   api_clear();
   if (!dz || !offsets || !db) return api_fail(HKX_ERR_ARG, "experts_bias_grad: a null pointer");
   if (!floating(db_dtype)) return api_fail(HKX_ERR_DTYPE, "experts_bias_grad: db is bf16, fp16 or fp32");
-  if (experts < 1 || experts > kMaxExperts || rows < 0 || n < 1 || n % 8 || lddz < n || lddz % 2 || !api_aligned(dz, 4))
+  if (experts < 1 || experts > kMaxExperts || rows < 0 || rows > kMostRows || n < 1 || n % 8 || lddz < n || lddz % 2 || !api_aligned(dz, 4))
     return api_fail(HKX_ERR_SHAPE, "experts_bias_grad: experts=%d rows=%d n=%d", experts, rows, n);
   hipLaunchKernelGGL(bias_grad_kernel, dim3((n + 127) / 128, experts), dim3(1024), 0, (hipStream_t)stream,
                      (const uint8_t*)dz, lddz * 2, offsets, db, db_dtype, rows, n);

@@ -430,7 +430,8 @@ size_t hkx_block_norm_backward_workspace(const HkxBlockNormGradArgs* args);
  * R rows stand in the order of their experts: rows offsets[e] .. offsets[e + 1] are expert e's (offsets of
  * experts + 1 int32 on the GPU, from 0, at most rows), those behind offsets[experts] are nobody's. A host need not
  * know them: grids are sized for any. Offsets out of order or past the rows are clamped, an index out of range reads
- * zeros: nothing outside the operands is touched. At most 1024 experts. */
+ * zeros: nothing outside the operands is touched. At most 1024 experts and 2^31 - 256
+ * rows. */
 
 #define HKX_EXPERTS_NT 0 /* C[r] = A[r or index[r]] . B_e^T, B_e (n, k) */
 #define HKX_EXPERTS_NN 1 /* C[r] = A[r] . B_e, B_e (k, n) */

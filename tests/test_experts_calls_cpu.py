@@ -1,6 +1,7 @@
 """Derivatives that hk.ops.experts, hk.ops.fp8 and hk.ops.block_norm do not take are refused, not dropped (no GPU: the
 library is a stub that launches nothing)."""
 
+import ctypes
 import types
 
 import pytest
@@ -152,3 +153,22 @@ def test_tokens_whose_plan_has_no_rows_have_a_gradient_of_zeros(stub, monkeypatc
     assert y.shape == (0, 40)
     dx, dw = torch.autograd.grad(y, (x, w), _t(0, 40))
     assert dx.shape == (12, 32) and dw.shape == (4, 40, 32) and not dx.any() and not dw.any()
+
+
+def test_rows_whose_tiles_an_int_does_not_count_are_refused():
+    """A group of rows is counted in tiles of up to 256: rows + 255 is an int too."""
+    L, at = nat.lib(), 1 << 20
+    most = 2 ** 31 - 1 - 255
+    for op, sizes in ((experts.NT, dict(k=8)), (experts.NN, dict(k=8)), (experts.TN, dict(m=8))):
+        g = nat.HkxExpertsGemmArgs()
+        g.size, g.op, g.ab_dtype, g.experts, g.n, g.kernel = ctypes.sizeof(g), op, nat.BF16, 2, 8, 4
+        g.a = g.b = g.c = g.offsets = at
+        g.lda = g.ldb = g.ldc = 8
+        g.b_expert = g.c_expert = 64
+        for name, v in sizes.items():
+            setattr(g, name, v)
+        for rows in (most + 1, 2 ** 31 - 1):
+            g.rows = rows
+            assert L.hkx_experts_gemm(ctypes.byref(g), None) == nat.ERR_SHAPE and "rows" in nat.last_error()
+    for rows in (most + 1, 2 ** 31 - 1):
+        assert L.hkx_experts_bias_grad(at, 8, at, at, nat.BF16, 2, rows, 8, None) == nat.ERR_SHAPE
