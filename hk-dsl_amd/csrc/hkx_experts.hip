@@ -625,12 +625,18 @@ int hkx_experts_route_backward(const void* logits, int64_t ld, int32_t dtype, co
   api_clear();
   if (!logits || !weights || !chosen || !dweights || !dlogits) return api_fail(HKX_ERR_ARG, "experts_route_backward: a null pointer");
   if (!floating(dtype)) return api_fail(HKX_ERR_DTYPE, "experts_route_backward: logits are bf16, fp16 or fp32");
-  if (t < 1 || e < 1 || e > kMaxRouted || k < 1 || k > kMaxChosen || k > e || ld < e || lddl < e || t >= 1 << 26)
+  if (t < 1 || e < 1 || e > kMaxRouted || k < 1 || k > kMaxChosen || k > e || ld < e || lddl < e)
     return api_fail(HKX_ERR_SHAPE, "experts_route_backward: t=%d e=%d k=%d", t, e, k);
-  const RouteGradArgs a{logits, ld, weights, chosen, dweights, dlogits, lddl, dtype, t, e, k, renormalize != 0};
   return api_launched(by_lane(e, [&](auto j) {
-    hipLaunchKernelGGL((route_grad_kernel<decltype(j)::value>), dim3((t + 3) / 4), dim3(256), 0, (hipStream_t)stream, a);
-    return hipGetLastError();
+    constexpr int64_t most = 1 << 25;  // tokens a launch: under 2^32 threads
+    for (int64_t i = 0; i < t; i += most) {
+      const int n = (int)std::min(most, t - i);
+      const RouteGradArgs a{(const uint8_t*)logits + i * ld * es(dtype), ld, weights + i * k, chosen + i * k, dweights + i * k,
+                            (uint8_t*)dlogits + i * lddl * es(dtype), lddl, dtype, n, e, k, renormalize != 0};
+      hipLaunchKernelGGL((route_grad_kernel<decltype(j)::value>), dim3((n + 3) / 4), dim3(256), 0, (hipStream_t)stream, a);
+      if (hipError_t rc = hipGetLastError()) return rc;
+    }
+    return hipSuccess;
   }), "experts route backward");
 }
 

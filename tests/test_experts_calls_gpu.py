@@ -34,3 +34,22 @@ def test_a_gathered_rows_gradient_is_rounded_once(t, e, k, n, d, dead, kernel): 
     # (the sums of a row, and then of k rows; the one rounding)
     err = (n + 2 + k) * 2.0 ** -23 * mag
     assert ((dx.double() - ref).abs() <= err + 2.0 ** -8 * (ref.abs() + err)).all()
+
+
+def test_the_routers_gradient_past_a_launch():
+    """More tokens than one launch takes: those at the seams have the gradients that they have by themselves."""
+    t, e = (1 << 26) + 5, 2
+    g = torch.Generator(device=DEV).manual_seed(3)
+    block = torch.randn(1 << 16, e, generator=g, device=DEV).to(BF16)
+    logits = torch.empty(t, e, dtype=BF16, device=DEV)
+    dw = torch.empty(t, 1, device=DEV)
+    for at in range(0, t, 1 << 16):
+        n = min(1 << 16, t - at)
+        logits[at:at + n] = block[:n]
+        dw[at:at + n] = block[:n, :1].float() + at / t
+    logits.requires_grad_()
+    (got,) = torch.autograd.grad(experts.route(logits, 1, renormalize=False)[0], logits, dw)
+    for at in (0, (1 << 25) - 7, (1 << 26) - 7, t - 11):
+        part = logits.detach()[at:at + 11].clone().requires_grad_()
+        (want,) = torch.autograd.grad(experts.route(part, 1, renormalize=False)[0], part, dw[at:at + 11].clone())
+        assert torch.equal(got[at:at + 11], want) and want.any()
