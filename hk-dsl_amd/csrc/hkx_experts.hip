@@ -678,23 +678,25 @@ int hkx_experts_gather_grad(const float* dr, int64_t lddr, const int32_t* slots,
     return api_fail(HKX_ERR_SHAPE, "experts_gather_grad: t=%d k=%d rows=%d d=%d", t, k, rows, d);
   if (!api_aligned(dr, 4) || !api_aligned(dx, 2)) return api_fail(HKX_ERR_SHAPE, "experts_gather_grad: the operands need their elements' alignment");
   if (t == 0) return HKX_OK;
-  const int64_t grid = (int64_t)t * ((d + 2047) / 2048);
-  if (grid >= 1 << 24) return api_fail(HKX_ERR_SHAPE, "experts_gather_grad: t=%d of d=%d are more than a launch takes; split the call", t, d);
   CombineArgs a{};
   a.y = dr;
-  a.slots = slots;
-  a.out = dx;
   a.ldy = lddr;
   a.ldo = lddx;
-  a.t = t;
   a.k = k;
   a.rows = rows;
   a.d = d;
-  if (d % 8 == 0 && whole(dr, lddr, HKX_FP32) && whole(dx, lddx, HKX_BF16))
-    hipLaunchKernelGGL((combine_kernel<HKX_FP32, true, HKX_BF16>), dim3((unsigned)grid), dim3(256), 0, (hipStream_t)stream, a);
-  else
-    hipLaunchKernelGGL((combine_kernel<HKX_FP32, false, HKX_BF16>), dim3((unsigned)grid), dim3(256), 0, (hipStream_t)stream, a);
-  return api_launched(hipGetLastError(), "experts gather grad");
+  const bool vec = d % 8 == 0 && whole(dr, lddr, HKX_FP32) && whole(dx, lddx, HKX_BF16);
+  const int64_t per = ((int64_t)d + 2047) / 2048, most = std::max<int64_t>(((1 << 24) - 1) / per, 1);  // under 2^32 threads a launch
+  for (int64_t i = 0; i < t; i += most) {
+    a.t = (int)std::min(most, t - i);
+    a.slots = slots + i * k;
+    a.out = (uint16_t*)dx + i * lddx;
+    const dim3 grid((unsigned)(a.t * per));
+    if (vec) hipLaunchKernelGGL((combine_kernel<HKX_FP32, true, HKX_BF16>), grid, dim3(256), 0, (hipStream_t)stream, a);
+    else hipLaunchKernelGGL((combine_kernel<HKX_FP32, false, HKX_BF16>), grid, dim3(256), 0, (hipStream_t)stream, a);
+    if (hipError_t e = hipGetLastError()) return api_launched(e, "experts gather grad");
+  }
+  return api_launched(hipSuccess, "experts gather grad");
 }
 
 int hkx_experts_combine_backward(const void* y, int64_t ldy, const void* dout, int64_t lddo, int32_t dtype, const int32_t* slots,

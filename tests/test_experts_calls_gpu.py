@@ -53,3 +53,23 @@ def test_the_routers_gradient_past_a_launch():
         part = logits.detach()[at:at + 11].clone().requires_grad_()
         (want,) = torch.autograd.grad(experts.route(part, 1, renormalize=False)[0], part, dw[at:at + 11].clone())
         assert torch.equal(got[at:at + 11], want) and want.any()
+
+
+def test_a_gathered_gradient_past_a_launch():
+    """More tokens than one launch of their rows' sum takes."""
+    t, d = (1 << 24) + 9, 8
+    g = torch.Generator(device=DEV).manual_seed(4)
+    x = torch.zeros(t, d, dtype=BF16, device=DEV, requires_grad=True)
+    w = torch.randint(-3, 4, (2, 8, d), generator=g, device=DEV).to(BF16)
+    half = t // 2
+    offsets = torch.tensor([0, half, t], dtype=torch.int32, device=DEV)
+    rows = torch.arange(t - 1, -1, -1, dtype=torch.int32, device=DEV)  # token t - 1 first
+    plan = experts.Plan(offsets, rows, rows.reshape(t, 1))
+    dy = torch.zeros(t, 8, dtype=BF16, device=DEV)
+    dy[:, 0] = (torch.arange(t, device=DEV) % 61).to(BF16)
+    (dx,) = torch.autograd.grad(experts.gemm(x, w, plan, gather=True), x, dy)
+    # (small whole numbers: exact)
+    for at in (0, t - half - 5, (1 << 23) - 5, (1 << 24) - 6, t - 10):
+        row = rows[at:at + 10].long()
+        want = dy[row, :1].float() * w[(row >= half).long(), 0].float()
+        assert torch.equal(dx[at:at + 10].float(), want) and want.any()
