@@ -172,3 +172,58 @@ def test_rows_whose_tiles_an_int_does_not_count_are_refused():
             assert L.hkx_experts_gemm(ctypes.byref(g), None) == nat.ERR_SHAPE and "rows" in nat.last_error()
     for rows in (most + 1, 2 ** 31 - 1):
         assert L.hkx_experts_bias_grad(at, 8, at, at, nat.BF16, 2, rows, 8, None) == nat.ERR_SHAPE
+
+
+def test_the_rows_gradients_refusals():
+    L, at = nat.lib(), 1 << 20
+    for rc, code in [
+        (L.hkx_experts_gather_grad(None, 8, at, at, 8, 4, 2, 8, 8, None), nat.ERR_ARG),
+        (L.hkx_experts_gather_grad(at, 8, None, at, 8, 4, 2, 8, 8, None), nat.ERR_ARG),
+        (L.hkx_experts_gather_grad(at, 8, at, None, 8, 4, 2, 8, 8, None), nat.ERR_ARG),
+        (L.hkx_experts_gather_grad(at, 7, at, at, 8, 4, 2, 8, 8, None), nat.ERR_SHAPE),
+        (L.hkx_experts_gather_grad(at, 8, at, at, 7, 4, 2, 8, 8, None), nat.ERR_SHAPE),
+        (L.hkx_experts_gather_grad(at, 8, at, at, 8, 4, 0, 8, 8, None), nat.ERR_SHAPE),
+        (L.hkx_experts_gather_grad(at, 8, at, at, 8, 4, 2, -1, 8, None), nat.ERR_SHAPE),
+        (L.hkx_experts_gather_grad(at + 2, 8, at, at, 8, 4, 2, 8, 8, None), nat.ERR_SHAPE),
+        (L.hkx_experts_gather_grad(at, 8, at, at + 1, 8, 4, 2, 8, 8, None), nat.ERR_SHAPE),
+        (L.hkx_experts_gather_grad(at, 8, at, at, 8, 0, 2, 8, 8, None), nat.OK),
+    ]:
+        assert rc == code, nat.last_error()
+
+
+@pytest.mark.parametrize("kw,code,match", [
+    (dict(op=experts.NT), nat.ERR_DTYPE, "fp32 where"), (dict(op=experts.TN, m=8, c_expert=64), nat.ERR_DTYPE, "fp32 where"),
+    (dict(c_dtype=nat.FP16), nat.ERR_DTYPE, "fp32 where"), (dict(c=(1 << 20) + 8), nat.ERR_SHAPE, "an fp32 C's 16"),
+    (dict(ldc=10), nat.ERR_SHAPE, "an fp32 C's 16"), (dict(ldc=1 << 22), nat.ERR_SHAPE, "4 GiB")])
+def test_an_fp32_product_is_the_rows_gradient_alone(kw, code, match):
+    at = 1 << 20
+    g = nat.HkxExpertsGemmArgs()
+    g.size, g.op, g.ab_dtype, g.c_dtype = ctypes.sizeof(g), experts.NN, nat.BF16, nat.FP32
+    g.experts, g.rows, g.n, g.k = 2, 24, 8, 8
+    g.a = g.b = g.c = g.offsets = at
+    g.lda = g.ldb = g.ldc = 8
+    g.b_expert = 64
+    for name, v in kw.items():
+        setattr(g, name, v)
+    assert nat.lib().hkx_experts_gemm(ctypes.byref(g), None) == code and match in nat.last_error()
+
+
+def test_only_a_gathered_rows_product_is_fp32(monkeypatch, stub):
+    seen = []
+
+    class Lib:
+        def __getattr__(self, name):
+            def call(*a):
+                if name == "hkx_experts_gemm":
+                    seen.append((a[0]._obj.op, a[0]._obj.c_dtype))
+                return 0
+            return call
+
+    monkeypatch.setattr(nat, "lib", lambda: Lib())
+    w = _t(4, 40, 32).requires_grad_()
+    for gather, x in ((False, _t(24, 32)), (True, _t(12, 32))):
+        x.requires_grad_()
+        torch.autograd.grad(experts.gemm(x, w, PLAN, gather=gather), (x, w), _t(24, 40))
+    bf16 = nat.BF16
+    assert seen == [(experts.NT, bf16), (experts.NN, bf16), (experts.TN, bf16),
+                    (experts.NT, bf16), (experts.NN, nat.FP32), (experts.TN, bf16)]
