@@ -10,6 +10,12 @@ from test_experts_gpu import BF16, DEV, _plan, kernel  # noqa: F401
 pytestmark = pytest.mark.gpu
 
 
+@pytest.fixture(autouse=True)
+def _hand_the_memory_back():
+    yield
+    torch.cuda.empty_cache()
+
+
 @pytest.mark.parametrize("t,e,k,n,d,dead", [(9, 4, 2, 40, 24, 1), (150, 6, 4, 136, 200, 9), (700, 8, 8, 128, 64, 33),
                                             (3000, 4, 4, 264, 520, 0), (600, 2, 2, 2824, 264, 5)])
 def test_a_gathered_rows_gradient_is_rounded_once(t, e, k, n, d, dead, kernel):  # noqa: F811
@@ -73,3 +79,22 @@ def test_a_gathered_gradient_past_a_launch():
         row = rows[at:at + 10].long()
         want = dy[row, :1].float() * w[(row >= half).long(), 0].float()
         assert torch.equal(dx[at:at + 10].float(), want) and want.any()
+
+
+def test_a_gathered_gradient_of_rows_past_4_gib(kernel):  # noqa: F811
+    """The rows' fp32 gradient is 5.4 GB; small whole numbers, so that it is exact."""
+    t, e, k, d = 66_001, 3, 5, 4096
+    g = torch.Generator(device=DEV).manual_seed(5)
+    x = torch.zeros(t, d, dtype=BF16, device=DEV, requires_grad=True)
+    w = torch.randint(-2, 3, (e, 8, d), generator=g, device=DEV).to(BF16)
+    slots = torch.randperm(t * k, generator=g, device=DEV).int().reshape(t, k)
+    rows = torch.empty(t * k, dtype=torch.int32, device=DEV)
+    rows[slots.flatten().long()] = torch.arange(t, dtype=torch.int32, device=DEV).repeat_interleave(k)
+    offsets = torch.tensor([0, 1001, 200_003, t * k], dtype=torch.int32, device=DEV)
+    dy = torch.randint(-1, 2, (t * k, 8), generator=g, device=DEV).to(BF16)
+    (dx,) = torch.autograd.grad(experts.gemm(x, w, experts.Plan(offsets, rows, slots), gather=True), x, dy)
+    for at in (0, t // 2, t - 300):
+        s = slots[at:at + 300].long()
+        of = torch.bucketize(s, offsets[1:].long(), right=True)
+        want = (dy[s].float().unsqueeze(3) * w[of].float()).sum((1, 2))
+        assert torch.equal(dx[at:at + 300].float(), want) and want.any()
