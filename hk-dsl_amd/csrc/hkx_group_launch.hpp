@@ -35,7 +35,8 @@ inline int group_kernel(const GroupArgs& a, int op, bool fp8, bool pair, int ker
 }
 
 // The 256-row kernel may split its last round along K: the bytes of workspace that takes (0: none; 24 units of K are
-// some 36 us a round).
+// some 36 us a round). Whether it does goes by the counts of rows, which the host does not know: the second launch, that of
+// the sums, comes in any case, 5 us of it where no tile is split.
 inline size_t group_ws_bytes(const GroupArgs& a, int op, bool fp8, bool pair, int kernel, int cus) {
   if (op == kGroupTN || (int64_t)a.k * (fp8 ? 1 : 2) < 24 * 128 || group_kernel(a, op, fp8, pair, kernel, cus) != kGroupQuad) return 0;
   return (size_t)std::max(cus / 256 * 256, 256) * 256 * 256 * 4;

@@ -8,14 +8,18 @@ to the tokens; forward and backward.
 
 or all of it as `experts.mlp(x, logits, k, gate_up, down)`. T tokens have k experts each: R = T k rows, in the order of
 (expert, token). How many each expert has is known to the GPU alone: nothing here waits for the GPU, and every
-call can be captured in a graph after a first call.
+call can be captured in a graph after a first call. (A captured backward pass: while an eager graph of the same leaves is
+alive, torch's engine joins that one's stream to the captured one, which ends the process; drop its results first.)
 
 A `Plan` is three int32 tensors on the GPU: offsets (E + 1), of expert e the rows offsets[e] .. offsets[e + 1], from
 0; rows (R), the token of each row, -1 behind the last; slots (T, k), the row of each choice, -1 for one that has no
-expert. To drop a choice, set its slot to -1 (its row is then computed, and passes no gradient). A token whose logits are all -inf (padding) has no rows, and its output is zero. Plans from elsewhere may
-leave out `rows` where no call gathers, and `slots` where none combines or has a gathered gradient. Offsets out of
-order or past the rows are clamped and an index out of range stands for a row of zeros: nothing is read or written
-outside the tensors.
+expert. To drop a choice, set its slot to -1 (its row is then computed, and passes no gradient). A token whose logits are
+all -inf (padding) has no rows, and its output is zero. Plans from elsewhere may leave out `rows` where no call gathers,
+and `slots` where none combines or has a gathered gradient. Offsets out of order or past the rows are clamped and an index
+out of range stands for a row of zeros: nothing is read or written outside the tensors.
+
+Derivatives are the backward pass's, of bf16 products: a forward-mode one, a second one, and one through 8-bit operands or
+their scales are refused.
 
 The rows behind the last expert's are zeros in a new output and stay as they were in one that is passed in.
 
@@ -131,7 +135,8 @@ def gemm(x, w, plan, *, gather=False, bias=None, silu_mul=False, scale_a=None, s
     * silu_mul: w[e] (and scale_b, bias) holds N gate rows, then N up rows: silu(z[:, :N]) * z[:, N:] of z (R, 2N);
     * out: bf16 (R, N) to write into (no gradient), columns next to each other.
 
-    K and N multiples of 8, an 8-bit K of 16; E up to 1024; an expert's w, and an x that is gathered, under 4 GiB.
+    K and N multiples of 8, an 8-bit K of 16; E up to 1024, R up to 2^31 - 256; an expert's w, and an x that is gathered,
+    under 4 GiB.
     Sums are fp32, rounded once. Differentiable in x, w and bias (bf16): with silu_mul z is kept in bf16 for the backward
     pass and its gradient, which the other products read, rounded to bf16; a gathered x's gradient adds a token's rows,
     which stay fp32 till then, in order of its choices. No atomics: the same bits every time."""
@@ -621,9 +626,9 @@ def mlp(x, logits, k, gate_up, down, *, gate_up_scale=None, down_scale=None, ren
     hk.ops.block_norm(quant="fp8") gives it: each product's rows are quantized by hk.ops.fp8.quant."""
     if (gate_up_scale is None) != (down_scale is None) or (isinstance(x, tuple) and down_scale is None):
         raise TypeError("experts.mlp: 8-bit weights come with both scales, a quantized x with 8-bit weights")
-    if (x[0] if isinstance(x, tuple) else x).shape[:1] != logits.shape[:1]:
-        raise ValueError(f"experts.mlp: x has {tuple((x[0] if isinstance(x, tuple) else x).shape)}, logits {tuple(logits.shape)}: "
-                         f"a row a token")
+    rows = x[0] if isinstance(x, tuple) else x
+    if rows.shape[:1] != logits.shape[:1]:
+        raise ValueError(f"experts.mlp: x has {tuple(rows.shape)}, logits {tuple(logits.shape)}: a row a token")
     weights, _, plan = route(logits, k, renormalize=renormalize)
     if gate_up_scale is None and down_scale is None:
         a = gemm(x, gate_up, plan, gather=True, silu_mul=True)

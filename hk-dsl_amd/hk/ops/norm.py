@@ -15,11 +15,11 @@ h is rounded only as it is stored.
 D up to 16384 (8192 where gradients are taken).
 
 quant="mxfp8" or "mxfp4" gives y as (q, s), the operand of an MX product (hk.ops.mxfp4.gemm), without
-another pass: q (..., D) float8_e4m3fn, or (..., D/2) packed codes, and s (..., D/32); D a multiple of 32. quant="fp8" gives the operands of hk.ops.scaled_mm and
-hk.ops.experts.gemm: q (..., D) float8_e4m3fn and s (..., 1) fp32, as hk.ops.fp8.quant makes them of the fp32 y;
-any D.
+another pass: q (..., D) float8_e4m3fn, or (..., D/2) packed codes, and s (..., D/32); D a multiple of 32.
+quant="fp8" gives the operands of hk.ops.scaled_mm and hk.ops.experts.gemm: q (..., D) float8_e4m3fn and
+s (..., 1) fp32, as hk.ops.fp8.quant makes them of the fp32 y; any D.
 
-Differentiable in x, residual, post, pre and gate (not through a quantized y): one backward pass over the
+Differentiable in x, residual, post, pre and gate (not through a quantized y, nor in forward mode): one backward pass over the
 same bytes, with the gradients of post, pre and a broadcast gate summed in a fixed order, a run of rows in
 fp32 and the runs in 64 bits.
 
