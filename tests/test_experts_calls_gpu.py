@@ -98,3 +98,60 @@ def test_a_gathered_gradient_of_rows_past_4_gib(kernel):  # noqa: F811
         of = torch.bucketize(s, offsets[1:].long(), right=True)
         want = (dy[s].float().unsqueeze(3) * w[of].float()).sum((1, 2))
         assert torch.equal(dx[at:at + 300].float(), want) and want.any()
+
+
+def _ints(*shape, seed):
+    """-2 .. 2: sums are exact in any order."""
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    out = torch.empty(shape, dtype=BF16, device=DEV)
+    flat, step = out.view(-1), 999_983 * 16
+    block = torch.randint(-2, 3, (step,), generator=g, device=DEV, dtype=torch.int8)
+    for at in range(0, flat.numel(), step):
+        flat[at:at + step] = block[:min(step, flat.numel() - at)]
+    return out
+
+
+@pytest.mark.parametrize("silu_mul", [False, True], ids=["plain", "paired"])
+def test_rows_gathered_from_just_under_4_gib(silu_mul, kernel):  # noqa: F811
+    """The largest x that a call gathers from: its last rows among them, and the gradients."""
+    t, k, n, r = 524_284, 4096, 72, 3001
+    x, w = _ints(t, k, seed=1), _ints(3, 2 * n if silu_mul else n, k, seed=2) * 2.0 ** -7
+    g = torch.Generator(device=DEV).manual_seed(3)
+    rows = torch.randperm(t, generator=g, device=DEV)[:r].int()
+    rows[:4] = torch.tensor([t - 1, 0, t - 2, t // 2], device=DEV)
+    rows[4:] = torch.where((rows[4:] >= t - 2) | (rows[4:] == 0) | (rows[4:] == t // 2), -1, rows[4:])
+    plan = experts.Plan(torch.tensor([0, 5, 1400, r - 9], dtype=torch.int32, device=DEV), rows)
+    own = x[rows.clamp(min=0).long()] * (rows >= 0).unsqueeze(1)
+    own[r - 9:] = 0
+    y = experts.gemm(x, w, plan, gather=True, silu_mul=silu_mul)
+    assert torch.equal(y, experts.gemm(own, w, plan._replace(rows=None), silu_mul=silu_mul)) and y[:4].any(1).all()
+    slots = torch.full((t, 1), -1, dtype=torch.int32, device=DEV)
+    live = torch.arange(r, device=DEV, dtype=torch.int32)[rows >= 0]
+    slots[rows[live.long()].long(), 0] = live
+    dy = _ints(r, n, seed=4)
+    leaf, one = x.requires_grad_(), own.requires_grad_()
+    w.requires_grad_()
+    dx, dw = torch.autograd.grad(experts.gemm(leaf, w, plan._replace(slots=slots), gather=True, silu_mul=silu_mul), (leaf, w), dy)
+    d1, w1 = torch.autograd.grad(experts.gemm(one, w, plan._replace(rows=None), silu_mul=silu_mul), (one, w), dy)
+    assert torch.equal(dw, w1) and dw.any()
+    assert torch.equal(dx[rows[live.long()].long()], d1[live.long()]) and d1[:4].any(1).all()
+    dx[rows[live.long()].long()] = 0
+    assert not dx.any()
+
+
+@pytest.mark.parametrize("silu_mul", [False, True], ids=["plain", "paired"])
+def test_an_experts_weight_of_just_under_4_gib(silu_mul, kernel):  # noqa: F811
+    """The largest w[e] that a call takes: columns at its ends and in the middle are what they are by themselves."""
+    n, k, r = 262_128, 8192, 300
+    w, x = _ints(1, n, k, seed=1) * 2.0 ** -7, _ints(r, k, seed=2)
+    plan = experts.Plan(torch.tensor([0, r - 4], dtype=torch.int32, device=DEV))
+    y = experts.gemm(x, w, plan, silu_mul=silu_mul)
+    half = n // 2
+    for at in (0, half // 2 + 8, half - 40):
+        if silu_mul:
+            part = torch.cat((w[:, at:at + 40], w[:, half + at:half + at + 40]), 1)
+        else:
+            at = 2 * at if at != half - 40 else n - 40
+            part = w[:, at:at + 40].contiguous()
+        assert torch.equal(y[:, at:at + 40], experts.gemm(x, part, plan, silu_mul=silu_mul)) and y[0, at:at + 40].any()
+    assert not y[r - 4:].any()
